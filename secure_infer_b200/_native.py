@@ -102,6 +102,43 @@ class Codec(ct.Structure):
     _fields_ = [("bits", ct.c_uint32), ("kind", ct.c_uint32), ("heads", ct.c_uint32), ("layer", ct.c_uint32)]
 
 
+class Pages(ct.Structure):
+    """secure_infer_pages (include/secure_infer_paged.h)."""
+    _fields_ = [("k", P), ("v", P), ("k_stride", ct.c_int64 * 3), ("v_stride", ct.c_int64 * 3), ("pages", U32),
+                ("heads", U32), ("dtype", U32), ("reserved", U32)]
+
+
+class Chunk(ct.Structure):
+    """secure_infer_chunk (include/secure_infer_paged.h)."""
+    _fields_ = [("block_table", P), ("cu_q", P), ("kv_lens", P), ("table_stride", ct.c_int64), ("table_width", U32),
+                ("seqs", U32), ("tokens", U32), ("max_q", U32)]
+
+
+class Tables(ct.Structure):
+    """secure_infer_tables (include/secure_infer_paged.h)."""
+    _fields_ = [("block_table", P), ("lens", P), ("refs", P), ("seqs", U32), ("width", U32), ("pages", U32),
+                ("reserved", U32)]
+
+
+class PageTensor(ct.Structure):
+    """secure_infer_page_tensor (include/secure_infer_paged.h)."""
+    _fields_ = [("base", P), ("page_stride", ct.c_int64)]
+
+
+# Operators on the paged cache.  Structures go by reference.
+PAGED_SIGNATURES = {
+    "secure_infer_paged_attend_workspace": ([], U64),
+    "secure_infer_paged_attend": ([P, P, P, P, U32, P, P, ct.c_float, U32, U32, P, P], I32),
+    "secure_infer_paged_append": ([P, P, P, P, U32, P, P, P, P, P, P, P, P, ct.c_int64, U32, U32, P], I32),
+    "secure_infer_paged_scratch": ([P, U32], U64),
+    "secure_infer_paged_copy": ([P, U32, U64, U32, P, P, U32, P], I32),
+    "secure_infer_paged_fork": ([P, U32, U64, P, P, P, P, U32, P, P, P], I32),
+    "secure_infer_paged_reserve": ([P, P, P, P, U32, P, P, P], I32),
+    "secure_infer_paged_free": ([P, P, P, U32, P, P], I32),
+    "secure_infer_paged_compact": ([P, U32, U64, P, P, P, P, P, P], I32),
+}
+HOST_SIGNATURES.update(PAGED_SIGNATURES)
+
 # SECURE_INFER_KIND_KV: a reload of 2n records, K packets first, V packets after.
 KIND_KV = 2
 

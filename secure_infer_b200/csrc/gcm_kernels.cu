@@ -1892,30 +1892,6 @@ cudaEvent_t prof_event()
     return e;
 }
 
-// Brackets one launch with timing events when profiling is on.
-class ProfileScope {
-public:
-    ProfileScope(uint32_t kind, cudaStream_t stream) : stream_(stream)
-    {
-        if (!g_prof_on.load(std::memory_order_relaxed)) return;
-        std::lock_guard<std::mutex> lock(g_prof_mu);
-        rec_ = ProfileRec{kind, prof_event(), prof_event()};
-        active_ = rec_.start && rec_.end && cudaEventRecord(rec_.start, stream) == cudaSuccess;
-    }
-    ~ProfileScope()
-    {
-        if (!active_) return;
-        std::lock_guard<std::mutex> lock(g_prof_mu);
-        cudaEventRecord(rec_.end, stream_);
-        g_prof_recs.push_back(rec_);
-    }
-
-private:
-    cudaStream_t stream_;
-    ProfileRec rec_{};
-    bool active_ = false;
-};
-
 template <bool A>
 int segment_launch_impl(const SegmentLaunch& args, size_t smem, int variant, cudaStream_t stream)
 {
@@ -1953,6 +1929,23 @@ int segment_launch_impl(const SegmentLaunch& args, size_t smem, int variant, cud
 
 }  // namespace
 
+ProfileScope::ProfileScope(uint32_t kind, cudaStream_t stream) : stream_(stream), kind_(kind)
+{
+    if (!g_prof_on.load(std::memory_order_relaxed)) return;
+    std::lock_guard<std::mutex> lock(g_prof_mu);
+    start_ = prof_event();
+    end_ = prof_event();
+    active_ = start_ && end_ && cudaEventRecord(start_, stream) == cudaSuccess;
+}
+
+ProfileScope::~ProfileScope()
+{
+    if (!active_) return;
+    std::lock_guard<std::mutex> lock(g_prof_mu);
+    cudaEventRecord(end_, stream_);
+    g_prof_recs.push_back(ProfileRec{kind_, start_, end_});
+}
+
 uint32_t set_layer_sm_limit(uint32_t sms) { return g_layer_sm_limit.exchange(sms); }
 
 void profile_enable(bool on) { g_prof_on.store(on); }
@@ -1985,7 +1978,10 @@ const char* kernel_kind_name(uint32_t kind)
     static const char* names[kKernKinds] = {"gcm_layer_ctr_kernel", "gcm_layer_verify_kernel", "gcm_layer_encrypt",
                                             "kv_encode_kernel", "gcm_segment_kernel", "gcm_ctr_kernel",
                                             "gcm_schedule_kernel", "auth_gate_kernel",
-                                            "gcm_layer_verify_inline_kernel", "gcm_layer_ctr_bs_kernel"};
+                                            "gcm_layer_verify_inline_kernel", "gcm_layer_ctr_bs_kernel",
+                                            "paged_attend_rows_kernel", "paged_attend_tiles_kernel",
+                                            "paged_attend_join_kernel", "paged_append_kernel", "page_copy_kernel",
+                                            "page_tables_kernel"};
     return kind < kKernKinds ? names[kind] : nullptr;
 }
 

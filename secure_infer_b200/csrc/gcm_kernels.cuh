@@ -164,7 +164,20 @@ int launch_layer_verify_inline(const LayerHeader& h, const LayerRec* rec, cudaSt
 // events on its stream; collect() sums device time and launches per kind.
 enum KernelKind : uint32_t {
     kKernLayerCtr = 0, kKernLayerVerify, kKernLayerEncrypt, kKernEncode, kKernSegment, kKernCtr, kKernSchedule,
-    kKernAuthGate, kKernLayerVerifyInline, kKernLayerCtrBitsliced, kKernKinds
+    kKernAuthGate, kKernLayerVerifyInline, kKernLayerCtrBitsliced, kKernAttendRows, kKernAttendTiles, kKernAttendJoin,
+    kKernAppend, kKernPageCopy, kKernTables, kKernKinds
+};
+// Brackets one launch with timing events while the profile is enabled.
+class ProfileScope {
+public:
+    ProfileScope(uint32_t kind, cudaStream_t stream);
+    ~ProfileScope();
+
+private:
+    cudaStream_t stream_;
+    uint32_t kind_ = 0;
+    cudaEvent_t start_ = nullptr, end_ = nullptr;
+    bool active_ = false;
 };
 void profile_enable(bool on);
 int profile_collect(double* total_us, uint64_t* launches, uint32_t kinds);

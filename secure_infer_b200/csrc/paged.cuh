@@ -1,0 +1,435 @@
+// paged.cuh -- what the kernels on the paged KV cache share: launch
+// descriptors, the walk over attention's work, barriers and copies.
+#pragma once
+
+#include <cstdint>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <type_traits>
+
+#include "../../include/secure_infer_paged.h"
+
+namespace sib {
+namespace paged {
+
+constexpr int kPage = 128;   // tokens of a page
+constexpr int kDim = 128;    // values of a head
+
+struct AttendParams {
+    const void* q;
+    int64_t q_token, q_head;        // strides, elements
+    const void* k;
+    const void* v;
+    int64_t k_stride[3], v_stride[3];
+    void* out;
+    float* lse;                     // or null
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* cu;
+    const int32_t* kv;
+    int32_t width, seqs, tokens, pages;
+    int32_t heads, group;           // KV heads, query heads of each
+    int32_t rows_min, rows_max;     // sequences with rows_min <= rows <= rows_max are this launch's
+    int32_t causal, window;
+    float scale_log2;               // scale * log2(e): the softmax runs in powers of two
+    uint32_t* counters;             // [grid], zero between launches
+    uint32_t* status;
+    float* slots;                   // [2 * grid] partial results
+};
+
+// Launchers (cudaError_t values).
+int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int m_tiles,
+                       uint32_t dtype, cudaStream_t stream);
+uint64_t attend_workspace_bytes();
+void attend_workspace(void* workspace, AttendParams* p);   // its counters, status word and slots
+
+struct AppendParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride[2], k_in[2], v_in[2];
+    void* q_out;
+    void* k_cache;
+    void* v_cache;
+    int64_t k_stride[3], v_stride[3];
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* cu;
+    const int32_t* kv;
+    const uint64_t* phase;
+    const uint32_t* axis;
+    const int32_t* positions;
+    int64_t position_stride;
+    int32_t width, seqs, tokens, pages, q_heads, heads, axes, interleaved;
+};
+int launch_append(const AppendParams& p, uint32_t dtype, cudaStream_t stream);
+
+constexpr int kCopyTensors = 240;   // tensors of one copy launch, passed by value
+struct CopyParams {
+    const int32_t* src;
+    const int32_t* dst;
+    const int32_t* count;           // entries of src and dst, or null: n
+    int32_t n, pages, tensors;
+    int64_t page_bytes;
+    secure_infer_page_tensor t[kCopyTensors];
+};
+int launch_page_copy(const secure_infer_page_tensor* tensors, uint32_t n_tensors, uint64_t page_bytes, uint32_t pages,
+                     const int32_t* src, const int32_t* dst, const int32_t* count, uint32_t n, cudaStream_t stream);
+
+enum TableOp : int32_t { kFork, kReserve, kFree, kCompact };
+struct TableParams {
+    secure_infer_tables in, out;
+    const int32_t* a;               // fork: parents; reserve, free: sequences
+    const int32_t* b;               // fork: children; reserve: new lengths
+    int32_t* granted;
+    int32_t* moved;
+    int32_t* live;
+    int32_t* scratch;
+    int32_t n;
+};
+int launch_tables(TableOp op, const TableParams& p, cudaStream_t stream);
+uint64_t table_scratch_ints(uint32_t seqs, uint32_t pages, uint32_t n);
+// Where a table kernel leaves the page copies to make, in scratch.
+struct CopyList {
+    int32_t *count, *src, *dst;
+};
+CopyList table_copy_list(int32_t* scratch, uint32_t pages);
+
+#ifdef __CUDACC__
+// ------------------------------------------------------------ device helpers
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void dependents_may_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// Waits for the phase of parity `parity`.  The wait is bounded: some seconds
+// of tries that the hardware suspends, after which `abort` is set and every
+// wait of the CTA gives up, so a protocol error ends the kernel instead of
+// hanging it.  Returns whether the phase completed.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* abort)
+{
+    for (int tries = 0; tries < (1 << 22); ++tries) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((tries & 63) == 63 && *abort) return false;
+    }
+    *abort = 1;
+    return false;
+}
+
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int half,
+                                              int head, int page)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(0), "r"(token), "r"(half), "r"(head), "r"(page)
+        : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t x);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x)
+{
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t x)
+{
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+// An infinity or a NaN in either half.
+template <typename T>
+__device__ __forceinline__ bool nonfinite2(uint32_t x)
+{
+    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return (x & e) == e || ((x >> 16) & e) == e;
+}
+
+// ------------------------------------------------- attention's work, in order
+//
+// A sequence's rows are (new token, query head of the group), flattened, so one
+// KV head's K and V serve the whole group.  A tile is kRows of them over one KV
+// head; its units are the pages that any of its rows sees (one empty unit if
+// none).  All units of a launch in the order sequence, tile, head, page are cut
+// into equal consecutive shares, one per CTA: every CTA gets the same work
+// whatever the lengths, and a long axis is split where there are few rows.
+struct Seq {
+    int n, kv, q0;   // new tokens, all tokens, first new token
+};
+
+__device__ __forceinline__ Seq load_seq(const AttendParams& p, int s)
+{
+    Seq r;
+    int a = p.cu[s], b = p.cu[s + 1];
+    a = max(0, min(a, p.tokens));
+    b = max(a, min(b, p.tokens));
+    r.q0 = a;
+    r.n = b - a;
+    r.kv = max(0, min(p.kv[s], p.width * kPage));
+    const int64_t rows = static_cast<int64_t>(r.n) * p.group;
+    if (rows < p.rows_min || rows > p.rows_max) r.n = 0;
+    return r;
+}
+
+struct Span {
+    int first, pages;   // page range of a tile
+    int lo, hi;         // keys that any row of it sees: [lo, hi)
+};
+
+__device__ __forceinline__ Span tile_span(const AttendParams& p, const Seq& s, int first_token, int last_token)
+{
+    Span r;
+    r.hi = p.causal ? min(s.kv, s.kv - s.n + last_token + 1) : s.kv;
+    r.lo = p.window ? max(0, s.kv - s.n + first_token - p.window + 1) : 0;
+    if (r.hi <= r.lo) {
+        r.lo = r.hi = r.first = 0;
+        r.pages = 1;
+    } else {
+        r.first = r.lo / kPage;
+        r.pages = (r.hi + kPage - 1) / kPage - r.first;
+    }
+    return r;
+}
+
+struct Walk {
+    int rows_per_tile;
+    int s, tile, tiles, head;
+    Seq q;
+    Span span;
+    int page;                // next unit of the tile: 0 .. span.pages
+    int first_token, last_token, rows;   // of the tile
+    int64_t tile_unit;       // unit number of the tile's first unit
+    int64_t left;            // units of this CTA not yet taken
+
+    __device__ __forceinline__ void set_tile(const AttendParams& p)
+    {
+        const int r0 = tile * rows_per_tile;
+        rows = min(rows_per_tile, q.n * p.group - r0);
+        first_token = r0 / p.group;
+        last_token = (r0 + rows - 1) / p.group;
+        span = tile_span(p, q, first_token, last_token);
+    }
+    // Past the last unit of a tile: the next head, tile or sequence.
+    __device__ __forceinline__ void next_tile(const AttendParams& p)
+    {
+        tile_unit += span.pages;
+        page = 0;
+        if (++head < p.heads) return;
+        head = 0;
+        if (++tile < tiles) {
+            set_tile(p);
+            return;
+        }
+        tile = 0;
+        do {
+            if (++s >= p.seqs) return;
+            q = load_seq(p, s);
+        } while (q.n == 0);
+        tiles = (q.n * p.group + rows_per_tile - 1) / rows_per_tile;
+        set_tile(p);
+    }
+};
+
+__device__ __forceinline__ int64_t seq_units(const AttendParams& p, const Seq& s, int rows_per_tile)
+{
+    if (s.n == 0) return 0;
+    int64_t pages = 0;
+    const int rows = s.n * p.group;
+    for (int r = 0; r < rows; r += rows_per_tile)
+        pages += tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages;
+    return pages * p.heads;
+}
+
+// The share of this CTA: [begin, begin + units) of `per` units each.
+struct Share {
+    int64_t per;      // units of a CTA
+    int64_t begin;    // first unit of this one
+    int seq;          // sequence of the first unit, -1: none
+    int64_t seq_unit; // unit number of that sequence's first unit
+    int64_t total;
+};
+
+// All threads of the block take part; `warp_sums` holds one value per warp.
+// At least min_units go to a CTA that has any, so short work is not split.
+template <int kThreads>
+__device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int min_units, Share* share,
+                                           int64_t* warp_sums)
+{
+    constexpr int kWarps = kThreads / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int64_t base = 0;
+    // Pass 0 sums the units; pass 1 finds the sequence that holds the first of this CTA's.
+    for (int pass = 0; pass < 2; ++pass) {
+        base = 0;
+        for (int s0 = 0; s0 < p.seqs; s0 += kThreads) {
+            const int s = s0 + tid;
+            const int64_t own = s < p.seqs ? seq_units(p, load_seq(p, s), rows_per_tile) : 0;
+            int64_t sum = own;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t up = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += up;
+            }
+            if (lane == 31) warp_sums[warp] = sum;
+            __syncthreads();
+            int64_t before = base;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) before += warp_sums[w];
+                base += warp_sums[w];
+            }
+            if (pass == 0 && p.seqs <= kThreads) {   // one round holds every sequence: no second pass
+                if (tid == 0) {
+                    share->total = base;
+                    share->seq = -1;
+                    int64_t per = (base + gridDim.x - 1) / gridDim.x;
+                    share->per = per < min_units ? min_units : per;
+                    share->begin = share->per * blockIdx.x;
+                }
+                __syncthreads();
+            }
+            if (pass == 1 || p.seqs <= kThreads) {
+                const int64_t first = before + sum - own;
+                if (own > 0 && share->begin >= first && share->begin < first + own) {
+                    share->seq = s;
+                    share->seq_unit = first;
+                }
+            }
+            __syncthreads();
+        }
+        if (p.seqs <= kThreads) break;
+        if (pass == 0) {
+            if (tid == 0) {
+                share->total = base;
+                share->seq = -1;
+                int64_t per = (base + gridDim.x - 1) / gridDim.x;
+                share->per = per < min_units ? min_units : per;
+                share->begin = share->per * blockIdx.x;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+__device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_tile, const Share& share)
+{
+    Walk w;
+    w.rows_per_tile = rows_per_tile;
+    w.left = 0;
+    if (share.seq < 0) return w;
+    w.left = min(share.per, share.total - share.begin);
+    w.s = share.seq;
+    w.q = load_seq(p, w.s);
+    w.tiles = (w.q.n * p.group + rows_per_tile - 1) / rows_per_tile;
+    w.tile = 0;
+    w.tile_unit = share.seq_unit;
+    w.set_tile(p);
+    int64_t skip = share.begin - share.seq_unit;
+    while (skip >= static_cast<int64_t>(w.span.pages) * p.heads) {
+        skip -= static_cast<int64_t>(w.span.pages) * p.heads;
+        w.tile_unit += static_cast<int64_t>(w.span.pages) * p.heads;
+        ++w.tile;
+        w.set_tile(p);
+    }
+    w.head = static_cast<int>(skip / w.span.pages);
+    w.page = static_cast<int>(skip % w.span.pages);
+    w.tile_unit += static_cast<int64_t>(w.head) * w.span.pages;
+    return w;
+}
+
+// Keys that row r of the tile sees: [lo, hi].
+__device__ __forceinline__ void row_keys(const AttendParams& p, const Seq& s, int token, int& lo, int& hi)
+{
+    hi = p.causal ? min(s.kv, s.kv - s.n + token + 1) - 1 : s.kv - 1;
+    lo = p.window ? max(0, s.kv - s.n + token - p.window + 1) : 0;
+}
+
+// One row over keys [a, b) by one warp, straight from the pages: lane l holds
+// values 4l .. 4l+3.  Only rows of a tile in which some row must not see an
+// infinite or NaN value that another one does see come here: in a matrix
+// product zero times such a value would be NaN.
+template <typename T>
+__device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q, const int32_t* table, int head, int a,
+                                               int b, float& m, float& l, float4& o)
+{
+    const int d = 4 * (threadIdx.x & 31);
+    const uint2 qx = *reinterpret_cast<const uint2*>(q + d);
+    const float2 q0 = unpack2<T>(qx.x), q1 = unpack2<T>(qx.y);
+    m = -INFINITY;
+    l = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = a; j < b; ++j) {
+        const int page = table[j / kPage];
+        float2 k0 = {0, 0}, k1 = {0, 0}, v0 = {0, 0}, v1 = {0, 0};
+        if (page >= 0 && page < p.pages) {
+            const uint2 kx = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.k) + page * p.k_stride[0] +
+                                                             (j % kPage) * p.k_stride[1] + head * p.k_stride[2] + d);
+            const uint2 vx = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.v) + page * p.v_stride[0] +
+                                                             (j % kPage) * p.v_stride[1] + head * p.v_stride[2] + d);
+            k0 = unpack2<T>(kx.x), k1 = unpack2<T>(kx.y), v0 = unpack2<T>(vx.x), v1 = unpack2<T>(vx.y);
+        }
+        float x = q0.x * k0.x + q0.y * k0.y + q1.x * k1.x + q1.y * k1.y;
+        for (int s = 16; s; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+        x *= p.scale_log2;
+        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.0f : top;
+        const float f = m == top ? 1.0f : exp2f(m - top), e = exp2f(x - base);
+        m = top;
+        l = l * f + e;
+        o.x = o.x * f + e * v0.x;
+        o.y = o.y * f + e * v0.y;
+        o.z = o.z * f + e * v1.x;
+        o.w = o.w * f + e * v1.y;
+    }
+}
+
+// Weight of a partial result with maximum m in a whole with maximum top.
+__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.0f : exp2f(m - top); }
+#endif  // __CUDACC__
+
+}  // namespace paged
+}  // namespace sib

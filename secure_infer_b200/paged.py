@@ -1,0 +1,396 @@
+"""Operators on the paged KV cache that reloads fill (include/secure_infer_paged.h).
+
+* ``append``  -- rotary positions (one or several axes) of a step's new queries
+  and keys, and the new keys' and values' way into their pages;
+* ``attend``  -- attention of the new tokens over the pages, from single tokens
+  to long chunks, ragged over sequences;
+* ``CachePages`` -- copies, forks, reserves, frees and compacts pages of all
+  layers.
+
+A layer's cache is K and V of ``[pages, 128, KV heads, 128]`` in bf16 or fp16,
+as ``NativeTransfer`` and ``LayerwiseReloader`` fill it.  Handles
+(``LayerPages``, ``CachePages``, ``Rotary``) are made once, a ``Chunk`` once per
+step for all its layers.  Calls run on the current stream and return without
+waiting; lengths, tables and page ids stay on the device.  Bad arguments raise
+``ValueError`` before anything is launched, a refused launch ``RuntimeError``.
+As everywhere in this package there is no fallback: the work goes through
+``libsecure_infer.so``.
+"""
+from __future__ import annotations
+
+import ctypes as ct
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _native
+
+PAGE = 128
+HEAD_DIM = 128
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _ints(t, what: str, device, dims: int) -> torch.Tensor:
+    """An int32 tensor of the device, as given or made from a list."""
+    if not isinstance(t, torch.Tensor):
+        t = torch.tensor(list(t), dtype=torch.int32, device=device)
+    _need(t.dtype == torch.int32 and t.ndim == dims and t.device == device,
+          f"{what} must be an int32 tensor of {dims} dimension(s) on {device}")
+    _need(t.numel() == 0 or t.stride(-1) == 1, f"{what} must be dense in its last dimension")
+    return t
+
+
+def _rows(t: torch.Tensor, what: str, tokens: int, dtype, device) -> tuple[int, int, int]:
+    """Heads and strides of [tokens, heads, 128]."""
+    _need(t.ndim == 3 and t.shape[0] == tokens and t.shape[2] == HEAD_DIM,
+          f"{what} must be [{tokens}, heads, {HEAD_DIM}], not {list(t.shape)}")
+    _need(t.dtype == dtype and t.device == device, f"{what} must be {dtype} on {device}")
+    st, sh, sd = t.stride()
+    # A single token or head has no stride of its own.
+    st = st if tokens > 1 else HEAD_DIM
+    sh = sh if t.shape[1] > 1 else HEAD_DIM
+    _need(sd == 1 and t.data_ptr() % 16 == 0 and st > 0 and sh > 0 and st % 8 == 0 and sh % 8 == 0,
+          f"{what}: a head's values must be adjacent, the address and strides multiples of 16 bytes")
+    return t.shape[1], st, sh
+
+
+class LayerPages:
+    """One layer's paged cache: ``k`` and ``v`` ``[pages, 128, heads, 128]`` of
+    one type, in any order of pages, tokens and heads in memory."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device, "K and V differ in shape, type or device")
+        _need(k.ndim == 4 and k.shape[0] > 0 and k.shape[1] == PAGE and k.shape[2] > 0 and k.shape[3] == HEAD_DIM,
+              f"a cache is [pages, {PAGE}, heads, {HEAD_DIM}], not {list(k.shape)}")
+        _need(k.dtype in _DTYPES, f"a cache holds bf16 or fp16, not {k.dtype}")
+        _need(k.is_cuda, "the cache must be on a CUDA device")
+        strides = []
+        for t in (k, v):
+            s = list(t.stride())
+            if t.shape[0] == 1:
+                s[0] = PAGE * HEAD_DIM * t.shape[2]
+            if t.shape[2] == 1:
+                s[2] = HEAD_DIM
+            _need(s[3] == 1 and t.data_ptr() % 16 == 0 and all(x > 0 and x % 8 == 0 for x in s[:3]),
+                  "a head's values must be adjacent, the cache's address and strides multiples of 16 bytes")
+            strides.append(s[:3])
+        self.k, self.v = k, v
+        self.pages, self.heads, self.dtype, self.device = k.shape[0], k.shape[2], k.dtype, k.device
+        self._c = _native.Pages(k.data_ptr(), v.data_ptr(), (ct.c_int64 * 3)(*strides[0]), (ct.c_int64 * 3)(*strides[1]),
+                                self.pages, self.heads, _DTYPES[k.dtype], 0)
+        self._ref = ct.byref(self._c)
+
+
+class Chunk:
+    """The new tokens of one step, ragged over its sequences.
+
+    ``block_table`` int32 ``[seqs, width]``: page of every 128 tokens (entries
+    past a sequence's length are not read); ``cu_q`` int32 ``[seqs + 1]``: where
+    each sequence's new tokens begin; ``kv_lens`` int32 ``[seqs]``: its tokens in
+    all, the new ones last.  ``max_q``: no sequence has more new tokens; given,
+    it lets steps of single tokens take their own path.  The tensors are kept
+    and read when the operators run, so a captured graph follows their contents.
+    """
+
+    def __init__(self, block_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q: int | None = None):
+        _need(isinstance(block_table, torch.Tensor) and block_table.is_cuda, "block_table must be on a CUDA device")
+        device = block_table.device
+        _ints(block_table, "block_table", device, 2)
+        _ints(cu_q, "cu_q", device, 1)
+        _ints(kv_lens, "kv_lens", device, 1)
+        seqs, width = block_table.shape
+        _need(seqs > 0 and width > 0, "block_table is empty")
+        _need(cu_q.shape[0] == seqs + 1 and kv_lens.shape[0] == seqs, "cu_q needs seqs + 1 entries, kv_lens seqs")
+        _need(max_q is None or max_q >= 0, "max_q is negative")
+        stride = block_table.stride(0) if seqs > 1 else width
+        _need(stride >= width, "block_table's rows overlap")
+        self.block_table, self.cu_q, self.kv_lens, self.device = block_table, cu_q, kv_lens, device
+        self._c = _native.Chunk(block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), stride, width, seqs, 0,
+                                max_q or 0)
+        self._ref = ct.byref(self._c)
+
+
+class Rotary:
+    """Rotary positions of 128-value heads: pair ``i`` turns by ``position *
+    base ** (-i / 64)`` radians.  ``sections``: how many of the 64 pairs, in
+    order, go by each axis of the positions (``(64,)``: one axis; ``(16, 24,
+    24)``: time, height, width).  ``interleaved``: pair ``i`` is elements ``2i``
+    and ``2i + 1`` instead of ``i`` and ``i + 64``."""
+
+    def __init__(self, base: float = 10000.0, sections=(64,), interleaved: bool = False, device="cuda"):
+        sections = [int(n) for n in sections]
+        _need(base > 0 and math.isfinite(base), "base must be positive")
+        _need(len(sections) > 0 and all(n >= 0 for n in sections) and sum(sections) == HEAD_DIM // 2,
+              f"sections must be counts that add up to {HEAD_DIM // 2}")
+        self.axes, self.interleaved = len(sections), bool(interleaved)
+        # Revolutions per position as a fraction of 2^64, so a position's angle is an exact product modulo one turn.
+        turns = [round(base ** (-i / 64) / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for i in range(HEAD_DIM // 2)]
+        self.phase = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
+        self.axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32, device=device)
+        self.device = self.phase.device
+
+
+def _call(name: str, device, *args) -> None:
+    lib = _native.lib()
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args)
+    else:
+        rc = getattr(lib, name)(*args)
+    if rc != 0:
+        raise RuntimeError(f"{name} refused its arguments or failed to launch")
+
+
+def append(pages: LayerPages, chunk: Chunk, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, *,
+           rotary: Rotary | None = None, positions: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """Write the chunk's ``k`` and ``v`` ``[tokens, heads, 128]`` into their
+    pages, keys turned by ``rotary``; returns ``q`` ``[tokens, q heads, 128]``
+    turned likewise (``out``, or a new tensor; ``None`` without ``q``).
+
+    ``positions`` int32 ``[axes, tokens]`` or ``[tokens]``; by default the
+    tokens' places in their sequences.  A token whose place lies outside its
+    sequence's pages is not written."""
+    tokens, device, dtype = k.shape[0], pages.device, pages.dtype
+    _need(chunk.device == device, "the chunk and the cache are on different devices")
+    heads, kt, kh = _rows(k, "k", tokens, dtype, device)
+    v_heads, vt, vh = _rows(v, "v", tokens, dtype, device)
+    _need(heads == pages.heads and v_heads == heads, f"k and v must have the cache's {pages.heads} heads")
+    q_heads, qs, q_ptr, out_ptr = 0, None, None, None
+    if q is not None:
+        q_heads, qt, qh = _rows(q, "q", tokens, dtype, device)
+        qs, q_ptr = (ct.c_int64 * 2)(qt, qh), q.data_ptr()
+        if out is None:
+            out = torch.empty((tokens, q_heads, HEAD_DIM), dtype=dtype, device=device)
+        else:
+            _need(out.shape == q.shape and out.dtype == dtype and out.device == device and out.is_contiguous() and
+                  out.data_ptr() % 16 == 0, "out must be dense, with q's shape, type and device")
+        out_ptr = out.data_ptr()
+    else:
+        _need(out is None, "out goes with q")
+    phase = axis = pos_ptr = None
+    pos_stride, axes, interleaved = 0, 1, 0
+    if rotary is not None:
+        _need(rotary.device == device, "rotary and the cache are on different devices")
+        phase, axis, axes, interleaved = rotary.phase.data_ptr(), rotary.axis.data_ptr(), rotary.axes, rotary.interleaved
+        if positions is not None:
+            positions = _ints(positions, "positions", device, positions.ndim)
+            if positions.ndim == 1:
+                _need(axes == 1, f"positions must be [{axes}, tokens]")
+                positions = positions[None]
+            _need(tuple(positions.shape) == (axes, tokens), f"positions must be [{axes}, {tokens}]")
+            pos_ptr, pos_stride = positions.data_ptr(), positions.stride(0) if axes > 1 else tokens
+            _need(pos_stride >= 0, "positions has a negative stride")
+    else:
+        _need(positions is None, "positions go with rotary")
+    if tokens == 0:
+        return out
+    chunk._c.tokens = tokens
+    _call("secure_infer_paged_append", device, pages._ref, chunk._ref, q_ptr, qs, q_heads, out_ptr, k.data_ptr(),
+          (ct.c_int64 * 2)(kt, kh), v.data_ptr(), (ct.c_int64 * 2)(vt, vh), phase, axis, pos_ptr, pos_stride, axes,
+          interleaved, torch.cuda.current_stream(device).cuda_stream)
+    return out
+
+
+_workspaces: dict = {}
+
+
+def attend_workspace(device) -> torch.Tensor:
+    """A workspace for ``attend``: one per stream that calls it."""
+    return torch.zeros(int(_native.lib().secure_infer_paged_attend_workspace()), dtype=torch.uint8, device=device)
+
+
+def _workspace(device, stream: int) -> torch.Tensor:
+    w = _workspaces.get((device, stream))
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attend's first call on a stream makes its workspace: make it before capturing, "
+                               "or pass workspace=attend_workspace(device)")
+        w = _workspaces[(device, stream)] = attend_workspace(device)
+    return w
+
+
+def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | None = None, causal: bool = True,
+           window: int = 0, return_lse: bool = False, out: torch.Tensor | None = None,
+           workspace: torch.Tensor | None = None):
+    """Attention of the chunk's queries ``[tokens, q heads, 128]`` over the
+    pages: query head ``h`` reads KV head ``h // (q heads / KV heads)``.
+
+    ``scale``: of the scores, 128 ** -0.5 by default.  ``causal``: the token at
+    position ``p`` sees keys ``0 .. p``, with ``window`` only the last
+    ``window`` of them; otherwise all of its sequence.  Returns ``[tokens,
+    q heads, 128]``, and with ``return_lse`` the natural logarithms of the
+    softmax sums, float32 ``[tokens, q heads]``, to join it with attention over
+    other keys.  A row that sees no key gives 0 and -inf.  ``workspace``:
+    ``attend_workspace(device)``, by default one that the current stream
+    keeps."""
+    device, dtype = pages.device, pages.dtype
+    _need(chunk.device == device, "the chunk and the cache are on different devices")
+    tokens = q.shape[0]
+    q_heads, qt, qh = _rows(q, "q", tokens, dtype, device)
+    _need(q_heads > 0 and q_heads % pages.heads == 0, f"q's heads must be a multiple of the cache's {pages.heads}")
+    _need(0 <= window < 1 << 31 and (causal or window == 0), "window must be zero or positive, and goes with causal")
+    if out is None:
+        out = torch.empty((tokens, q_heads, HEAD_DIM), dtype=dtype, device=device)
+    else:
+        _need(out.shape == q.shape and out.dtype == dtype and out.device == device and out.is_contiguous() and
+              out.data_ptr() % 16 == 0, "out must be dense, with q's shape, type and device")
+    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=device) if return_lse else None
+    if tokens > 0:
+        stream = torch.cuda.current_stream(device).cuda_stream
+        if workspace is None:
+            workspace = _workspace(device, stream)
+        else:
+            _need(workspace.device == device and workspace.is_contiguous() and workspace.data_ptr() % 256 == 0 and
+                  workspace.numel() * workspace.element_size() >= _native.lib().secure_infer_paged_attend_workspace(),
+                  "workspace must come from attend_workspace of the cache's device")
+        chunk._c.tokens = tokens
+        _call("secure_infer_paged_attend", device, pages._ref, chunk._ref, q.data_ptr(), (ct.c_int64 * 2)(qt, qh),
+              q_heads, out.data_ptr(), lse.data_ptr() if return_lse else None,
+              HEAD_DIM ** -0.5 if scale is None else float(scale), 1 if causal else 0, window, workspace.data_ptr(),
+              stream)
+    return (out, lse) if return_lse else out
+
+
+class PageTables(NamedTuple):
+    """Who holds which page: ``block_table`` int32 ``[seqs, width]``, ``lens``
+    int32 ``[seqs]`` tokens held, ``refs`` int32 ``[pages]`` rows that hold a
+    page (0: free).  A sequence of n tokens holds ``ceil(n / 128)`` pages."""
+    block_table: torch.Tensor
+    lens: torch.Tensor
+    refs: torch.Tensor
+
+
+class CachePages:
+    """The pages of a whole cache, ``kv_caches[layer] = [K, V]`` as
+    ``LayerwiseReloader`` takes it; ``layers[l]`` is layer l's ``LayerPages``.
+
+    The table operations return new tables and leave the given ones as they
+    are, so work in flight may go on reading those."""
+
+    def __init__(self, kv_caches):
+        self.layers = [LayerPages(k, v) for k, v in kv_caches]
+        _need(len(self.layers) > 0, "a cache has at least one layer")
+        first = self.layers[0]
+        self.pages, self.device = first.pages, first.device
+        tensors = [t for layer in self.layers for t in (layer.k, layer.v)]
+        _need(all(t.shape == first.k.shape and t.dtype == first.dtype and t.device == first.device for t in tensors),
+              "the layers' caches differ in shape, type or device")
+        self.page_bytes = first.k[0].numel() * first.k.element_size()
+        arr = (_native.PageTensor * len(tensors))()
+        for i, t in enumerate(tensors):
+            inner = sorted((s, n) for s, n in zip(t.stride()[1:], t.shape[1:]) if n > 1)
+            dense, expect = True, 1
+            for s, n in inner:
+                dense, expect = dense and s == expect, expect * n
+            stride = t.stride(0) * t.element_size() if t.shape[0] > 1 else self.page_bytes
+            _need(dense and stride >= self.page_bytes, "a page's values must fill one block of memory")
+            arr[i].base, arr[i].page_stride = t.data_ptr(), stride
+        self._tensors = arr
+
+    def _check(self, t: PageTables) -> _native.Tables:
+        _need(isinstance(t, PageTables), "tables must be PageTables")
+        for x, what, dims in ((t.block_table, "block_table", 2), (t.lens, "lens", 1), (t.refs, "refs", 1)):
+            _need(isinstance(x, torch.Tensor), f"{what} must be a tensor")
+            _ints(x, what, self.device, dims)
+            _need(x.is_contiguous(), f"{what} must be dense")
+        seqs, width = t.block_table.shape
+        _need(seqs > 0 and width > 0, "block_table is empty")
+        _need(t.lens.shape[0] == seqs and t.refs.shape[0] == self.pages,
+              "lens needs an entry for each row of the block table, refs one for each page")
+        return _native.Tables(t.block_table.data_ptr(), t.lens.data_ptr(), t.refs.data_ptr(), seqs, width, self.pages, 0)
+
+    def _outputs(self, t: PageTables, out: PageTables | None):
+        c = self._check(t)
+        if out is None:
+            out = PageTables(*(torch.empty_like(x) for x in t))
+        else:
+            self._check(out)
+            _need(all(a.shape == b.shape for a, b in zip(t, out)), "out differs in shape from the tables")
+            for a in t:
+                for b in out:
+                    lo, hi = max(a.data_ptr(), b.data_ptr()), min(a.data_ptr() + 4 * a.numel(), b.data_ptr() + 4 * b.numel())
+                    _need(lo >= hi, "out overlaps the tables")
+        return c, out, _native.Tables(out.block_table.data_ptr(), out.lens.data_ptr(), out.refs.data_ptr(), c.seqs,
+                                      c.width, c.pages, 0)
+
+    def _scratch(self, c: _native.Tables, n: int) -> torch.Tensor:
+        return torch.empty(int(_native.lib().secure_infer_paged_scratch(ct.byref(c), n)), dtype=torch.uint8,
+                           device=self.device)
+
+    def _pair(self, a, b, names) -> tuple[torch.Tensor, torch.Tensor]:
+        a, b = _ints(a, names[0], self.device, 1), _ints(b, names[1], self.device, 1)
+        _need(a.shape == b.shape, f"{names[0]} and {names[1]} differ in length")
+        return a, b
+
+    def copy(self, src, dst) -> None:
+        """Copy pages ``src[i]`` to ``dst[i]`` in every layer.  No page may be
+        written twice, or written and read; pairs outside the cache are skipped.
+        Lists are checked here, device tensors are the caller's to keep so."""
+        if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
+            src, dst = [int(i) for i in src], [int(i) for i in dst]
+            _need(len(set(dst)) == len(dst) and not set(dst) & set(src), "a page is written twice, or written and read")
+            _need(all(0 <= i < self.pages for i in src + dst), "page outside the cache")
+        src, dst = self._pair(src, dst, ("src", "dst"))
+        _call("secure_infer_paged_copy", self.device, self._tensors, len(self._tensors), self.page_bytes, self.pages,
+              src.data_ptr(), dst.data_ptr(), src.shape[0], torch.cuda.current_stream(self.device).cuda_stream)
+
+    def fork(self, tables: PageTables, parents, children, out: PageTables | None = None):
+        """Give the empty sequence ``children[i]`` the tokens of ``parents[i]``:
+        it shares the full pages, and a partial last one is copied to the lowest
+        free page in every layer.  Returns the new tables and ``granted`` int32
+        ``[n]``: 0 where the child is not empty or named twice, an index is out
+        of range, or pages ran out (requests are served in order)."""
+        a, b = self._pair(parents, children, ("parents", "children"))
+        c, out, o = self._outputs(tables, out)
+        n = a.shape[0]
+        granted = torch.empty(n, dtype=torch.int32, device=self.device)
+        scratch = self._scratch(c, n)
+        _call("secure_infer_paged_fork", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
+              ct.byref(o), a.data_ptr(), b.data_ptr(), n, granted.data_ptr(), scratch.data_ptr(),
+              torch.cuda.current_stream(self.device).cuda_stream)
+        return out, granted
+
+    def reserve(self, tables: PageTables, seqs, lens, out: PageTables | None = None):
+        """Grow sequence ``seqs[i]`` to ``lens[i]`` tokens on the lowest free
+        pages.  Returns the new tables and ``granted`` int32 ``[n]``: 0 where it
+        would shrink or not fit the table, is named twice, its partial last page
+        is shared, or pages ran out (requests are served in order)."""
+        a, b = self._pair(seqs, lens, ("seqs", "lens"))
+        c, out, o = self._outputs(tables, out)
+        n = a.shape[0]
+        granted = torch.empty(n, dtype=torch.int32, device=self.device)
+        scratch = self._scratch(c, n)
+        _call("secure_infer_paged_reserve", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), b.data_ptr(), n,
+              granted.data_ptr(), scratch.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+        return out, granted
+
+    def free(self, tables: PageTables, seqs, out: PageTables | None = None) -> PageTables:
+        """Empty the sequences ``seqs``; a page that no other row holds becomes
+        free.  Returns the new tables."""
+        a = _ints(seqs, "seqs", self.device, 1)
+        c, out, o = self._outputs(tables, out)
+        scratch = self._scratch(c, a.shape[0])
+        _call("secure_infer_paged_free", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), a.shape[0],
+              scratch.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+        return out
+
+    def compact(self, tables: PageTables, out: PageTables | None = None):
+        """Move the used pages to the lowest places, in every layer: with
+        ``live`` pages in use, the i-th used page at or above ``live`` goes to
+        the i-th free one below.  Returns the new tables, ``moved`` int32
+        ``[pages]`` (where each page is now, -1 for a free one) and ``live``
+        int32 ``[1]``."""
+        c, out, o = self._outputs(tables, out)
+        moved = torch.empty(self.pages, dtype=torch.int32, device=self.device)
+        live = torch.empty(1, dtype=torch.int32, device=self.device)
+        scratch = self._scratch(c, 0)
+        _call("secure_infer_paged_compact", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
+              ct.byref(o), moved.data_ptr(), live.data_ptr(), scratch.data_ptr(),
+              torch.cuda.current_stream(self.device).cuda_stream)
+        return out, moved, live

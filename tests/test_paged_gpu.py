@@ -1,0 +1,658 @@
+"""Operators on the paged cache against their definitions in 64 bits: attention
+of a chunk, rotary append, and the page tables against a plain Python model.
+
+Bounds.  An output of ``attend`` is rounded once (eps |o|), and each weight is
+rounded once to the cache's type for the product with the values: eps times the
+softmax of |v|.  Scores, exponentials and sums are 32-bit: 128 products of a
+score lose at most 128 2^-24 of sum |q k|, below 2e-4 at these inputs, which is
+a relative 2e-4 of every weight.  fp16 weights below 2^-14 round to multiples of
+2^-24: up to 2^-25 |v| per key.  ``append`` rounds once, after angles that are
+exact to 2^-24 of a turn."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+# Unit roundoff: 8 and 11 significant bits.
+EPS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+@pytest.fixture(scope="module")
+def paged():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from secure_infer_b200 import paged
+    return paged
+
+
+class Case:
+    """Random pages for sequences of (new, all) tokens; unwritten slots, unused
+    pages and one page that no table names hold NaN."""
+
+    def __init__(self, paged, lens, heads, kv_heads, dtype=torch.bfloat16, seed=0, layout="plain", spare=3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.lens, self.dtype, self.group = lens, dtype, heads // kv_heads
+        used = [-(-kv // 128) for _, kv in lens]
+        pages = sum(used) + spare
+        order = torch.randperm(pages, generator=g, device="cuda").tolist()
+        width = max(1, max(used)) + 2
+        table = torch.full((len(lens), width), -1, dtype=torch.int32)
+        at = 0
+        for s, n in enumerate(used):
+            table[s, :n] = torch.tensor(order[at:at + n], dtype=torch.int32)
+            at += n
+        if layout == "heads":      # [pages, heads, 128, 128] seen as [pages, 128, heads, 128]
+            kv = [torch.full((pages, kv_heads, 128, 128), math.nan, dtype=dtype, device="cuda").transpose(1, 2)
+                  for _ in range(2)]
+        elif layout == "joint":    # K and V of a page side by side
+            both = torch.full((pages, 2, 128, kv_heads, 128), math.nan, dtype=dtype, device="cuda")
+            kv = [both[:, 0], both[:, 1]]
+        else:
+            kv = [torch.full((pages, 128, kv_heads, 128), math.nan, dtype=dtype, device="cuda") for _ in range(2)]
+        self.rows = []
+        for s, (_, n) in enumerate(lens):
+            k, v = (torch.randn((n, kv_heads, 128), generator=g, device="cuda", dtype=dtype) for _ in range(2))
+            for c, x in zip(kv, (k, v)):
+                for i in range(0, n, 128):
+                    c[table[s, i // 128].item(), :min(128, n - i)] = x[i:i + 128]
+            self.rows.append([k, v])
+        self.k, self.v = kv
+        self.cu = [0]
+        for n, _ in lens:
+            self.cu.append(self.cu[-1] + n)
+        self.q = 2 * torch.randn((self.cu[-1], heads, 128), generator=g, device="cuda", dtype=dtype)
+        self.table = table.cuda()
+        self.pages = paged.LayerPages(self.k, self.v)
+        self.chunk = paged.Chunk(self.table, torch.tensor(self.cu, dtype=torch.int32, device="cuda"),
+                                 torch.tensor([n for _, n in lens], dtype=torch.int32, device="cuda"),
+                                 max_q=max(n for n, _ in lens))
+
+    def set_row(self, s, token, head, k=None, v=None):
+        page, slot = self.table[s, token // 128].item(), token % 128
+        for which, x in ((0, k), (1, v)):
+            if x is not None:
+                (self.k, self.v)[which][page, slot, head] = x
+                self.rows[s][which][token, head] = x
+
+    def expected(self, causal=True, window=0, scale=None):
+        """(out, lse, bound) in 64 bits.  Hidden keys are left out, not weighted with zero."""
+        scale = 128 ** -0.5 if scale is None else scale
+        eps = EPS[self.dtype]
+        out = torch.zeros(self.q.shape, dtype=torch.float64, device="cuda")
+        bound = torch.zeros_like(out)
+        lse = torch.full(self.q.shape[:2], -math.inf, dtype=torch.float64, device="cuda")
+        for s, (n, kv) in enumerate(self.lens):
+            if n == 0 or kv == 0:
+                continue
+            k, v = (x.double().repeat_interleave(self.group, 1) for x in self.rows[s])
+            x = torch.einsum("qhd,khd->hqk", self.q[self.cu[s]:self.cu[s + 1]].double(), k) * scale
+            pos = torch.arange(kv - n, kv, device="cuda")[:, None]
+            key = torch.arange(kv, device="cuda")[None]
+            hidden = (key > pos) if causal else torch.zeros((n, kv), dtype=torch.bool, device="cuda")
+            if window:
+                hidden |= pos - key >= window
+            x = x.masked_fill(hidden, -math.inf)
+            some = ~hidden.all(1)
+            w = torch.softmax(x, -1).masked_fill(hidden, 0.0)
+            bad = ~torch.isfinite(v)
+            o = torch.einsum("hqk,khd->qhd", w, v.masked_fill(bad, 0.0))
+            # Visible infinities and NaN reach the rows that see them.
+            if bad.any():
+                seen = (~hidden).double()
+                for value in (math.inf, -math.inf, math.nan):
+                    at = torch.isnan(v) if math.isnan(value) else v == value
+                    o = torch.where(torch.einsum("qk,khd->qhd", seen, at.double()) > 0, o + value, o)
+            mass = torch.einsum("hqk,khd->qhd", w, v.abs().masked_fill(bad, 0.0))
+            tail = kv * 2.0 ** -25 * v.abs().masked_fill(bad, 0.0).amax() if self.dtype == torch.float16 else 0.0
+            rows = slice(self.cu[s], self.cu[s + 1])
+            out[rows] = torch.where(some[:, None, None], o, 0.0)
+            bound[rows] = eps * o.abs() + (eps + 2e-4) * mass + tail + 1e-7
+            lse[rows] = torch.where(some[:, None], torch.logsumexp(x, -1).T, -math.inf)
+        return out, lse, bound
+
+    def check(self, got, lse=None, **kw):
+        out, want_lse, bound = self.expected(**kw)
+        got = got.double()
+        fine = torch.isfinite(out)
+        assert torch.equal(torch.isnan(got), torch.isnan(out))
+        assert torch.equal(got[~fine & ~torch.isnan(out)], out[~fine & ~torch.isnan(out)])
+        over = ((got - out).abs() - bound)[fine]
+        assert over.numel() == 0 or over.max() <= 0, f"off by {over.max().item()} over the bound"
+        if lse is not None:
+            assert torch.equal(torch.isinf(lse), torch.isinf(want_lse))
+            some = ~torch.isinf(want_lse)
+            assert not some.any() or (lse.double() - want_lse)[some].abs().max() <= 3e-4
+
+
+EDGES = [1, 2, 15, 16, 17, 31, 33, 127, 128, 129, 255, 256, 257, 640, 1000]
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (28, 4), (8, 1), (4, 4), (7, 1), (40, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_single_tokens_at_page_edges(paged, heads, kv_heads, dtype):
+    c = Case(paged, [(1, n) for n in EDGES], heads, kv_heads, dtype)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("n", [2, 3, 5, 8, 13, 16, 17])
+@pytest.mark.parametrize("heads,kv_heads", [(16, 4), (7, 1)])
+def test_drafts(paged, n, heads, kv_heads):
+    c = Case(paged, [(n, n), (n, 128), (n, 129 + n), (n, 700)], heads, kv_heads, seed=n)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (28, 4), (3, 3), (160, 1)])
+@pytest.mark.parametrize("lens", [[(100, 100)], [(129, 300)], [(257, 1500)], [(64, 128), (0, 50), (200, 1000), (1, 900)],
+                                  [(511, 640), (33, 33)]])
+def test_chunks(paged, heads, kv_heads, lens):
+    c = Case(paged, lens, heads, kv_heads, seed=len(lens))
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("window", [1, 2, 64, 127, 128, 129, 500])
+@pytest.mark.parametrize("lens", [[(1, n) for n in (1, 100, 128, 129, 777)], [(5, 700), (5, 5)], [(200, 900), (70, 70)]])
+def test_window(paged, window, lens):
+    c = Case(paged, lens, 8, 2, seed=window)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, window=window, return_lse=True)
+    c.check(out, lse, window=window)
+
+
+@pytest.mark.parametrize("lens", [[(1, 300)], [(9, 300), (4, 4)], [(150, 400), (150, 150)]])
+def test_every_key(paged, lens):
+    c = Case(paged, lens, 8, 2)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, causal=False, return_lse=True)
+    c.check(out, lse, causal=False)
+
+
+@pytest.mark.parametrize("lens", [[(0, 0), (1, 40), (0, 300), (1, 128), (0, 0)], [(3, 0), (1, 0)], [(1, 0), (200, 0), (130, 50)]])
+def test_empty_sequences_and_rows(paged, lens):
+    """Slots without new tokens, sequences without tokens, and more new tokens than the sequence holds: the rows
+    before its first token see nothing."""
+    c = Case(paged, lens, 8, 2)
+    out = torch.full_like(c.q, math.nan)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True, out=out)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("lens", [[(4, 200)], [(16, 130)], [(140, 400)], [(300, 300)]])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_values_that_later_tokens_hold_do_not_leak(paged, lens, value):
+    """A row is what it is whatever the keys after it hold; rows that see the value get it."""
+    c = Case(paged, lens, 8, 2, seed=3)
+    n, kv = lens[0]
+    c.set_row(0, kv - n // 2, 1, k=1.0, v=value)
+    c.set_row(0, kv - 2, 0, k=value if not math.isinf(value) else 7.0)
+    out = paged.attend(c.pages, c.chunk, c.q)
+    first = n - 2
+    got, (want, _, bound) = out.double(), c.expected()
+    # Rows before any such key, and after it for the value (the key's NaN makes whole rows of head 0's group NaN).
+    h = c.group
+    assert torch.isfinite(got[:first, :h]).all()
+    assert ((got - want).abs() <= bound)[:first, :h].all()
+    if math.isnan(value):
+        assert torch.isnan(got[first:, :h]).all()
+    before, after = got[:n - n // 2, h:], got[n - n // 2:, h:]
+    assert ((before - want[:n - n // 2, h:]).abs() <= bound[:n - n // 2, h:]).all()
+    assert torch.isnan(after).all() if math.isnan(value) else torch.equal(after, torch.full_like(after, value))
+
+
+def test_keys_left_of_a_window_may_hold_anything(paged):
+    """Pages before a sliding window may have been given away: their table entries are stale."""
+    c = Case(paged, [(1, 1000), (6, 1000), (150, 1000)], 8, 2)
+    want = paged.attend(c.pages, c.chunk, c.q, window=200)
+    c.check(want, window=200)
+    for s, first in ((0, 800), (1, 795), (2, 651)):
+        for p in range(first // 128):
+            page = c.table[s, p].item()
+            c.k[page] = math.nan
+            c.v[page] = math.nan
+        for x in (c.k, c.v):
+            x[c.table[s, first // 128].item(), :first % 128] = math.nan
+        c.table[s, :first // 128] = -7
+    assert torch.equal(paged.attend(c.pages, c.chunk, c.q, window=200), want)
+
+
+@pytest.mark.parametrize("layout", ["heads", "joint"])
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 77)], [(3, 300)], [(150, 500)]])
+def test_layouts_and_strides(paged, layout, lens):
+    c = Case(paged, lens, 12, 2, layout=layout)
+    qkv = torch.randn((c.q.shape[0], 12 + 4, 128), device="cuda").to(c.dtype)
+    qkv[:, 2:14] = c.q
+    table = torch.full((len(lens), c.table.shape[1] + 5), 99, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    chunk = paged.Chunk(table[:, :c.table.shape[1]], c.chunk.cu_q, c.chunk.kv_lens)
+    c.check(paged.attend(c.pages, chunk, qkv[:, 2:14]))
+
+
+def test_scale(paged):
+    c = Case(paged, [(1, 300), (40, 200)], 8, 2)
+    for scale in (0.3, -0.05, 0.0):
+        c.check(paged.attend(c.pages, c.chunk, c.q, scale=scale), scale=scale)
+
+
+def test_large_scores(paged):
+    """Scores of some thousands: only the running maximum keeps the exponentials in range."""
+    c = Case(paged, [(1, 1000), (100, 700)], 4, 1)
+    c.q.mul_(64)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+    want, want_lse, _ = c.expected()
+    assert torch.isfinite(out).all()
+    # The scores' own 32-bit error grows with them: 128 2^-24 sum |q k| scale is below 0.02 here.
+    assert (lse.double() - want_lse).abs().max() <= 2e-2
+    assert (out.double() - want).abs().max() <= 0.05 * want.abs().max()
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(1, 20000)], 8, 1), ([(1, 5000), (1, 10)], 8, 8), ([(7, 9000)], 8, 1),
+                                                 ([(100, 9000)], 8, 1), ([(1, 3), (300, 6000), (1, 2222)], 16, 2)])
+def test_split_contexts_and_their_repetition(paged, lens, heads, kv_heads):
+    """One long context is cut over many CTAs; repeated calls give the same bits whatever CTA finishes last."""
+    c = Case(paged, lens, heads, kv_heads)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+    c.check(out, lse)
+    for _ in range(20):
+        again, again_lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, again_lse)
+
+
+def test_many_sequences(paged):
+    """More sequences than a block has threads."""
+    c = Case(paged, [(i % 4 != 3, 1 + (i * 37) % 300) for i in range(1500)], 4, 2)
+    c.lens = [(int(n), kv) for n, kv in c.lens]
+    c.check(paged.attend(c.pages, c.chunk, c.q))
+
+
+def test_joining_two_halves(paged):
+    """The statistics join attention over two sets of keys to attention over both."""
+    c = Case(paged, [(1, 512)], 8, 2)
+    whole, whole_lse = paged.attend(c.pages, c.chunk, c.q, causal=False, return_lse=True)
+    parts = []
+    for a, b in ((0, 2), (2, 4)):
+        chunk = paged.Chunk(c.table[:, a:b].contiguous(), c.chunk.cu_q,
+                            torch.tensor([256], dtype=torch.int32, device="cuda"), max_q=1)
+        parts.append(paged.attend(c.pages, chunk, c.q, causal=False, return_lse=True))
+    lse = torch.logaddexp(parts[0][1], parts[1][1])
+    out = sum(o.float() * torch.exp(l - lse)[..., None] for o, l in parts)
+    assert (lse - whole_lse).abs().max() <= 1e-5
+    assert (out - whole.float()).abs().max() <= 2 ** -7 * whole.float().abs().max()
+
+
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 2000)], [(6, 900)], [(200, 1200), (1, 50)]])
+def test_other_streams_and_graphs(paged, lens):
+    c = Case(paged, lens, 8, 2)
+    want = paged.attend(c.pages, c.chunk, c.q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = paged.attend(c.pages, c.chunk, c.q)
+    side.synchronize()
+    assert torch.equal(got, want)
+    workspace, out = paged.attend_workspace("cuda:0"), torch.empty_like(c.q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.attend(c.pages, c.chunk, c.q, out=out, workspace=workspace)
+    # Same shapes, other contents.
+    c.chunk.kv_lens.sub_(1)
+    c.lens = [(n, kv - 1) for n, kv in c.lens]
+    for s, (_, kv) in enumerate(c.lens):
+        c.rows[s] = [x[:kv] for x in c.rows[s]]
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    c.check(out)
+
+
+def test_pages_past_two_gigabytes(paged):
+    """Offsets of a large cache need more than 32 bits."""
+    if torch.cuda.get_device_properties(0).total_memory < 60 << 30:
+        pytest.skip("needs 20 GB")
+    pages = 20000
+    k, v = (torch.zeros((pages, 128, 8, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    c = Case(paged, [(1, 256), (130, 256), (2, 256)], 32, 8, spare=0)
+    table = c.table.clone()
+    table[:, :2] = torch.tensor([[19999, 17000], [16384, 19998], [3, 16383]], dtype=torch.int32)
+    for s in range(3):
+        for i in range(2):
+            k[table[s, i]], v[table[s, i]] = c.k[c.table[s, i]], c.v[c.table[s, i]]
+    layer, chunk = paged.LayerPages(k, v), paged.Chunk(table, c.chunk.cu_q, c.chunk.kv_lens)
+    c.check(paged.attend(layer, chunk, c.q))
+    new = torch.randn((133, 8, 128), device="cuda").to(torch.bfloat16)
+    paged.append(layer, chunk, None, new, new)
+    assert torch.equal(k[17000, 127], new[0]) and torch.equal(v[19998, 127], new[130])
+    whole = paged.CachePages([[k, v]])
+    whole.copy([19998], [9])
+    assert torch.equal(k[9], k[19998]) and torch.equal(v[9], v[19998])
+
+
+# ------------------------------------------------------------------- append
+
+def turned(x, positions, sections, base, interleaved):
+    """x [tokens, heads, 128] in 64 bits."""
+    axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    freq = torch.exp(-torch.arange(64, dtype=torch.float64) / 64 * math.log(base)).cuda()
+    angle = positions.double()[axis].T * freq
+    cos, sin = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    x = x.double()
+    a, b = (x[..., 0::2], x[..., 1::2]) if interleaved else (x[..., :64], x[..., 64:])
+    u, w = a * cos - b * sin, b * cos + a * sin
+    return torch.stack((u, w), -1).flatten(-2) if interleaved else torch.cat((u, w), -1)
+
+
+def near(got, want, dtype):
+    # One rounding to the type, and 1e-6 of each term of the turn.
+    return (got.double() - want).abs() <= EPS[dtype] * want.abs() + 2e-5
+
+
+@pytest.mark.parametrize("lens", [[(1, 1)], [(1, 200), (0, 0), (1, 129), (1, 128)], [(300, 300), (5, 900), (0, 40)]])
+@pytest.mark.parametrize("sections,interleaved", [((64,), False), ((64,), True), ((16, 24, 24), False), ((0, 40, 24), True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_append(paged, lens, sections, interleaved, dtype):
+    c = Case(paged, lens, 12, 2, dtype)
+    tokens = c.cu[-1]
+    qkv = torch.randn((tokens, 16, 128), device="cuda").to(dtype)
+    q, k, v = qkv[:, :12], qkv[:, 12:14], qkv[:, 14:]
+    rotary = paged.Rotary(base=500000.0, sections=sections, interleaved=interleaved, device="cuda:0")
+    positions = torch.randint(0, 1 << 20, (len(sections), tokens), dtype=torch.int32, device="cuda")
+    before = [c.k.clone(), c.v.clone()]
+    out = paged.append(c.pages, c.chunk, q, k, v, rotary=rotary, positions=positions)
+    assert near(out, turned(q, positions, sections, 500000.0, interleaved), dtype).all()
+    want_k = turned(k, positions, sections, 500000.0, interleaved)
+    touched = torch.zeros(c.k.shape[:2], dtype=torch.bool, device="cuda")
+    for s, (n, kv) in enumerate(lens):
+        for i in range(n):
+            page, slot, t = c.table[s, (kv - n + i) // 128].item(), (kv - n + i) % 128, c.cu[s] + i
+            touched[page, slot] = True
+            assert near(c.k[page, slot], want_k[t], dtype).all()
+            assert torch.equal(c.v[page, slot], v[t])
+    for now, old in ((c.k, before[0]), (c.v, before[1])):
+        assert torch.equal(now[~touched].view(torch.int16), old[~touched].view(torch.int16))
+
+
+def test_append_default_positions_and_plain_copy(paged):
+    c = Case(paged, [(3, 130), (1, 1)], 4, 2)
+    k, v = (torch.randn((4, 2, 128), device="cuda").to(c.dtype) for _ in range(2))
+    assert paged.append(c.pages, c.chunk, None, k, v) is None
+    assert torch.equal(c.k[c.table[0, 0], 127], k[0]) and torch.equal(c.k[c.table[0, 1], 1], k[2])
+    rotary = paged.Rotary(device="cuda:0")
+    q = torch.randn((4, 4, 128), device="cuda").to(c.dtype)
+    out = paged.append(c.pages, c.chunk, q, k, v, rotary=rotary)
+    places = torch.tensor([[127, 128, 129, 0]], device="cuda")
+    assert near(out, turned(q, places, (64,), 10000.0, False), c.dtype).all()
+    same = paged.append(c.pages, c.chunk, q, k, v, rotary=rotary, positions=places[0].int(), out=torch.empty_like(q))
+    assert torch.equal(same, out)
+
+
+def test_append_leaves_what_has_no_place(paged):
+    """Entries outside the cache, places outside the table, tokens of nobody: queries turn, nothing is written."""
+    c = Case(paged, [(4, 300), (2, 10)], 4, 2)
+    c.table[0, 2] = 10 ** 6
+    c.table[1, 0] = -1
+    before = c.k.clone()
+    k, v = (torch.randn((9, 2, 128), device="cuda").to(c.dtype) for _ in range(2))
+    q = torch.randn((9, 4, 128), device="cuda").to(c.dtype)
+    out = paged.append(c.pages, c.chunk, q, k, v)
+    assert torch.equal(out, q) and torch.equal(c.k.view(torch.int16), before.view(torch.int16))
+    chunk = paged.Chunk(c.table, c.chunk.cu_q, torch.tensor([2, 5000], dtype=torch.int32, device="cuda"))
+    paged.append(c.pages, chunk, q, k, v)
+    page = c.table[0, 0].item()
+    assert torch.equal(c.k[page, 0], k[2]) and torch.equal(c.k[page, 1], k[3])
+    before[page, :2] = k[2:4]
+    assert torch.equal(c.k.view(torch.int16), before.view(torch.int16))
+
+
+def test_rotary_keeps_its_precision_far_out(paged):
+    """At position 2^30 a 32-bit product of position and frequency would be off by whole turns."""
+    c = Case(paged, [(1, 1)], 2, 2)
+    q = torch.randn((1, 2, 128), device="cuda").to(c.dtype)
+    positions = torch.tensor([[(1 << 30) + 12345]], dtype=torch.int32, device="cuda")
+    out = paged.append(c.pages, c.chunk, q, q, q, rotary=paged.Rotary(device="cuda:0"), positions=positions)
+    assert near(out, turned(q, positions, (64,), 10000.0, False), c.dtype).all()
+
+
+# ------------------------------------------------------------------- tables
+
+def model_of(paged, seqs, width, pages, seed, share=True):
+    """Random tables and the cache of three layers behind them."""
+    r = torch.Generator().manual_seed(seed)
+    table, lens, refs = torch.full((seqs, width), -1, dtype=torch.int32), torch.zeros(seqs, dtype=torch.int32), [0] * pages
+    order, at = torch.randperm(pages, generator=r).tolist(), 0
+    for s in range(seqs):
+        if s % 3 == 2:
+            continue
+        n = int(torch.randint(0, width * 128 + 1, (1,), generator=r))
+        used = -(-n // 128)
+        if at + used > pages * 2 // 3:
+            continue
+        row = order[at:at + used]
+        at += used
+        if share and s and lens[0] >= 128 and used > 1:
+            row[0] = int(table[0, 0])
+            at -= 1
+            order[at - len(row) + 1:at] = row[1:]
+        for p in row:
+            refs[p] += 1
+        table[s, :used] = torch.tensor(row, dtype=torch.int32)
+        lens[s] = n
+    data = torch.randint(-30000, 30000, (3, 2, pages, 128, 1, 128), dtype=torch.int16, device="cuda").view(torch.bfloat16)
+    tables = paged.PageTables(table.cuda(), lens.cuda(), torch.tensor(refs, dtype=torch.int32, device="cuda"))
+    return tables, data, paged.CachePages([[d[0], d[1]] for d in data])
+
+
+def bits(x):
+    return x.view(torch.int16)
+
+
+def consistent(t, extra=None):
+    """Every used entry is a page, and each page's count is the rows that hold it."""
+    table, lens, refs = (x.cpu() for x in t)
+    counts = torch.zeros_like(refs)
+    for row, n in zip(table, lens.tolist()):
+        used = -(-n // 128)
+        assert (row[:used] >= 0).all()
+        for p in row[:used].tolist():
+            counts[p] += 1
+    return torch.equal(counts, refs)
+
+
+@pytest.mark.parametrize("seqs,width,pages", [(8, 4, 40), (100, 9, 500), (1200, 3, 3000), (5, 70, 9001)])
+def test_fork(paged, seqs, width, pages):
+    t, data, cache = model_of(paged, seqs, width, pages, seqs)
+    old = [x.clone() for x in t]
+    image = data.clone()
+    lens = t.lens.tolist()
+    empty, full = [s for s in range(seqs) if lens[s] == 0], [s for s in range(seqs) if lens[s]]
+    pairs = [(full[i % len(full)], e) for i, e in enumerate(empty)]
+    pairs[1:1] = [(full[0], full[-1]), (full[0], empty[0]), (-1, empty[-1]), (full[0], seqs), (seqs, empty[-1])]
+    new, granted = cache.fork(t, [p for p, _ in pairs], [c for _, c in pairs])
+    assert all(torch.equal(a, b) for a, b in zip(t, old))
+    free = [p for p in range(pages) if old[2][p] == 0]
+    table, now, refs = old[0].cpu().clone(), old[1].cpu().clone(), old[2].cpu().clone()
+    want, taken, seen, asked = [], [], set(), 0
+    for parent, child in pairs:
+        ok = 0 <= parent < seqs and 0 <= child < seqs and child not in seen and lens[child] == 0
+        if 0 <= child < seqs:
+            seen.add(child)
+        need = int(ok and lens[parent] % 128 != 0)
+        ok = ok and (not need or asked + need <= len(free))
+        asked += need
+        want.append(int(ok))
+        if ok:
+            k = lens[parent] // 128
+            table[child] = -1
+            table[child, :k] = old[0][parent, :k].cpu()
+            for p in table[child, :k].tolist():
+                refs[p] += 1
+            if need:
+                table[child, k] = free[asked - 1]
+                refs[free[asked - 1]] += 1
+                taken.append((int(old[0][parent, k]), free[asked - 1]))
+            now[child] = lens[parent]
+    assert granted.tolist() == want
+    assert torch.equal(new.block_table.cpu(), table) and torch.equal(new.lens.cpu(), now) and torch.equal(new.refs.cpu(), refs)
+    assert consistent(new)
+    for src, dst in taken:
+        image[:, :, dst] = image[:, :, src]
+    assert torch.equal(bits(data), bits(image))
+
+
+def test_fork_until_pages_run_out(paged):
+    t, data, cache = model_of(paged, 12, 6, 30, 1, share=False)
+    lens = t.lens.tolist()
+    parent = next(s for s in range(12) if lens[s] % 128)
+    refs = torch.ones_like(t.refs)
+    refs[[7, 21]] = 0
+    tight = paged.PageTables(t.block_table, t.lens, refs)
+    children = [s for s in range(12) if lens[s] == 0]
+    assert len(children) >= 4
+    new, granted = cache.fork(tight, [parent] * len(children), children)
+    assert granted.tolist() == [1, 1] + [0] * (len(children) - 2)
+    k = lens[parent] // 128
+    assert new.block_table[children[0], k] == 7 and new.block_table[children[1], k] == 21
+    assert (new.lens[children[2:]] == 0).all()
+
+
+@pytest.mark.parametrize("seqs,width,pages", [(8, 4, 40), (300, 9, 1500), (1200, 3, 3000)])
+def test_reserve(paged, seqs, width, pages):
+    t, data, cache = model_of(paged, seqs, width, pages, seqs + 1)
+    old = [x.cpu().clone() for x in t]
+    lens = old[1].tolist()
+    r = torch.Generator().manual_seed(5)
+    asks = [(s, min(width * 128, lens[s] + int(torch.randint(0, 300, (1,), generator=r)))) for s in range(seqs)]
+    asks[2:2] = [(0, lens[0] - 1 if lens[0] else 1), (1, width * 128 + 1), (-1, 5), (seqs, 5)]
+    new, granted = cache.reserve(t, [s for s, _ in asks], [n for _, n in asks])
+    free = [p for p in range(pages) if old[2][p] == 0]
+    table, now, refs, asked, seen = old[0].clone(), old[1].clone(), old[2].clone(), 0, set()
+    want = []
+    for s, n in asks:
+        ok = 0 <= s < seqs and s not in seen
+        seen.add(s)
+        ok = ok and lens[s] <= n <= width * 128
+        if ok and n > lens[s] and lens[s] % 128:
+            ok = old[2][old[0][s, lens[s] // 128]] == 1
+        need = -(-n // 128) - -(-lens[s] // 128) if ok else 0
+        ok = ok and (need == 0 or asked + need <= len(free))
+        if ok:
+            table[s, -(-lens[s] // 128):-(-n // 128)] = torch.tensor(free[asked:asked + need], dtype=torch.int32)
+            refs[free[asked:asked + need]] = 1
+            now[s] = n
+        asked += need
+        want.append(int(ok))
+    assert granted.tolist() == want and 0 < sum(want) < len(want)
+    assert torch.equal(new.block_table.cpu(), table) and torch.equal(new.lens.cpu(), now) and torch.equal(new.refs.cpu(), refs)
+    assert consistent(new)
+
+
+@pytest.mark.parametrize("seqs,width,pages", [(8, 4, 40), (300, 9, 1500), (1200, 3, 3000)])
+def test_free(paged, seqs, width, pages):
+    t, data, cache = model_of(paged, seqs, width, pages, seqs + 2)
+    old = [x.cpu().clone() for x in t]
+    ended = list(range(0, seqs, 2)) + [0, -1, seqs, 2]
+    new = cache.free(t, ended)
+    table, lens, refs = (x.clone() for x in old)
+    for s in range(0, seqs, 2):
+        for p in table[s, :-(-int(lens[s]) // 128)].tolist():
+            refs[p] -= 1
+        table[s], lens[s] = -1, 0
+    assert torch.equal(new.block_table.cpu(), table) and torch.equal(new.lens.cpu(), lens) and torch.equal(new.refs.cpu(), refs)
+    assert consistent(new)
+    assert torch.equal(cache.free(t, []).block_table, t.block_table)
+
+
+@pytest.mark.parametrize("seqs,width,pages", [(8, 4, 40), (100, 9, 500), (1200, 3, 3000), (5, 70, 9001), (1, 1, 1)])
+def test_compact(paged, seqs, width, pages):
+    t, data, cache = model_of(paged, seqs, width, pages, seqs + 3)
+    old = [x.cpu().clone() for x in t]
+    image = data.clone()
+    new, moved, live = cache.compact(t)
+    used = [p for p in range(pages) if old[2][p] > 0]
+    n = len(used)
+    sources, holes = [p for p in used if p >= n], [p for p in range(n) if old[2][p] == 0]
+    where = {p: p for p in used} | dict(zip(sources, holes))
+    assert live.tolist() == [n] and moved.tolist() == [where.get(p, -1) for p in range(pages)]
+    refs = torch.zeros_like(old[2])
+    for p, q in where.items():
+        refs[q] = old[2][p]
+    assert torch.equal(new.refs.cpu(), refs) and torch.equal(new.lens.cpu(), old[1]) and consistent(new)
+    for s in range(seqs):
+        k = -(-int(old[1][s]) // 128)
+        assert new.block_table[s, :k].tolist() == [where[p] for p in old[0][s, :k].tolist()]
+        assert (new.block_table[s, k:] == -1).all()
+    for src, dst in zip(sources, holes):
+        image[:, :, dst] = image[:, :, src]
+    assert torch.equal(bits(data), bits(image))
+
+
+def test_copy_and_layouts(paged):
+    data = torch.randint(-30000, 30000, (130, 20, 2, 128, 2, 128), dtype=torch.int16, device="cuda").view(torch.bfloat16)
+    cache = paged.CachePages([[d[:, 0], d[:, 1].view(20, 2, 128, 128).transpose(1, 2)] for d in data])   # 260 tensors
+    image = data.clone()
+    cache.copy([3, 19, 0], [4, 2, 7])
+    image[:, [4, 2, 7]] = image[:, [3, 19, 0]]
+    assert torch.equal(bits(data), bits(image))
+    cache.copy(torch.tensor([-1, 20, 5], dtype=torch.int32, device="cuda"), torch.tensor([1, 1, 99], dtype=torch.int32, device="cuda"))
+    cache.copy([], [])
+    assert torch.equal(bits(data), bits(image))
+
+
+# ----------------------------------------------------------------- refusals
+
+def test_refusals(paged):
+    c = Case(paged, [(1, 300), (2, 20)], 8, 2)
+    q = c.q
+    bad = [
+        lambda: paged.attend(c.pages, c.chunk, q[:, :7]),
+        lambda: paged.attend(c.pages, c.chunk, q[..., :64]),
+        lambda: paged.attend(c.pages, c.chunk, q.half()),
+        lambda: paged.attend(c.pages, c.chunk, q.cpu()),
+        lambda: paged.attend(c.pages, c.chunk, torch.empty((3, 8, 132), dtype=c.dtype, device="cuda")[..., 2:130]),
+        lambda: paged.attend(c.pages, c.chunk, q, window=-1),
+        lambda: paged.attend(c.pages, c.chunk, q, window=5, causal=False),
+        lambda: paged.attend(c.pages, c.chunk, q, out=torch.empty_like(q)[:2]),
+        lambda: paged.attend(c.pages, c.chunk, q, workspace=torch.zeros(64, dtype=torch.uint8, device="cuda")),
+        lambda: paged.LayerPages(c.k, c.v[:-1]),
+        lambda: paged.LayerPages(c.k[:, :64], c.v[:, :64]),
+        lambda: paged.LayerPages(c.k.float(), c.v.float()),
+        lambda: paged.LayerPages(c.k.cpu(), c.v.cpu()),
+        lambda: paged.Chunk(c.table.long(), c.chunk.cu_q, c.chunk.kv_lens),
+        lambda: paged.Chunk(c.table, c.chunk.cu_q[:-1], c.chunk.kv_lens),
+        lambda: paged.Chunk(c.table, c.chunk.cu_q, c.chunk.kv_lens.cpu()),
+        lambda: paged.Chunk(c.table, c.chunk.cu_q, c.chunk.kv_lens, max_q=-1),
+        lambda: paged.append(c.pages, c.chunk, q, q, q),
+        lambda: paged.append(c.pages, c.chunk, q, q[:, :2], q[:2, :2]),
+        lambda: paged.append(c.pages, c.chunk, None, q[:, :2], q[:, :2], out=q),
+        lambda: paged.append(c.pages, c.chunk, q, q[:, :2], q[:, :2], positions=c.chunk.kv_lens),
+        lambda: paged.append(c.pages, c.chunk, q, q[:, :2], q[:, :2], rotary=paged.Rotary(sections=(32, 32), device="cuda:0"),
+                             positions=torch.zeros(3, dtype=torch.int32, device="cuda")),
+        lambda: paged.Rotary(sections=(10, 20), device="cuda:0"),
+        lambda: paged.Rotary(base=0.0, device="cuda:0"),
+        lambda: paged.CachePages([]),
+        lambda: paged.CachePages([[c.k, c.v], [c.k[:-1], c.v[:-1]]]),
+    ]
+    cache = paged.CachePages([[c.k, c.v]])
+    t = paged.PageTables(c.table.contiguous(), c.chunk.kv_lens, torch.ones(cache.pages, dtype=torch.int32, device="cuda"))
+    bad += [
+        lambda: cache.copy([1], [1]),
+        lambda: cache.copy([1, 2], [3, 3]),
+        lambda: cache.copy([1], [2, 3]),
+        lambda: cache.copy([1], [cache.pages]),
+        lambda: cache.free(t, torch.tensor([0], device="cuda")),
+        lambda: cache.free(t._replace(refs=t.refs[:-1]), [0]),
+        lambda: cache.free(t, [0], out=t),
+        lambda: cache.free(tuple(t), [0]),
+        lambda: cache.fork(t, [0], [1, 2]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    # Nothing of it ran, and the operators still work.
+    c.check(paged.attend(c.pages, c.chunk, c.q))
+    empty = paged.attend(c.pages, c.chunk, q[:0])
+    assert empty.shape == (0, 8, 128)
