@@ -18,6 +18,12 @@ namespace paged {
 constexpr int kPage = 128;   // tokens of a page
 constexpr int kDim = 128;    // values of a head
 
+// What a CTA's last unit of a cut tile leaves for the join.
+struct Cut {
+    int32_t valid, cta0, rows, token0, head;
+    int32_t n, kv, q0;
+};
+
 struct AttendParams {
     const void* q;
     int64_t q_token, q_head;        // strides, elements
@@ -37,12 +43,16 @@ struct AttendParams {
     float scale_log2;               // scale * log2(e): the softmax runs in powers of two
     uint32_t* counters;             // [grid], zero between launches
     uint32_t* status;
+    Cut* cuts;                      // [grid]
     float* slots;                   // [2 * grid] partial results
 };
 
 // Launchers (cudaError_t values).
 int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int m_tiles,
                        uint32_t dtype, cudaStream_t stream);
+// q_map: boxes of [128 / group tokens][group heads][64 values].
+int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                        const AttendParams& p, uint32_t dtype, cudaStream_t stream);
 uint64_t attend_workspace_bytes();
 void attend_workspace(void* workspace, AttendParams* p);   // its counters, status word and slots
 

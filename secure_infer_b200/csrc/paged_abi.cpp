@@ -63,6 +63,24 @@ bool page_map(CUtensorMap* map, const secure_infer_pages* p, const void* base, c
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Queries as [half of a head][token][query head][64 values], in boxes of a KV
+// head's group by 128 / group tokens.
+bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, const int64_t* stride, uint32_t tokens, uint32_t heads,
+              uint32_t group)
+{
+    const cuuint64_t dims[4] = {64, heads, tokens, 2};
+    const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(stride[1]) * 2, static_cast<cuuint64_t>(stride[0]) * 2, 128};
+    const cuuint32_t box[4] = {64, group, 128 / group, 1}, step[4] = {1, 1, 1, 1};
+    const auto type = dtype == SECURE_INFER_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const auto encode = tensor_map_encoder();
+    return encode != nullptr &&
+           encode(map, type, 4, const_cast<void*>(q), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr uint32_t kFewRows = 64;
+
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)
 {
     return in != nullptr && out != nullptr && in->block_table != nullptr && in->lens != nullptr && in->refs != nullptr &&
@@ -128,13 +146,27 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     p.causal = causal != 0;
     p.window = static_cast<int32_t>(window);
     p.scale_log2 = scale * 1.4426950408889634f;
+    // Hidden scores are -inf before they are scaled, so the scale is never zero; at 1e-30 all weights are 1.
+    if (p.scale_log2 > -1e-30f && p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
     attend_workspace(workspace, &p);
-    CUtensorMap k_map, v_map;
-    if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
+    const auto st = static_cast<cudaStream_t>(stream);
+    // Up to kFewRows rows per KV head a sequence is bound by reading K and V once, which the kernel for few rows does
+    // with less latency; more rows are worth tiles of 128.
+    const bool tiles = max_rows > kFewRows && group <= 128;
+    CUtensorMap q_map, k_map, v_map;
+    if (!tiles || chunk->seqs > 1) {
+        if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
+            return -1;
+        p.rows_max = tiles ? kFewRows : INT_MAX;
+        if (launch_attend_rows(k_map, v_map, p, max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4, pages->dtype, st) != 0) return -1;
+        p.rows_min = kFewRows + 1;
+        p.rows_max = INT_MAX;
+    }
+    if (!tiles) return 0;
+    if (!page_map(&k_map, pages, pages->k, pages->k_stride, kPage) || !page_map(&v_map, pages, pages->v, pages->v_stride, kPage) ||
+        !rows_map(&q_map, pages->dtype, q, q_stride, chunk->tokens, q_heads, group))
         return -1;
-    return launch_attend_rows(k_map, v_map, p, max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4, pages->dtype, static_cast<cudaStream_t>(stream)) == 0
-               ? 0
-               : -1;
+    return launch_attend_tiles(q_map, k_map, v_map, p, pages->dtype, st) == 0 ? 0 : -1;
 }
 
 SI_EXPORT int secure_infer_paged_append(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,

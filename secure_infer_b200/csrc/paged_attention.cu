@@ -15,9 +15,10 @@ namespace sib {
 namespace paged {
 namespace {
 
-// Workspace: counters, the status word, then partial results.
+// Workspace: counters, the status word, cuts, then partial results.
 constexpr int kMaxGrid = 256;
-constexpr uint64_t kSlotOffset = 4096;
+constexpr uint64_t kCutOffset = 4096;
+constexpr uint64_t kSlotOffset = kCutOffset + kMaxGrid * sizeof(Cut);
 
 // ---------------------------------------------------------------- few rows
 //
@@ -434,9 +435,565 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     }
 }
 
+
+// --------------------------------------------------------------- many rows
+//
+// Chunks: both products on the tcgen05 tensor cores, bound by them and by the
+// exponentials (a 128 x 128 tile takes 1024 clocks of each).  One CTA per SM
+// takes two tiles of up to 128 rows (whole tokens) that share every page.  A
+// warp loads pages by TMA through a ring of five 32 KiB buffers, a warp issues
+// the products, and a warpgroup per tile holds one row per thread: scores from
+// tensor memory, maximum, weights back over the scores in the cache's type,
+// from where the second product reads them.  While one tile's softmax runs the
+// other's products do.  The accumulated values are only rescaled when a row's
+// maximum grew by more than 2^8 since the last time; weights up to 2^8 are as
+// exact as weights up to 1, and the sums are 32-bit.  Tensor memory: scores
+// (and weights) of the tiles at columns 0 and 128, values at 256 and 384.
+constexpr int kTileThreads = 384;   // two softmax warpgroups; producer, products, two checkers
+constexpr int kRing = 5;
+constexpr uint32_t kTileBytes = 128 * kDim * 2;
+constexpr uint32_t kTilesSmem = 1024 + (2 + kRing) * kTileBytes;
+constexpr int kTileRows = 256;
+constexpr int kTileSlot = kTileRows * (kDim + 2);
+constexpr float kRescale = 8.0f;
+
+template <int kCols>
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[kCols], uint32_t addr);
+template <>
+__device__ __forceinline__ void tmem_load<32>(uint32_t (&r)[32], uint32_t addr)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+template <>
+__device__ __forceinline__ void tmem_load<16>(uint32_t (&r)[16], uint32_t addr)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit_to(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Shared-memory operand in the 128-byte swizzle, 8-row groups 1024 bytes apart;
+// `half`: bytes between the two 64-value halves of an operand whose rows run
+// along the product's sum (V).
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t half)
+{
+    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | static_cast<uint64_t>(half >> 4) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+__device__ __forceinline__ void product_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t accumulate)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int token, int half)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(0), "r"(head), "r"(token), "r"(half)
+        : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads, 1)
+paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttendParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kRing + 2 + 6 + 3];
+    __shared__ Share share;
+    __shared__ int64_t warp_sums[kTileThreads / 32];
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int stop;
+    __shared__ volatile int irregular[2];   // what each checker found in the item
+
+    const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t q_smem = smem, ring = smem + 2 * kTileBytes;
+    auto kv_full = [&](int i) { return smem_addr(&bars[i]); };
+    auto kv_empty = [&](int i) { return smem_addr(&bars[kRing + i]); };
+    const uint32_t q_full = smem_addr(&bars[2 * kRing]), q_empty = q_full + 8;
+    auto s_full = [&](int w) { return smem_addr(&bars[2 * kRing + 2 + w]); };
+    auto p_ready = [&](int w) { return smem_addr(&bars[2 * kRing + 4 + w]); };
+    auto o_full = [&](int w) { return smem_addr(&bars[2 * kRing + 6 + w]); };
+    const uint32_t checked = smem_addr(&bars[2 * kRing + 8]), taken = checked + 8, drained = checked + 16;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < kRing; ++i) {
+            barrier_init(kv_full(i), 1);
+            barrier_init(kv_empty(i), 3);    // the products' commit and both checkers
+        }
+        barrier_init(q_full, 1);
+        barrier_init(q_empty, 1);
+        for (int w = 0; w < 2; ++w) {
+            barrier_init(s_full(w), 1);
+            barrier_init(p_ready(w), 4);
+            barrier_init(o_full(w), 1);
+        }
+        barrier_init(checked, 2);
+        barrier_init(taken, 8);
+        barrier_init(drained, 1);
+        stop = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        tmem_fence_before();
+    }
+    wait_for_earlier_kernels();
+    const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
+    find_share<kTileThreads>(p, 2 * rows_per_tile, 1, &share, warp_sums);
+    dependents_may_launch();
+    tmem_fence_after();
+    const uint32_t tmem = tmem_base;
+    Walk w = start_walk(p, 2 * rows_per_tile, share);
+
+    // 384 threads at 168 registers: 208 for the softmax warpgroups and 88 for the third make the same sum.
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // Producer.
+            uint32_t n = 0, item = 0;
+            while (w.left > 0 && !stop) {
+                const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+                if (lane == 0) {
+                    if (item > 0) barrier_wait(q_empty, (item - 1) & 1, &stop);
+                    if (!stop) {
+                        const int tiles = w.rows > rows_per_tile ? 2 : 1;
+                        barrier_expect(q_full, tiles * 2 * rows_per_tile * 128);
+                        for (int t = 0; t < tiles; ++t)
+                            for (int h = 0; h < 2; ++h)
+                                tma_load_rows(q_smem + t * kTileBytes + h * (kTileBytes / 2), &q_map, q_full, w.head * p.group,
+                                              w.q.q0 + w.first_token + t * tokens, h);
+                    }
+                }
+                __syncwarp();
+                const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
+                for (int i0 = 0; i0 < pages; i0 += 32) {
+                    const int id = i0 + lane < pages && w.span.hi > 0 ? row[i0 + lane] : -1;
+                    for (int i = i0; i < min(pages, i0 + 32); ++i) {
+                        const int page = __shfl_sync(0xffffffffu, id, i - i0);
+                        for (int kv = 0; kv < 2; ++kv, ++n) {
+                            const uint32_t slot = n % kRing, turn = n / kRing;
+                            if (lane != 0 || stop || (turn > 0 && !barrier_wait(kv_empty(slot), (turn - 1) & 1, &stop))) continue;
+                            barrier_expect(kv_full(slot), kTileBytes);
+                            tma_load_page(ring + slot * kTileBytes, kv ? &v_map : &k_map, kv_full(slot), 0, 0, w.head, page);
+                        }
+                    }
+                    __syncwarp();
+                }
+                ++item;
+                w.left -= pages;
+                if (w.left > 0) w.next_tile(p);
+            }
+            if (lane == 0) {
+                for (uint32_t u = n > kRing ? n - kRing : 0; u < n; ++u) barrier_wait(kv_full(u % kRing), (u / kRing) & 1, &stop);
+                if (stop) atomicOr(p.status, 1u);
+            }
+            __syncwarp();
+        } else if (warp == 9) {
+            // Products.
+            constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+            constexpr uint32_t desc = 1u << 4 | type << 7 | type << 10 | (128u >> 3) << 17 | (128u >> 4) << 24;
+            constexpr uint32_t desc_v = desc | 1u << 16;   // V's rows run along the sum
+            uint32_t n = 0, item = 0, ready = 0;           // buffers taken, items, softmax tiles per warpgroup
+            auto scores = [&](int t, uint32_t slot) {
+                if (lane == 0) {
+    #pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t at = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
+                        product_smem(tmem + t * 128, operand(q_smem + t * kTileBytes + at, 16),
+                                     operand(ring + slot * kTileBytes + at, 16), desc, k > 0);
+                    }
+                    commit_to(s_full(t));
+                }
+            };
+            bool ok = true;
+            while (ok && w.left > 0) {
+                const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+                const int tiles = w.rows > rows_per_tile ? 2 : 1;
+                uint32_t slot = n % kRing;
+                ok = barrier_wait(q_full, item & 1, &stop) && barrier_wait(kv_full(slot), (n / kRing) & 1, &stop);
+                if (!ok) break;
+                tmem_fence_after();
+                for (int t = 0; t < tiles; ++t) scores(t, slot);
+                if (lane == 0) {
+                    commit_to(kv_empty(slot));
+                    if (pages == 1) commit_to(q_empty);
+                }
+                ++n;
+                for (int i = 0; ok && i < pages; ++i) {
+                    const uint32_t v_slot = n % kRing, k_slot = (n + 1) % kRing;
+                    const bool more = i + 1 < pages;
+                    ok = barrier_wait(kv_full(v_slot), (n / kRing) & 1, &stop);
+                    if (!ok) break;
+                    // Values of keys that no row sees were never written or belong to others: weights of zero do not
+                    // silence a NaN there, so within the 16-key steps that are multiplied they become zero.
+                    const int key0 = (w.span.first + w.page + i) * kPage;
+                    const int lo = max(0, min(kPage, w.span.lo - key0)), hi = max(0, min(kPage, w.span.hi - key0));
+                    const int step0 = lo >> 4, step1 = hi > lo ? (hi + 15) >> 4 : step0;
+                    if (lo & 15 || hi & 15) {
+                        for (int side = 0; side < 2; ++side) {
+                            const int a = side ? hi : step0 * 16, b = side ? min(kPage, step1 * 16) : lo;
+                            for (int c = lane; c < (b - a) * 16; c += 32) {
+                                const uint32_t at = ring + v_slot * kTileBytes + (c & 8 ? kTileBytes / 2 : 0) + (a + (c >> 4)) * 128 + (c & 7) * 16;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    for (int t = 0; ok && t < tiles; ++t) {
+                        ok = barrier_wait(p_ready(t), ready & 1, &stop);
+                        if (ok && t == 0 && more) ok = barrier_wait(kv_full(k_slot), ((n + 1) / kRing) & 1, &stop);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        if (lane == 0) {
+                            // A page that no row sees still sets the values to zero where it is the first.
+                            const int s0 = step1 > step0 ? step0 : 0, s1 = step1 > step0 ? step1 : (i == 0 ? 1 : 0);
+                            for (int k = s0; k < s1; ++k)
+                                product_tmem(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
+                                             operand(ring + v_slot * kTileBytes + k * 2048, kTileBytes / 2), desc_v,
+                                             i > 0 || k > s0);
+                            if (!more) commit_to(o_full(t));
+                        }
+                        if (more) scores(t, k_slot);
+                    }
+                    ++ready;
+                    if (lane == 0) {
+                        commit_to(kv_empty(v_slot));
+                        if (more) commit_to(kv_empty(k_slot));
+                        if (i + 2 == pages) commit_to(q_empty);
+                    }
+                    n += more ? 2 : 1;
+                }
+                ++item;
+                w.left -= pages;
+                if (w.left > 0) w.next_tile(p);
+            }
+            // Nothing of this warp is in flight when tensor memory is given back.
+            if (lane == 0) {
+                commit_to(drained);
+                barrier_wait(drained, 0, &stop);
+            }
+            __syncwarp();
+        } else if (warp >= 10) {
+            // Checkers: an infinity or NaN among values that some rows see and others do not, where zero weights would
+            // carry it over.  Each takes one half of the 128 values.
+            uint32_t n = 0, item = 0;
+            while (w.left > 0 && !stop) {
+                const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+                int lo_all, hi_all, unused;   // keys that all rows see
+                row_keys(p, w.q, w.last_token, lo_all, unused);
+                row_keys(p, w.q, w.first_token, unused, hi_all);
+                bool odd = false;
+                for (int i = 0; i < pages; ++i) {
+                    const int key0 = (w.span.first + w.page + i) * kPage;
+                    for (int kv = 0; kv < 2; ++kv, ++n) {
+                        const uint32_t slot = n % kRing;
+                        if (!barrier_wait(kv_full(slot), (n / kRing) & 1, &stop)) break;
+                        if (kv == 1 && w.first_token != w.last_token && (key0 < lo_all || key0 + kPage - 1 > hi_all)) {
+                            const int a = max(0, w.span.lo - key0), b = min(kPage, w.span.hi - key0);
+                            for (int c = lane; c < kPage * 8; c += 32) {
+                                const int key = c >> 3;
+                                if (key < a || key >= b || (key0 + key >= lo_all && key0 + key <= hi_all)) continue;
+                                uint4 x;
+                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                             : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                             : "r"(ring + slot * kTileBytes + (warp - 10) * (kTileBytes / 2) + c * 16));
+                                odd |= nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) || nonfinite2<T>(x.w);
+                            }
+                        }
+                        __syncwarp();
+                        if (lane == 0) barrier_arrive(kv_empty(slot));
+                    }
+                }
+                // The flag is the previous item's until the softmax has read it.
+                if (item > 0) barrier_wait(taken, (item - 1) & 1, &stop);
+                odd = __any_sync(0xffffffffu, odd);
+                if (lane == 0) irregular[warp - 10] = odd;
+                __syncwarp();
+                if (lane == 0) barrier_arrive(checked);
+                ++item;
+                w.left -= pages;
+                if (w.left > 0) w.next_tile(p);
+            }
+        }
+    } else {
+        // Softmax: one row per thread.
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+        const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+        const float scale = fabsf(p.scale_log2);
+        const bool flip = p.scale_log2 < 0.0f;
+        uint32_t turn = 0, done = 0, item = 0;   // completions of s_full and o_full taken
+        bool ok = true;
+        while (ok && w.left > 0) {
+            const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+            const bool used = t == 0 || w.rows > rows_per_tile;
+            const int token = w.first_token + t * tokens + row / p.group;   // of the sequence's new ones
+            const bool valid = row < rows_per_tile && t * rows_per_tile + row < w.rows;
+            int lo, hi;
+            row_keys(p, w.q, min(token, w.last_token), lo, hi);
+            int lo_all, hi_all, unused;
+            row_keys(p, w.q, w.last_token, lo_all, unused);
+            row_keys(p, w.q, w.first_token, unused, hi_all);
+            float m = -INFINITY, l = 0.0f;
+            if (used) {
+                for (int i = 0; i < pages; ++i) {
+                    ok = barrier_wait(s_full(t), turn & 1, &stop);
+                    ++turn;
+                    if (!ok) break;
+                    tmem_fence_after();
+                    const int key0 = (w.span.first + w.page + i) * kPage;
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_load<32>(s[c], s_at + c * 32);
+                    tmem_wait_loads();
+                    if (flip) {
+#pragma unroll
+                        for (int c = 0; c < 128; ++c) s[c >> 5][c & 31] ^= 0x80000000u;
+                    }
+                    if (key0 < lo_all || key0 + kPage - 1 > hi_all) {
+                        const int a = lo - key0, b = hi - key0;
+#pragma unroll
+                        for (int c = 0; c < 128; ++c)
+                            if (c < a || c > b) s[c >> 5][c & 31] = 0xff800000u;
+                    }
+                    float top = m;
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) top = fmaxf(top, __uint_as_float(s[c >> 5][c & 31]));
+                    if (i == 0) {
+                        m = top;
+                    } else if (__any_sync(0xffffffffu, (top - m) * scale > kRescale)) {
+                        const float f = m == top ? 1.0f : exp2_approx((m - top) * scale);
+                        m = top;
+                        l *= f;
+#pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t o[16];
+                            tmem_load<16>(o, o_at + c * 16);
+                            tmem_wait_loads();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_store(o_at + c * 16, o);
+                        }
+                        tmem_wait_stores();
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m * scale;
+                    float sum[4] = {};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w2[32];   // weights rounded to the cache's type; their sum is not
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float x = __uint_as_float(s[c * 2 + (j >> 4)][(j & 15) * 2]);
+                            const float y = __uint_as_float(s[c * 2 + (j >> 4)][(j & 15) * 2 + 1]);
+                            const float ex = exp2_approx(fmaf(x, scale, -base)), ey = exp2_approx(fmaf(y, scale, -base));
+                            sum[j & 3] += ex + ey;
+                            w2[j] = pack2<T>(ex, ey);
+                        }
+                        tmem_store(s_at + c * 32, w2);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_stores();
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(p_ready(t));
+                }
+                if (ok) ok = barrier_wait(o_full(t), done & 1, &stop);
+                ++done;
+            }
+            if (ok) ok = barrier_wait(checked, item & 1, &stop);
+            if (!ok) break;
+            tmem_fence_after();
+            const int64_t tile_end = w.tile_unit + w.span.pages;
+            const int cta0 = static_cast<int>(w.tile_unit / share.per), cta1 = static_cast<int>((tile_end - 1) / share.per);
+            float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kTileSlot;
+            const bool split = cta1 > cta0;
+            const bool by_definition = irregular[0] || irregular[1];
+            __syncwarp();
+            if (lane == 0) barrier_arrive(taken);
+            if (by_definition) {
+                const int ka = (w.span.first + w.page) * kPage, kb = ka + pages * kPage;
+                for (int r = (warp & 3) * 32; r < (warp & 3) * 32 + 32; ++r) {
+                    const int tile_row = t * rows_per_tile + r;
+                    if (r >= rows_per_tile || tile_row >= w.rows) break;
+                    const int tok = w.first_token + tile_row / p.group, g = tile_row % p.group;
+                    int a, b;
+                    row_keys(p, w.q, tok, a, b);
+                    float mm, ll;
+                    float4 x;
+                    row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + tok) * p.q_token +
+                                                (w.head * p.group + g) * p.q_head,
+                                         p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, kb), mm, ll, x);
+                    if (split) {
+                        *reinterpret_cast<float4*>(slot + (t * 128 + r) * kDim + lane * 4) = x;
+                        if (lane == 0) {
+                            slot[kTileRows * kDim + t * 128 + r] = mm;
+                            slot[kTileRows * kDim + kTileRows + t * 128 + r] = ll;
+                        }
+                    } else {
+                        const float inv = 1.0f / ll;
+                        const int64_t at = static_cast<int64_t>(w.q.q0 + tok) * p.heads * p.group + w.head * p.group + g;
+                        uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+                        if (b < a) packed = make_uint2(0, 0);
+                        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
+                        if (p.lse != nullptr && lane == 0)
+                            p.lse[at] = b >= a ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
+                    }
+                }
+            } else if (used) {
+                const float inv = 1.0f / l;
+                const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + row % p.group;
+                T* out = static_cast<T*>(p.out) + at * kDim;
+                float* part = slot + (t * 128 + row) * kDim;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[32];
+                    tmem_load<32>(o, o_at + c * 32);
+                    tmem_wait_loads();
+                    if (!valid) continue;
+                    if (split) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<uint4*>(part + c * 32 + j * 4) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    } else {
+                        const bool some = hi >= lo;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t x[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                x[k] = some ? pack2<T>(__uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
+                            *reinterpret_cast<uint4*>(out + c * 32 + j * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                }
+                if (valid) {
+                    const float top = m * scale;
+                    if (split) {
+                        slot[kTileRows * kDim + t * 128 + row] = top;
+                        slot[kTileRows * kDim + kTileRows + t * 128 + row] = l;
+                    } else if (p.lse != nullptr) {
+                        p.lse[at] = hi >= lo ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                    }
+                }
+                tmem_fence_before();
+            }
+            // Only the first tile of a CTA can have begun in an earlier one.
+            if (tid == 0 && item == 0) {
+                Cut cut{};
+                if (split && cta0 < static_cast<int>(blockIdx.x) && w.page + pages == w.span.pages)
+                    cut = Cut{1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
+                p.cuts[blockIdx.x] = cut;
+            }
+            ++item;
+            w.left -= pages;
+            if (w.left > 0) w.next_tile(p);
+        }
+        if (tid == 0 && share.seq < 0) p.cuts[blockIdx.x] = Cut{};
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// Joins the pieces of tiles that were cut over CTAs: a warp per row.
+constexpr int kJoinThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const __grid_constant__ AttendParams p)
+{
+    wait_for_earlier_kernels();
+    dependents_may_launch();
+    const Cut cut = p.cuts[blockIdx.y];
+    if (!cut.valid) return;
+    const int rows_per_tile = 128 / p.group * p.group;
+    const int lane = threadIdx.x & 31, tile_row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+    if (tile_row >= cut.rows) return;
+    const int pieces = blockIdx.y - cut.cta0 + 1;
+    const int r = tile_row < rows_per_tile ? tile_row : 128 + tile_row - rows_per_tile;
+    auto piece = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cut.cta0 + i) + (i == 0)) * kTileSlot; };
+    float top = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, piece(i)[kTileRows * kDim + r]);
+    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+        const float* src = piece(i);
+        const float f = join_weight(src[kTileRows * kDim + r], top);
+        const float4 y = *reinterpret_cast<const float4*>(src + r * kDim + lane * 4);
+        sum += f * src[kTileRows * kDim + kTileRows + r];
+        x.x += f * y.x;
+        x.y += f * y.y;
+        x.z += f * y.z;
+        x.w += f * y.w;
+    }
+    const Seq s{cut.n, cut.kv, cut.q0};
+    const int token = cut.token0 + tile_row / p.group, g = tile_row % p.group;
+    int a, b;
+    row_keys(p, s, token, a, b);
+    const float inv = 1.0f / sum;
+    const int64_t at = static_cast<int64_t>(cut.q0 + token) * p.heads * p.group + cut.head * p.group + g;
+    uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    if (b < a) packed = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
+    if (p.lse != nullptr && lane == 0) p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
 struct Device {
     int sms = 0;
     bool rows_set[2][kMaxRowTiles] = {};
+    bool tiles_set[2] = {};
 };
 std::mutex g_mu;
 Device g_devices[64];
@@ -474,7 +1031,56 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
     return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, kTiles>, k_map, v_map, p);
 }
 
+template <typename T>
+int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p,
+                 cudaStream_t stream)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int sms;
+    {
+        std::lock_guard<std::mutex> lock(g_mu);
+        Device& d = g_devices[dev & 63];
+        if (d.sms == 0) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+        bool& set = d.tiles_set[std::is_same<T, __half>::value];
+        if (!set) {
+            const cudaError_t e = cudaFuncSetAttribute(paged_attend_tiles_kernel<T>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kTilesSmem);
+            if (e != cudaSuccess) return e;
+            set = true;
+        }
+        sms = d.sms < kMaxGrid ? d.sms : kMaxGrid;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = kTilesSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    {
+        ProfileScope prof(kKernAttendTiles, stream);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attend_tiles_kernel<T>, q_map, k_map, v_map, p);
+        if (e != cudaSuccess) return e;
+    }
+    cfg.gridDim = dim3(kTileRows / (kJoinThreads / 32), sms);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = 0;
+    ProfileScope prof(kKernAttendJoin, stream);
+    return cudaLaunchKernelEx(&cfg, paged_attend_join_kernel<T>, p);
+}
+
 }  // namespace
+
+int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                        const AttendParams& p, uint32_t dtype, cudaStream_t stream)
+{
+    return dtype == SECURE_INFER_FP16 ? launch_tiles<__half>(q_map, k_map, v_map, p, stream)
+                                      : launch_tiles<__nv_bfloat16>(q_map, k_map, v_map, p, stream);
+}
 
 int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int m_tiles,
                        uint32_t dtype, cudaStream_t stream)
@@ -490,13 +1096,14 @@ int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const
 
 uint64_t attend_workspace_bytes()
 {
-    return kSlotOffset + static_cast<uint64_t>(2 * kMaxGrid) * kRowSlot * sizeof(float);
+    return kSlotOffset + static_cast<uint64_t>(2 * kMaxGrid) * kTileSlot * sizeof(float);
 }
 
 void attend_workspace(void* workspace, AttendParams* p)
 {
     p->counters = static_cast<uint32_t*>(workspace);
     p->status = p->counters + kMaxGrid;
+    p->cuts = reinterpret_cast<Cut*>(static_cast<char*>(workspace) + kCutOffset);
     p->slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotOffset);
 }
 
