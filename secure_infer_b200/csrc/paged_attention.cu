@@ -537,6 +537,59 @@ __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
+// Two 32-bit floats in a register pair.
+__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair(float x, float y) { return pair(__float_as_uint(x), __float_as_uint(y)); }
+__device__ __forceinline__ float2 unpair(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair on the multiply-add units, for x <= 126: x = n + f with n the
+// nearest integer, 2^f by the polynomial of degree 4 with the least largest
+// relative error on [-1/2, 1/2] (2.7e-6, by Remez's exchange), n added to the
+// exponent.  Below -126 it stays at 2^-126.  NaN does not survive.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x2)
+{
+    constexpr float kRound = 12582912.0f;   // 1.5 2^23: the sum's last bits are n
+    float2 x = unpair(x2);
+    x2 = pair(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    const uint64_t t = add2(x2, pair(kRound, kRound));
+    const uint64_t n = add2(t, pair(-kRound, -kRound));
+    const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x2);
+    uint64_t y = fma2(pair(0.009570102f, 0.009570102f), f, pair(0.05591786f, 0.05591786f));
+    y = fma2(y, f, pair(0.24024744f, 0.24024744f));
+    y = fma2(y, f, pair(0.6931218f, 0.6931218f));
+    y = fma2(y, f, pair(0.9999993f, 0.9999993f));
+    const float2 r = unpair(y), e = unpair(t);
+    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(e.x) << 23)),
+                       __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(e.y) << 23)));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -547,6 +600,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     __shared__ Share share;
     __shared__ int64_t warp_sums[kTileThreads / 32];
     __shared__ uint32_t tmem_base;
+    __shared__ Walk walks[8];   // the softmax warps', who need their registers
     __shared__ volatile int stop;
     __shared__ volatile int irregular[2];   // what each checker found in the item
 
@@ -594,6 +648,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     tmem_fence_after();
     const uint32_t tmem = tmem_base;
     Walk w = start_walk(p, 2 * rows_per_tile, share);
+    if (warp < 8 && lane == 0) walks[warp] = w;
+    __syncwarp();
 
     // 384 threads at 168 registers: 208 for the softmax warpgroups and 88 for the third make the same sum.
     if (warp >= 8) {
@@ -774,6 +830,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
         const float scale = fabsf(p.scale_log2);
         const bool flip = p.scale_log2 < 0.0f;
+        Walk& w = walks[warp];
         uint32_t turn = 0, done = 0, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
         while (ok && w.left > 0) {
@@ -786,6 +843,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             int lo_all, hi_all, unused;
             row_keys(p, w.q, w.last_token, lo_all, unused);
             row_keys(p, w.q, w.first_token, unused, hi_all);
+            const int first_key = (w.span.first + w.page) * kPage;
             float m = -INFINITY, l = 0.0f;
             if (used) {
                 for (int i = 0; i < pages; ++i) {
@@ -793,7 +851,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     ++turn;
                     if (!ok) break;
                     tmem_fence_after();
-                    const int key0 = (w.span.first + w.page + i) * kPage;
+                    const int key0 = first_key + i * kPage;
                     uint32_t s[4][32];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) tmem_load<32>(s[c], s_at + c * 32);
@@ -802,18 +860,23 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 #pragma unroll
                         for (int c = 0; c < 128; ++c) s[c >> 5][c & 31] ^= 0x80000000u;
                     }
-                    if (key0 < lo_all || key0 + kPage - 1 > hi_all) {
+                    const bool masked = key0 < lo_all || key0 + kPage - 1 > hi_all;
+                    if (masked) {
                         const int a = lo - key0, b = hi - key0;
 #pragma unroll
                         for (int c = 0; c < 128; ++c)
                             if (c < a || c > b) s[c >> 5][c & 31] = 0xff800000u;
                     }
-                    float top = m;
+                    float tops[4] = {m, m, m, m};
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) top = fmaxf(top, __uint_as_float(s[c >> 5][c & 31]));
+                    for (int c = 0; c < 128; c += 2)
+                        tops[(c >> 1) & 3] = max3_nan(tops[(c >> 1) & 3], __uint_as_float(s[c >> 5][c & 31]),
+                                                      __uint_as_float(s[c >> 5][(c & 31) + 1]));
+                    float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                    if (top == INFINITY) top = NAN;   // a NaN or infinite score makes its row NaN
                     if (i == 0) {
                         m = top;
-                    } else if (__any_sync(0xffffffffu, (top - m) * scale > kRescale)) {
+                    } else if (__any_sync(0xffffffffu, !((top - m) * scale <= kRescale) && top != -INFINITY)) {
                         const float f = m == top ? 1.0f : exp2_approx((m - top) * scale);
                         m = top;
                         l *= f;
@@ -829,21 +892,35 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         tmem_wait_stores();
                     }
                     const float base = m == -INFINITY ? 0.0f : m * scale;
-                    float sum[4] = {};
+                    const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+                    uint64_t sum[4] = {};
+                    // Weights are rounded to the cache's type for the product; their sum is not.  A third of the
+                    // exponentials go to the multiply-add units, which levels these with the special function units:
+                    // all on the latter would take as long as the products.  Masked tiles have exact zeros.
+                    auto weights = [&](auto poly) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w2[32];   // weights rounded to the cache's type; their sum is not
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t w2[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float x = __uint_as_float(s[c * 2 + (j >> 4)][(j & 15) * 2]);
-                            const float y = __uint_as_float(s[c * 2 + (j >> 4)][(j & 15) * 2 + 1]);
-                            const float ex = exp2_approx(fmaf(x, scale, -base)), ey = exp2_approx(fmaf(y, scale, -base));
-                            sum[j & 3] += ex + ey;
-                            w2[j] = pack2<T>(ex, ey);
+                            for (int j = 0; j < 32; ++j) {
+                                const uint64_t x = fma2(pair(s[c * 2 + (j >> 4)][(j & 15) * 2], s[c * 2 + (j >> 4)][(j & 15) * 2 + 1]), scale2, base2);
+                                float2 e;
+                                if (decltype(poly)::value && j % 3 == 1) {
+                                    e = exp2_poly(x);
+                                } else {
+                                    const float2 y = unpair(x);
+                                    e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                                }
+                                sum[j & 3] = add2(sum[j & 3], pair(e.x, e.y));
+                                w2[j] = pack2<T>(e.x, e.y);
+                            }
+                            tmem_store(s_at + c * 32, w2);
                         }
-                        tmem_store(s_at + c * 32, w2);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    };
+                    if (masked) weights(std::false_type{});
+                    else weights(std::true_type{});
+                    const float2 sums = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+                    l += sums.x + sums.y;
                     tmem_wait_stores();
                     tmem_fence_before();
                     __syncwarp();
@@ -937,8 +1014,12 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 p.cuts[blockIdx.x] = cut;
             }
             ++item;
-            w.left -= pages;
-            if (w.left > 0) w.next_tile(p);
+            __syncwarp();
+            if (lane == 0) {
+                w.left -= pages;
+                if (w.left > 0) w.next_tile(p);
+            }
+            __syncwarp();
         }
         if (tid == 0 && share.seq < 0) p.cuts[blockIdx.x] = Cut{};
     }
