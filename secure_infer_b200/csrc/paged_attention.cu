@@ -508,18 +508,27 @@ __device__ __forceinline__ void commit_to(uint32_t bar)
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Shared-memory operand in the 128-byte swizzle, 8-row groups 1024 bytes apart;
-// `half`: bytes between the two 64-value halves of an operand whose rows run
-// along the product's sum (V).
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t half)
+// Two 32-bit values in a register pair.
+__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y)
 {
-    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | static_cast<uint64_t>(half >> 4) << 16 |
-           static_cast<uint64_t>(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
 }
-__device__ __forceinline__ void product_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate)
+// Shared-memory operands lie in the 128-byte swizzle, groups of eight 128-byte
+// rows 1024 bytes apart.  A descriptor's low word holds the address and, for an
+// operand whose rows run along the product's sum (V), the bytes between the two
+// halves of 64 values; its high word is the same for all.  Advancing along the
+// sum adds to the low word.
+constexpr uint32_t kOperandHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t half) { return (addr >> 4 & 0x3fff) | (half >> 4) << 16; }
+__device__ __forceinline__ uint64_t operand_at(uint32_t low, uint32_t bytes) { return pair(low + (bytes >> 4), kOperandHigh); }
+
+template <bool kAdd>
+__device__ __forceinline__ void product_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t desc)
 {
     asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+                 "l"(a), "l"(b), "r"(desc), "n"(kAdd)
                  : "memory");
 }
 __device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, uint32_t accumulate)
@@ -527,6 +536,13 @@ __device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint64_t b,
     asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
                  "r"(a), "l"(b), "r"(desc), "r"(accumulate)
                  : "memory");
+}
+// One lane of a converged warp, the same one at every call.
+__device__ __forceinline__ bool elected()
+{
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+    return r != 0;
 }
 
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int token, int half)
@@ -537,13 +553,6 @@ __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-// Two 32-bit floats in a register pair.
-__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
-    return r;
-}
 __device__ __forceinline__ uint64_t pair(float x, float y) { return pair(__float_as_uint(x), __float_as_uint(y)); }
 __device__ __forceinline__ float2 unpair(uint64_t v)
 {
@@ -701,15 +710,14 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             constexpr uint32_t desc_v = desc | 1u << 16;   // V's rows run along the sum
             uint32_t n = 0, item = 0, ready = 0;           // buffers taken, items, softmax tiles per warpgroup
             auto scores = [&](int t, uint32_t slot) {
-                if (lane == 0) {
-    #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t at = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
-                        product_smem(tmem + t * 128, operand(q_smem + t * kTileBytes + at, 16),
-                                     operand(ring + slot * kTileBytes + at, 16), desc, k > 0);
-                    }
-                    commit_to(s_full(t));
+                const uint32_t q = operand(q_smem + t * kTileBytes, 0), k = operand(ring + slot * kTileBytes, 0), d = tmem + t * 128;
+                product_smem<false>(d, operand_at(q, 0), operand_at(k, 0), desc);
+#pragma unroll
+                for (int i = 1; i < 8; ++i) {
+                    const uint32_t at = (i >> 2) * (kTileBytes / 2) + (i & 3) * 32;
+                    product_smem<true>(d, operand_at(q, at), operand_at(k, at), desc);
                 }
+                commit_to(s_full(t));
             };
             bool ok = true;
             while (ok && w.left > 0) {
@@ -719,11 +727,12 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 ok = barrier_wait(q_full, item & 1, &stop) && barrier_wait(kv_full(slot), (n / kRing) & 1, &stop);
                 if (!ok) break;
                 tmem_fence_after();
-                for (int t = 0; t < tiles; ++t) scores(t, slot);
-                if (lane == 0) {
+                if (elected()) {
+                    for (int t = 0; t < tiles; ++t) scores(t, slot);
                     commit_to(kv_empty(slot));
                     if (pages == 1) commit_to(q_empty);
                 }
+                __syncwarp();
                 ++n;
                 for (int i = 0; ok && i < pages; ++i) {
                     const uint32_t v_slot = n % kRing, k_slot = (n + 1) % kRing;
@@ -746,28 +755,35 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
+                    const uint32_t v = operand(ring + v_slot * kTileBytes, kTileBytes / 2);
                     for (int t = 0; ok && t < tiles; ++t) {
                         ok = barrier_wait(p_ready(t), ready & 1, &stop);
                         if (ok && t == 0 && more) ok = barrier_wait(kv_full(k_slot), ((n + 1) / kRing) & 1, &stop);
                         if (!ok) break;
                         tmem_fence_after();
-                        if (lane == 0) {
-                            // A page that no row sees still sets the values to zero where it is the first.
-                            const int s0 = step1 > step0 ? step0 : 0, s1 = step1 > step0 ? step1 : (i == 0 ? 1 : 0);
-                            for (int k = s0; k < s1; ++k)
-                                product_tmem(tmem + 256 + t * 128, tmem + t * 128 + k * 8,
-                                             operand(ring + v_slot * kTileBytes + k * 2048, kTileBytes / 2), desc_v,
-                                             i > 0 || k > s0);
-                            if (!more) commit_to(o_full(t));
+                        if (elected()) {
+                            const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128;
+                            if (step0 == 0 && step1 == 8) {
+                                product_tmem(d, a, operand_at(v, 0), desc_v, i > 0);
+#pragma unroll
+                                for (int k = 1; k < 8; ++k) product_tmem(d, a + k * 8, operand_at(v, k * 2048), desc_v, 1);
+                            } else {
+                                // A page that no row sees still sets the values to zero where it is the first.
+                                const int s0 = step1 > step0 ? step0 : 0, s1 = step1 > step0 ? step1 : (i == 0 ? 1 : 0);
+                                for (int k = s0; k < s1; ++k)
+                                    product_tmem(d, a + k * 8, operand_at(v, k * 2048), desc_v, i > 0 || k > s0);
+                            }
+                            if (more) scores(t, k_slot);
+                            else commit_to(o_full(t));
+                            if (t + 1 == tiles) {
+                                commit_to(kv_empty(v_slot));
+                                if (more) commit_to(kv_empty(k_slot));
+                                if (i + 2 == pages) commit_to(q_empty);
+                            }
                         }
-                        if (more) scores(t, k_slot);
+                        __syncwarp();
                     }
                     ++ready;
-                    if (lane == 0) {
-                        commit_to(kv_empty(v_slot));
-                        if (more) commit_to(kv_empty(k_slot));
-                        if (i + 2 == pages) commit_to(q_empty);
-                    }
                     n += more ? 2 : 1;
                 }
                 ++item;
