@@ -128,24 +128,32 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Waits for the phase of parity `parity`.  The wait is bounded: some seconds
-// of tries that the hardware suspends, after which `abort` is set and every
-// wait of the CTA gives up, so a protocol error ends the kernel instead of
-// hanging it.  Returns whether the phase completed.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* abort)
+__device__ __forceinline__ bool barrier_done(uint32_t bar, uint32_t parity)
 {
-    for (int tries = 0; tries < (1 << 22); ++tries) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((tries & 63) == 63 && *abort) return false;
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+
+// Waits for the phase of parity `parity`.  The wait is bounded: some seconds
+// after its start `stop` is set and every wait of the CTA gives up, so a
+// protocol error ends the kernel instead of hanging it.  Returns whether the
+// phase completed.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* stop)
+{
+    if (barrier_done(bar, parity)) return true;
+    const long long start = clock64();
+    while (!barrier_done(bar, parity)) {
+        if (*stop) return false;
+        if (clock64() - start > (1ll << 33)) {
+            *stop = 1;
+            return false;
+        }
     }
-    *abort = 1;
-    return false;
+    return true;
 }
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int half,
@@ -210,6 +218,7 @@ __device__ __forceinline__ bool nonfinite2(uint32_t x)
 // none).  All units of a launch in the order sequence, tile, head, page are cut
 // into equal consecutive shares, one per CTA: every CTA gets the same work
 // whatever the lengths, and a long axis is split where there are few rows.
+// Units are counted in 32 bits; the host refuses more.
 struct Seq {
     int n, kv, q0;   // new tokens, all tokens, first new token
 };
@@ -248,16 +257,32 @@ __device__ __forceinline__ Span tile_span(const AttendParams& p, const Seq& s, i
     return r;
 }
 
+// A launch's units cut into consecutive shares of `per` or, for the first
+// `more` CTAs, per + 1 units; `ctas` of the grid have one.
+struct Share {
+    int32_t per, more, ctas, total;
+    int32_t begin, units;      // of this CTA
+    int32_t seq, seq_unit;     // sequence of its first unit, and that sequence's first unit
+
+    __device__ __forceinline__ int begin_of(int cta) const { return cta * per + min(cta, more); }
+    __device__ __forceinline__ int owner(int unit) const
+    {
+        const int cut = more * (per + 1);
+        return unit < cut ? unit / (per + 1) : more + (unit - cut) / per;
+    }
+};
+
 struct Walk {
     int rows_per_tile;
     int s, tile, tiles, head;
     Seq q;
     Span span;
-    int page;                // next unit of the tile: 0 .. span.pages
+    int page;                            // next unit of the tile: 0 .. span.pages
     int first_token, last_token, rows;   // of the tile
-    int64_t tile_unit;       // unit number of the tile's first unit
-    int64_t left;            // units of this CTA not yet taken
+    int tile_unit;                       // number of the tile's first unit
+    int left;                            // units of this CTA not yet taken
 
+    __device__ __forceinline__ int take() const { return min(left, span.pages - page); }
     __device__ __forceinline__ void set_tile(const AttendParams& p)
     {
         const int r0 = tile * rows_per_tile;
@@ -266,9 +291,11 @@ struct Walk {
         last_token = (r0 + rows - 1) / p.group;
         span = tile_span(p, q, first_token, last_token);
     }
-    // Past the last unit of a tile: the next head, tile or sequence.
-    __device__ __forceinline__ void next_tile(const AttendParams& p)
+    // After `taken` units: the next head, tile or sequence.
+    __device__ __forceinline__ void advance(const AttendParams& p, int taken)
     {
+        left -= taken;
+        if (left <= 0) return;
         tile_unit += span.pages;
         page = 0;
         if (++head < p.heads) return;
@@ -279,7 +306,10 @@ struct Walk {
         }
         tile = 0;
         do {
-            if (++s >= p.seqs) return;
+            if (++s >= p.seqs) {   // only if lengths changed under the kernel
+                left = 0;
+                return;
+            }
             q = load_seq(p, s);
         } while (q.n == 0);
         tiles = (q.n * p.group + rows_per_tile - 1) / rows_per_tile;
@@ -287,79 +317,69 @@ struct Walk {
     }
 };
 
-__device__ __forceinline__ int64_t seq_units(const AttendParams& p, const Seq& s, int rows_per_tile)
+__device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile)
 {
     if (s.n == 0) return 0;
-    int64_t pages = 0;
+    int pages = 0;
     const int rows = s.n * p.group;
     for (int r = 0; r < rows; r += rows_per_tile)
         pages += tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages;
     return pages * p.heads;
 }
 
-// The share of this CTA: [begin, begin + units) of `per` units each.
-struct Share {
-    int64_t per;      // units of a CTA
-    int64_t begin;    // first unit of this one
-    int seq;          // sequence of the first unit, -1: none
-    int64_t seq_unit; // unit number of that sequence's first unit
-    int64_t total;
-};
-
 // All threads of the block take part; `warp_sums` holds one value per warp.
 // At least min_units go to a CTA that has any, so short work is not split.
 template <int kThreads>
 __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int min_units, Share* share,
-                                           int64_t* warp_sums)
+                                           int32_t* warp_sums)
 {
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int64_t base = 0;
-    // Pass 0 sums the units; pass 1 finds the sequence that holds the first of this CTA's.
-    for (int pass = 0; pass < 2; ++pass) {
-        base = 0;
+    Share r;
+    r.begin = r.total = 0;
+    // The first pass sums the units, the second finds the sequence that holds this CTA's first; where every sequence
+    // has a thread one pass does both.
+    const bool one = p.seqs <= kThreads;
+    for (int pass = one ? 1 : 0; pass < 2; ++pass) {
+        int base = 0;
         for (int s0 = 0; s0 < p.seqs; s0 += kThreads) {
             const int s = s0 + tid;
-            const int64_t own = s < p.seqs ? seq_units(p, load_seq(p, s), rows_per_tile) : 0;
-            int64_t sum = own;
+            const int own = s < p.seqs ? seq_units(p, load_seq(p, s), rows_per_tile) : 0;
+            int sum = own;
             for (int d = 1; d < 32; d <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, sum, d);
+                const int up = __shfl_up_sync(0xffffffffu, sum, d);
                 if (lane >= d) sum += up;
             }
             if (lane == 31) warp_sums[warp] = sum;
             __syncthreads();
-            int64_t before = base;
+            int before = base;
+#pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) before += warp_sums[w];
-                base += warp_sums[w];
+                const int x = warp_sums[w];
+                if (w < warp) before += x;
+                base += x;
             }
-            if (pass == 0 && p.seqs <= kThreads) {   // one round holds every sequence: no second pass
+            if (one || (pass == 0 && s0 + kThreads >= p.seqs)) {
+                r.total = base;
+                r.ctas = max(1, min(static_cast<int>(gridDim.x), base / min_units));
+                r.per = base / r.ctas;
+                r.more = base - r.per * r.ctas;
+                const int c = blockIdx.x;
+                r.begin = r.begin_of(c);
+                r.units = c < r.ctas ? r.per + (c < r.more) : 0;
                 if (tid == 0) {
-                    share->total = base;
-                    share->seq = -1;
-                    int64_t per = (base + gridDim.x - 1) / gridDim.x;
-                    share->per = per < min_units ? min_units : per;
-                    share->begin = share->per * blockIdx.x;
+                    r.seq = -1;
+                    r.seq_unit = 0;
+                    *share = r;
                 }
                 __syncthreads();
             }
-            if (pass == 1 || p.seqs <= kThreads) {
-                const int64_t first = before + sum - own;
-                if (own > 0 && share->begin >= first && share->begin < first + own) {
+            if (pass == 1) {
+                const int first = before + sum - own;
+                if (r.units > 0 && own > 0 && r.begin >= first && r.begin < first + own) {
                     share->seq = s;
                     share->seq_unit = first;
                 }
-            }
-            __syncthreads();
-        }
-        if (p.seqs <= kThreads) break;
-        if (pass == 0) {
-            if (tid == 0) {
-                share->total = base;
-                share->seq = -1;
-                int64_t per = (base + gridDim.x - 1) / gridDim.x;
-                share->per = per < min_units ? min_units : per;
-                share->begin = share->per * blockIdx.x;
             }
             __syncthreads();
         }
@@ -372,23 +392,23 @@ __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_t
     w.rows_per_tile = rows_per_tile;
     w.left = 0;
     if (share.seq < 0) return w;
-    w.left = min(share.per, share.total - share.begin);
+    w.left = share.units;
     w.s = share.seq;
     w.q = load_seq(p, w.s);
     w.tiles = (w.q.n * p.group + rows_per_tile - 1) / rows_per_tile;
     w.tile = 0;
     w.tile_unit = share.seq_unit;
     w.set_tile(p);
-    int64_t skip = share.begin - share.seq_unit;
-    while (skip >= static_cast<int64_t>(w.span.pages) * p.heads) {
-        skip -= static_cast<int64_t>(w.span.pages) * p.heads;
-        w.tile_unit += static_cast<int64_t>(w.span.pages) * p.heads;
+    int skip = share.begin - share.seq_unit;
+    while (skip >= w.span.pages * p.heads) {
+        skip -= w.span.pages * p.heads;
+        w.tile_unit += w.span.pages * p.heads;
         ++w.tile;
         w.set_tile(p);
     }
-    w.head = static_cast<int>(skip / w.span.pages);
-    w.page = static_cast<int>(skip % w.span.pages);
-    w.tile_unit += static_cast<int64_t>(w.head) * w.span.pages;
+    w.head = skip / w.span.pages;
+    w.page = skip - w.head * w.span.pages;
+    w.tile_unit += w.head * w.span.pages;
     return w;
 }
 

@@ -117,6 +117,9 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     const uint32_t max_q = chunk->max_q == 0 || chunk->max_q > chunk->tokens ? chunk->tokens : chunk->max_q;
     const uint64_t max_rows = static_cast<uint64_t>(max_q) * group;
     if (max_rows > INT_MAX) return -1;
+    // Units of work (a page for 16 rows and a KV head) are counted in 32 bits.
+    const uint64_t tiles16 = static_cast<uint64_t>(chunk->tokens) * group / 16 + chunk->seqs;
+    if (tiles16 * pages->heads > INT_MAX || tiles16 * pages->heads * chunk->table_width > INT_MAX) return -1;
 
     AttendParams p;
     std::memset(&p, 0, sizeof(p));

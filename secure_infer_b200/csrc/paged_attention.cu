@@ -89,7 +89,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
     __shared__ Share share;
-    __shared__ int64_t warp_sums[kRowsThreads / 32];
+    __shared__ int32_t warp_sums[kRowsThreads / 32];
     __shared__ volatile int stop;   // a wait ran out
     __shared__ int irregular, last_piece, give_up;
 
@@ -124,16 +124,16 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
-        int64_t unit = 0;
+        uint32_t unit = 0;
         while (w.left > 0 && !stop) {
-            const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+            const int pages = w.take();
             const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
             for (int i0 = 0; i0 < pages; i0 += 32) {
                 const int id = i0 + lane < pages && w.span.hi > 0 ? row[i0 + lane] : -1;
                 for (int i = i0; i < min(pages, i0 + 32); ++i, ++unit) {
                     const int page = __shfl_sync(0xffffffffu, id, i - i0);
-                    const int stage = static_cast<int>(unit % kRowsStages);
-                    const uint32_t turn = static_cast<uint32_t>(unit / kRowsStages);
+                    const int stage = unit % kRowsStages;
+                    const uint32_t turn = unit / kRowsStages;
                     if (lane != 0 || stop || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, &stop))) continue;
                     const int first = (w.span.first + w.page + i) * kPage;
                     const int qa = max(0, w.span.lo - first) / kQuarter;
@@ -150,23 +150,22 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 }
                 __syncwarp();
             }
-            w.left -= pages;
-            if (w.left > 0) w.next_tile(p);
+            w.advance(p, pages);
         }
         // Copies still in flight land before the CTA's shared memory goes away.
         if (lane == 0) {
-            for (int64_t u = max(int64_t(0), unit - kRowsStages); u < unit; ++u) {
-                barrier_wait(k_full(u % kRowsStages), static_cast<uint32_t>(u / kRowsStages) & 1, &stop);
-                barrier_wait(v_full(u % kRowsStages), static_cast<uint32_t>(u / kRowsStages) & 1, &stop);
+            for (uint32_t u = unit > kRowsStages ? unit - kRowsStages : 0; u < unit; ++u) {
+                barrier_wait(k_full(u % kRowsStages), (u / kRowsStages) & 1, &stop);
+                barrier_wait(v_full(u % kRowsStages), (u / kRowsStages) & 1, &stop);
             }
             if (stop) atomicOr(p.status, 1u);
         }
         return;
     }
 
-    int64_t unit = 0;
+    uint32_t unit = 0;
     while (w.left > 0) {
-        const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+        const int pages = w.take();
         // The tile's rows, 256 bytes each, in 16-byte pieces swizzled against bank conflicts.
         const int r0 = w.tile * kRows;
         for (int c = tid; c < kRows * 16; c += 32 * kRowsWarps) {
@@ -201,8 +200,8 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const bool idle = row_tile * 16 >= w.rows;   // no row of this warp's sixteen is used
 
         for (int i = 0; i < pages; ++i, ++unit) {
-            const int stage = static_cast<int>(unit % kRowsStages);
-            const uint32_t parity = static_cast<uint32_t>(unit / kRowsStages) & 1;
+            const int stage = unit % kRowsStages;
+            const uint32_t parity = unit / kRowsStages & 1;
             const int page_key = (w.span.first + w.page + i) * kPage;
             if (!barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop)) break;
 #pragma unroll
@@ -307,8 +306,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (tid == 0) give_up = stop;
         rows_sync();
         if (give_up) break;
-        const int64_t tile_end = w.tile_unit + w.span.pages;
-        const int cta0 = static_cast<int>(w.tile_unit / share.per), cta1 = static_cast<int>((tile_end - 1) / share.per);
+        const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
         const bool split = cta1 > cta0;
         float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
         const bool by_definition = irregular != 0;
@@ -430,8 +428,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             if (tid == 0) irregular = 0;
         }
         rows_sync();
-        w.left -= pages;
-        if (w.left > 0) w.next_tile(p);
+        w.advance(p, pages);
     }
 }
 
@@ -441,18 +438,19 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // Chunks: both products on the tcgen05 tensor cores, bound by them and by the
 // exponentials (a 128 x 128 tile takes 1024 clocks of each).  One CTA per SM
 // takes two tiles of up to 128 rows (whole tokens) that share every page.  A
-// warp loads pages by TMA through a ring of five 32 KiB buffers, a warp issues
-// the products, and a warpgroup per tile holds one row per thread: scores from
+// warp loads pages by TMA through a ring of five 32 KiB buffers, a warp per tile
+// issues its products, and two warpgroups per tile hold a row in two threads: scores from
 // tensor memory, maximum, weights back over the scores in the cache's type,
 // from where the second product reads them.  While one tile's softmax runs the
 // other's products do.  The accumulated values are only rescaled when a row's
 // maximum grew by more than 2^8 since the last time; weights up to 2^8 are as
 // exact as weights up to 1, and the sums are 32-bit.  Tensor memory: scores
 // (and weights) of the tiles at columns 0 and 128, values at 256 and 384.
-constexpr int kTileThreads = 384;   // two softmax warpgroups; producer, products, two checkers
+constexpr int kSoftWarps = 16;       // four warpgroups: two tiles, two halves of a page's keys
+constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, checker
 constexpr int kRing = 5;
 constexpr uint32_t kTileBytes = 128 * kDim * 2;
-constexpr uint32_t kTilesSmem = 1024 + (2 + kRing) * kTileBytes;
+constexpr int kItems = 8;
 constexpr int kTileRows = 256;
 constexpr int kTileSlot = kTileRows * (kDim + 2);
 constexpr float kRescale = 8.0f;
@@ -599,84 +597,120 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t x2)
                        __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(e.y) << 23)));
 }
 
+// A CTA's piece of a tile, from the producer for the other warps.  The producer
+// is less than kItems pieces ahead of the last of them: it needs the first
+// product of the piece before, and buffers that the checker gives back, who
+// waits for every softmax warp.
+struct Item {
+    Seq q;
+    Span span;
+    int s, head, page, pages;            // pages [page, page + pages) of the tile's
+    int first_token, last_token, rows;
+    int tile_unit;
+    int more;                            // another piece follows
+
+    __device__ __forceinline__ int first_key() const { return (span.first + page) * kPage; }
+};
+
+struct TilesControl {
+    uint64_t kv_full[kRing], kv_empty[kRing], q_full, q_empty;
+    uint64_t s_full[2], p_ready[2], o_full[2], drained[2], turn[2];
+    uint64_t checked, taken, item_full[kItems];
+    Item items[kItems];
+    float exchange[2][2][128];           // between a row's two threads
+    int32_t warp_sums[kTileThreads / 32];
+    Share share;
+    uint32_t tmem;
+    int irregular;                       // what the checker found in the piece
+    int stop;                            // a wait ran out
+};
+constexpr uint32_t kControlBytes = 4096 - 1024;   // the first KiB of shared memory is the driver's
+static_assert(sizeof(TilesControl) <= kControlBytes, "control block");
+constexpr uint32_t kTilesSmem = kControlBytes + (2 + kRing) * kTileBytes;
+
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttendParams p)
 {
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kRing + 2 + 6 + 3];
-    __shared__ Share share;
-    __shared__ int64_t warp_sums[kTileThreads / 32];
-    __shared__ uint32_t tmem_base;
-    __shared__ Walk walks[8];   // the softmax warps', who need their registers
-    __shared__ volatile int stop;
-    __shared__ volatile int irregular[2];   // what each checker found in the item
-
-    const uint32_t smem = (smem_addr(smem_raw) + 1023) & ~1023u;
-    const uint32_t q_smem = smem, ring = smem + 2 * kTileBytes;
-    auto kv_full = [&](int i) { return smem_addr(&bars[i]); };
-    auto kv_empty = [&](int i) { return smem_addr(&bars[kRing + i]); };
-    const uint32_t q_full = smem_addr(&bars[2 * kRing]), q_empty = q_full + 8;
-    auto s_full = [&](int w) { return smem_addr(&bars[2 * kRing + 2 + w]); };
-    auto p_ready = [&](int w) { return smem_addr(&bars[2 * kRing + 4 + w]); };
-    auto o_full = [&](int w) { return smem_addr(&bars[2 * kRing + 6 + w]); };
-    const uint32_t checked = smem_addr(&bars[2 * kRing + 8]), taken = checked + 8, drained = checked + 16;
+    TilesControl& c = *reinterpret_cast<TilesControl*>(smem_raw);
+    volatile int* const stop = &c.stop;
+    const uint32_t q_smem = smem_addr(smem_raw) + kControlBytes, ring = q_smem + 2 * kTileBytes;
+    if (q_smem & 1023) {   // the swizzle needs it; shared memory would have to start elsewhere
+        if (threadIdx.x == 0) atomicOr(p.status, 2u);
+        return;
+    }
+    auto kv_full = [&](int i) { return smem_addr(&c.kv_full[i]); };
+    auto kv_empty = [&](int i) { return smem_addr(&c.kv_empty[i]); };
+    const uint32_t q_full = smem_addr(&c.q_full), q_empty = smem_addr(&c.q_empty);
+    auto s_full = [&](int w) { return smem_addr(&c.s_full[w]); };
+    auto p_ready = [&](int w) { return smem_addr(&c.p_ready[w]); };
+    auto o_full = [&](int w) { return smem_addr(&c.o_full[w]); };
+    auto turn = [&](int w) { return smem_addr(&c.turn[w]); };
+    auto drained = [&](int w) { return smem_addr(&c.drained[w]); };
+    auto item_full = [&](uint32_t i) { return smem_addr(&c.item_full[i % kItems]); };
+    const uint32_t checked = smem_addr(&c.checked), taken = smem_addr(&c.taken);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) {
             barrier_init(kv_full(i), 1);
-            barrier_init(kv_empty(i), 3);    // the products' commit and both checkers
+            barrier_init(kv_empty(i), 3);    // each tile's products and the checker
         }
         barrier_init(q_full, 1);
-        barrier_init(q_empty, 1);
+        barrier_init(q_empty, 2);
         for (int w = 0; w < 2; ++w) {
             barrier_init(s_full(w), 1);
-            barrier_init(p_ready(w), 4);
+            barrier_init(p_ready(w), kSoftWarps / 2);
             barrier_init(o_full(w), 1);
+            barrier_init(drained(w), 1);
+            barrier_init(turn(w), 1);
         }
-        barrier_init(checked, 2);
-        barrier_init(taken, 8);
-        barrier_init(drained, 1);
-        stop = 0;
+        barrier_init(checked, 1);
+        barrier_init(taken, kSoftWarps);
+        for (int i = 0; i < kItems; ++i) barrier_init(item_full(i), 1);
+        c.stop = 0;
+        c.irregular = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_base)) : "memory");
+    if (warp == kSoftWarps + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&c.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tmem_fence_before();
     }
     wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads>(p, 2 * rows_per_tile, 1, &share, warp_sums);
+    find_share<kTileThreads>(p, 2 * rows_per_tile, 1, &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
-    const uint32_t tmem = tmem_base;
-    Walk w = start_walk(p, 2 * rows_per_tile, share);
-    if (warp < 8 && lane == 0) walks[warp] = w;
-    __syncwarp();
+    const uint32_t tmem = c.tmem;
+    const bool any = c.share.seq >= 0;
 
-    // 384 threads at 168 registers: 208 for the softmax warpgroups and 88 for the third make the same sum.
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 8) {
+    // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.
+    if (warp >= kSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == kSoftWarps) {
             // Producer.
+            Walk w = start_walk(p, 2 * rows_per_tile, c.share);
             uint32_t n = 0, item = 0;
-            while (w.left > 0 && !stop) {
-                const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+            while (w.left > 0 && !*stop) {
+                const int pages = w.take();
                 if (lane == 0) {
-                    if (item > 0) barrier_wait(q_empty, (item - 1) & 1, &stop);
-                    if (!stop) {
+                    if (item > 0) barrier_wait(q_empty, (item - 1) & 1, stop);
+                    c.items[item % kItems] = Item{w.q, w.span, w.s, w.head, w.page, pages, w.first_token, w.last_token,
+                                                  w.rows, w.tile_unit, w.left > pages};
+                    barrier_arrive(item_full(item));
+                    if (!*stop) {
                         const int tiles = w.rows > rows_per_tile ? 2 : 1;
                         barrier_expect(q_full, tiles * 2 * rows_per_tile * 128);
                         for (int t = 0; t < tiles; ++t)
                             for (int h = 0; h < 2; ++h)
-                                tma_load_rows(q_smem + t * kTileBytes + h * (kTileBytes / 2), &q_map, q_full, w.head * p.group,
-                                              w.q.q0 + w.first_token + t * tokens, h);
+                                tma_load_rows(q_smem + t * kTileBytes + h * (kTileBytes / 2), &q_map, q_full,
+                                              w.head * p.group, w.q.q0 + w.first_token + t * tokens, h);
                     }
                 }
                 __syncwarp();
@@ -686,8 +720,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     for (int i = i0; i < min(pages, i0 + 32); ++i) {
                         const int page = __shfl_sync(0xffffffffu, id, i - i0);
                         for (int kv = 0; kv < 2; ++kv, ++n) {
-                            const uint32_t slot = n % kRing, turn = n / kRing;
-                            if (lane != 0 || stop || (turn > 0 && !barrier_wait(kv_empty(slot), (turn - 1) & 1, &stop))) continue;
+                            const uint32_t slot = n % kRing, turns = n / kRing;
+                            if (lane != 0 || *stop || (turns > 0 && !barrier_wait(kv_empty(slot), (turns - 1) & 1, stop))) continue;
                             barrier_expect(kv_full(slot), kTileBytes);
                             tma_load_page(ring + slot * kTileBytes, kv ? &v_map : &k_map, kv_full(slot), 0, 0, w.head, page);
                         }
@@ -695,131 +729,146 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     __syncwarp();
                 }
                 ++item;
-                w.left -= pages;
-                if (w.left > 0) w.next_tile(p);
+                w.advance(p, pages);
             }
             if (lane == 0) {
-                for (uint32_t u = n > kRing ? n - kRing : 0; u < n; ++u) barrier_wait(kv_full(u % kRing), (u / kRing) & 1, &stop);
-                if (stop) atomicOr(p.status, 1u);
+                for (uint32_t u = n > kRing ? n - kRing : 0; u < n; ++u) barrier_wait(kv_full(u % kRing), (u / kRing) & 1, stop);
+                if (*stop) atomicOr(p.status, 1u);
             }
             __syncwarp();
-        } else if (warp == 9) {
-            // Products.
+        } else if (warp < kSoftWarps + 3) {
+            // Products, a warp per tile, in turns of one page: while one tile's products run the other warp has done
+            // its waiting, and the two softmax warpgroups stay half a page apart instead of fighting for the same units.
+            const int t = warp - kSoftWarps - 1;
             constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
             constexpr uint32_t desc = 1u << 4 | type << 7 | type << 10 | (128u >> 3) << 17 | (128u >> 4) << 24;
             constexpr uint32_t desc_v = desc | 1u << 16;   // V's rows run along the sum
-            uint32_t n = 0, item = 0, ready = 0;           // buffers taken, items, softmax tiles per warpgroup
-            auto scores = [&](int t, uint32_t slot) {
-                const uint32_t q = operand(q_smem + t * kTileBytes, 0), k = operand(ring + slot * kTileBytes, 0), d = tmem + t * 128;
-                product_smem<false>(d, operand_at(q, 0), operand_at(k, 0), desc);
+            const uint32_t q = operand(q_smem + t * kTileBytes, 0), s_at = tmem + t * 128, o_at = tmem + 256 + t * 128;
+            uint32_t n = 0, item = 0, ready = 0, turns = 0;   // buffers and items taken, softmax tiles, turns
+            auto my_turn = [&](bool both) {
+                if (!both) return true;
+                const bool mine = t == 0 && turns == 0 ? true : barrier_wait(turn(t), (turns - (t == 0)) & 1, stop);
+                ++turns;
+                return mine;
+            };
+            auto scores = [&](uint32_t slot) {
+                const uint32_t k = operand(ring + slot * kTileBytes, 0);
+                product_smem<false>(s_at, operand_at(q, 0), operand_at(k, 0), desc);
 #pragma unroll
                 for (int i = 1; i < 8; ++i) {
                     const uint32_t at = (i >> 2) * (kTileBytes / 2) + (i & 3) * 32;
-                    product_smem<true>(d, operand_at(q, at), operand_at(k, at), desc);
+                    product_smem<true>(s_at, operand_at(q, at), operand_at(k, at), desc);
                 }
                 commit_to(s_full(t));
+                commit_to(kv_empty(slot));
             };
             bool ok = true;
-            while (ok && w.left > 0) {
-                const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
-                const int tiles = w.rows > rows_per_tile ? 2 : 1;
-                uint32_t slot = n % kRing;
-                ok = barrier_wait(q_full, item & 1, &stop) && barrier_wait(kv_full(slot), (n / kRing) & 1, &stop);
+            while (ok && any) {
+                ok = barrier_wait(item_full(item), (item / kItems) & 1, stop) && barrier_wait(q_full, item & 1, stop);
                 if (!ok) break;
-                tmem_fence_after();
-                if (elected()) {
-                    for (int t = 0; t < tiles; ++t) scores(t, slot);
-                    commit_to(kv_empty(slot));
-                    if (pages == 1) commit_to(q_empty);
-                }
-                __syncwarp();
-                ++n;
-                for (int i = 0; ok && i < pages; ++i) {
-                    const uint32_t v_slot = n % kRing, k_slot = (n + 1) % kRing;
-                    const bool more = i + 1 < pages;
-                    ok = barrier_wait(kv_full(v_slot), (n / kRing) & 1, &stop);
-                    if (!ok) break;
-                    // Values of keys that no row sees were never written or belong to others: weights of zero do not
-                    // silence a NaN there, so within the 16-key steps that are multiplied they become zero.
-                    const int key0 = (w.span.first + w.page + i) * kPage;
-                    const int lo = max(0, min(kPage, w.span.lo - key0)), hi = max(0, min(kPage, w.span.hi - key0));
-                    const int step0 = lo >> 4, step1 = hi > lo ? (hi + 15) >> 4 : step0;
-                    if (lo & 15 || hi & 15) {
-                        for (int side = 0; side < 2; ++side) {
-                            const int a = side ? hi : step0 * 16, b = side ? min(kPage, step1 * 16) : lo;
-                            for (int c = lane; c < (b - a) * 16; c += 32) {
-                                const uint32_t at = ring + v_slot * kTileBytes + (c & 8 ? kTileBytes / 2 : 0) + (a + (c >> 4)) * 128 + (c & 7) * 16;
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                            }
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
+                const Item& w = c.items[item % kItems];
+                const int pages = w.pages;
+                const bool last = !w.more;
+                if (t == 1 && w.rows <= rows_per_tile) {
+                    // No second tile: its share of the buffers is given back as they fill.
+                    for (int i = 0; ok && i < 2 * pages; ++i, ++n) {
+                        ok = barrier_wait(kv_full(n % kRing), (n / kRing) & 1, stop);
+                        if (ok && lane == 0) barrier_arrive(kv_empty(n % kRing));
                     }
-                    const uint32_t v = operand(ring + v_slot * kTileBytes, kTileBytes / 2);
-                    for (int t = 0; ok && t < tiles; ++t) {
-                        ok = barrier_wait(p_ready(t), ready & 1, &stop);
-                        if (ok && t == 0 && more) ok = barrier_wait(kv_full(k_slot), ((n + 1) / kRing) & 1, &stop);
+                    if (lane == 0) barrier_arrive(q_empty);
+                } else {
+                    const bool both = w.rows > rows_per_tile;
+                    ok = ok && barrier_wait(kv_full(n % kRing), (n / kRing) & 1, stop) && my_turn(both);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    if (elected()) {
+                        scores(n % kRing);
+                        if (both) barrier_arrive(turn(1 - t));
+                        if (pages == 1) commit_to(q_empty);
+                    }
+                    __syncwarp();
+                    ++n;
+                    for (int i = 0; i < pages; ++i) {
+                        const uint32_t v_slot = n % kRing, k_slot = (n + 1) % kRing;
+                        const bool more = i + 1 < pages;
+                        ok = barrier_wait(kv_full(v_slot), (n / kRing) & 1, stop);
+                        // Values of keys that no row sees were never written or belong to others: weights of zero do
+                        // not silence a NaN there, so within the 16-key steps that are multiplied they become zero.
+                        const int key0 = w.first_key() + i * kPage;
+                        const int lo = max(0, min(kPage, w.span.lo - key0)), hi = max(0, min(kPage, w.span.hi - key0));
+                        const int step0 = lo >> 4, step1 = hi > lo ? (hi + 15) >> 4 : step0;
+                        if (lo & 15 || hi & 15) {
+                            for (int side = 0; side < 2; ++side) {
+                                const int a = side ? hi : step0 * 16, b = side ? min(kPage, step1 * 16) : lo;
+                                for (int x = lane; x < (b - a) * 16; x += 32) {
+                                    const uint32_t at = ring + v_slot * kTileBytes + (x & 8 ? kTileBytes / 2 : 0) +
+                                                        (a + (x >> 4)) * 128 + (x & 7) * 16;
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                                }
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                        if (ok && more) ok = barrier_wait(kv_full(k_slot), ((n + 1) / kRing) & 1, stop);
+                        ok = ok && barrier_wait(p_ready(t), ready & 1, stop) && my_turn(both);
                         if (!ok) break;
+                        ++ready;
                         tmem_fence_after();
                         if (elected()) {
-                            const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128;
+                            const uint32_t v = operand(ring + v_slot * kTileBytes, kTileBytes / 2);
                             if (step0 == 0 && step1 == 8) {
-                                product_tmem(d, a, operand_at(v, 0), desc_v, i > 0);
+                                product_tmem(o_at, s_at, operand_at(v, 0), desc_v, i > 0);
 #pragma unroll
-                                for (int k = 1; k < 8; ++k) product_tmem(d, a + k * 8, operand_at(v, k * 2048), desc_v, 1);
+                                for (int k = 1; k < 8; ++k) product_tmem(o_at, s_at + k * 8, operand_at(v, k * 2048), desc_v, 1);
                             } else {
                                 // A page that no row sees still sets the values to zero where it is the first.
                                 const int s0 = step1 > step0 ? step0 : 0, s1 = step1 > step0 ? step1 : (i == 0 ? 1 : 0);
                                 for (int k = s0; k < s1; ++k)
-                                    product_tmem(d, a + k * 8, operand_at(v, k * 2048), desc_v, i > 0 || k > s0);
+                                    product_tmem(o_at, s_at + k * 8, operand_at(v, k * 2048), desc_v, i > 0 || k > s0);
                             }
-                            if (more) scores(t, k_slot);
+                            if (more) scores(k_slot);
                             else commit_to(o_full(t));
-                            if (t + 1 == tiles) {
-                                commit_to(kv_empty(v_slot));
-                                if (more) commit_to(kv_empty(k_slot));
-                                if (i + 2 == pages) commit_to(q_empty);
-                            }
+                            commit_to(kv_empty(v_slot));
+                            if (i + 2 == pages) commit_to(q_empty);
+                            if (both) barrier_arrive(turn(1 - t));
                         }
                         __syncwarp();
+                        n += more ? 2 : 1;
                     }
-                    ++ready;
-                    n += more ? 2 : 1;
                 }
                 ++item;
-                w.left -= pages;
-                if (w.left > 0) w.next_tile(p);
+                if (last) break;
             }
             // Nothing of this warp is in flight when tensor memory is given back.
-            if (lane == 0) {
-                commit_to(drained);
-                barrier_wait(drained, 0, &stop);
-            }
+            if (elected()) commit_to(drained(t));
             __syncwarp();
-        } else if (warp >= 10) {
-            // Checkers: an infinity or NaN among values that some rows see and others do not, where zero weights would
-            // carry it over.  Each takes one half of the 128 values.
+            barrier_wait(drained(t), 0, stop);
+        } else {
+            // Checker: an infinity or NaN among values that some rows see and others do not, where weights of zero
+            // would carry it over.
             uint32_t n = 0, item = 0;
-            while (w.left > 0 && !stop) {
-                const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+            while (any) {
+                if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
+                const Item w = c.items[item % kItems];
+                const int pages = w.pages;
                 int lo_all, hi_all, unused;   // keys that all rows see
                 row_keys(p, w.q, w.last_token, lo_all, unused);
                 row_keys(p, w.q, w.first_token, unused, hi_all);
                 bool odd = false;
                 for (int i = 0; i < pages; ++i) {
-                    const int key0 = (w.span.first + w.page + i) * kPage;
+                    const int key0 = w.first_key() + i * kPage;
                     for (int kv = 0; kv < 2; ++kv, ++n) {
                         const uint32_t slot = n % kRing;
-                        if (!barrier_wait(kv_full(slot), (n / kRing) & 1, &stop)) break;
+                        if (!barrier_wait(kv_full(slot), (n / kRing) & 1, stop)) break;
                         if (kv == 1 && w.first_token != w.last_token && (key0 < lo_all || key0 + kPage - 1 > hi_all)) {
                             const int a = max(0, w.span.lo - key0), b = min(kPage, w.span.hi - key0);
-                            for (int c = lane; c < kPage * 8; c += 32) {
-                                const int key = c >> 3;
+                            for (int piece = lane; piece < kPage * 16; piece += 32) {
+                                const int key = piece >> 3 & 127;
                                 if (key < a || key >= b || (key0 + key >= lo_all && key0 + key <= hi_all)) continue;
                                 uint4 x;
                                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                              : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                                             : "r"(ring + slot * kTileBytes + (warp - 10) * (kTileBytes / 2) + c * 16));
+                                             : "r"(ring + slot * kTileBytes + piece * 16));
                                 odd |= nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) || nonfinite2<T>(x.w);
                             }
                         }
@@ -828,29 +877,32 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                 }
                 // The flag is the previous item's until the softmax has read it.
-                if (item > 0) barrier_wait(taken, (item - 1) & 1, &stop);
+                if (item > 0) barrier_wait(taken, (item - 1) & 1, stop);
                 odd = __any_sync(0xffffffffu, odd);
-                if (lane == 0) irregular[warp - 10] = odd;
+                if (lane == 0) c.irregular = odd;
                 __syncwarp();
                 if (lane == 0) barrier_arrive(checked);
                 ++item;
-                w.left -= pages;
-                if (w.left > 0) w.next_tile(p);
+                if (!w.more) break;
             }
         }
     } else {
-        // Softmax: one row per thread.
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int t = warp >> 2, row = tid & 127;
+        // Softmax: a row of a tile by two threads, each with half of a page's keys.  After a wait that ran out the
+        // loops run on without waiting, so the two keep meeting.
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int t = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-        const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+        const uint32_t s_at = tmem + lanes + t * 128 + half * 64, w_at = tmem + lanes + t * 128 + half * 32;
+        const uint32_t o_at = tmem + lanes + 256 + t * 128 + half * 64;
         const float scale = fabsf(p.scale_log2);
         const bool flip = p.scale_log2 < 0.0f;
-        Walk& w = walks[warp];
-        uint32_t turn = 0, done = 0, item = 0;   // completions of s_full and o_full taken
+        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+        uint32_t seen = 0, done = 0, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
-        while (ok && w.left > 0) {
-            const int pages = static_cast<int>(min(w.left, static_cast<int64_t>(w.span.pages - w.page)));
+        while (any) {
+            if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
+            const Item& w = c.items[item % kItems];
+            const int pages = w.pages;
             const bool used = t == 0 || w.rows > rows_per_tile;
             const int token = w.first_token + t * tokens + row / p.group;   // of the sequence's new ones
             const bool valid = row < rows_per_tile && t * rows_per_tile + row < w.rows;
@@ -859,36 +911,42 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             int lo_all, hi_all, unused;
             row_keys(p, w.q, w.last_token, lo_all, unused);
             row_keys(p, w.q, w.first_token, unused, hi_all);
-            const int first_key = (w.span.first + w.page) * kPage;
+            const int first_key = w.first_key() + half * 64;
             float m = -INFINITY, l = 0.0f;
             if (used) {
                 for (int i = 0; i < pages; ++i) {
-                    ok = barrier_wait(s_full(t), turn & 1, &stop);
-                    ++turn;
-                    if (!ok) break;
+                    ok = ok && barrier_wait(s_full(t), seen & 1, stop);
+                    ++seen;
                     tmem_fence_after();
                     const int key0 = first_key + i * kPage;
-                    uint32_t s[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_load<32>(s[c], s_at + c * 32);
+                    uint32_t s[2][32];
+                    tmem_load<32>(s[0], s_at);
+                    tmem_load<32>(s[1], s_at + 32);
                     tmem_wait_loads();
                     if (flip) {
 #pragma unroll
-                        for (int c = 0; c < 128; ++c) s[c >> 5][c & 31] ^= 0x80000000u;
+                        for (int j = 0; j < 64; ++j) s[j >> 5][j & 31] ^= 0x80000000u;
                     }
-                    const bool masked = key0 < lo_all || key0 + kPage - 1 > hi_all;
+                    const bool masked = key0 < lo_all || key0 + 63 > hi_all;
                     if (masked) {
                         const int a = lo - key0, b = hi - key0;
 #pragma unroll
-                        for (int c = 0; c < 128; ++c)
-                            if (c < a || c > b) s[c >> 5][c & 31] = 0xff800000u;
+                        for (int j = 0; j < 64; ++j)
+                            if (j < a || j > b) s[j >> 5][j & 31] = 0xff800000u;
                     }
                     float tops[4] = {m, m, m, m};
 #pragma unroll
-                    for (int c = 0; c < 128; c += 2)
-                        tops[(c >> 1) & 3] = max3_nan(tops[(c >> 1) & 3], __uint_as_float(s[c >> 5][c & 31]),
-                                                      __uint_as_float(s[c >> 5][(c & 31) + 1]));
+                    for (int j = 0; j < 64; j += 2)
+                        tops[(j >> 1) & 3] = max3_nan(tops[(j >> 1) & 3], __uint_as_float(s[j >> 5][j & 31]),
+                                                      __uint_as_float(s[j >> 5][(j & 31) + 1]));
                     float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                    // The row's other thread.  Its scores are in registers by now too, so weights may cover scores.
+                    c.exchange[t][half][row] = top;
+                    tmem_fence_before();
+                    meet();
+                    tmem_fence_after();
+                    const float other = c.exchange[t][half ^ 1][row];
+                    top = max3_nan(top, other, other);
                     if (top == INFINITY) top = NAN;   // a NaN or infinite score makes its row NaN
                     if (i == 0) {
                         m = top;
@@ -897,41 +955,38 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         m = top;
                         l *= f;
 #pragma unroll 1
-                        for (int c = 0; c < 8; ++c) {
+                        for (int d = 0; d < 64; d += 16) {
                             uint32_t o[16];
-                            tmem_load<16>(o, o_at + c * 16);
+                            tmem_load<16>(o, o_at + d);
                             tmem_wait_loads();
 #pragma unroll
                             for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tmem_store(o_at + c * 16, o);
+                            tmem_store(o_at + d, o);
                         }
                         tmem_wait_stores();
                     }
                     const float base = m == -INFINITY ? 0.0f : m * scale;
                     const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
                     uint64_t sum[4] = {};
-                    // Weights are rounded to the cache's type for the product; their sum is not.  A third of the
+                    // Weights are rounded to the cache's type for the product; their sum is not.  A quarter of the
                     // exponentials go to the multiply-add units, which levels these with the special function units:
                     // all on the latter would take as long as the products.  Masked tiles have exact zeros.
                     auto weights = [&](auto poly) {
+                        uint32_t w2[32];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t w2[32];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const uint64_t x = fma2(pair(s[c * 2 + (j >> 4)][(j & 15) * 2], s[c * 2 + (j >> 4)][(j & 15) * 2 + 1]), scale2, base2);
-                                float2 e;
-                                if (decltype(poly)::value && j % 3 == 1) {
-                                    e = exp2_poly(x);
-                                } else {
-                                    const float2 y = unpair(x);
-                                    e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                                }
-                                sum[j & 3] = add2(sum[j & 3], pair(e.x, e.y));
-                                w2[j] = pack2<T>(e.x, e.y);
+                        for (int j = 0; j < 32; ++j) {
+                            const uint64_t x = fma2(pair(s[j >> 4][(j & 15) * 2], s[j >> 4][(j & 15) * 2 + 1]), scale2, base2);
+                            float2 e;
+                            if (decltype(poly)::value && j % 4 == 1) {
+                                e = exp2_poly(x);
+                            } else {
+                                const float2 y = unpair(x);
+                                e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                             }
-                            tmem_store(s_at + c * 32, w2);
+                            sum[j & 3] = add2(sum[j & 3], pair(e.x, e.y));
+                            w2[j] = pack2<T>(e.x, e.y);
                         }
+                        tmem_store(w_at, w2);
                     };
                     if (masked) weights(std::false_type{});
                     else weights(std::true_type{});
@@ -942,22 +997,22 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     __syncwarp();
                     if (lane == 0) barrier_arrive(p_ready(t));
                 }
-                if (ok) ok = barrier_wait(o_full(t), done & 1, &stop);
+                ok = ok && barrier_wait(o_full(t), done & 1, stop);
                 ++done;
+                c.exchange[t][half][row] = l;
+                meet();
+                l += c.exchange[t][half ^ 1][row];
+                meet();   // read before the next page's maxima come
             }
-            if (ok) ok = barrier_wait(checked, item & 1, &stop);
-            if (!ok) break;
+            ok = ok && barrier_wait(checked, item & 1, stop);
             tmem_fence_after();
-            const int64_t tile_end = w.tile_unit + w.span.pages;
-            const int cta0 = static_cast<int>(w.tile_unit / share.per), cta1 = static_cast<int>((tile_end - 1) / share.per);
+            const int cta0 = c.share.owner(w.tile_unit), cta1 = c.share.owner(w.tile_unit + w.span.pages - 1);
             float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kTileSlot;
             const bool split = cta1 > cta0;
-            const bool by_definition = irregular[0] || irregular[1];
-            __syncwarp();
-            if (lane == 0) barrier_arrive(taken);
+            const bool by_definition = *static_cast<volatile int*>(&c.irregular) != 0;
             if (by_definition) {
-                const int ka = (w.span.first + w.page) * kPage, kb = ka + pages * kPage;
-                for (int r = (warp & 3) * 32; r < (warp & 3) * 32 + 32; ++r) {
+                const int ka = w.first_key(), kb = ka + pages * kPage;
+                for (int r = (warp & 3) * 32 + half; r < (warp & 3) * 32 + 32; r += 2) {
                     const int tile_row = t * rows_per_tile + r;
                     if (r >= rows_per_tile || tile_row >= w.rows) break;
                     const int tok = w.first_token + tile_row / p.group, g = tile_row % p.group;
@@ -987,18 +1042,18 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             } else if (used) {
                 const float inv = 1.0f / l;
                 const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + row % p.group;
-                T* out = static_cast<T*>(p.out) + at * kDim;
-                float* part = slot + (t * 128 + row) * kDim;
+                T* out = static_cast<T*>(p.out) + at * kDim + half * 64;
+                float* part = slot + (t * 128 + row) * kDim + half * 64;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int d = 0; d < 64; d += 32) {
                     uint32_t o[32];
-                    tmem_load<32>(o, o_at + c * 32);
+                    tmem_load<32>(o, o_at + d);
                     tmem_wait_loads();
                     if (!valid) continue;
                     if (split) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint4*>(part + c * 32 + j * 4) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                            *reinterpret_cast<uint4*>(part + d + j * 4) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                     } else {
                         const bool some = hi >= lo;
 #pragma unroll
@@ -1007,11 +1062,11 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
                                 x[k] = some ? pack2<T>(__uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
-                            *reinterpret_cast<uint4*>(out + c * 32 + j * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+                            *reinterpret_cast<uint4*>(out + d + j * 8) = make_uint4(x[0], x[1], x[2], x[3]);
                         }
                     }
                 }
-                if (valid) {
+                if (valid && half == 0) {
                     const float top = m * scale;
                     if (split) {
                         slot[kTileRows * kDim + t * 128 + row] = top;
@@ -1029,19 +1084,17 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     cut = Cut{1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
                 p.cuts[blockIdx.x] = cut;
             }
+            const bool last = !w.more;
             ++item;
             __syncwarp();
-            if (lane == 0) {
-                w.left -= pages;
-                if (w.left > 0) w.next_tile(p);
-            }
-            __syncwarp();
+            if (lane == 0) barrier_arrive(taken);
+            if (last) break;
         }
-        if (tid == 0 && share.seq < 0) p.cuts[blockIdx.x] = Cut{};
+        if (tid == 0 && !any) p.cuts[blockIdx.x] = Cut{};
     }
     tmem_fence_before();
     __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // Joins the pieces of tiles that were cut over CTAs: a warp per row.
