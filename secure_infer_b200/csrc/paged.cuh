@@ -202,12 +202,27 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t x)
     return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-// An infinity or a NaN in either half.
+// Sums of products with zero: NaN in either half as soon as an infinity or a
+// NaN was among the values.
 template <typename T>
-__device__ __forceinline__ bool nonfinite2(uint32_t x)
+__device__ __forceinline__ uint32_t zero_sum(uint32_t sum, uint32_t x);
+template <>
+__device__ __forceinline__ uint32_t zero_sum<__nv_bfloat16>(uint32_t sum, uint32_t x)
 {
-    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    return (x & e) == e || ((x >> 16) & e) == e;
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+    return sum;
+}
+template <>
+__device__ __forceinline__ uint32_t zero_sum<__half>(uint32_t sum, uint32_t x)
+{
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0u));
+    return sum;
+}
+template <typename T>
+__device__ __forceinline__ bool zero_sum_odd(uint32_t sum)
+{
+    const float2 x = unpack2<T>(sum);
+    return x.x != x.x || x.y != x.y;
 }
 
 // ------------------------------------------------- attention's work, in order

@@ -270,7 +270,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     const int key = key0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
                     if (key >= w.span.lo && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
                 }
-                bool odd = false;
+                uint32_t odd = 0;
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
                     uint32_t b[4];
@@ -281,13 +281,13 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             b[j] &= keep[j & 1];
-                            odd |= nonfinite2<T>(b[j]);
+                            odd = zero_sum<T>(odd, b[j]);
                         }
                     }
                     mma16816<T>(o[2 * d], weight, b[0], b[1]);
                     mma16816<T>(o[2 * d + 1], weight, b[2], b[3]);
                 }
-                if (odd && w.first_token != w.last_token) irregular = 1;
+                if (w.first_token != w.last_token && zero_sum_odd<T>(odd)) irregular = 1;
             }
             __syncwarp();
             if (lane == 0) barrier_arrive(empty(stage));
@@ -854,22 +854,26 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 int lo_all, hi_all, unused;   // keys that all rows see
                 row_keys(p, w.q, w.last_token, lo_all, unused);
                 row_keys(p, w.q, w.first_token, unused, hi_all);
-                bool odd = false;
+                uint32_t odd = 0;
                 for (int i = 0; i < pages; ++i) {
                     const int key0 = w.first_key() + i * kPage;
                     for (int kv = 0; kv < 2; ++kv, ++n) {
                         const uint32_t slot = n % kRing;
                         if (!barrier_wait(kv_full(slot), (n / kRing) & 1, stop)) break;
                         if (kv == 1 && w.first_token != w.last_token && (key0 < lo_all || key0 + kPage - 1 > hi_all)) {
+                            // Two keys at a time: left of what all rows see, then right of it.
                             const int a = max(0, w.span.lo - key0), b = min(kPage, w.span.hi - key0);
-                            for (int piece = lane; piece < kPage * 16; piece += 32) {
-                                const int key = piece >> 3 & 127;
-                                if (key < a || key >= b || (key0 + key >= lo_all && key0 + key <= hi_all)) continue;
-                                uint4 x;
-                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                             : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                                             : "r"(ring + slot * kTileBytes + piece * 16));
-                                odd |= nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) || nonfinite2<T>(x.w);
+                            for (int side = 0; side < 2; ++side) {
+                                const int k0 = side ? max(a, hi_all + 1 - key0) : a, k1 = side ? b : min(b, lo_all - key0);
+                                const uint32_t at = ring + slot * kTileBytes + (lane & 8 ? kTileBytes / 2 : 0) + (lane & 7) * 16;
+#pragma unroll 8
+                                for (int key = k0 + (lane >> 4); key < k1; key += 2) {
+                                    uint4 x;
+                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                                 : "r"(at + key * 128));
+                                    odd = zero_sum<T>(zero_sum<T>(zero_sum<T>(zero_sum<T>(odd, x.x), x.y), x.z), x.w);
+                                }
                             }
                         }
                         __syncwarp();
@@ -878,8 +882,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 }
                 // The flag is the previous item's until the softmax has read it.
                 if (item > 0) barrier_wait(taken, (item - 1) & 1, stop);
-                odd = __any_sync(0xffffffffu, odd);
-                if (lane == 0) c.irregular = odd;
+                const bool found = __any_sync(0xffffffffu, zero_sum_odd<T>(odd));
+                if (lane == 0) c.irregular = found;
                 __syncwarp();
                 if (lane == 0) barrier_arrive(checked);
                 ++item;
@@ -896,7 +900,15 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         const uint32_t o_at = tmem + lanes + 256 + t * 128 + half * 64;
         const float scale = fabsf(p.scale_log2);
         const bool flip = p.scale_log2 < 0.0f;
-        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+        // The two warps that hold a tile's 32 rows: whether any of their threads says so.
+        auto meet_or = [&](bool x) {
+            uint32_t r;
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.aligned.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+                         : "=r"(r)
+                         : "r"(1 + t * 4 + (warp & 3)), "r"(static_cast<uint32_t>(x))
+                         : "memory");
+            return r != 0;
+        };
         uint32_t seen = 0, done = 0, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
         while (any) {
@@ -911,7 +923,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             int lo_all, hi_all, unused;
             row_keys(p, w.q, w.last_token, lo_all, unused);
             row_keys(p, w.q, w.first_token, unused, hi_all);
-            const int first_key = w.first_key() + half * 64;
+            const int page_key = w.first_key(), first_key = page_key + half * 64;
             float m = -INFINITY, l = 0.0f;
             if (used) {
                 for (int i = 0; i < pages; ++i) {
@@ -919,79 +931,105 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     ++seen;
                     tmem_fence_after();
                     const int key0 = first_key + i * kPage;
-                    uint32_t s[2][32];
-                    tmem_load<32>(s[0], s_at);
-                    tmem_load<32>(s[1], s_at + 32);
-                    tmem_wait_loads();
-                    if (flip) {
-#pragma unroll
-                        for (int j = 0; j < 64; ++j) s[j >> 5][j & 31] ^= 0x80000000u;
-                    }
-                    const bool masked = key0 < lo_all || key0 + 63 > hi_all;
-                    if (masked) {
-                        const int a = lo - key0, b = hi - key0;
-#pragma unroll
-                        for (int j = 0; j < 64; ++j)
-                            if (j < a || j > b) s[j >> 5][j & 31] = 0xff800000u;
-                    }
-                    float tops[4] = {m, m, m, m};
-#pragma unroll
-                    for (int j = 0; j < 64; j += 2)
-                        tops[(j >> 1) & 3] = max3_nan(tops[(j >> 1) & 3], __uint_as_float(s[j >> 5][j & 31]),
-                                                      __uint_as_float(s[j >> 5][(j & 31) + 1]));
-                    float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-                    // The row's other thread.  Its scores are in registers by now too, so weights may cover scores.
-                    c.exchange[t][half][row] = top;
-                    tmem_fence_before();
-                    meet();
-                    tmem_fence_after();
-                    const float other = c.exchange[t][half ^ 1][row];
-                    top = max3_nan(top, other, other);
-                    if (top == INFINITY) top = NAN;   // a NaN or infinite score makes its row NaN
-                    if (i == 0) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, !((top - m) * scale <= kRescale) && top != -INFINITY)) {
-                        const float f = m == top ? 1.0f : exp2_approx((m - top) * scale);
-                        m = top;
-                        l *= f;
-#pragma unroll 1
-                        for (int d = 0; d < 64; d += 16) {
-                            uint32_t o[16];
-                            tmem_load<16>(o, o_at + d);
-                            tmem_wait_loads();
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tmem_store(o_at + d, o);
-                        }
-                        tmem_wait_stores();
-                    }
-                    const float base = m == -INFINITY ? 0.0f : m * scale;
-                    const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
-                    uint64_t sum[4] = {};
-                    // Weights are rounded to the cache's type for the product; their sum is not.  A quarter of the
-                    // exponentials go to the multiply-add units, which levels these with the special function units:
-                    // all on the latter would take as long as the products.  Masked tiles have exact zeros.
-                    auto weights = [&](auto poly) {
-                        uint32_t w2[32];
+                    // By the whole page, so that a row's two threads agree.
+                    const int page0 = page_key + i * kPage;
+                    const bool masked = page0 < lo_all || page0 + kPage - 1 > hi_all;
+                    bool fresh = i == 0 || masked || flip;
+                    if (!fresh) {
+                        // The usual page: weights by the maximum so far, while the page's own is found.
+                        uint32_t s[2][32], w2[32];
+                        tmem_load<32>(s[0], s_at);
+                        tmem_load<32>(s[1], s_at + 32);
+                        tmem_wait_loads();
+                        const float base = m == -INFINITY ? 0.0f : m * scale;
+                        const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+                        uint64_t sum[2] = {};
+                        float tops[2] = {m, m};
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const uint64_t x = fma2(pair(s[j >> 4][(j & 15) * 2], s[j >> 4][(j & 15) * 2 + 1]), scale2, base2);
+                            const uint32_t s0 = s[j >> 4][(j & 15) * 2], s1 = s[j >> 4][(j & 15) * 2 + 1];
+                            const uint64_t x = fma2(pair(s0, s1), scale2, base2);
+                            tops[j & 1] = max3_nan(tops[j & 1], __uint_as_float(s0), __uint_as_float(s1));
                             float2 e;
-                            if (decltype(poly)::value && j % 4 == 1) {
+                            // A quarter of the exponentials go to the multiply-add units, which levels these with the
+                            // special function units.
+                            if (j % 4 == 1) {
                                 e = exp2_poly(x);
                             } else {
                                 const float2 y = unpair(x);
                                 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                             }
-                            sum[j & 3] = add2(sum[j & 3], pair(e.x, e.y));
+                            sum[j & 1] = add2(sum[j & 1], pair(e.x, e.y));
+                            // Weights are rounded to the cache's type for the product; their sum is not.
                             w2[j] = pack2<T>(e.x, e.y);
                         }
-                        tmem_store(w_at, w2);
-                    };
-                    if (masked) weights(std::false_type{});
-                    else weights(std::true_type{});
-                    const float2 sums = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-                    l += sums.x + sums.y;
+                        const float top = max3_nan(tops[0], tops[1], tops[1]);
+                        // Weights may cover scores once the row's other thread has read its own.
+                        tmem_fence_before();
+                        fresh = meet_or(!((top - m) * scale <= kRescale) && top != -INFINITY);
+                        tmem_fence_after();
+                        if (!fresh) {
+                            tmem_store(w_at, w2);
+                            const float2 sums = unpair(add2(sum[0], sum[1]));
+                            l += sums.x + sums.y;
+                        }
+                    }
+                    if (fresh) {
+                        // The first page, one whose mask hides keys, or one that some row's maximum outgrew.
+                        uint32_t s[2][32];
+                        tmem_load<32>(s[0], s_at);
+                        tmem_load<32>(s[1], s_at + 32);
+                        tmem_wait_loads();
+                        if (flip) {
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) s[j >> 5][j & 31] ^= 0x80000000u;
+                        }
+                        if (masked) {
+                            const int a = lo - key0, b = hi - key0;
+#pragma unroll
+                            for (int j = 0; j < 64; ++j)
+                                if (j < a || j > b) s[j >> 5][j & 31] = 0xff800000u;
+                        }
+                        float tops[4] = {m, m, m, m};
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2)
+                            tops[(j >> 1) & 3] = max3_nan(tops[(j >> 1) & 3], __uint_as_float(s[j >> 5][j & 31]),
+                                                          __uint_as_float(s[j >> 5][(j & 31) + 1]));
+                        float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                        // And the row's other thread's.
+                        c.exchange[t][half][row] = top;
+                        tmem_fence_before();
+                        meet_or(false);
+                        tmem_fence_after();
+                        const float other = c.exchange[t][half ^ 1][row];
+                        top = max3_nan(top, other, other);
+                        if (top == INFINITY) top = NAN;   // a NaN or infinite score makes its row NaN
+                        if (i > 0) {
+                            const float f = m == top ? 1.0f : exp2_approx((m - top) * scale);
+                            l *= f;
+#pragma unroll 1
+                            for (int d = 0; d < 64; d += 16) {
+                                uint32_t o[16];
+                                tmem_load<16>(o, o_at + d);
+                                tmem_wait_loads();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                tmem_store(o_at + d, o);
+                            }
+                        }
+                        m = top;
+                        const float base = m == -INFINITY ? 0.0f : m * scale;
+                        float sum[4] = {};
+#pragma unroll
+                        for (int j = 0; j < 64; j += 2) {
+                            const float e0 = exp2_approx(fmaf(__uint_as_float(s[j >> 5][j & 31]), scale, -base));
+                            const float e1 = exp2_approx(fmaf(__uint_as_float(s[j >> 5][(j & 31) + 1]), scale, -base));
+                            sum[(j >> 1) & 3] += e0 + e1;
+                            s[j >> 6][j >> 1] = pack2<T>(e0, e1);
+                        }
+                        tmem_store(w_at, s[0]);
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    }
                     tmem_wait_stores();
                     tmem_fence_before();
                     __syncwarp();
@@ -1000,9 +1038,9 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 ok = ok && barrier_wait(o_full(t), done & 1, stop);
                 ++done;
                 c.exchange[t][half][row] = l;
-                meet();
+                meet_or(false);
                 l += c.exchange[t][half ^ 1][row];
-                meet();   // read before the next page's maxima come
+                meet_or(false);   // read before the next page's maxima come
             }
             ok = ok && barrier_wait(checked, item & 1, stop);
             tmem_fence_after();
