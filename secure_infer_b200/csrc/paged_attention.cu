@@ -438,7 +438,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // Chunks: both products on the tcgen05 tensor cores, bound by them and by the
 // exponentials (a 128 x 128 tile takes 1024 clocks of each).  One CTA per SM
 // takes two tiles of up to 128 rows (whole tokens) that share every page.  A
-// warp loads pages by TMA through a ring of five 32 KiB buffers, a warp per tile
+// warp loads pages by TMA through a ring of four 32 KiB buffers, a warp per tile
 // issues its products, and two warpgroups per tile hold a row in two threads: scores from
 // tensor memory, maximum, weights back over the scores in the cache's type,
 // from where the second product reads them.  While one tile's softmax runs the
@@ -448,7 +448,8 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // (and weights) of the tiles at columns 0 and 128, values at 256 and 384.
 constexpr int kSoftWarps = 16;       // four warpgroups: two tiles, two halves of a page's keys
 constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, checker
-constexpr int kRing = 5;
+constexpr int kRing = 4;
+constexpr uint32_t kStageBytes = 32 * 64;   // 64 bytes of a softmax warp's rows, on their way to coalesced stores
 constexpr uint32_t kTileBytes = 128 * kDim * 2;
 constexpr int kItems = 8;
 constexpr int kTileRows = 256;
@@ -626,7 +627,7 @@ struct TilesControl {
 };
 constexpr uint32_t kControlBytes = 4096 - 1024;   // the first KiB of shared memory is the driver's
 static_assert(sizeof(TilesControl) <= kControlBytes, "control block");
-constexpr uint32_t kTilesSmem = kControlBytes + (2 + kRing) * kTileBytes;
+constexpr uint32_t kTilesSmem = kControlBytes + (2 + kRing) * kTileBytes + kSoftWarps * kStageBytes;
 
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -985,10 +986,13 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             for (int j = 0; j < 64; ++j) s[j >> 5][j & 31] ^= 0x80000000u;
                         }
                         if (masked) {
-                            const int a = lo - key0, b = hi - key0;
+                            // Bits of the keys from lo to hi.
+                            const int a = max(0, lo - key0), b = min(63, hi - key0);
+                            const uint64_t bits = b < a ? 0 : (~0ull << a) & (~0ull >> (63 - b));
+                            const uint32_t keep[2] = {static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32)};
 #pragma unroll
                             for (int j = 0; j < 64; ++j)
-                                if (j < a || j > b) s[j >> 5][j & 31] = 0xff800000u;
+                                if (!(keep[j >> 5] >> (j & 31) & 1)) s[j >> 5][j & 31] = 0xff800000u;
                         }
                         float tops[4] = {m, m, m, m};
 #pragma unroll
@@ -1004,7 +1008,9 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         const float other = c.exchange[t][half ^ 1][row];
                         top = max3_nan(top, other, other);
                         if (top == INFINITY) top = NAN;   // a NaN or infinite score makes its row NaN
-                        if (i > 0) {
+                        if (i == 0) {
+                            m = top;
+                        } else if (__any_sync(0xffffffffu, !((top - m) * scale <= kRescale) && top != -INFINITY)) {
                             const float f = m == top ? 1.0f : exp2_approx((m - top) * scale);
                             l *= f;
 #pragma unroll 1
@@ -1016,8 +1022,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                                 for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
                                 tmem_store(o_at + d, o);
                             }
+                            m = top;
                         }
-                        m = top;
                         const float base = m == -INFINITY ? 0.0f : m * scale;
                         float sum[4] = {};
 #pragma unroll
@@ -1078,30 +1084,63 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                 }
             } else if (used) {
-                const float inv = 1.0f / l;
+                // Rows leave through a warp's own piece of shared memory, 64 bytes of each at a time, so that a store
+                // covers whole sectors: eight rows by four lanes.
+                const float inv = hi >= lo ? 1.0f / l : 0.0f;
                 const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + row % p.group;
-                T* out = static_cast<T*>(p.out) + at * kDim + half * 64;
-                float* part = slot + (t * 128 + row) * kDim + half * 64;
+                const uint32_t stage = ring + kRing * kTileBytes + warp * kStageBytes;
+                const int valid_rows = min(rows_per_tile, w.rows - t * rows_per_tile) - (warp & 3) * 32;
+                auto put = [&](const uint32_t (&x)[16]) {
 #pragma unroll
-                for (int d = 0; d < 64; d += 32) {
-                    uint32_t o[32];
-                    tmem_load<32>(o, o_at + d);
-                    tmem_wait_loads();
-                    if (!valid) continue;
-                    if (split) {
+                    for (int j = 0; j < 4; ++j)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)),
+                                     "r"(x[4 * j]), "r"(x[4 * j + 1]), "r"(x[4 * j + 2]), "r"(x[4 * j + 3])
+                                     : "memory");
+                    __syncwarp();
+                };
+                auto get = [&](int r) {
+                    uint4 x;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                 : "r"(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4))
+                                 : "memory");
+                    return x;
+                };
+                if (split) {
+                    float* part = slot + (t * 128 + (warp & 3) * 32) * kDim + half * 64 + (lane & 3) * 4;
+#pragma unroll 1
+                    for (int d = 0; d < 64; d += 16) {
+                        uint32_t o[16];
+                        tmem_load<16>(o, o_at + d);
+                        tmem_wait_loads();
+                        put(o);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint4*>(part + d + j * 4) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                    } else {
-                        const bool some = hi >= lo;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t x[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                x[k] = some ? pack2<T>(__uint_as_float(o[8 * j + 2 * k]) * inv, __uint_as_float(o[8 * j + 2 * k + 1]) * inv) : 0u;
-                            *reinterpret_cast<uint4*>(out + d + j * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = k * 8 + (lane >> 2);
+                            const uint4 x = get(r);
+                            if (r < valid_rows) *reinterpret_cast<uint4*>(part + r * kDim + d) = x;
                         }
+                        __syncwarp();
+                    }
+                } else {
+                    T* out = static_cast<T*>(p.out) + half * 64 + (lane & 3) * 8;
+#pragma unroll 1
+                    for (int d = 0; d < 64; d += 32) {
+                        uint32_t o[32], x[16];
+                        tmem_load<32>(o, o_at + d);
+                        tmem_wait_loads();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            x[j] = hi >= lo ? pack2<T>(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv) : 0u;
+                        put(x);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int r = k * 8 + (lane >> 2);
+                            const int64_t to = __shfl_sync(0xffffffffu, at, r);
+                            const uint4 y = get(r);
+                            if (r < valid_rows) *reinterpret_cast<uint4*>(out + to * kDim + d) = y;
+                        }
+                        __syncwarp();
                     }
                 }
                 if (valid && half == 0) {
