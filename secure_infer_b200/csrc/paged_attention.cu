@@ -603,14 +603,21 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t x2)
 // product of the piece before, and buffers that the checker gives back, who
 // waits for every softmax warp.
 struct Item {
-    Seq q;
     Span span;
-    int s, head, page, pages;            // pages [page, page + pages) of the tile's
-    int first_token, last_token, rows;
-    int tile_unit;
-    int more;                            // another piece follows
+    int s, head, pages, rows;
+    int first_key;               // of the piece
+    int pos, last_pos, last_key; // of the tile's first and last token, and of the sequence
+    int lo_all, hi_all;          // keys that every row sees
+    int q0;                      // the tile's first token among all
+    int slot;                    // where a part of a cut tile goes, -1: the tile is whole
+    int more;                    // another piece follows
 
-    __device__ __forceinline__ int first_key() const { return (span.first + page) * kPage; }
+    // Keys that the row at position p sees: [lo, hi].
+    __device__ __forceinline__ void keys(const AttendParams& a, int p, int& lo, int& hi) const
+    {
+        hi = a.causal ? min(last_key, p) : last_key;
+        lo = a.window ? max(0, p - a.window + 1) : 0;
+    }
 };
 
 struct TilesControl {
@@ -702,9 +709,31 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 const int pages = w.take();
                 if (lane == 0) {
                     if (item > 0) barrier_wait(q_empty, (item - 1) & 1, stop);
-                    c.items[item % kItems] = Item{w.q, w.span, w.s, w.head, w.page, pages, w.first_token, w.last_token,
-                                                  w.rows, w.tile_unit, w.left > pages};
+                    Item& it = c.items[item % kItems];
+                    it.span = w.span;
+                    it.s = w.s;
+                    it.head = w.head;
+                    it.pages = pages;
+                    it.rows = w.rows;
+                    it.first_key = (w.span.first + w.page) * kPage;
+                    it.pos = w.q.kv - w.q.n + w.first_token;
+                    it.last_pos = it.pos + w.last_token - w.first_token;
+                    it.last_key = w.q.kv - 1;
+                    int unused;
+                    it.keys(p, it.last_pos, it.lo_all, unused);
+                    it.keys(p, it.pos, unused, it.hi_all);
+                    it.q0 = w.q.q0 + w.first_token;
+                    const int cta0 = c.share.owner(w.tile_unit), cta1 = c.share.owner(w.tile_unit + w.span.pages - 1);
+                    it.slot = cta1 > cta0 ? 2 * static_cast<int>(blockIdx.x) + (cta0 == static_cast<int>(blockIdx.x)) : -1;
+                    it.more = w.left > pages;
                     barrier_arrive(item_full(item));
+                    // Only the first tile of a CTA can have begun in an earlier one.
+                    if (item == 0) {
+                        Cut cut{};
+                        if (cta0 < static_cast<int>(blockIdx.x) && w.page + pages == w.span.pages)
+                            cut = Cut{1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
+                        p.cuts[blockIdx.x] = cut;
+                    }
                     if (!*stop) {
                         const int tiles = w.rows > rows_per_tile ? 2 : 1;
                         barrier_expect(q_full, tiles * 2 * rows_per_tile * 128);
@@ -795,7 +824,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         ok = barrier_wait(kv_full(v_slot), (n / kRing) & 1, stop);
                         // Values of keys that no row sees were never written or belong to others: weights of zero do
                         // not silence a NaN there, so within the 16-key steps that are multiplied they become zero.
-                        const int key0 = w.first_key() + i * kPage;
+                        const int key0 = w.first_key + i * kPage;
                         const int lo = max(0, min(kPage, w.span.lo - key0)), hi = max(0, min(kPage, w.span.hi - key0));
                         const int step0 = lo >> 4, step1 = hi > lo ? (hi + 15) >> 4 : step0;
                         if (lo & 15 || hi & 15) {
@@ -851,17 +880,14 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             while (any) {
                 if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
                 const Item w = c.items[item % kItems];
-                const int pages = w.pages;
-                int lo_all, hi_all, unused;   // keys that all rows see
-                row_keys(p, w.q, w.last_token, lo_all, unused);
-                row_keys(p, w.q, w.first_token, unused, hi_all);
+                const int pages = w.pages, lo_all = w.lo_all, hi_all = w.hi_all;
                 uint32_t odd = 0;
                 for (int i = 0; i < pages; ++i) {
-                    const int key0 = w.first_key() + i * kPage;
+                    const int key0 = w.first_key + i * kPage;
                     for (int kv = 0; kv < 2; ++kv, ++n) {
                         const uint32_t slot = n % kRing;
                         if (!barrier_wait(kv_full(slot), (n / kRing) & 1, stop)) break;
-                        if (kv == 1 && w.first_token != w.last_token && (key0 < lo_all || key0 + kPage - 1 > hi_all)) {
+                        if (kv == 1 && w.pos != w.last_pos && (key0 < lo_all || key0 + kPage - 1 > hi_all)) {
                             // Two keys at a time: left of what all rows see, then right of it.
                             const int a = max(0, w.span.lo - key0), b = min(kPage, w.span.hi - key0);
                             for (int side = 0; side < 2; ++side) {
@@ -910,6 +936,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                          : "memory");
             return r != 0;
         };
+        const int token = row / p.group, g = row % p.group;   // within the tile
+        const int rel = token * p.heads * p.group + g;        // rows of the output from the tile's first
         uint32_t seen = 0, done = 0, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
         while (any) {
@@ -917,14 +945,10 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             const Item& w = c.items[item % kItems];
             const int pages = w.pages;
             const bool used = t == 0 || w.rows > rows_per_tile;
-            const int token = w.first_token + t * tokens + row / p.group;   // of the sequence's new ones
-            const bool valid = row < rows_per_tile && t * rows_per_tile + row < w.rows;
             int lo, hi;
-            row_keys(p, w.q, min(token, w.last_token), lo, hi);
-            int lo_all, hi_all, unused;
-            row_keys(p, w.q, w.last_token, lo_all, unused);
-            row_keys(p, w.q, w.first_token, unused, hi_all);
-            const int page_key = w.first_key(), first_key = page_key + half * 64;
+            w.keys(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
+            const int lo_all = w.lo_all, hi_all = w.hi_all;
+            const int page_key = w.first_key, first_key = page_key + half * 64;
             float m = -INFINITY, l = 0.0f;
             if (used) {
                 for (int i = 0; i < pages; ++i) {
@@ -1050,22 +1074,22 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             }
             ok = ok && barrier_wait(checked, item & 1, stop);
             tmem_fence_after();
-            const int cta0 = c.share.owner(w.tile_unit), cta1 = c.share.owner(w.tile_unit + w.span.pages - 1);
-            float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kTileSlot;
-            const bool split = cta1 > cta0;
+            const bool split = w.slot >= 0;
+            float* slot = p.slots + static_cast<int64_t>(w.slot) * kTileSlot;
+            // Output row of the tile's first row.
+            const int64_t out0 = static_cast<int64_t>(w.q0 + t * tokens) * p.heads * p.group + w.head * p.group;
+            const int valid_rows = min(rows_per_tile, w.rows - t * rows_per_tile);
             const bool by_definition = *static_cast<volatile int*>(&c.irregular) != 0;
             if (by_definition) {
-                const int ka = w.first_key(), kb = ka + pages * kPage;
-                for (int r = (warp & 3) * 32 + half; r < (warp & 3) * 32 + 32; r += 2) {
-                    const int tile_row = t * rows_per_tile + r;
-                    if (r >= rows_per_tile || tile_row >= w.rows) break;
-                    const int tok = w.first_token + tile_row / p.group, g = tile_row % p.group;
+                const int ka = page_key, kb = ka + pages * kPage;
+                for (int r = (warp & 3) * 32 + half; r < min((warp & 3) * 32 + 32, valid_rows); r += 2) {
+                    const int tok = t * tokens + r / p.group;
                     int a, b;
-                    row_keys(p, w.q, tok, a, b);
+                    w.keys(p, w.pos + tok, a, b);
                     float mm, ll;
                     float4 x;
-                    row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + tok) * p.q_token +
-                                                (w.head * p.group + g) * p.q_head,
+                    row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q0 + tok) * p.q_token +
+                                                (w.head * p.group + r % p.group) * p.q_head,
                                          p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, kb), mm, ll, x);
                     if (split) {
                         *reinterpret_cast<float4*>(slot + (t * 128 + r) * kDim + lane * 4) = x;
@@ -1075,7 +1099,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         }
                     } else {
                         const float inv = 1.0f / ll;
-                        const int64_t at = static_cast<int64_t>(w.q.q0 + tok) * p.heads * p.group + w.head * p.group + g;
+                        const int64_t at = out0 + r / p.group * p.heads * p.group + r % p.group;
                         uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
                         if (b < a) packed = make_uint2(0, 0);
                         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
@@ -1087,9 +1111,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 // Rows leave through a warp's own piece of shared memory, 64 bytes of each at a time, so that a store
                 // covers whole sectors: eight rows by four lanes.
                 const float inv = hi >= lo ? 1.0f / l : 0.0f;
-                const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + row % p.group;
                 const uint32_t stage = ring + kRing * kTileBytes + warp * kStageBytes;
-                const int valid_rows = min(rows_per_tile, w.rows - t * rows_per_tile) - (warp & 3) * 32;
+                const int valid = valid_rows - (warp & 3) * 32;
                 auto put = [&](const uint32_t (&x)[16]) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -1118,12 +1141,12 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         for (int k = 0; k < 4; ++k) {
                             const int r = k * 8 + (lane >> 2);
                             const uint4 x = get(r);
-                            if (r < valid_rows) *reinterpret_cast<uint4*>(part + r * kDim + d) = x;
+                            if (r < valid) *reinterpret_cast<uint4*>(part + r * kDim + d) = x;
                         }
                         __syncwarp();
                     }
                 } else {
-                    T* out = static_cast<T*>(p.out) + half * 64 + (lane & 3) * 8;
+                    T* out = static_cast<T*>(p.out) + out0 * kDim + half * 64 + (lane & 3) * 8;
 #pragma unroll 1
                     for (int d = 0; d < 64; d += 32) {
                         uint32_t o[32], x[16];
@@ -1136,30 +1159,23 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const int r = k * 8 + (lane >> 2);
-                            const int64_t to = __shfl_sync(0xffffffffu, at, r);
+                            const int64_t to = __shfl_sync(0xffffffffu, rel, r);
                             const uint4 y = get(r);
-                            if (r < valid_rows) *reinterpret_cast<uint4*>(out + to * kDim + d) = y;
+                            if (r < valid) *reinterpret_cast<uint4*>(out + to * kDim + d) = y;
                         }
                         __syncwarp();
                     }
                 }
-                if (valid && half == 0) {
+                if (row < valid_rows && half == 0) {
                     const float top = m * scale;
                     if (split) {
                         slot[kTileRows * kDim + t * 128 + row] = top;
                         slot[kTileRows * kDim + kTileRows + t * 128 + row] = l;
                     } else if (p.lse != nullptr) {
-                        p.lse[at] = hi >= lo ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                        p.lse[out0 + rel] = hi >= lo ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
                     }
                 }
                 tmem_fence_before();
-            }
-            // Only the first tile of a CTA can have begun in an earlier one.
-            if (tid == 0 && item == 0) {
-                Cut cut{};
-                if (split && cta0 < static_cast<int>(blockIdx.x) && w.page + pages == w.span.pages)
-                    cut = Cut{1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
-                p.cuts[blockIdx.x] = cut;
             }
             const bool last = !w.more;
             ++item;
