@@ -41,7 +41,7 @@ struct AttendParams {
     int32_t rows_min, rows_max;     // sequences with rows_min <= rows <= rows_max are this launch's
     int32_t causal, window;
     float scale_log2;               // scale * log2(e): the softmax runs in powers of two
-    uint32_t* counters;             // [grid], zero between launches
+    uint32_t* counters;             // three of each CTA, zero between launches
     uint32_t* status;
     Cut* cuts;                      // [grid]
     float* slots;                   // [2 * grid] partial results
@@ -473,7 +473,7 @@ __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q
 }
 
 // Weight of a partial result with maximum m in a whole with maximum top.
-__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.0f : exp2f(m - top); }
+__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.0f : exp2_approx(m - top); }
 #endif  // __CUDACC__
 
 }  // namespace paged

@@ -161,7 +161,9 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
         if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
             return -1;
         p.rows_max = tiles ? kFewRows : INT_MAX;
-        if (launch_attend_rows(k_map, v_map, p, max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4, pages->dtype, st) != 0) return -1;
+        // Beside tiles the few rows are mostly single tokens.
+        if (launch_attend_rows(k_map, v_map, p, tiles || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4, pages->dtype, st) != 0)
+            return -1;
         p.rows_min = kFewRows + 1;
         p.rows_max = INT_MAX;
     }

@@ -20,6 +20,41 @@ constexpr int kMaxGrid = 256;
 constexpr uint64_t kCutOffset = 4096;
 constexpr uint64_t kSlotOffset = kCutOffset + kMaxGrid * sizeof(Cut);
 
+// One row of n <= 32 partial results, by a warp: lane l gets values 4l .. 4l+3
+// of the sum, and all lanes the maximum and the sum of weights.  stats(i):
+// where piece i keeps the row's maximum, `sums` floats before its sum;
+// values(i): its 128 values.
+template <class Stats, class Values>
+__device__ __forceinline__ void join_row(int n, Stats stats, int sums, Values values, float4& x, float& top, float& sum)
+{
+    const int lane = threadIdx.x & 31;
+    const float m = lane < n ? __ldcg(stats(lane)) : -INFINITY, l = lane < n ? __ldcg(stats(lane) + sums) : 0.0f;
+    x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // The first values are on their way while the weights are found.
+    constexpr int kBatch = 6;
+    float4 y[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+        if (i < n) y[i] = __ldcg(reinterpret_cast<const float4*>(values(i)) + lane);
+    top = m;
+    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float f = join_weight(m, top);
+    sum = lane < n ? f * l : 0.0f;
+    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (i0 + i >= n) break;
+            const float w = __shfl_sync(0xffffffffu, f, i0 + i);
+            x.x += w * y[i].x;
+            x.y += w * y[i].y;
+            x.z += w * y[i].z;
+            x.w += w * y[i].w;
+            if (i0 + kBatch + i < n) y[i] = __ldcg(reinterpret_cast<const float4*>(values(i0 + kBatch + i)) + lane);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- few rows
 //
 // Single tokens and short drafts: at most 16 * kTiles rows per KV head and
@@ -42,6 +77,9 @@ constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRowTiles
                                2 * kRowsWarps * 16 * 4;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowsMinUnits = 1;
+// Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
+// more in a second step.
+constexpr int kJoinRows = 160;
 constexpr int kRowSlot = kMaxRowTiles * 16 * (kDim + 2);
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
@@ -382,33 +420,40 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         }
 
         if (split) {
-            // The last CTA of the tile joins its pieces.
-            __threadfence();
-            rows_sync();
-            const int pieces = cta1 - cta0 + 1;
-            if (tid == 0) last_piece = atomicInc(&p.counters[cta0], pieces - 1) == static_cast<uint32_t>(pieces - 1);
-            rows_sync();
-            if (last_piece) {
+            // Piece i of the tile is CTA cta0 + i's.  The last CTA to finish joins them; where that is much to read for
+            // one CTA, in two steps: the last of each group of neighbours joins these into its first, the last group
+            // those.  Either way in the order of the pieces.
+            const int pieces = cta1 - cta0 + 1, mine = static_cast<int>(blockIdx.x) - cta0;
+            auto slot_of = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cta0 + i) + (i == 0)) * kRowSlot; };
+            int group = pieces;
+            if (pieces * w.rows > kJoinRows || pieces > 32) {
+                group = 2;
+                while (group * group < pieces) ++group;
+            }
+            int first = mine / group * group, n = min(group, pieces - first), step = 1;
+            uint32_t* counter = &p.counters[2 * (cta0 + first) + (first == 0)];
+            for (;;) {
                 __threadfence();
-                auto piece = [&](int i) {
-                    return p.slots + static_cast<int64_t>(2 * (cta0 + i) + (i == 0)) * kRowSlot;
-                };
+                rows_sync();
+                if (tid == 0) last_piece = atomicInc(counter, n - 1) == static_cast<uint32_t>(n - 1);
+                rows_sync();
+                if (!last_piece) break;
+                __threadfence();
+                const bool final = step > 1 || n == pieces;
                 for (int r = warp; r < w.rows; r += kRowsWarps) {
-                    float top = -INFINITY;
-                    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(piece(i) + kRows * kDim + r));
-                    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float sum = 0.0f;
-#pragma unroll 4
-                    for (int i = 0; i < pieces; ++i) {
-                        const float* src = piece(i);
-                        const float f = join_weight(__ldcg(src + kRows * kDim + r), top);
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(src + r * kDim + lane * 4));
-                        sum += f * __ldcg(src + kRows * kDim + kRows + r);
-                        x.x += f * y.x;
-                        x.y += f * y.y;
-                        x.z += f * y.z;
-                        x.w += f * y.w;
+                    float4 x;
+                    float top, sum;
+                    join_row(
+                        n, [&](int i) { return slot_of(first + i * step) + kRows * kDim + r; }, kRows,
+                        [&](int i) { return slot_of(first + i * step) + r * kDim; }, x, top, sum);
+                    if (!final) {
+                        float* to = slot_of(first);
+                        *reinterpret_cast<float4*>(to + r * kDim + lane * 4) = x;
+                        if (lane == 0) {
+                            to[kRows * kDim + r] = top;
+                            to[kRows * kDim + kRows + r] = sum;
+                        }
+                        continue;
                     }
                     const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
                     int a, b;
@@ -421,6 +466,11 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     if (p.lse != nullptr && lane == 0)
                         p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
                 }
+                if (final) break;
+                first = 0;
+                step = group;
+                n = (pieces + group - 1) / group;
+                counter = &p.counters[2 * kMaxGrid + cta0];
             }
         }
         if (by_definition) {
@@ -1204,22 +1254,20 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     if (tile_row >= cut.rows) return;
     const int pieces = blockIdx.y - cut.cta0 + 1;
     const int r = tile_row < rows_per_tile ? tile_row : 128 + tile_row - rows_per_tile;
-    auto piece = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cut.cta0 + i) + (i == 0)) * kTileSlot; };
-    float top = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, piece(i)[kTileRows * kDim + r]);
-    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    // 32 pieces at a time.
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-        const float* src = piece(i);
-        const float f = join_weight(src[kTileRows * kDim + r], top);
-        const float4 y = *reinterpret_cast<const float4*>(src + r * kDim + lane * 4);
-        sum += f * src[kTileRows * kDim + kTileRows + r];
-        x.x += f * y.x;
-        x.y += f * y.y;
-        x.z += f * y.z;
-        x.w += f * y.w;
+    float sum = 0.0f, top = -INFINITY;
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+        auto piece = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cut.cta0 + i0 + i) + (i0 + i == 0)) * kTileSlot; };
+        float4 y;
+        float part_top, part_sum;
+        join_row(
+            min(32, pieces - i0), [&](int i) { return piece(i) + kTileRows * kDim + r; }, kTileRows,
+            [&](int i) { return piece(i) + r * kDim; }, y, part_top, part_sum);
+        const float both = fmaxf(top, part_top), f = join_weight(top, both), g = join_weight(part_top, both);
+        x = make_float4(f * x.x + g * y.x, f * x.y + g * y.y, f * x.z + g * y.z, f * x.w + g * y.w);
+        sum = f * sum + g * part_sum;
+        top = both;
     }
     const Seq s{cut.n, cut.kv, cut.q0};
     const int token = cut.token0 + tile_row / p.group, g = tile_row % p.group;
@@ -1345,7 +1393,7 @@ uint64_t attend_workspace_bytes()
 void attend_workspace(void* workspace, AttendParams* p)
 {
     p->counters = static_cast<uint32_t*>(workspace);
-    p->status = p->counters + kMaxGrid;
+    p->status = p->counters + 3 * kMaxGrid;
     p->cuts = reinterpret_cast<Cut*>(static_cast<char*>(workspace) + kCutOffset);
     p->slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotOffset);
 }
