@@ -233,7 +233,9 @@ __device__ __forceinline__ bool zero_sum_odd(uint32_t sum)
 // none).  All units of a launch in the order sequence, tile, head, page are cut
 // into equal consecutive shares, one per CTA: every CTA gets the same work
 // whatever the lengths, and a long axis is split where there are few rows.
-// Units are counted in 32 bits; the host refuses more.
+// What a tile takes besides its pages (its queries, its end) counts as `cost`
+// units more, before its pages.  Units are counted in 32 bits; the host refuses
+// more.
 struct Seq {
     int n, kv, q0;   // new tokens, all tokens, first new token
 };
@@ -288,13 +290,13 @@ struct Share {
 };
 
 struct Walk {
-    int rows_per_tile;
+    int rows_per_tile, cost;
     int s, tile, tiles, head;
     Seq q;
     Span span;
     int page;                            // next unit of the tile: 0 .. span.pages
     int first_token, last_token, rows;   // of the tile
-    int tile_unit;                       // number of the tile's first unit
+    int tile_unit;                       // number of the tile's first page
     int left;                            // units of this CTA not yet taken
 
     __device__ __forceinline__ int take() const { return min(left, span.pages - page); }
@@ -310,8 +312,9 @@ struct Walk {
     __device__ __forceinline__ void advance(const AttendParams& p, int taken)
     {
         left -= taken;
+        if (left > 0) left -= cost;
         if (left <= 0) return;
-        tile_unit += span.pages;
+        tile_unit += span.pages + cost;
         page = 0;
         if (++head < p.heads) return;
         head = 0;
@@ -332,20 +335,20 @@ struct Walk {
     }
 };
 
-__device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile)
+__device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost)
 {
     if (s.n == 0) return 0;
     int pages = 0;
     const int rows = s.n * p.group;
     for (int r = 0; r < rows; r += rows_per_tile)
-        pages += tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages;
+        pages += tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages + cost;
     return pages * p.heads;
 }
 
 // All threads of the block take part; `warp_sums` holds one value per warp.
 // At least min_units go to a CTA that has any, so short work is not split.
 template <int kThreads>
-__device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int min_units, Share* share,
+__device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int cost, int min_units, Share* share,
                                            int32_t* warp_sums)
 {
     constexpr int kWarps = kThreads / 32;
@@ -359,7 +362,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
         int base = 0;
         for (int s0 = 0; s0 < p.seqs; s0 += kThreads) {
             const int s = s0 + tid;
-            const int own = s < p.seqs ? seq_units(p, load_seq(p, s), rows_per_tile) : 0;
+            const int own = s < p.seqs ? seq_units(p, load_seq(p, s), rows_per_tile, cost) : 0;
             int sum = own;
             for (int d = 1; d < 32; d <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, sum, d);
@@ -401,10 +404,11 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
     }
 }
 
-__device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_tile, const Share& share)
+__device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_tile, int cost, const Share& share)
 {
     Walk w;
     w.rows_per_tile = rows_per_tile;
+    w.cost = cost;
     w.left = 0;
     if (share.seq < 0) return w;
     w.left = share.units;
@@ -414,16 +418,19 @@ __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_t
     w.tile = 0;
     w.tile_unit = share.seq_unit;
     w.set_tile(p);
-    int skip = share.begin - share.seq_unit;
-    while (skip >= w.span.pages * p.heads) {
-        skip -= w.span.pages * p.heads;
-        w.tile_unit += w.span.pages * p.heads;
+    int skip = share.begin - share.seq_unit, units = w.span.pages + cost;
+    while (skip >= units * p.heads) {
+        skip -= units * p.heads;
+        w.tile_unit += units * p.heads;
         ++w.tile;
         w.set_tile(p);
+        units = w.span.pages + cost;
     }
-    w.head = skip / w.span.pages;
-    w.page = skip - w.head * w.span.pages;
-    w.tile_unit += w.head * w.span.pages;
+    w.head = skip / units;
+    skip -= w.head * units;
+    w.tile_unit += w.head * units + cost;
+    w.page = max(0, skip - cost);
+    w.left = max(0, w.left - max(0, cost - skip));   // a share of nothing but cost has no page
     return w;
 }
 

@@ -72,11 +72,11 @@ constexpr int kQuarter = 32;                              // tokens of one TMA b
 constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 tokens][64 values]
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
 constexpr int kMaxRowTiles = 4;
-constexpr uint32_t kJoinBytes = kRowsWarps * 8 * 64 * 4;  // 8 rows x 64 columns of every warp
-constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRowTiles * 16 * 256 + kJoinBytes +
+constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRowTiles * 16 * 256 +
                                2 * kRowsWarps * 16 * 4;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowsMinUnits = 1;
+constexpr int kRowsCost = 1;   // pages that a tile's end is worth
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
 // more in a second step.
 constexpr int kJoinRows = 160;
@@ -135,8 +135,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     const uint32_t k_smem = smem_addr(base), v_smem = k_smem + kRowsStages * kPageTile;
     const uint32_t q_smem = v_smem + kRowsStages * kPageTile;
     uint8_t* q_bytes = base + 2 * kRowsStages * kPageTile;
-    float* join = reinterpret_cast<float*>(q_bytes + kMaxRowTiles * 16 * 256);
-    float* join_m = join + kJoinBytes / 4;
+    float* join_m = reinterpret_cast<float*>(q_bytes + kMaxRowTiles * 16 * 256);
     float* join_l = join_m + kRowsWarps * 16;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row_tile = warp / kSlices;
@@ -156,9 +155,9 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     wait_for_earlier_kernels();
-    find_share<kRowsThreads>(p, kRows, kRowsMinUnits, &share, warp_sums);
+    find_share<kRowsThreads>(p, kRows, kRowsCost, kRowsMinUnits, &share, warp_sums);
     dependents_may_launch();
-    Walk w = start_walk(p, kRows, share);
+    Walk w = start_walk(p, kRows, kRowsCost, share);
 
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
@@ -216,8 +215,9 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             }
             *reinterpret_cast<uint4*>(q_bytes + r * 256 + ((piece ^ (r & 7)) << 4)) = x;
         }
-        rows_sync();
-
+        const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
+        const bool split = cta1 > cta0;
+        float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
         int lo[2], hi[2];   // keys that this thread's rows see
         int all_lo, all_hi; // keys that every row of the tile sees
         {
@@ -236,42 +236,60 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[d][c] = 0.0f;
         const bool idle = row_tile * 16 >= w.rows;   // no row of this warp's sixteen is used
+        rows_sync();
 
         for (int i = 0; i < pages; ++i, ++unit) {
             const int stage = unit % kRowsStages;
             const uint32_t parity = unit / kRowsStages & 1;
-            const int page_key = (w.span.first + w.page + i) * kPage;
-            if (!barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop)) break;
+            // This warp's 16 kTiles keys of the page.
+            const int first16 = warp % kSlices * kTiles, key0 = (w.span.first + w.page + i) * kPage + first16 * 16;
+            if (!barrier_wait(k_full(stage), parity, &stop)) break;
+            const bool mine = !idle && key0 < w.span.hi && key0 + 16 * kTiles > w.span.lo;
+            const bool whole = key0 >= all_lo && key0 + 16 * kTiles - 1 <= all_hi;
+            auto slice = [&](int sub) {
+                return stage * kPageTile + ((first16 + sub) >> 1) * kQuarterBytes + ((first16 + sub) & 1) * 16 * 128;
+            };
+            uint32_t weight[kTiles][4];
+            if (mine) {
+                // One chain of products per eight keys; where there are few, two of them.
+                constexpr int kChains = kTiles == 1 ? 2 : 1;
+                float s[kTiles][2][4], s2[2][4];
 #pragma unroll
-            for (int sub = 0; sub < kTiles; ++sub) {
-                const int slot16 = (warp % kSlices) * kTiles + sub, key0 = page_key + slot16 * 16;
-                if (idle || key0 >= w.span.hi || key0 + 16 <= w.span.lo) continue;
-                const uint32_t slice = stage * kPageTile + (slot16 >> 1) * kQuarterBytes + (slot16 & 1) * 16 * 128;
-                const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
-                float s[2][4] = {};
+                for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                    for (int sub = 0; sub < kTiles; ++sub) s[sub][0][c] = s[sub][1][c] = 0.0f;
+                    s2[0][c] = s2[1][c] = 0.0f;
+                }
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {   // 16 values of the head at a time
-                    uint32_t a[4], b[4];
-                    const int key = (lane & 7) + ((lane >> 4) << 3), chunk = (d & 3) * 2 + ((lane >> 3) & 1);
-                    ldmatrix4(b, k_smem + slice + (d >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
+                    uint32_t q[4];
                     const int r = row_tile * 16 + (lane & 15), piece = d * 2 + (lane >> 4);
-                    ldmatrix4(a, q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
-                    mma16816<T>(s[0], a, b[0], b[1]);
-                    mma16816<T>(s[1], a, b[2], b[3]);
+                    ldmatrix4(q, q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int sub = 0; sub < kTiles; ++sub) {
+                        uint32_t b[4];
+                        const int key = (lane & 7) + ((lane >> 4) << 3), chunk = (d & 3) * 2 + ((lane >> 3) & 1);
+                        ldmatrix4(b, k_smem + slice(sub) + (d >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
+                        const bool second = kChains == 2 && (d & 1);
+                        mma16816<T>(second ? s2[0] : s[sub][0], q, b[0], b[1]);
+                        mma16816<T>(second ? s2[1] : s[sub][1], q, b[2], b[3]);
+                    }
                 }
                 float top[2] = {m[0], m[1]};
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int sub = 0; sub < kTiles; ++sub)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float x = s[n][c] * p.scale_log2;
-                        if (!whole) {
-                            const int key = key0 + n * 8 + (lane & 3) * 2 + (c & 1);
-                            if (key < lo[c >> 1] || key > hi[c >> 1]) x = -INFINITY;
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float x = (kChains == 2 ? s[sub][n][c] + s2[n][c] : s[sub][n][c]) * p.scale_log2;
+                            if (!whole) {
+                                const int key = key0 + sub * 16 + n * 8 + (lane & 3) * 2 + (c & 1);
+                                if (key < lo[c >> 1] || key > hi[c >> 1]) x = -INFINITY;
+                            }
+                            s[sub][n][c] = x;
+                            top[c >> 1] = fmaxf(top[c >> 1], x);
                         }
-                        s[n][c] = x;
-                        top[c >> 1] = fmaxf(top[c >> 1], x);
-                    }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
@@ -291,47 +309,54 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     }
                 }
                 const float base0 = top[0] == -INFINITY ? 0.0f : top[0], base1 = top[1] == -INFINITY ? 0.0f : top[1];
-                uint32_t weight[4];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float e0 = exp2_approx(s[n][0] - base0), e1 = exp2_approx(s[n][1] - base0);
-                    const float e2 = exp2_approx(s[n][2] - base1), e3 = exp2_approx(s[n][3] - base1);
-                    l[0] += e0 + e1;
-                    l[1] += e2 + e3;
-                    // Weights are rounded to the cache's type for the product; their sum is not.
-                    weight[2 * n] = pack2<T>(e0, e1);
-                    weight[2 * n + 1] = pack2<T>(e2, e3);
-                }
-                uint32_t keep[2] = {0, 0};   // values of keys that some row sees: this lane's keys 2t, 2t + 1 and 8 more
+                for (int sub = 0; sub < kTiles; ++sub)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int key = key0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
-                    if (key >= w.span.lo && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
-                }
+                    for (int n = 0; n < 2; ++n) {
+                        const float e0 = exp2_approx(s[sub][n][0] - base0), e1 = exp2_approx(s[sub][n][1] - base0);
+                        const float e2 = exp2_approx(s[sub][n][2] - base1), e3 = exp2_approx(s[sub][n][3] - base1);
+                        l[0] += e0 + e1;
+                        l[1] += e2 + e3;
+                        // Weights are rounded to the cache's type for the product; their sum is not.
+                        weight[sub][2 * n] = pack2<T>(e0, e1);
+                        weight[sub][2 * n + 1] = pack2<T>(e2, e3);
+                    }
+            }
+            if (!barrier_wait(v_full(stage), parity, &stop)) break;
+            if (mine) {
                 uint32_t odd = 0;
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    uint32_t b[4];
-                    const int key = lane & 15, chunk = (d & 3) * 2 + (lane >> 4);
-                    ldmatrix4_trans(b, v_smem + slice + (d >> 2) * (kQuarterBytes / 2) + key * 128 +
-                                           ((chunk ^ (key & 7)) << 4));
-                    if (!whole) {
+                for (int sub = 0; sub < kTiles; ++sub) {
+                    uint32_t keep[2] = {0, 0};   // values of keys that some row sees: this lane's keys 2t, 2t + 1, and 8 more
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            b[j] &= keep[j & 1];
-                            odd = zero_sum<T>(odd, b[j]);
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = key0 + sub * 16 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
+                        if (key >= w.span.lo && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
                     }
-                    mma16816<T>(o[2 * d], weight, b[0], b[1]);
-                    mma16816<T>(o[2 * d + 1], weight, b[2], b[3]);
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) {
+                        uint32_t b[4];
+                        const int key = lane & 15, chunk = (d & 3) * 2 + (lane >> 4);
+                        ldmatrix4_trans(b, v_smem + slice(sub) + (d >> 2) * (kQuarterBytes / 2) + key * 128 +
+                                               ((chunk ^ (key & 7)) << 4));
+                        if (!whole) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                b[j] &= keep[j & 1];
+                                odd = zero_sum<T>(odd, b[j]);
+                            }
+                        }
+                        mma16816<T>(o[2 * d], weight[sub], b[0], b[1]);
+                        mma16816<T>(o[2 * d + 1], weight[sub], b[2], b[3]);
+                    }
                 }
-                if (w.first_token != w.last_token && zero_sum_odd<T>(odd)) irregular = 1;
+                if (!whole && w.first_token != w.last_token && zero_sum_odd<T>(odd)) irregular = 1;
             }
             __syncwarp();
-            if (lane == 0) barrier_arrive(empty(stage));
+            if (lane == 0 && i + 1 < pages) barrier_arrive(empty(stage));
         }
 
-        // Join the warps' results.
+        // Join the warps' results where the last page lay: its buffers are given back afterwards.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -344,80 +369,76 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (tid == 0) give_up = stop;
         rows_sync();
         if (give_up) break;
-        const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
-        const bool split = cta1 > cta0;
-        float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
+        const int last_stage = (unit - 1) % kRowsStages;
         const bool by_definition = irregular != 0;
-
-        auto emit2 = [&](int r, int col, float2 x, float mm, float ll) {
-            if (split) {
-                *reinterpret_cast<float2*>(slot + r * kDim + col) = x;
-                if (col == 0) {
-                    slot[kRows * kDim + r] = mm;
-                    slot[kRows * kDim + kRows + r] = ll;
-                }
-                return;
-            }
-            const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
-            int a, b;
-            row_keys(p, w.q, token, a, b);
-            const float inv = 1.0f / ll;
-            const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + g;
-            *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at * kDim + col) =
-                b >= a ? pack2<T>(x.x * inv, x.y * inv) : 0u;
-            if (p.lse != nullptr && col == 0)
-                p.lse[at] = b >= a ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
-        };
-
-        if (!by_definition) {
+        // Warp i's [16 rows][128] floats, columns swizzled by the row against bank conflicts.
+        auto joined = [&](int i) { return base + ((i < 4 ? 0 : kRowsStages) + last_stage) * kPageTile + (i & 3) * 8192; };
+        if (!idle) {
+            uint8_t* to = joined(warp) + (lane >> 2) * 512;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (h * 8 >= w.rows) continue;   // the same for all threads
+                if (row_tile * 16 + h * 8 >= w.rows) break;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                    for (int d = 0; d < 8; ++d)
-                        *reinterpret_cast<float2*>(join + warp * 512 + (lane >> 2) * 64 + d * 8 + (lane & 3) * 2) =
-                            make_float2(o[half * 8 + d][2 * h], o[half * 8 + d][2 * h + 1]);
-                    rows_sync();
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        const int r = t * 16 + h * 8 + warp;
-                        if (r >= w.rows) continue;
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int i = t * kSlices; i < (t + 1) * kSlices; ++i)
-                            top = fmaxf(top, join_m[i * 16 + h * 8 + warp]);
-                        float2 x = make_float2(0.0f, 0.0f);
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int i = t * kSlices; i < (t + 1) * kSlices; ++i) {
-                            const float f = join_weight(join_m[i * 16 + h * 8 + warp], top);
-                            const float2 y = *reinterpret_cast<const float2*>(join + i * 512 + warp * 64 + lane * 2);
-                            sum += f * join_l[i * 16 + h * 8 + warp];
-                            x.x += f * y.x;
-                            x.y += f * y.y;
-                        }
-                        emit2(r, half * 64 + lane * 2, x, top, sum);
-                    }
-                    rows_sync();
-                }
-            }
-        } else {
-            const int ka = (w.span.first + w.page) * kPage, kb = ka + pages * kPage;
-            for (int r = warp; r < w.rows; r += kRowsWarps) {
-                const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
-                int a, b;
-                row_keys(p, w.q, token, a, b);
-                float mm, ll;
-                float4 x;
-                row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
-                                            (w.head * p.group + g) * p.q_head,
-                                     p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, kb), mm, ll, x);
-                emit2(r, lane * 4, make_float2(x.x, x.y), mm, ll);
-                emit2(r, lane * 4 + 2, make_float2(x.z, x.w), mm, ll);
+                for (int d = 0; d < 16; ++d)
+                    *reinterpret_cast<float2*>(to + h * 4096 + ((d * 8 + (lane & 3) * 2) ^ ((lane >> 2 & 3) << 3)) * 4) =
+                        make_float2(o[d][2 * h], o[d][2 * h + 1]);
             }
         }
+        rows_sync();
+#pragma unroll 1
+        for (int r = warp; r < w.rows; r += kRowsWarps) {
+            const int token = (r0 + r) / p.group, g = (r0 + r) - token * p.group;
+            int a, b;
+            row_keys(p, w.q, token, a, b);
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float top, sum;
+            if (by_definition) {
+                const int ka = (w.span.first + w.page) * kPage;
+                row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
+                                            (w.head * p.group + g) * p.q_head,
+                                     p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, ka + pages * kPage), top,
+                                     sum, x);
+            } else {
+                const int from = (r >> 4) * kSlices, row = r & 15;
+                const int stat = (from + (lane & (kSlices - 1))) * 16 + row;
+                const float mi = join_m[stat];
+                top = mi;
+#pragma unroll
+                for (int d = 1; d < kSlices; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float f = join_weight(mi, top);
+                sum = f * join_l[stat];
+#pragma unroll
+                for (int d = 1; d < kSlices; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+#pragma unroll
+                for (int i = 0; i < kSlices; ++i) {
+                    const float wi = __shfl_sync(0xffffffffu, f, i);
+                    const float4 y = *reinterpret_cast<const float4*>(joined(from + i) + row * 512 + ((lane * 4) ^ ((row & 3) << 3)) * 4);
+                    x.x += wi * y.x;
+                    x.y += wi * y.y;
+                    x.z += wi * y.z;
+                    x.w += wi * y.w;
+                }
+            }
+            if (split) {
+                *reinterpret_cast<float4*>(slot + r * kDim + lane * 4) = x;
+                if (lane == 0) {
+                    slot[kRows * kDim + r] = top;
+                    slot[kRows * kDim + kRows + r] = sum;
+                }
+            } else {
+                const float inv = 1.0f / sum;
+                const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + g;
+                uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+                if (b < a) packed = make_uint2(0, 0);
+                *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
+                if (p.lse != nullptr && lane == 0)
+                    p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+            }
+        }
+        // Reads and writes of this page's buffers come before the next copy into them.
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive(empty(last_stage));
 
         if (split) {
             // Piece i of the tile is CTA cta0 + i's.  The last CTA to finish joins them; where that is much to read for
@@ -505,6 +526,7 @@ constexpr int kItems = 8;
 constexpr int kTileRows = 256;
 constexpr int kTileSlot = kTileRows * (kDim + 2);
 constexpr float kRescale = 8.0f;
+constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
 
 template <int kCols>
 __device__ __forceinline__ void tmem_load(uint32_t (&r)[kCols], uint32_t addr);
@@ -742,18 +764,18 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads>(p, 2 * rows_per_tile, 1, &c.share, c.warp_sums);
+    find_share<kTileThreads>(p, 2 * rows_per_tile, kTilesCost, 1, &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
-    const bool any = c.share.seq >= 0;
+    Walk w = start_walk(p, 2 * rows_per_tile, kTilesCost, c.share);
+    const bool any = w.left > 0;
 
     // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.
     if (warp >= kSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == kSoftWarps) {
             // Producer.
-            Walk w = start_walk(p, 2 * rows_per_tile, c.share);
             uint32_t n = 0, item = 0;
             while (w.left > 0 && !*stop) {
                 const int pages = w.take();
@@ -775,7 +797,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     it.q0 = w.q.q0 + w.first_token;
                     const int cta0 = c.share.owner(w.tile_unit), cta1 = c.share.owner(w.tile_unit + w.span.pages - 1);
                     it.slot = cta1 > cta0 ? 2 * static_cast<int>(blockIdx.x) + (cta0 == static_cast<int>(blockIdx.x)) : -1;
-                    it.more = w.left > pages;
+                    it.more = w.left > pages + w.cost;
                     barrier_arrive(item_full(item));
                     // Only the first tile of a CTA can have begun in an earlier one.
                     if (item == 0) {
