@@ -79,7 +79,7 @@ bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, const int64_t* st
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr uint32_t kFewRows = 64;
+constexpr uint32_t kFewRows = 32;
 
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)
 {
@@ -162,8 +162,8 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
             return -1;
         p.rows_max = tiles ? kFewRows : INT_MAX;
         // Beside tiles the few rows are mostly single tokens.
-        if (launch_attend_rows(k_map, v_map, p, tiles || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4, pages->dtype, st) != 0)
-            return -1;
+        const uint64_t rows = tiles ? group : max_rows;
+        if (launch_attend_rows(k_map, v_map, p, rows <= 8 ? 8 : rows <= 16 ? 16 : 32, pages->dtype, st) != 0) return -1;
         p.rows_min = kFewRows + 1;
         p.rows_max = INT_MAX;
     }

@@ -57,30 +57,33 @@ __device__ __forceinline__ void join_row(int n, Stats stats, int sums, Values va
 
 // ---------------------------------------------------------------- few rows
 //
-// Single tokens and short drafts: at most 16 * kTiles rows per KV head and
-// tile, bound by reading K and V once.  One CTA per SM; a producer warp keeps
-// three pages (64 KiB each, K and V) in flight by TMA; each of eight warps takes
-// 16 rows and a slice of each page's keys: scores by m16n8k16 with the rows as
-// M, their own running maximum and sum, and the values' product, so no warp
-// waits for another inside the loop.  The results join in shared memory at the tile's end,
-// and a tile cut over several CTAs is joined by the last of them to finish, in
-// the order of the cuts, so results do not depend on the order of arrival.
+// Single tokens and short drafts: up to 32 rows per KV head and tile, bound by
+// reading K and V once.  One CTA per SM; a producer warp keeps three pages
+// (64 KiB each, K and V) in flight by TMA.  Each of eight warps takes up to 16
+// rows and a slice of each page's keys, with its own running maximum and sum,
+// so no warp waits for another inside the loop.  The products are m16n8k16 with
+// the keys (then the values of a head) as M and eight rows as N: a group of
+// eight query heads or fewer fills one N, where rows as M would pad them to
+// sixteen, and these instructions are slow enough here to matter (about 20
+// clocks of a quarter SM).  The results join in shared memory at the tile's
+// end, and a tile cut over several CTAs is joined by the last of them to
+// finish, in the order of the cuts, so results do not depend on the order of
+// arrival.
 constexpr int kRowsWarps = 8;
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 constexpr int kRowsStages = 3;
 constexpr int kQuarter = 32;                              // tokens of one TMA box
 constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 tokens][64 values]
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
-constexpr int kMaxRowTiles = 4;
-constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRowTiles * 16 * 256 +
-                               2 * kRowsWarps * 16 * 4;
+constexpr int kMaxRows = 32;
+constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRows * 256 + 2 * kRowsWarps * 16 * 4;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowsMinUnits = 1;
 constexpr int kRowsCost = 1;   // pages that a tile's end is worth
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
 // more in a second step.
 constexpr int kJoinRows = 160;
-constexpr int kRowSlot = kMaxRowTiles * 16 * (kDim + 2);
+constexpr int kRowSlot = kMaxRows * (kDim + 2);
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -114,16 +117,25 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// An 8 x 8 block of pairs of 16-bit values, transposed over the warp.
+__device__ __forceinline__ uint32_t transposed(uint32_t x)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
 // Barrier of the eight computing warps.
 __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory"); }
 
-template <typename T, int kTiles>
+// kNs groups of eight rows per warp; the warps hold kTiles times that many rows.
+template <typename T, int kNs, int kTiles>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                          const __grid_constant__ AttendParams p)
 {
-    constexpr int kRows = 16 * kTiles;            // eight warps: kTiles times 16 rows, kSlices slices of a page's keys
-    constexpr int kSlices = kRowsWarps / kTiles;
+    constexpr int kWarpRows = 8 * kNs, kRows = kWarpRows * kTiles;
+    constexpr int kSlices = kRowsWarps / kTiles;   // of a page's keys
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
     __shared__ Share share;
@@ -135,7 +147,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     const uint32_t k_smem = smem_addr(base), v_smem = k_smem + kRowsStages * kPageTile;
     const uint32_t q_smem = v_smem + kRowsStages * kPageTile;
     uint8_t* q_bytes = base + 2 * kRowsStages * kPageTile;
-    float* join_m = reinterpret_cast<float*>(q_bytes + kMaxRowTiles * 16 * 256);
+    float* join_m = reinterpret_cast<float*>(q_bytes + kMaxRows * 256);
     float* join_l = join_m + kRowsWarps * 16;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row_tile = warp / kSlices;
@@ -218,137 +230,126 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
         const bool split = cta1 > cta0;
         float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
-        int lo[2], hi[2];   // keys that this thread's rows see
-        int all_lo, all_hi; // keys that every row of the tile sees
+        int lo[kNs][2], hi[kNs][2];   // keys that this thread's rows see
+        int all_lo, all_hi;           // keys that every row of the tile sees
         {
             int unused;
             row_keys(p, w.q, w.last_token, all_lo, unused);
             row_keys(p, w.q, w.first_token, unused, all_hi);
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = row_tile * 16 + h * 8 + (lane >> 2);
-            row_keys(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[h], hi[h]);
+        for (int n = 0; n < kNs; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = row_tile * kWarpRows + n * 8 + (lane & 3) * 2 + e;
+                row_keys(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[n][e], hi[n][e]);
+            }
+        // Sums of values: o[j][n] holds values 16 j + lane / 4 (+ 8) of rows 8 n + 2 (lane % 4) (+ 1).
+        float m[kNs][2], l[kNs][2], o[8][kNs][4];
+#pragma unroll
+        for (int n = 0; n < kNs; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[j][n][c] = 0.0f;
         }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[16][4];
-#pragma unroll
-        for (int d = 0; d < 16; ++d)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[d][c] = 0.0f;
-        const bool idle = row_tile * 16 >= w.rows;   // no row of this warp's sixteen is used
+        const bool idle = row_tile * kWarpRows >= w.rows;   // no row of this warp's is used
         rows_sync();
+        uint32_t q[kNs][4][4];   // 32 values of eight rows each
+#pragma unroll
+        for (int n = 0; n < kNs; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int r = row_tile * kWarpRows + n * 8 + (lane & 7), piece = d * 4 + (lane >> 3);
+                ldmatrix4(q[n][d], q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
+            }
 
         for (int i = 0; i < pages; ++i, ++unit) {
             const int stage = unit % kRowsStages;
             const uint32_t parity = unit / kRowsStages & 1;
-            // This warp's 16 kTiles keys of the page.
-            const int first16 = warp % kSlices * kTiles, key0 = (w.span.first + w.page + i) * kPage + first16 * 16;
-            if (!barrier_wait(k_full(stage), parity, &stop)) break;
-            const bool mine = !idle && key0 < w.span.hi && key0 + 16 * kTiles > w.span.lo;
-            const bool whole = key0 >= all_lo && key0 + 16 * kTiles - 1 <= all_hi;
-            auto slice = [&](int sub) {
-                return stage * kPageTile + ((first16 + sub) >> 1) * kQuarterBytes + ((first16 + sub) & 1) * 16 * 128;
-            };
-            uint32_t weight[kTiles][4];
-            if (mine) {
-                // One chain of products per eight keys; where there are few, two of them.
-                constexpr int kChains = kTiles == 1 ? 2 : 1;
-                float s[kTiles][2][4], s2[2][4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                    for (int sub = 0; sub < kTiles; ++sub) s[sub][0][c] = s[sub][1][c] = 0.0f;
-                    s2[0][c] = s2[1][c] = 0.0f;
-                }
+            const int page_key = (w.span.first + w.page + i) * kPage;
+            if (!barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop)) break;
+#pragma unroll 1
+            for (int sub = 0; sub < kTiles; ++sub) {
+                // 16 keys.
+                const int first16 = warp % kSlices * kTiles + sub, key0 = page_key + first16 * 16;
+                if (idle || key0 >= w.span.hi || key0 + 16 <= w.span.lo) continue;
+                const uint32_t slice = stage * kPageTile + (first16 >> 1) * kQuarterBytes + (first16 & 1) * 16 * 128;
+                const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
+                float s[kNs][2][4] = {};   // two chains of products
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {   // 16 values of the head at a time
-                    uint32_t q[4];
-                    const int r = row_tile * 16 + (lane & 15), piece = d * 2 + (lane >> 4);
-                    ldmatrix4(q, q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
+                    uint32_t a[4];
+                    const int key = lane & 15, chunk = (d & 3) * 2 + (lane >> 4);
+                    ldmatrix4(a, k_smem + slice + (d >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
 #pragma unroll
-                    for (int sub = 0; sub < kTiles; ++sub) {
-                        uint32_t b[4];
-                        const int key = (lane & 7) + ((lane >> 4) << 3), chunk = (d & 3) * 2 + ((lane >> 3) & 1);
-                        ldmatrix4(b, k_smem + slice(sub) + (d >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
-                        const bool second = kChains == 2 && (d & 1);
-                        mma16816<T>(second ? s2[0] : s[sub][0], q, b[0], b[1]);
-                        mma16816<T>(second ? s2[1] : s[sub][1], q, b[2], b[3]);
-                    }
+                    for (int n = 0; n < kNs; ++n)
+                        mma16816<T>(s[n][d & 1], a, q[n][d >> 1][(d & 1) * 2], q[n][d >> 1][(d & 1) * 2 + 1]);
                 }
-                float top[2] = {m[0], m[1]};
+                uint32_t weight[kNs][2];
 #pragma unroll
-                for (int sub = 0; sub < kTiles; ++sub)
+                for (int n = 0; n < kNs; ++n) {
+                    float x[4], top[2] = {m[n][0], m[n][1]};
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int c = 0; c < 4; ++c) {
+                        x[c] = (s[n][0][c] + s[n][1][c]) * p.scale_log2;
+                        if (!whole) {
+                            const int key = key0 + (lane >> 2) + (c >> 1) * 8;
+                            if (key < lo[n][c & 1] || key > hi[n][c & 1]) x[c] = -INFINITY;
+                        }
+                        top[c & 1] = fmaxf(top[c & 1], x[c]);
+                    }
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float x = (kChains == 2 ? s[sub][n][c] + s2[n][c] : s[sub][n][c]) * p.scale_log2;
-                            if (!whole) {
-                                const int key = key0 + sub * 16 + n * 8 + (lane & 3) * 2 + (c & 1);
-                                if (key < lo[c >> 1] || key > hi[c >> 1]) x = -INFINITY;
+                    for (int d = 4; d < 32; d <<= 1) {
+                        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+                        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+                    }
+                    if (__any_sync(0xffffffffu, top[0] != m[n][0] || top[1] != m[n][1])) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float f = m[n][e] == top[e] ? 1.0f : exp2_approx(m[n][e] - top[e]);
+                            m[n][e] = top[e];
+                            l[n][e] *= f;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                o[j][n][e] *= f;
+                                o[j][n][e + 2] *= f;
                             }
-                            s[sub][n][c] = x;
-                            top[c >> 1] = fmaxf(top[c >> 1], x);
-                        }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                }
-                if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float f = m[h] == top[h] ? 1.0f : exp2_approx(m[h] - top[h]);
-                        m[h] = top[h];
-                        l[h] *= f;
-#pragma unroll
-                        for (int d = 0; d < 16; ++d) {
-                            o[d][2 * h] *= f;
-                            o[d][2 * h + 1] *= f;
                         }
                     }
+                    const float base0 = top[0] == -INFINITY ? 0.0f : top[0], base1 = top[1] == -INFINITY ? 0.0f : top[1];
+                    const float e0 = exp2_approx(x[0] - base0), e1 = exp2_approx(x[1] - base1);
+                    const float e2 = exp2_approx(x[2] - base0), e3 = exp2_approx(x[3] - base1);
+                    l[n][0] += e0 + e2;
+                    l[n][1] += e1 + e3;
+                    // Weights are rounded to the cache's type for the product; their sum is not.  Keys by rows become
+                    // rows by keys.
+                    weight[n][0] = transposed(pack2<T>(e0, e1));
+                    weight[n][1] = transposed(pack2<T>(e2, e3));
                 }
-                const float base0 = top[0] == -INFINITY ? 0.0f : top[0], base1 = top[1] == -INFINITY ? 0.0f : top[1];
+                uint32_t keep[2] = {0, 0};   // values of keys that some row sees: this lane's keys 2t, 2t + 1, and 8 more
 #pragma unroll
-                for (int sub = 0; sub < kTiles; ++sub)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const float e0 = exp2_approx(s[sub][n][0] - base0), e1 = exp2_approx(s[sub][n][1] - base0);
-                        const float e2 = exp2_approx(s[sub][n][2] - base1), e3 = exp2_approx(s[sub][n][3] - base1);
-                        l[0] += e0 + e1;
-                        l[1] += e2 + e3;
-                        // Weights are rounded to the cache's type for the product; their sum is not.
-                        weight[sub][2 * n] = pack2<T>(e0, e1);
-                        weight[sub][2 * n + 1] = pack2<T>(e2, e3);
-                    }
-            }
-            if (!barrier_wait(v_full(stage), parity, &stop)) break;
-            if (mine) {
+                for (int j = 0; j < 4; ++j) {
+                    const int key = key0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
+                    if (key >= w.span.lo && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
+                }
                 uint32_t odd = 0;
 #pragma unroll
-                for (int sub = 0; sub < kTiles; ++sub) {
-                    uint32_t keep[2] = {0, 0};   // values of keys that some row sees: this lane's keys 2t, 2t + 1, and 8 more
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t a[4];
+                    const int key = (lane & 7) + ((lane >> 4) << 3), chunk = (j & 3) * 2 + ((lane >> 3) & 1);
+                    ldmatrix4_trans(a, v_smem + slice + (j >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
+                    if (!whole) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int key = key0 + sub * 16 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
-                        if (key >= w.span.lo && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
-                    }
-#pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        uint32_t b[4];
-                        const int key = lane & 15, chunk = (d & 3) * 2 + (lane >> 4);
-                        ldmatrix4_trans(b, v_smem + slice(sub) + (d >> 2) * (kQuarterBytes / 2) + key * 128 +
-                                               ((chunk ^ (key & 7)) << 4));
-                        if (!whole) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                b[j] &= keep[j & 1];
-                                odd = zero_sum<T>(odd, b[j]);
-                            }
+                        for (int c = 0; c < 4; ++c) {
+                            a[c] &= keep[c >> 1];
+                            odd = zero_sum<T>(odd, a[c]);
                         }
-                        mma16816<T>(o[2 * d], weight[sub], b[0], b[1]);
-                        mma16816<T>(o[2 * d + 1], weight[sub], b[2], b[3]);
                     }
+#pragma unroll
+                    for (int n = 0; n < kNs; ++n) mma16816<T>(o[j][n], a, weight[n][0], weight[n][1]);
                 }
                 if (!whole && w.first_token != w.last_token && zero_sum_odd<T>(odd)) irregular = 1;
             }
@@ -358,14 +359,16 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 
         // Join the warps' results where the last page lay: its buffers are given back afterwards.
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if ((lane & 3) == 0) {
-                join_m[warp * 16 + h * 8 + (lane >> 2)] = m[h];
-                join_l[warp * 16 + h * 8 + (lane >> 2)] = l[h];
+        for (int n = 0; n < kNs; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+                if (lane < 4) {
+                    join_m[warp * 16 + n * 8 + lane * 2 + e] = m[n][e];
+                    join_l[warp * 16 + n * 8 + lane * 2 + e] = l[n][e];
+                }
             }
-        }
         if (tid == 0) give_up = stop;
         rows_sync();
         if (give_up) break;
@@ -374,15 +377,16 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         // Warp i's [16 rows][128] floats, columns swizzled by the row against bank conflicts.
         auto joined = [&](int i) { return base + ((i < 4 ? 0 : kRowsStages) + last_stage) * kPageTile + (i & 3) * 8192; };
         if (!idle) {
-            uint8_t* to = joined(warp) + (lane >> 2) * 512;
+            uint8_t* to = joined(warp);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (row_tile * 16 + h * 8 >= w.rows) break;
+            for (int n = 0; n < kNs; ++n)
 #pragma unroll
-                for (int d = 0; d < 16; ++d)
-                    *reinterpret_cast<float2*>(to + h * 4096 + ((d * 8 + (lane & 3) * 2) ^ ((lane >> 2 & 3) << 3)) * 4) =
-                        make_float2(o[d][2 * h], o[d][2 * h + 1]);
-            }
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int r = n * 8 + (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
+                        *reinterpret_cast<float*>(to + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][n][c];
+                    }
         }
         rows_sync();
 #pragma unroll 1
@@ -399,7 +403,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                                      p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, ka + pages * kPage), top,
                                      sum, x);
             } else {
-                const int from = (r >> 4) * kSlices, row = r & 15;
+                const int from = r / kWarpRows * kSlices, row = r % kWarpRows;
                 const int stat = (from + (lane & (kSlices - 1))) * 16 + row;
                 const float mi = join_m[stat];
                 top = mi;
@@ -412,7 +416,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
                 for (int i = 0; i < kSlices; ++i) {
                     const float wi = __shfl_sync(0xffffffffu, f, i);
-                    const float4 y = *reinterpret_cast<const float4*>(joined(from + i) + row * 512 + ((lane * 4) ^ ((row & 3) << 3)) * 4);
+                    const float4 y = *reinterpret_cast<const float4*>(joined(from + i) + row * 512 + ((lane * 4) ^ ((row >> 1 & 3) << 3)) * 4);
                     x.x += wi * y.x;
                     x.y += wi * y.y;
                     x.z += wi * y.z;
@@ -1305,13 +1309,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
 
 struct Device {
     int sms = 0;
-    bool rows_set[2][kMaxRowTiles] = {};
+    bool rows_set[2][3] = {};
     bool tiles_set[2] = {};
 };
 std::mutex g_mu;
 Device g_devices[64];
 
-template <typename T, int kTiles>
+template <typename T, int kNs, int kTiles>
 int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, cudaStream_t stream)
 {
     int dev = 0;
@@ -1321,9 +1325,9 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
         if (d.sms == 0) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-        bool& set = d.rows_set[std::is_same<T, __half>::value][kTiles - 1];
+        bool& set = d.rows_set[std::is_same<T, __half>::value][kNs + kTiles - 2];
         if (!set) {
-            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, kTiles>,
+            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, kNs, kTiles>,
                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
             if (e != cudaSuccess) return e;
             set = true;
@@ -1341,7 +1345,15 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     ProfileScope prof(kKernAttendRows, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, kTiles>, k_map, v_map, p);
+    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, kNs, kTiles>, k_map, v_map, p);
+}
+
+template <typename T>
+int launch_rows_for(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows, cudaStream_t stream)
+{
+    return rows <= 8    ? launch_rows<T, 1, 1>(k_map, v_map, p, stream)
+           : rows <= 16 ? launch_rows<T, 2, 1>(k_map, v_map, p, stream)
+                        : launch_rows<T, 2, 2>(k_map, v_map, p, stream);
 }
 
 template <typename T>
@@ -1395,16 +1407,11 @@ int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, cons
                                       : launch_tiles<__nv_bfloat16>(q_map, k_map, v_map, p, stream);
 }
 
-int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int m_tiles,
+int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows,
                        uint32_t dtype, cudaStream_t stream)
 {
-    if (dtype == SECURE_INFER_FP16)
-        return m_tiles == 1   ? launch_rows<__half, 1>(k_map, v_map, p, stream)
-               : m_tiles == 2 ? launch_rows<__half, 2>(k_map, v_map, p, stream)
-                              : launch_rows<__half, 4>(k_map, v_map, p, stream);
-    return m_tiles == 1   ? launch_rows<__nv_bfloat16, 1>(k_map, v_map, p, stream)
-           : m_tiles == 2 ? launch_rows<__nv_bfloat16, 2>(k_map, v_map, p, stream)
-                          : launch_rows<__nv_bfloat16, 4>(k_map, v_map, p, stream);
+    return dtype == SECURE_INFER_FP16 ? launch_rows_for<__half>(k_map, v_map, p, rows, stream)
+                                      : launch_rows_for<__nv_bfloat16>(k_map, v_map, p, rows, stream);
 }
 
 uint64_t attend_workspace_bytes()
