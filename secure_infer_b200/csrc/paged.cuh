@@ -48,7 +48,7 @@ struct AttendParams {
 };
 
 // Launchers (cudaError_t values).
-// Tiles of up to `rows` rows (8, 16 or 32); any number of them.
+// Tiles of up to `rows` rows (8 or 16); any number of them.
 int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows,
                        uint32_t dtype, cudaStream_t stream);
 // q_map: boxes of [128 / group tokens][group heads][64 values].

@@ -57,11 +57,11 @@ __device__ __forceinline__ void join_row(int n, Stats stats, int sums, Values va
 
 // ---------------------------------------------------------------- few rows
 //
-// Single tokens and short drafts: up to 32 rows per KV head and tile, bound by
+// Single tokens and short drafts: up to 16 rows per KV head and tile, bound by
 // reading K and V once.  One CTA per SM; a producer warp keeps three pages
-// (64 KiB each, K and V) in flight by TMA.  Each of eight warps takes up to 16
-// rows and a slice of each page's keys, with its own running maximum and sum,
-// so no warp waits for another inside the loop.  The products are m16n8k16 with
+// (64 KiB each, K and V) in flight by TMA.  Each of eight warps takes 16 keys of
+// each page, with its own running maximum and sum, so no warp waits for another
+// inside the loop.  The products are m16n8k16 with
 // the keys (then the values of a head) as M and eight rows as N: a group of
 // eight query heads or fewer fills one N, where rows as M would pad them to
 // sixteen, and these instructions are slow enough here to matter (about 20
@@ -75,7 +75,7 @@ constexpr int kRowsStages = 3;
 constexpr int kQuarter = 32;                              // tokens of one TMA box
 constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 tokens][64 values]
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
-constexpr int kMaxRows = 32;
+constexpr int kMaxRows = 16;
 constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRows * 256 + 2 * kRowsWarps * 16 * 4;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowsMinUnits = 1;
@@ -128,14 +128,13 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x)
 // Barrier of the eight computing warps.
 __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory"); }
 
-// kNs groups of eight rows per warp; the warps hold kTiles times that many rows.
-template <typename T, int kNs, int kTiles>
+// kNs groups of eight rows.
+template <typename T, int kNs>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                          const __grid_constant__ AttendParams p)
 {
-    constexpr int kWarpRows = 8 * kNs, kRows = kWarpRows * kTiles;
-    constexpr int kSlices = kRowsWarps / kTiles;   // of a page's keys
+    constexpr int kRows = 8 * kNs;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
     __shared__ Share share;
@@ -150,7 +149,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     float* join_m = reinterpret_cast<float*>(q_bytes + kMaxRows * 256);
     float* join_l = join_m + kRowsWarps * 16;
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row_tile = warp / kSlices;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto k_full = [&](int s) { return smem_addr(&bars[s]); };
     auto v_full = [&](int s) { return smem_addr(&bars[kRowsStages + s]); };
     auto empty = [&](int s) { return smem_addr(&bars[2 * kRowsStages + s]); };
@@ -241,7 +240,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         for (int n = 0; n < kNs; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int r = row_tile * kWarpRows + n * 8 + (lane & 3) * 2 + e;
+                const int r = n * 8 + (lane & 3) * 2 + e;
                 row_keys(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[n][e], hi[n][e]);
             }
         // Sums of values: o[j][n] holds values 16 j + lane / 4 (+ 8) of rows 8 n + 2 (lane % 4) (+ 1).
@@ -255,38 +254,38 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[j][n][c] = 0.0f;
         }
-        const bool idle = row_tile * kWarpRows >= w.rows;   // no row of this warp's is used
         rows_sync();
-        uint32_t q[kNs][4][4];   // 32 values of eight rows each
+        // 32 values of eight rows; one group of rows stays in registers, two would not fit beside the sums.
+        auto load_q = [&](uint32_t (&x)[4], int n, int d) {
+            const int r = n * 8 + (lane & 7), piece = d * 4 + (lane >> 3);
+            ldmatrix4(x, q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
+        };
+        uint32_t q[kNs][4][4];
+        if (kNs == 1)
 #pragma unroll
-        for (int n = 0; n < kNs; ++n)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const int r = row_tile * kWarpRows + n * 8 + (lane & 7), piece = d * 4 + (lane >> 3);
-                ldmatrix4(q[n][d], q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
-            }
+            for (int d = 0; d < 4; ++d) load_q(q[0][d], 0, d);
+        const int groups = (w.rows + 7) / 8;   // that are used
 
         for (int i = 0; i < pages; ++i, ++unit) {
             const int stage = unit % kRowsStages;
             const uint32_t parity = unit / kRowsStages & 1;
-            const int page_key = (w.span.first + w.page + i) * kPage;
+            const int key0 = (w.span.first + w.page + i) * kPage + warp * 16;   // of this warp's keys
             if (!barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop)) break;
-#pragma unroll 1
-            for (int sub = 0; sub < kTiles; ++sub) {
-                // 16 keys.
-                const int first16 = warp % kSlices * kTiles + sub, key0 = page_key + first16 * 16;
-                if (idle || key0 >= w.span.hi || key0 + 16 <= w.span.lo) continue;
-                const uint32_t slice = stage * kPageTile + (first16 >> 1) * kQuarterBytes + (first16 & 1) * 16 * 128;
+            if (key0 < w.span.hi && key0 + 16 > w.span.lo) {
+                const uint32_t slice = stage * kPageTile + (warp >> 1) * kQuarterBytes + (warp & 1) * 16 * 128;
                 const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
                 float s[kNs][2][4] = {};   // two chains of products
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {   // 16 values of the head at a time
+                    if (kNs > 1 && (d & 1) == 0)
+#pragma unroll
+                        for (int n = 0; n < kNs; ++n) load_q(q[n][d >> 1], n, d >> 1);
                     uint32_t a[4];
                     const int key = lane & 15, chunk = (d & 3) * 2 + (lane >> 4);
                     ldmatrix4(a, k_smem + slice + (d >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
 #pragma unroll
                     for (int n = 0; n < kNs; ++n)
-                        mma16816<T>(s[n][d & 1], a, q[n][d >> 1][(d & 1) * 2], q[n][d >> 1][(d & 1) * 2 + 1]);
+                        if (n < groups) mma16816<T>(s[n][d & 1], a, q[n][d >> 1][(d & 1) * 2], q[n][d >> 1][(d & 1) * 2 + 1]);
                 }
                 uint32_t weight[kNs][2];
 #pragma unroll
@@ -349,7 +348,8 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                         }
                     }
 #pragma unroll
-                    for (int n = 0; n < kNs; ++n) mma16816<T>(o[j][n], a, weight[n][0], weight[n][1]);
+                    for (int n = 0; n < kNs; ++n)
+                        if (n < groups) mma16816<T>(o[j][n], a, weight[n][0], weight[n][1]);
                 }
                 if (!whole && w.first_token != w.last_token && zero_sum_odd<T>(odd)) irregular = 1;
             }
@@ -376,17 +376,16 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const bool by_definition = irregular != 0;
         // Warp i's [16 rows][128] floats, columns swizzled by the row against bank conflicts.
         auto joined = [&](int i) { return base + ((i < 4 ? 0 : kRowsStages) + last_stage) * kPageTile + (i & 3) * 8192; };
-        if (!idle) {
-            uint8_t* to = joined(warp);
 #pragma unroll
-            for (int n = 0; n < kNs; ++n)
+        for (int n = 0; n < kNs; ++n) {
+            if (n >= groups) break;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int r = n * 8 + (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
-                        *reinterpret_cast<float*>(to + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][n][c];
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    const int r = n * 8 + (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
+                    *reinterpret_cast<float*>(joined(warp) + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][n][c];
+                }
         }
         rows_sync();
 #pragma unroll 1
@@ -403,20 +402,19 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                                      p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, ka + pages * kPage), top,
                                      sum, x);
             } else {
-                const int from = r / kWarpRows * kSlices, row = r % kWarpRows;
-                const int stat = (from + (lane & (kSlices - 1))) * 16 + row;
+                const int stat = (lane & (kRowsWarps - 1)) * 16 + r;
                 const float mi = join_m[stat];
                 top = mi;
 #pragma unroll
-                for (int d = 1; d < kSlices; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                for (int d = 1; d < kRowsWarps; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                 const float f = join_weight(mi, top);
                 sum = f * join_l[stat];
 #pragma unroll
-                for (int d = 1; d < kSlices; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                for (int d = 1; d < kRowsWarps; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
 #pragma unroll
-                for (int i = 0; i < kSlices; ++i) {
+                for (int i = 0; i < kRowsWarps; ++i) {
                     const float wi = __shfl_sync(0xffffffffu, f, i);
-                    const float4 y = *reinterpret_cast<const float4*>(joined(from + i) + row * 512 + ((lane * 4) ^ ((row >> 1 & 3) << 3)) * 4);
+                    const float4 y = *reinterpret_cast<const float4*>(joined(i) + r * 512 + ((lane * 4) ^ ((r >> 1 & 3) << 3)) * 4);
                     x.x += wi * y.x;
                     x.y += wi * y.y;
                     x.z += wi * y.z;
@@ -1309,13 +1307,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
 
 struct Device {
     int sms = 0;
-    bool rows_set[2][3] = {};
+    bool rows_set[2][2] = {};
     bool tiles_set[2] = {};
 };
 std::mutex g_mu;
 Device g_devices[64];
 
-template <typename T, int kNs, int kTiles>
+template <typename T, int kNs>
 int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, cudaStream_t stream)
 {
     int dev = 0;
@@ -1325,9 +1323,9 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
         if (d.sms == 0) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-        bool& set = d.rows_set[std::is_same<T, __half>::value][kNs + kTiles - 2];
+        bool& set = d.rows_set[std::is_same<T, __half>::value][kNs - 1];
         if (!set) {
-            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, kNs, kTiles>,
+            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, kNs>,
                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
             if (e != cudaSuccess) return e;
             set = true;
@@ -1345,15 +1343,13 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     ProfileScope prof(kKernAttendRows, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, kNs, kTiles>, k_map, v_map, p);
+    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, kNs>, k_map, v_map, p);
 }
 
 template <typename T>
 int launch_rows_for(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows, cudaStream_t stream)
 {
-    return rows <= 8    ? launch_rows<T, 1, 1>(k_map, v_map, p, stream)
-           : rows <= 16 ? launch_rows<T, 2, 1>(k_map, v_map, p, stream)
-                        : launch_rows<T, 2, 2>(k_map, v_map, p, stream);
+    return rows <= 8 ? launch_rows<T, 1>(k_map, v_map, p, stream) : launch_rows<T, 2>(k_map, v_map, p, stream);
 }
 
 template <typename T>
