@@ -58,8 +58,8 @@ typedef struct {
     uint32_t max_q;
 } secure_infer_chunk;
 
-/* Attention of the chunk over the pages.  q: [tokens][q_heads][128] with
- * strides q_stride (token, head) in elements, q_heads a multiple of the KV
+/* Attention of the chunk over the pages.  q: [tokens][q_heads][128] with its
+ * strides in elements, q_heads a multiple of the KV
  * heads (query head h reads KV head h / (q_heads / heads)).  out:
  * [tokens][q_heads][128], dense.  lse: null, or [tokens][q_heads] natural
  * logarithms of the softmax sums, for joining with attention over other keys.
@@ -71,8 +71,8 @@ typedef struct {
  * calls leave it ready for the next. */
 uint64_t secure_infer_paged_attend_workspace(void);
 int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
-                              const int64_t* q_stride, uint32_t q_heads, void* out, float* lse, float scale,
-                              uint32_t causal, uint32_t window, void* workspace, void* stream);
+                              int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
+                              float scale, uint32_t causal, uint32_t window, void* workspace, void* stream);
 
 /* Rotary positions and the chunk's way into its pages.  q (may be null), k and
  * v: [tokens][heads][128] with their strides (token, head).  Pair i of a head
@@ -83,10 +83,10 @@ int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infe
  * the sequence.  Turned q goes to q_out, dense; turned k and plain v to their
  * slots.  Tokens whose slot lies outside the cache are not written. */
 int secure_infer_paged_append(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
-                              const int64_t* q_stride, uint32_t q_heads, void* q_out, const void* k,
-                              const int64_t* k_stride, const void* v, const int64_t* v_stride,
-                              const uint64_t* phase, const uint32_t* axis, const int32_t* positions,
-                              int64_t position_stride, uint32_t axes, uint32_t interleaved, void* stream);
+                              int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* q_out,
+                              const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                              int64_t v_token_stride, int64_t v_head_stride, const uint64_t* phase,
+                              const uint32_t* axis, const int32_t* positions, int64_t position_stride, uint32_t axes, uint32_t interleaved, void* stream);
 
 /* Tables of a cache: block_table [seqs][width], tokens held per sequence, and
  * how many rows hold each page (0: free).  A sequence of n tokens holds

@@ -12,6 +12,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_build" / "libsecure_infer.so"
 
 P, U64, U32, I32, SZ = ct.c_void_p, ct.c_uint64, ct.c_uint32, ct.c_int, ct.c_size_t
+I64 = ct.c_int64
 PP = ct.POINTER(ct.c_void_p)
 U32P = ct.POINTER(ct.c_uint32)
 U64P = ct.POINTER(ct.c_uint64)
@@ -128,8 +129,8 @@ class PageTensor(ct.Structure):
 # Operators on the paged cache.  Structures go by reference.
 PAGED_SIGNATURES = {
     "secure_infer_paged_attend_workspace": ([], U64),
-    "secure_infer_paged_attend": ([P, P, P, P, U32, P, P, ct.c_float, U32, U32, P, P], I32),
-    "secure_infer_paged_append": ([P, P, P, P, U32, P, P, P, P, P, P, P, P, ct.c_int64, U32, U32, P], I32),
+    "secure_infer_paged_attend": ([P, P, P, I64, I64, U32, P, P, ct.c_float, U32, U32, P, P], I32),
+    "secure_infer_paged_append": ([P, P, P, I64, I64, U32, P, P, I64, I64, P, I64, I64, P, P, P, I64, U32, U32, P], I32),
     "secure_infer_paged_scratch": ([P, U32], U64),
     "secure_infer_paged_copy": ([P, U32, U64, U32, P, P, U32, P], I32),
     "secure_infer_paged_fork": ([P, U32, U64, P, P, P, P, U32, P, P, P], I32),

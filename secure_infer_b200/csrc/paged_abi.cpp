@@ -65,11 +65,11 @@ bool page_map(CUtensorMap* map, const secure_infer_pages* p, const void* base, c
 
 // Queries as [half of a head][token][query head][64 values], in boxes of a KV
 // head's group by 128 / group tokens.
-bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, const int64_t* stride, uint32_t tokens, uint32_t heads,
-              uint32_t group)
+bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, int64_t token_stride, int64_t head_stride, uint32_t tokens,
+              uint32_t heads, uint32_t group)
 {
     const cuuint64_t dims[4] = {64, heads, tokens, 2};
-    const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(stride[1]) * 2, static_cast<cuuint64_t>(stride[0]) * 2, 128};
+    const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2, 128};
     const cuuint32_t box[4] = {64, group, 128 / group, 1}, step[4] = {1, 1, 1, 1};
     const auto type = dtype == SECURE_INFER_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const auto encode = tensor_map_encoder();
@@ -107,15 +107,16 @@ bool tensors_ok(const secure_infer_page_tensor* t, uint32_t n, uint64_t page_byt
 SI_EXPORT uint64_t secure_infer_paged_attend_workspace(void) { return attend_workspace_bytes(); }
 
 SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
-                                        const int64_t* q_stride, uint32_t q_heads, void* out, float* lse, float scale,
-                                        uint32_t causal, uint32_t window, void* workspace, void* stream)
+                                        int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out,
+                                        float* lse, float scale, uint32_t causal, uint32_t window, void* workspace,
+                                        void* stream)
 {
-    if (!pages_ok(pages) || !chunk_ok(chunk) || q_stride == nullptr || q_heads == 0 || q_heads > (1u << 16) ||
+    if (!pages_ok(pages) || !chunk_ok(chunk) || q_heads == 0 || q_heads > (1u << 16) ||
         q_heads % pages->heads != 0 || (window != 0 && !causal) || window > INT_MAX || workspace == nullptr ||
         (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
         return -1;
     if (chunk->tokens == 0) return 0;
-    if (!aligned16(q) || !aligned16(out) || !stride_ok(q_stride[0]) || !stride_ok(q_stride[1])) return -1;
+    if (!aligned16(q) || !aligned16(out) || !stride_ok(q_token_stride) || !stride_ok(q_head_stride)) return -1;
     const uint32_t group = q_heads / pages->heads;
     const uint32_t max_q = chunk->max_q == 0 || chunk->max_q > chunk->tokens ? chunk->tokens : chunk->max_q;
     const uint64_t max_rows = static_cast<uint64_t>(max_q) * group;
@@ -127,8 +128,8 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     AttendParams p;
     std::memset(&p, 0, sizeof(p));
     p.q = q;
-    p.q_token = q_stride[0];
-    p.q_head = q_stride[1];
+    p.q_token = q_token_stride;
+    p.q_head = q_head_stride;
     p.k = pages->k;
     p.v = pages->v;
     for (int i = 0; i < 3; ++i) {
@@ -172,37 +173,39 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     }
     if (!tiles) return 0;
     if (!page_map(&k_map, pages, pages->k, pages->k_stride, kPage) || !page_map(&v_map, pages, pages->v, pages->v_stride, kPage) ||
-        !rows_map(&q_map, pages->dtype, q, q_stride, chunk->tokens, q_heads, group))
+        !rows_map(&q_map, pages->dtype, q, q_token_stride, q_head_stride, chunk->tokens, q_heads, group))
         return -1;
     return launch_attend_tiles(q_map, k_map, v_map, p, pages->dtype, st) == 0 ? 0 : -1;
 }
 
 SI_EXPORT int secure_infer_paged_append(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
-                                        const int64_t* q_stride, uint32_t q_heads, void* q_out, const void* k,
-                                        const int64_t* k_stride, const void* v, const int64_t* v_stride,
-                                        const uint64_t* phase, const uint32_t* axis, const int32_t* positions,
-                                        int64_t position_stride, uint32_t axes, uint32_t interleaved, void* stream)
+                                        int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* q_out,
+                                        const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                        int64_t v_token_stride, int64_t v_head_stride, const uint64_t* phase,
+                                        const uint32_t* axis, const int32_t* positions, int64_t position_stride,
+                                        uint32_t axes, uint32_t interleaved, void* stream)
 {
-    if (!pages_ok(pages) || !chunk_ok(chunk) || k_stride == nullptr || v_stride == nullptr || q_heads > (1u << 16) ||
-        (phase == nullptr) != (axis == nullptr) || (positions != nullptr && (axes == 0 || axes > 64 || position_stride < 0)))
+    if (!pages_ok(pages) || !chunk_ok(chunk) || q_heads > (1u << 16) || (phase == nullptr) != (axis == nullptr) ||
+        (positions != nullptr && (axes == 0 || axes > 64 || position_stride < 0)))
         return -1;
     if (chunk->tokens == 0) return 0;
-    if (!aligned16(k) || !aligned16(v)) return -1;
-    for (int i = 0; i < 2; ++i)
-        if (!stride_ok(k_stride[i]) || !stride_ok(v_stride[i])) return -1;
-    if (q != nullptr && (!aligned16(q) || !aligned16(q_out) || q_stride == nullptr || q_heads == 0 ||
-                         !stride_ok(q_stride[0]) || !stride_ok(q_stride[1])))
+    if (!aligned16(k) || !aligned16(v) || !stride_ok(k_token_stride) || !stride_ok(k_head_stride) ||
+        !stride_ok(v_token_stride) || !stride_ok(v_head_stride))
+        return -1;
+    if (q != nullptr && (!aligned16(q) || !aligned16(q_out) || q_heads == 0 || !stride_ok(q_token_stride) ||
+                         !stride_ok(q_head_stride)))
         return -1;
     AppendParams p;
     std::memset(&p, 0, sizeof(p));
     p.q = q;
     p.k = k;
     p.v = v;
-    for (int i = 0; i < 2; ++i) {
-        p.q_stride[i] = q != nullptr ? q_stride[i] : 0;
-        p.k_in[i] = k_stride[i];
-        p.v_in[i] = v_stride[i];
-    }
+    p.q_stride[0] = q_token_stride;
+    p.q_stride[1] = q_head_stride;
+    p.k_in[0] = k_token_stride;
+    p.k_in[1] = k_head_stride;
+    p.v_in[0] = v_token_stride;
+    p.v_in[1] = v_head_stride;
     p.q_out = q_out;
     p.k_cache = pages->k;
     p.v_cache = pages->v;

@@ -40,24 +40,49 @@ def _ints(t, what: str, device, dims: int) -> torch.Tensor:
     """An int32 tensor of the device, as given or made from a list."""
     if not isinstance(t, torch.Tensor):
         t = torch.tensor(list(t), dtype=torch.int32, device=device)
-    _need(t.dtype == torch.int32 and t.ndim == dims and t.device == device,
-          f"{what} must be an int32 tensor of {dims} dimension(s) on {device}")
-    _need(t.numel() == 0 or t.stride(-1) == 1, f"{what} must be dense in its last dimension")
+    if t.dtype is not torch.int32 or t.ndim != dims or t.device != device:
+        raise ValueError(f"{what} must be an int32 tensor of {dims} dimension(s) on {device}")
+    if t.stride(-1) != 1 and t.numel() != 0:
+        raise ValueError(f"{what} must be dense in its last dimension")
     return t
 
 
+# Reading the current stream's handle costs a twentieth of building a Stream object, where torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _stream(device) -> int:
+    return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
+
+
 def _rows(t: torch.Tensor, what: str, tokens: int, dtype, device) -> tuple[int, int, int]:
-    """Heads and strides of [tokens, heads, 128]."""
-    _need(t.ndim == 3 and t.shape[0] == tokens and t.shape[2] == HEAD_DIM,
-          f"{what} must be [{tokens}, heads, {HEAD_DIM}], not {list(t.shape)}")
-    _need(t.dtype == dtype and t.device == device, f"{what} must be {dtype} on {device}")
+    """Heads and strides of [tokens, heads, 128].  On the way of every call:
+    texts are only made where something is wrong."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != HEAD_DIM:
+        raise ValueError(f"{what} must be [{tokens}, heads, {HEAD_DIM}], not {list(shape)}")
+    if t.dtype is not dtype or t.device != device:
+        raise ValueError(f"{what} must be {dtype} on {device}")
     st, sh, sd = t.stride()
     # A single token or head has no stride of its own.
-    st = st if tokens > 1 else HEAD_DIM
-    sh = sh if t.shape[1] > 1 else HEAD_DIM
-    _need(sd == 1 and t.data_ptr() % 16 == 0 and st > 0 and sh > 0 and st % 8 == 0 and sh % 8 == 0,
-          f"{what}: a head's values must be adjacent, the address and strides multiples of 16 bytes")
-    return t.shape[1], st, sh
+    if tokens <= 1:
+        st = HEAD_DIM
+    if shape[1] <= 1:
+        sh = HEAD_DIM
+    if sd != 1 or st <= 0 or sh <= 0 or (st | sh) & 7 or t.data_ptr() & 15:
+        raise ValueError(f"{what}: a head's values must be adjacent, the address and strides multiples of 16 bytes")
+    return shape[1], st, sh
+
+
+def _like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    """A dense output of q's shape, or the given one checked."""
+    if out is None:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous() \
+            or out.data_ptr() & 15:
+        raise ValueError("out must be dense, with q's shape, type and device")
+    return out
 
 
 class LayerPages:
@@ -134,15 +159,16 @@ class Rotary:
         self.phase = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
         self.axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32, device=device)
         self.device = self.phase.device
+        self._phase, self._axis = self.phase.data_ptr(), self.axis.data_ptr()
 
 
 def _call(name: str, device, *args) -> None:
-    lib = _native.lib()
+    function = getattr(_native.lib(), name)
     if device.index is not None and device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args)
+            rc = function(*args)
     else:
-        rc = getattr(lib, name)(*args)
+        rc = function(*args)
     if rc != 0:
         raise RuntimeError(f"{name} refused its arguments or failed to launch")
 
@@ -157,43 +183,42 @@ def append(pages: LayerPages, chunk: Chunk, q: torch.Tensor | None, k: torch.Ten
     tokens' places in their sequences.  A token whose place lies outside its
     sequence's pages is not written."""
     tokens, device, dtype = k.shape[0], pages.device, pages.dtype
-    _need(chunk.device == device, "the chunk and the cache are on different devices")
+    if chunk.device != device:
+        raise ValueError("the chunk and the cache are on different devices")
     heads, kt, kh = _rows(k, "k", tokens, dtype, device)
     v_heads, vt, vh = _rows(v, "v", tokens, dtype, device)
-    _need(heads == pages.heads and v_heads == heads, f"k and v must have the cache's {pages.heads} heads")
-    q_heads, qs, q_ptr, out_ptr = 0, None, None, None
+    if heads != pages.heads or v_heads != heads:
+        raise ValueError(f"k and v must have the cache's {pages.heads} heads")
+    q_heads = qt = qh = 0
+    q_ptr = out_ptr = None
     if q is not None:
         q_heads, qt, qh = _rows(q, "q", tokens, dtype, device)
-        qs, q_ptr = (ct.c_int64 * 2)(qt, qh), q.data_ptr()
-        if out is None:
-            out = torch.empty((tokens, q_heads, HEAD_DIM), dtype=dtype, device=device)
-        else:
-            _need(out.shape == q.shape and out.dtype == dtype and out.device == device and out.is_contiguous() and
-                  out.data_ptr() % 16 == 0, "out must be dense, with q's shape, type and device")
-        out_ptr = out.data_ptr()
-    else:
-        _need(out is None, "out goes with q")
+        out = _like(q, out)
+        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    elif out is not None:
+        raise ValueError("out goes with q")
     phase = axis = pos_ptr = None
-    pos_stride, axes, interleaved = 0, 1, 0
+    pos_stride, axes, interleaved = 0, 1, False
     if rotary is not None:
-        _need(rotary.device == device, "rotary and the cache are on different devices")
-        phase, axis, axes, interleaved = rotary.phase.data_ptr(), rotary.axis.data_ptr(), rotary.axes, rotary.interleaved
+        if rotary.device != device:
+            raise ValueError("rotary and the cache are on different devices")
+        phase, axis, axes, interleaved = rotary._phase, rotary._axis, rotary.axes, rotary.interleaved
         if positions is not None:
-            positions = _ints(positions, "positions", device, positions.ndim)
-            if positions.ndim == 1:
-                _need(axes == 1, f"positions must be [{axes}, tokens]")
-                positions = positions[None]
-            _need(tuple(positions.shape) == (axes, tokens), f"positions must be [{axes}, {tokens}]")
+            _ints(positions, "positions", device, positions.ndim)
+            shape = tuple(positions.shape)
+            if shape != (axes, tokens) and not (axes == 1 and shape == (tokens,)):
+                raise ValueError(f"positions must be [{axes}, {tokens}]")
             pos_ptr, pos_stride = positions.data_ptr(), positions.stride(0) if axes > 1 else tokens
-            _need(pos_stride >= 0, "positions has a negative stride")
-    else:
-        _need(positions is None, "positions go with rotary")
+            if pos_stride < 0:
+                raise ValueError("positions has a negative stride")
+    elif positions is not None:
+        raise ValueError("positions go with rotary")
     if tokens == 0:
         return out
-    chunk._c.tokens = tokens
-    _call("secure_infer_paged_append", device, pages._ref, chunk._ref, q_ptr, qs, q_heads, out_ptr, k.data_ptr(),
-          (ct.c_int64 * 2)(kt, kh), v.data_ptr(), (ct.c_int64 * 2)(vt, vh), phase, axis, pos_ptr, pos_stride, axes,
-          interleaved, torch.cuda.current_stream(device).cuda_stream)
+    if chunk._c.tokens != tokens:
+        chunk._c.tokens = tokens
+    _call("secure_infer_paged_append", device, pages._ref, chunk._ref, q_ptr, qt, qh, q_heads, out_ptr, k.data_ptr(), kt,
+          kh, v.data_ptr(), vt, vh, phase, axis, pos_ptr, pos_stride, axes, interleaved, _stream(device))
     return out
 
 
@@ -229,41 +254,42 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
     other keys.  A row that sees no key gives 0 and -inf.  ``workspace``:
     ``attend_workspace(device)``, by default one that the current stream
     keeps."""
-    device, dtype = pages.device, pages.dtype
-    _need(chunk.device == device, "the chunk and the cache are on different devices")
-    tokens = q.shape[0]
-    q_heads, qt, qh = _rows(q, "q", tokens, dtype, device)
-    _need(q_heads > 0 and q_heads % pages.heads == 0, f"q's heads must be a multiple of the cache's {pages.heads}")
-    _need(0 <= window < 1 << 31 and (causal or window == 0), "window must be zero or positive, and goes with causal")
-    if out is None:
-        out = torch.empty((tokens, q_heads, HEAD_DIM), dtype=dtype, device=device)
-    else:
-        _need(out.shape == q.shape and out.dtype == dtype and out.device == device and out.is_contiguous() and
-              out.data_ptr() % 16 == 0, "out must be dense, with q's shape, type and device")
+    device, tokens = pages.device, q.shape[0]
+    if chunk.device != device:
+        raise ValueError("the chunk and the cache are on different devices")
+    q_heads, qt, qh = _rows(q, "q", tokens, pages.dtype, device)
+    if q_heads == 0 or q_heads % pages.heads:
+        raise ValueError(f"q's heads must be a multiple of the cache's {pages.heads}")
+    if not 0 <= window < 1 << 31 or (window and not causal):
+        raise ValueError("window must be zero or positive, and goes with causal")
+    out = _like(q, out)
     lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=device) if return_lse else None
     if tokens > 0:
-        stream = torch.cuda.current_stream(device).cuda_stream
+        stream = _stream(device)
         if workspace is None:
             workspace = _workspace(device, stream)
-        else:
-            _need(workspace.device == device and workspace.is_contiguous() and workspace.data_ptr() % 256 == 0 and
-                  workspace.numel() * workspace.element_size() >= _native.lib().secure_infer_paged_attend_workspace(),
-                  "workspace must come from attend_workspace of the cache's device")
-        chunk._c.tokens = tokens
-        _call("secure_infer_paged_attend", device, pages._ref, chunk._ref, q.data_ptr(), (ct.c_int64 * 2)(qt, qh),
-              q_heads, out.data_ptr(), lse.data_ptr() if return_lse else None,
-              HEAD_DIM ** -0.5 if scale is None else float(scale), 1 if causal else 0, window, workspace.data_ptr(),
-              stream)
+        elif workspace.device != device or not workspace.is_contiguous() or workspace.data_ptr() & 255 or \
+                workspace.numel() * workspace.element_size() < _native.lib().secure_infer_paged_attend_workspace():
+            raise ValueError("workspace must come from attend_workspace of the cache's device")
+        if chunk._c.tokens != tokens:
+            chunk._c.tokens = tokens
+        _call("secure_infer_paged_attend", device, pages._ref, chunk._ref, q.data_ptr(), qt, qh, q_heads, out.data_ptr(),
+              lse.data_ptr() if return_lse else None, HEAD_DIM ** -0.5 if scale is None else scale, bool(causal), window,
+              workspace.data_ptr(), stream)
     return (out, lse) if return_lse else out
 
 
-class PageTables(NamedTuple):
-    """Who holds which page: ``block_table`` int32 ``[seqs, width]``, ``lens``
-    int32 ``[seqs]`` tokens held, ``refs`` int32 ``[pages]`` rows that hold a
-    page (0: free).  A sequence of n tokens holds ``ceil(n / 128)`` pages."""
+class _Tables(NamedTuple):
     block_table: torch.Tensor
     lens: torch.Tensor
     refs: torch.Tensor
+
+
+class PageTables(_Tables):
+    """Who holds which page: ``block_table`` int32 ``[seqs, width]``, ``lens``
+    int32 ``[seqs]`` tokens held, ``refs`` int32 ``[pages]`` rows that hold a
+    page (0: free).  A sequence of n tokens holds ``ceil(n / 128)`` pages."""
+    _checked = None   # the C structure, once a cache has looked the tensors over
 
 
 class CachePages:
@@ -294,7 +320,10 @@ class CachePages:
         self._tensors = arr
 
     def _check(self, t: PageTables) -> _native.Tables:
-        _need(isinstance(t, PageTables), "tables must be PageTables")
+        if not isinstance(t, PageTables):
+            raise ValueError("tables must be PageTables")
+        if t._checked is not None and t._checked[0] is self:
+            return t._checked[1]
         for x, what, dims in ((t.block_table, "block_table", 2), (t.lens, "lens", 1), (t.refs, "refs", 1)):
             _need(isinstance(x, torch.Tensor), f"{what} must be a tensor")
             _ints(x, what, self.device, dims)
@@ -303,29 +332,33 @@ class CachePages:
         _need(seqs > 0 and width > 0, "block_table is empty")
         _need(t.lens.shape[0] == seqs and t.refs.shape[0] == self.pages,
               "lens needs an entry for each row of the block table, refs one for each page")
-        return _native.Tables(t.block_table.data_ptr(), t.lens.data_ptr(), t.refs.data_ptr(), seqs, width, self.pages, 0)
+        return self._remember(t, seqs, width)
+
+    def _remember(self, t: PageTables, seqs: int, width: int) -> _native.Tables:
+        c = _native.Tables(t.block_table.data_ptr(), t.lens.data_ptr(), t.refs.data_ptr(), seqs, width, self.pages, 0)
+        t._checked = (self, c)
+        return c
 
     def _outputs(self, t: PageTables, out: PageTables | None):
         c = self._check(t)
         if out is None:
-            out = PageTables(*(torch.empty_like(x) for x in t))
-        else:
-            self._check(out)
-            _need(all(a.shape == b.shape for a, b in zip(t, out)), "out differs in shape from the tables")
-            for a in t:
-                for b in out:
-                    lo, hi = max(a.data_ptr(), b.data_ptr()), min(a.data_ptr() + 4 * a.numel(), b.data_ptr() + 4 * b.numel())
-                    _need(lo >= hi, "out overlaps the tables")
-        return c, out, _native.Tables(out.block_table.data_ptr(), out.lens.data_ptr(), out.refs.data_ptr(), c.seqs,
-                                      c.width, c.pages, 0)
+            out = PageTables(torch.empty_like(t.block_table), torch.empty_like(t.lens), torch.empty_like(t.refs))
+            return c, out, self._remember(out, c.seqs, c.width)
+        o = self._check(out)
+        _need(all(a.shape == b.shape for a, b in zip(t, out)), "out differs in shape from the tables")
+        for a in t:
+            for b in out:
+                lo, hi = max(a.data_ptr(), b.data_ptr()), min(a.data_ptr() + 4 * a.numel(), b.data_ptr() + 4 * b.numel())
+                _need(lo >= hi, "out overlaps the tables")
+        return c, out, o
 
     def _scratch(self, c: _native.Tables, n: int) -> torch.Tensor:
-        return torch.empty(int(_native.lib().secure_infer_paged_scratch(ct.byref(c), n)), dtype=torch.uint8,
-                           device=self.device)
+        return torch.empty(_native.lib().secure_infer_paged_scratch(ct.byref(c), n), dtype=torch.uint8, device=self.device)
 
     def _pair(self, a, b, names) -> tuple[torch.Tensor, torch.Tensor]:
         a, b = _ints(a, names[0], self.device, 1), _ints(b, names[1], self.device, 1)
-        _need(a.shape == b.shape, f"{names[0]} and {names[1]} differ in length")
+        if a.shape != b.shape:
+            raise ValueError(f"{names[0]} and {names[1]} differ in length")
         return a, b
 
     def copy(self, src, dst) -> None:
@@ -338,7 +371,7 @@ class CachePages:
             _need(all(0 <= i < self.pages for i in src + dst), "page outside the cache")
         src, dst = self._pair(src, dst, ("src", "dst"))
         _call("secure_infer_paged_copy", self.device, self._tensors, len(self._tensors), self.page_bytes, self.pages,
-              src.data_ptr(), dst.data_ptr(), src.shape[0], torch.cuda.current_stream(self.device).cuda_stream)
+              src.data_ptr(), dst.data_ptr(), src.shape[0], _stream(self.device))
 
     def fork(self, tables: PageTables, parents, children, out: PageTables | None = None):
         """Give the empty sequence ``children[i]`` the tokens of ``parents[i]``:
@@ -353,7 +386,7 @@ class CachePages:
         scratch = self._scratch(c, n)
         _call("secure_infer_paged_fork", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
               ct.byref(o), a.data_ptr(), b.data_ptr(), n, granted.data_ptr(), scratch.data_ptr(),
-              torch.cuda.current_stream(self.device).cuda_stream)
+              _stream(self.device))
         return out, granted
 
     def reserve(self, tables: PageTables, seqs, lens, out: PageTables | None = None):
@@ -367,7 +400,7 @@ class CachePages:
         granted = torch.empty(n, dtype=torch.int32, device=self.device)
         scratch = self._scratch(c, n)
         _call("secure_infer_paged_reserve", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), b.data_ptr(), n,
-              granted.data_ptr(), scratch.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+              granted.data_ptr(), scratch.data_ptr(), _stream(self.device))
         return out, granted
 
     def free(self, tables: PageTables, seqs, out: PageTables | None = None) -> PageTables:
@@ -377,7 +410,7 @@ class CachePages:
         c, out, o = self._outputs(tables, out)
         scratch = self._scratch(c, a.shape[0])
         _call("secure_infer_paged_free", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), a.shape[0],
-              scratch.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+              scratch.data_ptr(), _stream(self.device))
         return out
 
     def compact(self, tables: PageTables, out: PageTables | None = None):
@@ -392,5 +425,5 @@ class CachePages:
         scratch = self._scratch(c, 0)
         _call("secure_infer_paged_compact", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
               ct.byref(o), moved.data_ptr(), live.data_ptr(), scratch.data_ptr(),
-              torch.cuda.current_stream(self.device).cuda_stream)
+              _stream(self.device))
         return out, moved, live

@@ -58,9 +58,9 @@ def good():
 def test_attend_and_append_refuse(lib, change):
     pages, chunk, stride = good()
     change(pages, chunk, stride)
-    assert lib.secure_infer_paged_attend(ct.byref(pages), ct.byref(chunk), A, stride, 32, A, None, 1.0, 1, 0, A, None) == -1
+    assert lib.secure_infer_paged_attend(ct.byref(pages), ct.byref(chunk), A, *stride, 32, A, None, 1.0, 1, 0, A, None) == -1
     if pages.heads != 3:   # any head count of its own goes with append
-        assert lib.secure_infer_paged_append(ct.byref(pages), ct.byref(chunk), A, stride, 32, A, A, stride, A, stride,
+        assert lib.secure_infer_paged_append(ct.byref(pages), ct.byref(chunk), A, *stride, 32, A, A, *stride, A, *stride,
                                              None, None, None, 0, 1, 0, None) == -1
 
 
@@ -68,18 +68,18 @@ def test_attend_refuses_more(lib):
     pages, chunk, stride = good()
     call = lib.secure_infer_paged_attend
     p, c = ct.byref(pages), ct.byref(chunk)
-    assert call(None, c, A, stride, 32, A, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, None, A, stride, 32, A, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, c, None, stride, 32, A, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, c, A, None, 32, A, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, c, A, stride, 0, A, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, c, A, stride, 33, A, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, c, A, stride, 32, A + 2, None, 1.0, 1, 0, A, None) == -1
-    assert call(p, c, A, stride, 32, A, None, 1.0, 0, 9, A, None) == -1      # a window needs the causal order
-    assert call(p, c, A, stride, 32, A, None, 1.0, 1, 0, None, None) == -1
-    assert call(p, c, A, stride, 32, A, None, 1.0, 1, 0, A + 16, None) == -1
+    assert call(None, c, A, *stride, 32, A, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, None, A, *stride, 32, A, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, c, None, *stride, 32, A, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, c, A, 4096, -128, 32, A, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, c, A, *stride, 0, A, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, c, A, *stride, 33, A, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, c, A, *stride, 32, A + 2, None, 1.0, 1, 0, A, None) == -1
+    assert call(p, c, A, *stride, 32, A, None, 1.0, 0, 9, A, None) == -1      # a window needs the causal order
+    assert call(p, c, A, *stride, 32, A, None, 1.0, 1, 0, None, None) == -1
+    assert call(p, c, A, *stride, 32, A, None, 1.0, 1, 0, A + 16, None) == -1
     chunk.tokens = 0
-    assert call(p, c, None, stride, 32, None, None, 1.0, 1, 0, A, None) == 0   # nothing to do
+    assert call(p, c, None, *stride, 32, None, None, 1.0, 1, 0, A, None) == 0   # nothing to do
     assert lib.secure_infer_paged_attend_workspace() > 0
 
 
@@ -88,10 +88,10 @@ def test_append_refuses_more(lib):
     p, c = ct.byref(pages), ct.byref(chunk)
 
     def call(q=A, k=A, v=A, out=A, qs=stride, heads=32, phase=None, axis=None, positions=None, pos_stride=0, axes=1):
-        return lib.secure_infer_paged_append(p, c, q, qs, heads, out, k, stride, v, stride, phase, axis, positions,
+        return lib.secure_infer_paged_append(p, c, q, *qs, heads, out, k, *stride, v, *stride, phase, axis, positions,
                                              pos_stride, axes, 0, None)
     assert call(k=None) == -1 and call(v=A + 2) == -1 and call(q=A + 4) == -1 and call(out=None) == -1
-    assert call(qs=None) == -1 and call(heads=0) == -1
+    assert call(qs=(4096, 0)) == -1 and call(heads=0) == -1
     assert call(phase=A) == -1 and call(axis=A) == -1
     assert call(phase=A, axis=A, positions=A, axes=0) == -1 and call(phase=A, axis=A, positions=A, pos_stride=-1) == -1
     chunk.tokens = 0
