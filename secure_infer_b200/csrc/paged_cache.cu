@@ -18,6 +18,7 @@ namespace {
 // pairs each, 16-byte accesses), a warp four rows at a time, and computes its
 // lanes' eight angles once for all rows that it turns.
 constexpr int kAppendThreads = 128;
+constexpr int kAppendBatch = 3;
 
 __device__ __forceinline__ int find_seq(const int32_t* cu, int seqs, int token)
 {
@@ -38,13 +39,31 @@ template <typename T>
 __global__ void __launch_bounds__(kAppendThreads)
 paged_append_kernel(const __grid_constant__ AppendParams p, int groups, int rows_per_warp)
 {
-    wait_for_earlier_kernels();
-    dependents_may_launch();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, sub = lane & 7;
     const int64_t work = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
     const int64_t token64 = work / groups;
+    wait_for_earlier_kernels();
+    dependents_may_launch();
     if (token64 >= p.tokens) return;
     const int token = static_cast<int>(token64), part = static_cast<int>(work % groups);
+    const int rotated = p.q_heads + p.heads;
+    const int row0 = part * rows_per_warp, row1 = min(row0 + rows_per_warp, rotated + p.heads);
+    const int lo = p.interleaved ? sub * 16 : sub * 8, hi = p.interleaved ? sub * 16 + 8 : 64 + sub * 8;
+    // Twelve rows are on their way before the token's place and angles are known.
+    uint4 a[kAppendBatch], b[kAppendBatch];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < kAppendBatch; ++i) {
+            const int row = first + 4 * i + (lane >> 3);
+            if (row >= row1) break;
+            const T* src = row < p.q_heads ? static_cast<const T*>(p.q) + token * p.q_stride[0] + row * p.q_stride[1]
+                           : row < rotated ? static_cast<const T*>(p.k) + token * p.k_in[0] + (row - p.q_heads) * p.k_in[1]
+                                           : static_cast<const T*>(p.v) + token * p.v_in[0] + (row - rotated) * p.v_in[1];
+            a[i] = *reinterpret_cast<const uint4*>(src + lo);
+            b[i] = *reinterpret_cast<const uint4*>(src + hi);
+        }
+    };
+    load(row0);
     const int s = find_seq(p.cu, p.seqs, token);
     const int first = p.cu[s], end = min(p.cu[s + 1], p.tokens), kv = p.kv[s];
     const bool owned = token >= first && token < end;   // else the token is nobody's: q turns, nothing is written
@@ -57,10 +76,7 @@ paged_append_kernel(const __grid_constant__ AppendParams p, int groups, int rows
             v_at = page * p.v_stride[0] + (pos % kPage) * p.v_stride[1];
         }
     }
-    const int sub = lane & 7;
     float cs[8], sn[8];
-    const int rotated = p.q_heads + p.heads;
-    const int row0 = part * rows_per_warp, row1 = min(row0 + rows_per_warp, p.q_heads + 2 * p.heads);
     const bool turn = p.phase != nullptr && row0 < rotated;
     if (turn) {
 #pragma unroll
@@ -73,45 +89,42 @@ paged_append_kernel(const __grid_constant__ AppendParams p, int groups, int rows
             sincospif(static_cast<float>(static_cast<int32_t>(frac >> 32)) * 0x1p-31f, &sn[i], &cs[i]);
         }
     }
-    const int lo = p.interleaved ? sub * 16 : sub * 8, hi = p.interleaved ? sub * 16 + 8 : 64 + sub * 8;
-    for (int row = row0 + (lane >> 3); row < row1; row += 4) {
-        const T* src;
-        T* dst = nullptr;
-        if (row < p.q_heads) {
-            src = static_cast<const T*>(p.q) + token * p.q_stride[0] + row * p.q_stride[1];
-            dst = static_cast<T*>(p.q_out) + (static_cast<int64_t>(token) * p.q_heads + row) * kDim;
-        } else if (row < rotated) {
-            src = static_cast<const T*>(p.k) + token * p.k_in[0] + (row - p.q_heads) * p.k_in[1];
-            if (k_at >= 0) dst = static_cast<T*>(p.k_cache) + k_at + (row - p.q_heads) * p.k_stride[2];
-        } else {
-            src = static_cast<const T*>(p.v) + token * p.v_in[0] + (row - rotated) * p.v_in[1];
-            if (v_at >= 0) dst = static_cast<T*>(p.v_cache) + v_at + (row - rotated) * p.v_stride[2];
-        }
-        if (dst == nullptr) continue;
-        uint4 a = *reinterpret_cast<const uint4*>(src + lo), b = *reinterpret_cast<const uint4*>(src + hi);
-        if (turn && row < rotated) {
-            uint32_t* x = &a.x;
-            uint32_t* y = &b.x;
-            if (p.interleaved) {
-                uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    for (int batch = row0; batch < row1; batch += 4 * kAppendBatch) {
+        if (batch > row0) load(batch);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 u = unpack2<T>(w[i]);
-                    w[i] = pack2<T>(u.x * cs[i] - u.y * sn[i], u.y * cs[i] + u.x * sn[i]);
-                }
-                a = make_uint4(w[0], w[1], w[2], w[3]);
-                b = make_uint4(w[4], w[5], w[6], w[7]);
-            } else {
+        for (int i = 0; i < kAppendBatch; ++i) {
+            const int row = batch + 4 * i + (lane >> 3);
+            if (row >= row1) break;
+            T* dst = nullptr;
+            if (row < p.q_heads)
+                dst = static_cast<T*>(p.q_out) + (static_cast<int64_t>(token) * p.q_heads + row) * kDim;
+            else if (row < rotated)
+                dst = k_at >= 0 ? static_cast<T*>(p.k_cache) + k_at + (row - p.q_heads) * p.k_stride[2] : nullptr;
+            else
+                dst = v_at >= 0 ? static_cast<T*>(p.v_cache) + v_at + (row - rotated) * p.v_stride[2] : nullptr;
+            if (dst == nullptr) continue;
+            if (turn && row < rotated) {
+                uint32_t w[8] = {a[i].x, a[i].y, a[i].z, a[i].w, b[i].x, b[i].y, b[i].z, b[i].w};
+                if (p.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 u = unpack2<T>(x[i]), v = unpack2<T>(y[i]);
-                    x[i] = pack2<T>(u.x * cs[2 * i] - v.x * sn[2 * i], u.y * cs[2 * i + 1] - v.y * sn[2 * i + 1]);
-                    y[i] = pack2<T>(v.x * cs[2 * i] + u.x * sn[2 * i], v.y * cs[2 * i + 1] + u.y * sn[2 * i + 1]);
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 u = unpack2<T>(w[j]);
+                        w[j] = pack2<T>(u.x * cs[j] - u.y * sn[j], u.y * cs[j] + u.x * sn[j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 u = unpack2<T>(w[j]), v = unpack2<T>(w[j + 4]);
+                        w[j] = pack2<T>(u.x * cs[2 * j] - v.x * sn[2 * j], u.y * cs[2 * j + 1] - v.y * sn[2 * j + 1]);
+                        w[j + 4] = pack2<T>(v.x * cs[2 * j] + u.x * sn[2 * j], v.y * cs[2 * j + 1] + u.y * sn[2 * j + 1]);
+                    }
                 }
+                a[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                b[i] = make_uint4(w[4], w[5], w[6], w[7]);
             }
+            *reinterpret_cast<uint4*>(dst + lo) = a[i];
+            *reinterpret_cast<uint4*>(dst + hi) = b[i];
         }
-        *reinterpret_cast<uint4*>(dst + lo) = a;
-        *reinterpret_cast<uint4*>(dst + hi) = b;
     }
 }
 
@@ -157,11 +170,18 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
 // barriers.  Ranks come from prefix sums in page or request order, so pages
 // are given and moved in one order whatever the timing; the only atomics are
 // integer additions to the counts and a minimum over request numbers.
-constexpr int kCluster = 8;
+constexpr int kMaxCluster = 8;
 constexpr int kTableThreads = 1024;
+// Entries up to which one CTA is faster than a cluster and its barriers.
+constexpr int64_t kOneCta = 16384;
 
+template <int kCluster>
 __device__ __forceinline__ void cluster_barrier()
 {
+    if (kCluster == 1) {
+        __syncthreads();
+        return;
+    }
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -200,7 +220,7 @@ __host__ __device__ inline Scratch scratch_of(int32_t* s, uint32_t pages, uint32
 {
     Scratch r;
     r.copies = s;                   // copies to make
-    r.counts = s + 32;              // [3][kCluster] per-CTA counts
+    r.counts = s + 32;              // [3][kMaxCluster] per-CTA counts
     r.first = s + 64;               // [pages] free pages, or copy sources
     r.second = r.first + pages;     // [pages] copy destinations
     r.owner = r.second + pages;     // [seqs] first request that names the sequence
@@ -211,7 +231,7 @@ __host__ __device__ inline Scratch scratch_of(int32_t* s, uint32_t pages, uint32
 
 __device__ __forceinline__ int pages_of(int tokens, int width) { return min((max(tokens, 0) + kPage - 1) / kPage, width); }
 
-template <int kOp>
+template <int kOp, int kCluster>
 __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __grid_constant__ TableParams p)
 {
     __shared__ int sums[33];
@@ -236,13 +256,13 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
     }
     if (kOp != kCompact)
         for (int i = all; i < seqs; i += stride) s.owner[i] = INT32_MAX, s.row_of[i] = -1;
-    cluster_barrier();
+    cluster_barrier<kCluster>();
 
     if (kOp == kFork || kOp == kReserve) {
         const int32_t* named = kOp == kFork ? p.b : p.a;
         for (int i = all; i < p.n; i += stride)
             if (named[i] >= 0 && named[i] < seqs) atomicMin(&s.owner[named[i]], i);
-        cluster_barrier();
+        cluster_barrier<kCluster>();
         int free_before = 0, free_all = 0;
         for (int c = 0; c < kCluster; ++c) {
             const int k = __ldcg(&s.counts[c]);
@@ -300,12 +320,12 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
             }
         }
         if (kOp == kFork && cta == 0 && tid == 0) *s.copies = min(needed, free_all);
-        cluster_barrier();
+        cluster_barrier<kCluster>();
     }
     if (kOp == kFree) {
         for (int i = all; i < p.n; i += stride)
             if (p.a[i] >= 0 && p.a[i] < seqs) s.row_of[p.a[i]] = i;
-        cluster_barrier();
+        cluster_barrier<kCluster>();
     }
     if (kOp == kCompact) {
         int live = 0;
@@ -323,7 +343,7 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
         if (tid == 0) s.counts[kCluster + cta] = total;
         block_prefix(movers, sums, total);
         if (tid == 0) s.counts[2 * kCluster + cta] = total;
-        cluster_barrier();
+        cluster_barrier<kCluster>();
         int hole0 = 0, mover0 = 0, moves = 0;
         for (int c = 0; c < kCluster; ++c) {
             if (c < cta) hole0 += __ldcg(&s.counts[kCluster + c]);
@@ -341,7 +361,7 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
             hole0 += n_holes;
             mover0 += n_movers;
         }
-        cluster_barrier();
+        cluster_barrier<kCluster>();
         for (int k = all; k < moves; k += stride) {
             const int from = __ldcg(&s.first[k]), to = __ldcg(&s.second[k]);
             p.moved[from] = to;
@@ -351,7 +371,7 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
             *s.copies = moves;
             *p.live = live;
         }
-        cluster_barrier();
+        cluster_barrier<kCluster>();
     }
 
     // The rows, a warp each.
@@ -411,8 +431,8 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
     }
 }
 
-template <int kOp>
-cudaError_t launch_op(const TableParams& p, cudaStream_t stream)
+template <int kOp, int kCluster>
+cudaError_t launch_op_on(const TableParams& p, cudaStream_t stream)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kCluster);
@@ -425,9 +445,16 @@ cudaError_t launch_op(const TableParams& p, cudaStream_t stream)
     attr[1].val.clusterDim.x = kCluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = kCluster > 1 ? 2 : 1;
     ProfileScope prof(kKernTables, stream);
-    return cudaLaunchKernelEx(&cfg, page_tables_kernel<kOp>, p);
+    return cudaLaunchKernelEx(&cfg, page_tables_kernel<kOp, kCluster>, p);
+}
+
+template <int kOp>
+cudaError_t launch_op(const TableParams& p, cudaStream_t stream)
+{
+    const int64_t entries = static_cast<int64_t>(p.in.seqs) * p.in.width + p.in.pages;
+    return entries <= kOneCta ? launch_op_on<kOp, 1>(p, stream) : launch_op_on<kOp, kMaxCluster>(p, stream);
 }
 
 int sm_count()
