@@ -1266,6 +1266,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 
 // Joins the pieces of tiles that were cut over CTAs: a warp per row.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinBlocks = kTileRows / (kJoinThreads / 32);   // for each CTA that may have ended a cut tile: a row per warp
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const __grid_constant__ AttendParams p)
 {
@@ -1274,9 +1275,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     const Cut cut = p.cuts[blockIdx.y];
     if (!cut.valid) return;
     const int rows_per_tile = 128 / p.group * p.group;
-    const int lane = threadIdx.x & 31, tile_row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-    if (tile_row >= cut.rows) return;
+    const int lane = threadIdx.x & 31;
     const int pieces = blockIdx.y - cut.cta0 + 1;
+    const int tile_row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+    if (tile_row >= cut.rows) return;
     const int r = tile_row < rows_per_tile ? tile_row : 128 + tile_row - rows_per_tile;
     // 32 pieces at a time.
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1387,7 +1389,7 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
         const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attend_tiles_kernel<T>, q_map, k_map, v_map, p);
         if (e != cudaSuccess) return e;
     }
-    cfg.gridDim = dim3(kTileRows / (kJoinThreads / 32), sms);
+    cfg.gridDim = dim3(kJoinBlocks, sms);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     ProfileScope prof(kKernAttendJoin, stream);

@@ -515,7 +515,9 @@ int launch_page_copy(const secure_infer_page_tensor* tensors, uint32_t n_tensors
         p.page_bytes = static_cast<int64_t>(page_bytes);
         for (int i = 0; i < p.tensors; ++i) p.t[i] = tensors[t0 + i];
         const int64_t pieces = static_cast<int64_t>((page_bytes + kCopyPiece - 1) / kCopyPiece) * p.tensors * n;
-        const int64_t cap = 8 * static_cast<int64_t>(sm_count());
+        // Many more blocks than fit at once, so that SMs with a shorter way to memory take more pieces: 1.07 GB in
+        // 179 us with the 8 blocks per SM that fit, 165 with 64; more cost a list shorter than its bound too much.
+        const int64_t cap = 64 * static_cast<int64_t>(sm_count());
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(static_cast<uint32_t>(pieces < cap ? pieces : cap));
         cfg.blockDim = dim3(kCopyThreads);
