@@ -512,17 +512,17 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // exponentials (a 128 x 128 tile takes 1024 clocks of each).  One CTA per SM
 // takes two tiles of up to 128 rows (whole tokens) that share every page.  A
 // warp loads pages by TMA through a ring of four 32 KiB buffers, a warp per tile
-// issues its products, and two warpgroups per tile hold a row in two threads: scores from
-// tensor memory, maximum, weights back over the scores in the cache's type,
+// issues its products, and sixteen warps do both tiles' softmax in turn: scores
+// from tensor memory, maximum, weights back over the scores in the cache's type,
 // from where the second product reads them.  While one tile's softmax runs the
 // other's products do.  The accumulated values are only rescaled when a row's
 // maximum grew by more than 2^8 since the last time; weights up to 2^8 are as
 // exact as weights up to 1, and the sums are 32-bit.  Tensor memory: scores
 // (and weights) of the tiles at columns 0 and 128, values at 256 and 384.
-constexpr int kSoftWarps = 16;       // four warpgroups: two tiles, two halves of a page's keys
+constexpr int kSoftWarps = 16;       // four warpgroups, each with a quarter of a page's keys
 constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, checker
 constexpr int kRing = 4;
-constexpr uint32_t kStageBytes = 32 * 64;   // 64 bytes of a softmax warp's rows, on their way to coalesced stores
+constexpr uint32_t kStageBytes = 32 * 32;   // 32 bytes of a softmax warp's rows, on their way to whole sectors
 constexpr uint32_t kTileBytes = 128 * kDim * 2;
 constexpr int kItems = 8;
 constexpr int kTileRows = 256;
@@ -559,17 +559,6 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[16
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&r)[32])
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -696,17 +685,17 @@ struct Item {
 
 struct TilesControl {
     uint64_t kv_full[kRing], kv_empty[kRing], q_full, q_empty;
-    uint64_t s_full[2], p_ready[2], o_full[2], drained[2], turn[2];
+    uint64_t s_full[2], p_ready[2], o_full[2], drained[2];
     uint64_t checked, taken, item_full[kItems];
     Item items[kItems];
-    float exchange[2][2][128];           // between a row's two threads
+    float exchange[2][4][128];           // between a row's four threads
     int32_t warp_sums[kTileThreads / 32];
     Share share;
     uint32_t tmem;
     int irregular;                       // what the checker found in the piece
     int stop;                            // a wait ran out
 };
-constexpr uint32_t kControlBytes = 4096 - 1024;   // the first KiB of shared memory is the driver's
+constexpr uint32_t kControlBytes = 8192 - 1024;   // the first KiB of shared memory is the driver's
 static_assert(sizeof(TilesControl) <= kControlBytes, "control block");
 constexpr uint32_t kTilesSmem = kControlBytes + (2 + kRing) * kTileBytes + kSoftWarps * kStageBytes;
 
@@ -729,7 +718,6 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     auto s_full = [&](int w) { return smem_addr(&c.s_full[w]); };
     auto p_ready = [&](int w) { return smem_addr(&c.p_ready[w]); };
     auto o_full = [&](int w) { return smem_addr(&c.o_full[w]); };
-    auto turn = [&](int w) { return smem_addr(&c.turn[w]); };
     auto drained = [&](int w) { return smem_addr(&c.drained[w]); };
     auto item_full = [&](uint32_t i) { return smem_addr(&c.item_full[i % kItems]); };
     const uint32_t checked = smem_addr(&c.checked), taken = smem_addr(&c.taken);
@@ -744,10 +732,9 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         barrier_init(q_empty, 2);
         for (int w = 0; w < 2; ++w) {
             barrier_init(s_full(w), 1);
-            barrier_init(p_ready(w), kSoftWarps / 2);
+            barrier_init(p_ready(w), kSoftWarps);
             barrier_init(o_full(w), 1);
             barrier_init(drained(w), 1);
-            barrier_init(turn(w), 1);
         }
         barrier_init(checked, 1);
         barrier_init(taken, kSoftWarps);
@@ -841,20 +828,13 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             }
             __syncwarp();
         } else if (warp < kSoftWarps + 3) {
-            // Products, a warp per tile, in turns of one page: while one tile's products run the other warp has done
-            // its waiting, and the two softmax warpgroups stay half a page apart instead of fighting for the same units.
+            // Products, a warp per tile.  The softmax warps take the tiles in turn, and so do these.
             const int t = warp - kSoftWarps - 1;
             constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
             constexpr uint32_t desc = 1u << 4 | type << 7 | type << 10 | (128u >> 3) << 17 | (128u >> 4) << 24;
             constexpr uint32_t desc_v = desc | 1u << 16;   // V's rows run along the sum
             const uint32_t q = operand(q_smem + t * kTileBytes, 0), s_at = tmem + t * 128, o_at = tmem + 256 + t * 128;
-            uint32_t n = 0, item = 0, ready = 0, turns = 0;   // buffers and items taken, softmax tiles, turns
-            auto my_turn = [&](bool both) {
-                if (!both) return true;
-                const bool mine = t == 0 && turns == 0 ? true : barrier_wait(turn(t), (turns - (t == 0)) & 1, stop);
-                ++turns;
-                return mine;
-            };
+            uint32_t n = 0, item = 0, ready = 0;   // buffers and pieces taken, softmax tiles
             auto scores = [&](uint32_t slot) {
                 const uint32_t k = operand(ring + slot * kTileBytes, 0);
                 product_smem<false>(s_at, operand_at(q, 0), operand_at(k, 0), desc);
@@ -881,13 +861,11 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                     if (lane == 0) barrier_arrive(q_empty);
                 } else {
-                    const bool both = w.rows > rows_per_tile;
-                    ok = ok && barrier_wait(kv_full(n % kRing), (n / kRing) & 1, stop) && my_turn(both);
+                    ok = ok && barrier_wait(kv_full(n % kRing), (n / kRing) & 1, stop);
                     if (!ok) break;
                     tmem_fence_after();
                     if (elected()) {
                         scores(n % kRing);
-                        if (both) barrier_arrive(turn(1 - t));
                         if (pages == 1) commit_to(q_empty);
                     }
                     __syncwarp();
@@ -914,7 +892,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             __syncwarp();
                         }
                         if (ok && more) ok = barrier_wait(kv_full(k_slot), ((n + 1) / kRing) & 1, stop);
-                        ok = ok && barrier_wait(p_ready(t), ready & 1, stop) && my_turn(both);
+                        ok = ok && barrier_wait(p_ready(t), ready & 1, stop);
                         if (!ok) break;
                         ++ready;
                         tmem_fence_after();
@@ -934,7 +912,6 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             else commit_to(o_full(t));
                             commit_to(kv_empty(v_slot));
                             if (i + 2 == pages) commit_to(q_empty);
-                            if (both) barrier_arrive(turn(1 - t));
                         }
                         __syncwarp();
                         n += more ? 2 : 1;
@@ -992,63 +969,59 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             }
         }
     } else {
-        // Softmax: a row of a tile by two threads, each with half of a page's keys.  After a wait that ran out the
-        // loops run on without waiting, so the two keep meeting.
+        // Softmax: a row by four threads, each with a quarter of a page's keys, the tiles in turn: while one tile's
+        // products run all warps are at the other.  After a wait that ran out the loops run on without waiting, so
+        // the four keep meeting.
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-        const int t = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
-        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-        const uint32_t s_at = tmem + lanes + t * 128 + half * 64, w_at = tmem + lanes + t * 128 + half * 32;
-        const uint32_t o_at = tmem + lanes + 256 + t * 128 + half * 64;
+        const int quarter = warp >> 2, rows0 = (warp & 3) * 32, row = rows0 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
         const float scale = fabsf(p.scale_log2);
         const bool flip = p.scale_log2 < 0.0f;
-        // The two warps that hold a tile's 32 rows: whether any of their threads says so.
+        // The four warps that hold the same 32 rows: whether any of their threads says so.
         auto meet_or = [&](bool x) {
             uint32_t r;
-            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.aligned.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.aligned.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
                          : "=r"(r)
-                         : "r"(1 + t * 4 + (warp & 3)), "r"(static_cast<uint32_t>(x))
+                         : "r"(1 + (warp & 3)), "r"(static_cast<uint32_t>(x))
                          : "memory");
             return r != 0;
         };
         const int token = row / p.group, g = row % p.group;   // within the tile
         const int rel = token * p.heads * p.group + g;        // rows of the output from the tile's first
-        uint32_t seen = 0, done = 0, item = 0;   // completions of s_full and o_full taken
+        uint32_t seen[2] = {0, 0}, done[2] = {0, 0}, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
         while (any) {
             if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
             const Item& w = c.items[item % kItems];
-            const int pages = w.pages;
-            const bool used = t == 0 || w.rows > rows_per_tile;
-            int lo, hi;
-            w.keys(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
-            const int lo_all = w.lo_all, hi_all = w.hi_all;
-            const int page_key = w.first_key, first_key = page_key + half * 64;
-            float m = -INFINITY, l = 0.0f;
-            if (used) {
-                for (int i = 0; i < pages; ++i) {
-                    ok = ok && barrier_wait(s_full(t), seen & 1, stop);
-                    ++seen;
+            const int pages = w.pages, tiles = w.rows > rows_per_tile ? 2 : 1;
+            const int lo_all = w.lo_all, hi_all = w.hi_all, page_key = w.first_key;
+            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+            for (int i = 0; i < pages; ++i) {
+                // By the whole page and both tiles, so that all threads agree.
+                const int page0 = page_key + i * kPage;
+                const bool masked = page0 < lo_all || page0 + kPage - 1 > hi_all;
+#pragma unroll 1
+                for (int t = 0; t < tiles; ++t) {
+                    ok = ok && barrier_wait(s_full(t), (t ? seen[1] : seen[0]) & 1, stop);
+                    if (t) ++seen[1];
+                    else ++seen[0];
                     tmem_fence_after();
-                    const int key0 = first_key + i * kPage;
-                    // By the whole page, so that a row's two threads agree.
-                    const int page0 = page_key + i * kPage;
-                    const bool masked = page0 < lo_all || page0 + kPage - 1 > hi_all;
+                    float m = t ? m1 : m0, l = t ? l1 : l0;
+                    const uint32_t s_at = lanes + t * 128 + quarter * 32, w_at = lanes + t * 128 + quarter * 16;
                     bool fresh = i == 0 || masked || flip;
                     if (!fresh) {
                         // The usual page: weights by the maximum so far, while the page's own is found.
-                        uint32_t s[2][32], w2[32];
-                        tmem_load<32>(s[0], s_at);
-                        tmem_load<32>(s[1], s_at + 32);
+                        uint32_t s[32], w2[16];
+                        tmem_load<32>(s, s_at);
                         tmem_wait_loads();
                         const float base = m == -INFINITY ? 0.0f : m * scale;
                         const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
                         uint64_t sum[2] = {};
                         float tops[2] = {m, m};
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const uint32_t s0 = s[j >> 4][(j & 15) * 2], s1 = s[j >> 4][(j & 15) * 2 + 1];
-                            const uint64_t x = fma2(pair(s0, s1), scale2, base2);
-                            tops[j & 1] = max3_nan(tops[j & 1], __uint_as_float(s0), __uint_as_float(s1));
+                        for (int j = 0; j < 16; ++j) {
+                            const uint64_t x = fma2(pair(s[2 * j], s[2 * j + 1]), scale2, base2);
+                            tops[j & 1] = max3_nan(tops[j & 1], __uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]));
                             float2 e;
                             // A quarter of the exponentials go to the multiply-add units, which levels these with the
                             // special function units.
@@ -1063,7 +1036,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             w2[j] = pack2<T>(e.x, e.y);
                         }
                         const float top = max3_nan(tops[0], tops[1], tops[1]);
-                        // Weights may cover scores once the row's other thread has read its own.
+                        // Weights may cover scores once the row's other threads have read theirs.
                         tmem_fence_before();
                         fresh = meet_or(!((top - m) * scale <= kRescale) && top != -INFINITY);
                         tmem_fence_after();
@@ -1075,44 +1048,44 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                     if (fresh) {
                         // The first page, one whose mask hides keys, or one that some row's maximum outgrew.
-                        uint32_t s[2][32];
-                        tmem_load<32>(s[0], s_at);
-                        tmem_load<32>(s[1], s_at + 32);
+                        uint32_t s[32];
+                        tmem_load<32>(s, s_at);
                         tmem_wait_loads();
                         if (flip) {
 #pragma unroll
-                            for (int j = 0; j < 64; ++j) s[j >> 5][j & 31] ^= 0x80000000u;
+                            for (int j = 0; j < 32; ++j) s[j] ^= 0x80000000u;
                         }
                         if (masked) {
                             // Bits of the keys from lo to hi.
-                            const int a = max(0, lo - key0), b = min(63, hi - key0);
-                            const uint64_t bits = b < a ? 0 : (~0ull << a) & (~0ull >> (63 - b));
-                            const uint32_t keep[2] = {static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32)};
+                            int lo, hi;
+                            w.keys(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
+                            const int a = max(0, lo - page0 - quarter * 32), b = min(31, hi - page0 - quarter * 32);
+                            const uint32_t keep = b < a ? 0 : (~0u << a) & (~0u >> (31 - b));
 #pragma unroll
-                            for (int j = 0; j < 64; ++j)
-                                if (!(keep[j >> 5] >> (j & 31) & 1)) s[j >> 5][j & 31] = 0xff800000u;
+                            for (int j = 0; j < 32; ++j)
+                                if (!(keep >> j & 1)) s[j] = 0xff800000u;
                         }
-                        float tops[4] = {m, m, m, m};
+                        float tops[2] = {m, m};
 #pragma unroll
-                        for (int j = 0; j < 64; j += 2)
-                            tops[(j >> 1) & 3] = max3_nan(tops[(j >> 1) & 3], __uint_as_float(s[j >> 5][j & 31]),
-                                                          __uint_as_float(s[j >> 5][(j & 31) + 1]));
-                        float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-                        // And the row's other thread's.
-                        c.exchange[t][half][row] = top;
+                        for (int j = 0; j < 32; j += 2)
+                            tops[(j >> 1) & 1] = max3_nan(tops[(j >> 1) & 1], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                        float top = max3_nan(tops[0], tops[1], tops[1]);
+                        // And the row's other threads'.
+                        c.exchange[t][quarter][row] = top;
                         tmem_fence_before();
                         meet_or(false);
                         tmem_fence_after();
-                        const float other = c.exchange[t][half ^ 1][row];
-                        top = max3_nan(top, other, other);
+                        const float* others = &c.exchange[t][0][row];
+                        top = max3_nan(max3_nan(others[0], others[128], others[256]), others[384], top);
                         if (top == INFINITY) top = NAN;   // a NaN or infinite score makes its row NaN
                         if (i == 0) {
                             m = top;
                         } else if (__any_sync(0xffffffffu, !((top - m) * scale <= kRescale) && top != -INFINITY)) {
                             const float f = m == top ? 1.0f : exp2_approx((m - top) * scale);
                             l *= f;
+                            const uint32_t o_at = lanes + 256 + t * 128 + quarter * 32;
 #pragma unroll 1
-                            for (int d = 0; d < 64; d += 16) {
+                            for (int d = 0; d < 32; d += 16) {
                                 uint32_t o[16];
                                 tmem_load<16>(o, o_at + d);
                                 tmem_wait_loads();
@@ -1123,116 +1096,123 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             m = top;
                         }
                         const float base = m == -INFINITY ? 0.0f : m * scale;
-                        float sum[4] = {};
+                        float sum[2] = {};
+                        uint32_t w2[16];
 #pragma unroll
-                        for (int j = 0; j < 64; j += 2) {
-                            const float e0 = exp2_approx(fmaf(__uint_as_float(s[j >> 5][j & 31]), scale, -base));
-                            const float e1 = exp2_approx(fmaf(__uint_as_float(s[j >> 5][(j & 31) + 1]), scale, -base));
-                            sum[(j >> 1) & 3] += e0 + e1;
-                            s[j >> 6][j >> 1] = pack2<T>(e0, e1);
+                        for (int j = 0; j < 16; ++j) {
+                            const float e0 = exp2_approx(fmaf(__uint_as_float(s[2 * j]), scale, -base));
+                            const float e1 = exp2_approx(fmaf(__uint_as_float(s[2 * j + 1]), scale, -base));
+                            sum[j & 1] += e0 + e1;
+                            w2[j] = pack2<T>(e0, e1);
                         }
-                        tmem_store(w_at, s[0]);
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        tmem_store(w_at, w2);
+                        l += sum[0] + sum[1];
                     }
+                    if (t) m1 = m, l1 = l;
+                    else m0 = m, l0 = l;
                     tmem_wait_stores();
                     tmem_fence_before();
                     __syncwarp();
                     if (lane == 0) barrier_arrive(p_ready(t));
                 }
-                ok = ok && barrier_wait(o_full(t), done & 1, stop);
-                ++done;
-                c.exchange[t][half][row] = l;
-                meet_or(false);
-                l += c.exchange[t][half ^ 1][row];
-                meet_or(false);   // read before the next page's maxima come
             }
             ok = ok && barrier_wait(checked, item & 1, stop);
-            tmem_fence_after();
-            const bool split = w.slot >= 0;
+            const bool split = w.slot >= 0, by_definition = *static_cast<volatile int*>(&c.irregular) != 0;
             float* slot = p.slots + static_cast<int64_t>(w.slot) * kTileSlot;
-            // Output row of the tile's first row.
-            const int64_t out0 = static_cast<int64_t>(w.q0 + t * tokens) * p.heads * p.group + w.head * p.group;
-            const int valid_rows = min(rows_per_tile, w.rows - t * rows_per_tile);
-            const bool by_definition = *static_cast<volatile int*>(&c.irregular) != 0;
-            if (by_definition) {
-                const int ka = page_key, kb = ka + pages * kPage;
-                for (int r = (warp & 3) * 32 + half; r < min((warp & 3) * 32 + 32, valid_rows); r += 2) {
-                    const int tok = t * tokens + r / p.group;
-                    int a, b;
-                    w.keys(p, w.pos + tok, a, b);
-                    float mm, ll;
-                    float4 x;
-                    row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q0 + tok) * p.q_token +
-                                                (w.head * p.group + r % p.group) * p.q_head,
-                                         p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, kb), mm, ll, x);
-                    if (split) {
-                        *reinterpret_cast<float4*>(slot + (t * 128 + r) * kDim + lane * 4) = x;
-                        if (lane == 0) {
-                            slot[kTileRows * kDim + t * 128 + r] = mm;
-                            slot[kTileRows * kDim + kTileRows + t * 128 + r] = ll;
+            const uint32_t stage = ring + kRing * kTileBytes + warp * kStageBytes;
+#pragma unroll 1
+            for (int t = 0; t < tiles; ++t) {
+                ok = ok && barrier_wait(o_full(t), (t ? done[1] : done[0]) & 1, stop);
+                if (t) ++done[1];
+                else ++done[0];
+                tmem_fence_after();
+                // Output row of the tile's first row, and how many of the warp's rows are used.
+                const int64_t out0 = static_cast<int64_t>(w.q0 + t * tokens) * p.heads * p.group + w.head * p.group;
+                const int valid = min(rows_per_tile, w.rows - t * rows_per_tile) - rows0;
+                if (by_definition) {
+                    for (int r = quarter; r < min(32, valid); r += 4) {
+                        const int tok = (rows0 + r) / p.group, head = (rows0 + r) % p.group;
+                        int a, b;
+                        w.keys(p, w.pos + t * tokens + tok, a, b);
+                        float mm, ll;
+                        float4 x;
+                        row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q0 + t * tokens + tok) * p.q_token +
+                                                    (w.head * p.group + head) * p.q_head,
+                                             p.table + w.s * p.table_stride, w.head, max(a, page_key),
+                                             min(b + 1, page_key + pages * kPage), mm, ll, x);
+                        if (split) {
+                            *reinterpret_cast<float4*>(slot + (t * 128 + rows0 + r) * kDim + lane * 4) = x;
+                            if (lane == 0) {
+                                slot[kTileRows * kDim + t * 128 + rows0 + r] = mm;
+                                slot[kTileRows * kDim + kTileRows + t * 128 + rows0 + r] = ll;
+                            }
+                        } else {
+                            const float inv = 1.0f / ll;
+                            const int64_t at = out0 + tok * p.heads * p.group + head;
+                            uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+                            if (b < a) packed = make_uint2(0, 0);
+                            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
+                            if (p.lse != nullptr && lane == 0)
+                                p.lse[at] = b >= a ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
                         }
-                    } else {
-                        const float inv = 1.0f / ll;
-                        const int64_t at = out0 + r / p.group * p.heads * p.group + r % p.group;
-                        uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-                        if (b < a) packed = make_uint2(0, 0);
-                        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
-                        if (p.lse != nullptr && lane == 0)
-                            p.lse[at] = b >= a ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
                     }
+                    continue;
                 }
-            } else if (used) {
-                // Rows leave through a warp's own piece of shared memory, 64 bytes of each at a time, so that a store
-                // covers whole sectors: eight rows by four lanes.
-                const float inv = hi >= lo ? 1.0f / l : 0.0f;
-                const uint32_t stage = ring + kRing * kTileBytes + warp * kStageBytes;
-                const int valid = valid_rows - (warp & 3) * 32;
-                auto put = [&](const uint32_t (&x)[16]) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((j ^ (lane >> 1 & 3)) << 4)),
-                                     "r"(x[4 * j]), "r"(x[4 * j + 1]), "r"(x[4 * j + 2]), "r"(x[4 * j + 3])
-                                     : "memory");
-                    __syncwarp();
+                c.exchange[t][quarter][row] = t ? l1 : l0;
+                meet_or(false);
+                const float* parts = &c.exchange[t][0][row];
+                const float l = (parts[0] + parts[128]) + (parts[256] + parts[384]);
+                meet_or(false);   // read before the next piece's maxima come
+                int lo, hi;
+                w.keys(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
+                const float inv = 1.0f / l;
+                // Rows leave through a warp's own piece of shared memory, 32 bytes of each at a time, so that a store
+                // covers whole sectors: sixteen rows by two lanes.
+                auto put = [&](uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, int j) {
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 32 + ((j ^ (lane >> 2 & 1)) << 4)),
+                                 "r"(x0), "r"(x1), "r"(x2), "r"(x3)
+                                 : "memory");
                 };
                 auto get = [&](int r) {
                     uint4 x;
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                  : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                                 : "r"(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4))
+                                 : "r"(stage + r * 32 + (((lane & 1) ^ (r >> 2 & 1)) << 4))
                                  : "memory");
                     return x;
                 };
+                uint32_t o[32];
+                tmem_load<32>(o, lanes + 256 + t * 128 + quarter * 32);
+                tmem_wait_loads();
                 if (split) {
-                    float* part = slot + (t * 128 + (warp & 3) * 32) * kDim + half * 64 + (lane & 3) * 4;
-#pragma unroll 1
-                    for (int d = 0; d < 64; d += 16) {
-                        uint32_t o[16];
-                        tmem_load<16>(o, o_at + d);
-                        tmem_wait_loads();
-                        put(o);
+                    float* part = slot + (t * 128 + rows0) * kDim + quarter * 32 + (lane & 1) * 4;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int r = k * 8 + (lane >> 2);
+                    for (int d = 0; d < 32; d += 8) {
+                        put(o[d], o[d + 1], o[d + 2], o[d + 3], 0);
+                        put(o[d + 4], o[d + 5], o[d + 6], o[d + 7], 1);
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int r = k * 16 + (lane >> 1);
                             const uint4 x = get(r);
                             if (r < valid) *reinterpret_cast<uint4*>(part + r * kDim + d) = x;
                         }
                         __syncwarp();
                     }
                 } else {
-                    T* out = static_cast<T*>(p.out) + out0 * kDim + half * 64 + (lane & 3) * 8;
-#pragma unroll 1
-                    for (int d = 0; d < 64; d += 32) {
-                        uint32_t o[32], x[16];
-                        tmem_load<32>(o, o_at + d);
-                        tmem_wait_loads();
+                    T* out = static_cast<T*>(p.out) + out0 * kDim + quarter * 32 + (lane & 1) * 8;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            x[j] = hi >= lo ? pack2<T>(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv) : 0u;
-                        put(x);
+                    for (int d = 0; d < 32; d += 16) {
+                        uint32_t x[8];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int r = k * 8 + (lane >> 2);
+                        for (int j = 0; j < 8; ++j)
+                            x[j] = hi >= lo ? pack2<T>(__uint_as_float(o[d + 2 * j]) * inv, __uint_as_float(o[d + 2 * j + 1]) * inv) : 0u;
+                        put(x[0], x[1], x[2], x[3], 0);
+                        put(x[4], x[5], x[6], x[7], 1);
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int r = k * 16 + (lane >> 1);
                             const int64_t to = __shfl_sync(0xffffffffu, rel, r);
                             const uint4 y = get(r);
                             if (r < valid) *reinterpret_cast<uint4*>(out + to * kDim + d) = y;
@@ -1240,8 +1220,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         __syncwarp();
                     }
                 }
-                if (row < valid_rows && half == 0) {
-                    const float top = m * scale;
+                if (lane < valid && quarter == 0) {
+                    const float top = (t ? m1 : m0) * scale;
                     if (split) {
                         slot[kTileRows * kDim + t * 128 + row] = top;
                         slot[kTileRows * kDim + kTileRows + t * 128 + row] = l;
