@@ -48,9 +48,8 @@ struct AttendParams {
 };
 
 // Launchers (cudaError_t values).
-// Tiles of up to `rows` rows (8 or 16); any number of them.
-int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows,
-                       uint32_t dtype, cudaStream_t stream);
+int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, uint32_t dtype,
+                       cudaStream_t stream);
 // q_map: boxes of [128 / group tokens][group heads][64 values].
 int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
                         const AttendParams& p, uint32_t dtype, cudaStream_t stream);
@@ -281,6 +280,7 @@ struct Share {
     int32_t per, more, ctas, total;
     int32_t begin, units;      // of this CTA
     int32_t seq, seq_unit;     // sequence of its first unit, and that sequence's first unit
+    Seq q;
 
     __device__ __forceinline__ int begin_of(int cta) const { return cta * per + min(cta, more); }
     __device__ __forceinline__ int owner(int unit) const
@@ -336,20 +336,24 @@ struct Walk {
     }
 };
 
-__device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost)
+// Units of a sequence; `largest`: of a tile.
+__device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost, int& largest)
 {
-    if (s.n == 0) return 0;
-    int pages = 0;
+    int units = 0;
     const int rows = s.n * p.group;
-    for (int r = 0; r < rows; r += rows_per_tile)
-        pages += tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages + cost;
-    return pages * p.heads;
+    for (int r = 0; r < rows; r += rows_per_tile) {
+        const int u = tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages + cost;
+        units += u;
+        largest = max(largest, u);
+    }
+    return units * p.heads;
 }
 
-// All threads of the block take part; `warp_sums` holds one value per warp.
-// At least min_units go to a CTA that has any, so short work is not split.
+// All threads of the block take part; `warp_sums` holds two values per warp.
+// Where no tile has more than `whole` units a CTA gets the largest one's:
+// cutting it would cost more than the few pages that it would save.
 template <int kThreads>
-__device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int cost, int min_units, Share* share,
+__device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int cost, int whole, Share* share,
                                            int32_t* warp_sums)
 {
     constexpr int kWarps = kThreads / 32;
@@ -360,16 +364,23 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
     // has a thread one pass does both.
     const bool one = p.seqs <= kThreads;
     for (int pass = one ? 1 : 0; pass < 2; ++pass) {
-        int base = 0;
+        int base = 0, largest = 0;
         for (int s0 = 0; s0 < p.seqs; s0 += kThreads) {
             const int s = s0 + tid;
-            const int own = s < p.seqs ? seq_units(p, load_seq(p, s), rows_per_tile, cost) : 0;
+            Seq q{};
+            int own_largest = 0;
+            if (s < p.seqs) q = load_seq(p, s);
+            const int own = seq_units(p, q, rows_per_tile, cost, own_largest);
             int sum = own;
             for (int d = 1; d < 32; d <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, sum, d);
                 if (lane >= d) sum += up;
             }
-            if (lane == 31) warp_sums[warp] = sum;
+            own_largest = __reduce_max_sync(0xffffffffu, own_largest);
+            if (lane == 31) {
+                warp_sums[warp] = sum;
+                warp_sums[kWarps + warp] = own_largest;
+            }
             __syncthreads();
             int before = base;
 #pragma unroll
@@ -377,10 +388,11 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
                 const int x = warp_sums[w];
                 if (w < warp) before += x;
                 base += x;
+                largest = max(largest, warp_sums[kWarps + w]);
             }
             if (one || (pass == 0 && s0 + kThreads >= p.seqs)) {
                 r.total = base;
-                r.ctas = max(1, min(static_cast<int>(gridDim.x), base / min_units));
+                r.ctas = max(1, min(static_cast<int>(gridDim.x), largest <= whole ? base / max(1, largest) : base));
                 r.per = base / r.ctas;
                 r.more = base - r.per * r.ctas;
                 const int c = blockIdx.x;
@@ -398,6 +410,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
                 if (r.units > 0 && own > 0 && r.begin >= first && r.begin < first + own) {
                     share->seq = s;
                     share->seq_unit = first;
+                    share->q = q;
                 }
             }
             __syncthreads();
@@ -414,7 +427,7 @@ __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_t
     if (share.seq < 0) return w;
     w.left = share.units;
     w.s = share.seq;
-    w.q = load_seq(p, w.s);
+    w.q = share.q;
     w.tiles = (w.q.n * p.group + rows_per_tile - 1) / rows_per_tile;
     w.tile = 0;
     w.tile_unit = share.seq_unit;

@@ -79,10 +79,11 @@ bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, int64_t token_str
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Rows per KV head up to which a sequence goes to the kernel for few rows.
-// Measured with 24 sequences of up to 4096 tokens, 8 KV heads: 12 rows 55 us
-// there; 32 rows 87 us there (in tiles of 16 warps' rows) and 75 us in tiles.
-constexpr uint32_t kFewRows = 16;
+// Rows per KV head up to which a sequence goes to the kernel for few rows, in
+// tiles of eight.  Measured with 24 sequences of up to 4096 tokens and 8 KV
+// heads: 20 rows 54 us there and 59 in tiles of 128, 32 rows 100 and 53; with
+// one of 300 tokens 7.3 and 14.0, 7.7 and 14.1.
+constexpr uint32_t kFewRows = 24;
 
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)
 {
@@ -121,9 +122,9 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     const uint32_t max_q = chunk->max_q == 0 || chunk->max_q > chunk->tokens ? chunk->tokens : chunk->max_q;
     const uint64_t max_rows = static_cast<uint64_t>(max_q) * group;
     if (max_rows > INT_MAX) return -1;
-    // Units of work (a page for 16 rows and a KV head) are counted in 32 bits.
-    const uint64_t tiles16 = static_cast<uint64_t>(chunk->tokens) * group / 16 + chunk->seqs;
-    if (tiles16 * pages->heads > INT_MAX || tiles16 * pages->heads * chunk->table_width > INT_MAX) return -1;
+    // Units of work (a page for eight rows and a KV head) are counted in 32 bits.
+    const uint64_t tiles8 = (static_cast<uint64_t>(chunk->tokens) * group / 8 + chunk->seqs) * pages->heads;
+    if (tiles8 > INT_MAX || tiles8 * (chunk->table_width + 1) > INT_MAX) return -1;
 
     AttendParams p;
     std::memset(&p, 0, sizeof(p));
@@ -165,9 +166,7 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
         if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
             return -1;
         p.rows_max = tiles ? kFewRows : INT_MAX;
-        // Beside tiles the few rows are mostly single tokens.
-        const uint64_t rows = tiles ? group : max_rows;
-        if (launch_attend_rows(k_map, v_map, p, rows <= 8 ? 8 : 16, pages->dtype, st) != 0) return -1;
+        if (launch_attend_rows(k_map, v_map, p, pages->dtype, st) != 0) return -1;
         p.rows_min = kFewRows + 1;
         p.rows_max = INT_MAX;
     }

@@ -57,7 +57,7 @@ __device__ __forceinline__ void join_row(int n, Stats stats, int sums, Values va
 
 // ---------------------------------------------------------------- few rows
 //
-// Single tokens and short drafts: up to 16 rows per KV head and tile, bound by
+// Single tokens and short drafts: tiles of eight rows of a KV head, bound by
 // reading K and V once.  One CTA per SM; a producer warp keeps three pages
 // (64 KiB each, K and V) in flight by TMA.  Each of eight warps takes 16 keys of
 // each page, with its own running maximum and sum, so no warp waits for another
@@ -75,15 +75,16 @@ constexpr int kRowsStages = 3;
 constexpr int kQuarter = 32;                              // tokens of one TMA box
 constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 tokens][64 values]
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
-constexpr int kMaxRows = 16;
-constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kMaxRows * 256 + 2 * kRowsWarps * 16 * 4;
+constexpr int kRows = 8;
+constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kRows * 256 + 2 * kRowsWarps * kRows * 4;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
-constexpr int kRowsMinUnits = 1;
+// One sequence of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
+constexpr int kRowsWhole = 4;
 constexpr int kRowsCost = 1;   // pages that a tile's end is worth
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
 // more in a second step.
 constexpr int kJoinRows = 160;
-constexpr int kRowSlot = kMaxRows * (kDim + 2);
+constexpr int kRowSlot = kRows * (kDim + 2);
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -128,17 +129,15 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x)
 // Barrier of the eight computing warps.
 __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory"); }
 
-// kNs groups of eight rows.
-template <typename T, int kNs>
+template <typename T>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                          const __grid_constant__ AttendParams p)
 {
-    constexpr int kRows = 8 * kNs;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
     __shared__ Share share;
-    __shared__ int32_t warp_sums[kRowsThreads / 32];
+    __shared__ int32_t warp_sums[2 * kRowsThreads / 32];
     __shared__ volatile int stop;   // a wait ran out
     __shared__ int irregular, last_piece, give_up;
 
@@ -146,8 +145,8 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     const uint32_t k_smem = smem_addr(base), v_smem = k_smem + kRowsStages * kPageTile;
     const uint32_t q_smem = v_smem + kRowsStages * kPageTile;
     uint8_t* q_bytes = base + 2 * kRowsStages * kPageTile;
-    float* join_m = reinterpret_cast<float*>(q_bytes + kMaxRows * 256);
-    float* join_l = join_m + kRowsWarps * 16;
+    float* join_m = reinterpret_cast<float*>(q_bytes + kRows * 256);
+    float* join_l = join_m + kRowsWarps * kRows;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto k_full = [&](int s) { return smem_addr(&bars[s]); };
@@ -166,7 +165,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     wait_for_earlier_kernels();
-    find_share<kRowsThreads>(p, kRows, kRowsCost, kRowsMinUnits, &share, warp_sums);
+    find_share<kRowsThreads>(p, kRows, kRowsCost, kRowsWhole, &share, warp_sums);
     dependents_may_launch();
     Walk w = start_walk(p, kRows, kRowsCost, share);
 
@@ -229,42 +228,31 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
         const bool split = cta1 > cta0;
         float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
-        int lo[kNs][2], hi[kNs][2];   // keys that this thread's rows see
-        int all_lo, all_hi;           // keys that every row of the tile sees
+        int lo[2], hi[2];   // keys that this thread's rows see
+        int all_lo, all_hi; // keys that every row of the tile sees
         {
             int unused;
             row_keys(p, w.q, w.last_token, all_lo, unused);
             row_keys(p, w.q, w.first_token, unused, all_hi);
         }
 #pragma unroll
-        for (int n = 0; n < kNs; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = n * 8 + (lane & 3) * 2 + e;
-                row_keys(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[n][e], hi[n][e]);
-            }
-        // Sums of values: o[j][n] holds values 16 j + lane / 4 (+ 8) of rows 8 n + 2 (lane % 4) (+ 1).
-        float m[kNs][2], l[kNs][2], o[8][kNs][4];
-#pragma unroll
-        for (int n = 0; n < kNs; ++n) {
-            m[n][0] = m[n][1] = -INFINITY;
-            l[n][0] = l[n][1] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[j][n][c] = 0.0f;
+        for (int e = 0; e < 2; ++e) {
+            const int r = (lane & 3) * 2 + e;
+            row_keys(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[e], hi[e]);
         }
-        rows_sync();
-        // 32 values of eight rows; one group of rows stays in registers, two would not fit beside the sums.
-        auto load_q = [&](uint32_t (&x)[4], int n, int d) {
-            const int r = n * 8 + (lane & 7), piece = d * 4 + (lane >> 3);
-            ldmatrix4(x, q_smem + r * 256 + ((piece ^ (r & 7)) << 4));
-        };
-        uint32_t q[kNs][4][4];
-        if (kNs == 1)
+        // Sums of values: o[j] holds values 16 j + lane / 4 (+ 8) of rows 2 (lane % 4) (+ 1).
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[8][4];
 #pragma unroll
-            for (int d = 0; d < 4; ++d) load_q(q[0][d], 0, d);
-        const int groups = (w.rows + 7) / 8;   // that are used
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[j][c] = 0.0f;
+        rows_sync();
+        uint32_t q[4][4];   // 32 values of the rows each
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const int r = lane & 7, piece = d * 4 + (lane >> 3);
+            ldmatrix4(q[d], q_smem + r * 256 + ((piece ^ r) << 4));
+        }
 
         for (int i = 0; i < pages; ++i, ++unit) {
             const int stage = unit % kRowsStages;
@@ -274,60 +262,50 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             if (key0 < w.span.hi && key0 + 16 > w.span.lo) {
                 const uint32_t slice = stage * kPageTile + (warp >> 1) * kQuarterBytes + (warp & 1) * 16 * 128;
                 const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
-                float s[kNs][2][4] = {};   // two chains of products
+                float s[2][4] = {};   // two chains of products
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {   // 16 values of the head at a time
-                    if (kNs > 1 && (d & 1) == 0)
-#pragma unroll
-                        for (int n = 0; n < kNs; ++n) load_q(q[n][d >> 1], n, d >> 1);
                     uint32_t a[4];
                     const int key = lane & 15, chunk = (d & 3) * 2 + (lane >> 4);
                     ldmatrix4(a, k_smem + slice + (d >> 2) * (kQuarterBytes / 2) + key * 128 + ((chunk ^ (key & 7)) << 4));
-#pragma unroll
-                    for (int n = 0; n < kNs; ++n)
-                        if (n < groups) mma16816<T>(s[n][d & 1], a, q[n][d >> 1][(d & 1) * 2], q[n][d >> 1][(d & 1) * 2 + 1]);
+                    mma16816<T>(s[d & 1], a, q[d >> 1][(d & 1) * 2], q[d >> 1][(d & 1) * 2 + 1]);
                 }
-                uint32_t weight[kNs][2];
+                float x[4], top[2] = {m[0], m[1]};
 #pragma unroll
-                for (int n = 0; n < kNs; ++n) {
-                    float x[4], top[2] = {m[n][0], m[n][1]};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        x[c] = (s[n][0][c] + s[n][1][c]) * p.scale_log2;
-                        if (!whole) {
-                            const int key = key0 + (lane >> 2) + (c >> 1) * 8;
-                            if (key < lo[n][c & 1] || key > hi[n][c & 1]) x[c] = -INFINITY;
-                        }
-                        top[c & 1] = fmaxf(top[c & 1], x[c]);
+                for (int c = 0; c < 4; ++c) {
+                    x[c] = (s[0][c] + s[1][c]) * p.scale_log2;
+                    if (!whole) {
+                        const int key = key0 + (lane >> 2) + (c >> 1) * 8;
+                        if (key < lo[c & 1] || key > hi[c & 1]) x[c] = -INFINITY;
                     }
+                    top[c & 1] = fmaxf(top[c & 1], x[c]);
+                }
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) {
-                        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
-                        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
-                    }
-                    if (__any_sync(0xffffffffu, top[0] != m[n][0] || top[1] != m[n][1])) {
+                for (int d = 4; d < 32; d <<= 1) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+                }
+                if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float f = m[n][e] == top[e] ? 1.0f : exp2_approx(m[n][e] - top[e]);
-                            m[n][e] = top[e];
-                            l[n][e] *= f;
+                    for (int e = 0; e < 2; ++e) {
+                        const float f = m[e] == top[e] ? 1.0f : exp2_approx(m[e] - top[e]);
+                        m[e] = top[e];
+                        l[e] *= f;
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                o[j][n][e] *= f;
-                                o[j][n][e + 2] *= f;
-                            }
+                        for (int j = 0; j < 8; ++j) {
+                            o[j][e] *= f;
+                            o[j][e + 2] *= f;
                         }
                     }
-                    const float base0 = top[0] == -INFINITY ? 0.0f : top[0], base1 = top[1] == -INFINITY ? 0.0f : top[1];
-                    const float e0 = exp2_approx(x[0] - base0), e1 = exp2_approx(x[1] - base1);
-                    const float e2 = exp2_approx(x[2] - base0), e3 = exp2_approx(x[3] - base1);
-                    l[n][0] += e0 + e2;
-                    l[n][1] += e1 + e3;
-                    // Weights are rounded to the cache's type for the product; their sum is not.  Keys by rows become
-                    // rows by keys.
-                    weight[n][0] = transposed(pack2<T>(e0, e1));
-                    weight[n][1] = transposed(pack2<T>(e2, e3));
                 }
+                const float base0 = top[0] == -INFINITY ? 0.0f : top[0], base1 = top[1] == -INFINITY ? 0.0f : top[1];
+                const float e0 = exp2_approx(x[0] - base0), e1 = exp2_approx(x[1] - base1);
+                const float e2 = exp2_approx(x[2] - base0), e3 = exp2_approx(x[3] - base1);
+                l[0] += e0 + e2;
+                l[1] += e1 + e3;
+                // Weights are rounded to the cache's type for the product; their sum is not.  Keys by rows become rows
+                // by keys.
+                const uint32_t weight0 = transposed(pack2<T>(e0, e1)), weight1 = transposed(pack2<T>(e2, e3));
                 uint32_t keep[2] = {0, 0};   // values of keys that some row sees: this lane's keys 2t, 2t + 1, and 8 more
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -347,9 +325,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                             odd = zero_sum<T>(odd, a[c]);
                         }
                     }
-#pragma unroll
-                    for (int n = 0; n < kNs; ++n)
-                        if (n < groups) mma16816<T>(o[j][n], a, weight[n][0], weight[n][1]);
+                    mma16816<T>(o[j], a, weight0, weight1);
                 }
                 if (!whole && w.first_token != w.last_token && zero_sum_odd<T>(odd)) irregular = 1;
             }
@@ -359,37 +335,31 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 
         // Join the warps' results where the last page lay: its buffers are given back afterwards.
 #pragma unroll
-        for (int n = 0; n < kNs; ++n)
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-                if (lane < 4) {
-                    join_m[warp * 16 + n * 8 + lane * 2 + e] = m[n][e];
-                    join_l[warp * 16 + n * 8 + lane * 2 + e] = l[n][e];
-                }
+            for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+            if (lane < 4) {
+                join_m[warp * kRows + lane * 2 + e] = m[e];
+                join_l[warp * kRows + lane * 2 + e] = l[e];
             }
+        }
         if (tid == 0) give_up = stop;
         rows_sync();
         if (give_up) break;
         const int last_stage = (unit - 1) % kRowsStages;
         const bool by_definition = irregular != 0;
-        // Warp i's [16 rows][128] floats, columns swizzled by the row against bank conflicts.
-        auto joined = [&](int i) { return base + ((i < 4 ? 0 : kRowsStages) + last_stage) * kPageTile + (i & 3) * 8192; };
+        // Warp i's [8 rows][128] floats, columns swizzled by the row against bank conflicts.
+        auto joined = [&](int i) { return base + last_stage * kPageTile + i * 4096; };
 #pragma unroll
-        for (int n = 0; n < kNs; ++n) {
-            if (n >= groups) break;
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int r = n * 8 + (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
-                    *reinterpret_cast<float*>(joined(warp) + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][n][c];
-                }
-        }
+            for (int c = 0; c < 4; ++c) {
+                const int r = (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
+                *reinterpret_cast<float*>(joined(warp) + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][c];
+            }
         rows_sync();
-#pragma unroll 1
-        for (int r = warp; r < w.rows; r += kRowsWarps) {
+        // A warp per row.
+        if (const int r = warp; r < w.rows) {
             const int token = (r0 + r) / p.group, g = (r0 + r) - token * p.group;
             int a, b;
             row_keys(p, w.q, token, a, b);
@@ -402,7 +372,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                                      p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, ka + pages * kPage), top,
                                      sum, x);
             } else {
-                const int stat = (lane & (kRowsWarps - 1)) * 16 + r;
+                const int stat = (lane & (kRowsWarps - 1)) * kRows + r;
                 const float mi = join_m[stat];
                 top = mi;
 #pragma unroll
@@ -463,7 +433,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 if (!last_piece) break;
                 __threadfence();
                 const bool final = step > 1 || n == pieces;
-                for (int r = warp; r < w.rows; r += kRowsWarps) {
+                if (const int r = warp; r < w.rows) {
                     float4 x;
                     float top, sum;
                     join_row(
@@ -476,18 +446,18 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                             to[kRows * kDim + r] = top;
                             to[kRows * kDim + kRows + r] = sum;
                         }
-                        continue;
+                    } else {
+                        const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
+                        int a, b;
+                        row_keys(p, w.q, token, a, b);
+                        const float inv = 1.0f / sum;
+                        const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + g;
+                        uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+                        if (b < a) packed = make_uint2(0, 0);
+                        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
+                        if (p.lse != nullptr && lane == 0)
+                            p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
                     }
-                    const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
-                    int a, b;
-                    row_keys(p, w.q, token, a, b);
-                    const float inv = 1.0f / sum;
-                    const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + g;
-                    uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-                    if (b < a) packed = make_uint2(0, 0);
-                    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
-                    if (p.lse != nullptr && lane == 0)
-                        p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
                 }
                 if (final) break;
                 first = 0;
@@ -689,7 +659,7 @@ struct TilesControl {
     uint64_t checked, taken, item_full[kItems];
     Item items[kItems];
     float exchange[2][4][128];           // between a row's four threads
-    int32_t warp_sums[kTileThreads / 32];
+    int32_t warp_sums[2 * kTileThreads / 32];
     Share share;
     uint32_t tmem;
     int irregular;                       // what the checker found in the piece
@@ -753,7 +723,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads>(p, 2 * rows_per_tile, kTilesCost, 1, &c.share, c.warp_sums);
+    find_share<kTileThreads>(p, 2 * rows_per_tile, kTilesCost, 0, &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
@@ -1289,13 +1259,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
 
 struct Device {
     int sms = 0;
-    bool rows_set[2][2] = {};
+    bool rows_set[2] = {};
     bool tiles_set[2] = {};
 };
 std::mutex g_mu;
 Device g_devices[64];
 
-template <typename T, int kNs>
+template <typename T>
 int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, cudaStream_t stream)
 {
     int dev = 0;
@@ -1305,9 +1275,9 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
         if (d.sms == 0) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
-        bool& set = d.rows_set[std::is_same<T, __half>::value][kNs - 1];
+        bool& set = d.rows_set[std::is_same<T, __half>::value];
         if (!set) {
-            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, kNs>,
+            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T>,
                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
             if (e != cudaSuccess) return e;
             set = true;
@@ -1325,13 +1295,7 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     ProfileScope prof(kKernAttendRows, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, kNs>, k_map, v_map, p);
-}
-
-template <typename T>
-int launch_rows_for(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows, cudaStream_t stream)
-{
-    return rows <= 8 ? launch_rows<T, 1>(k_map, v_map, p, stream) : launch_rows<T, 2>(k_map, v_map, p, stream);
+    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T>, k_map, v_map, p);
 }
 
 template <typename T>
@@ -1385,11 +1349,11 @@ int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, cons
                                       : launch_tiles<__nv_bfloat16>(q_map, k_map, v_map, p, stream);
 }
 
-int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, int rows,
-                       uint32_t dtype, cudaStream_t stream)
+int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, uint32_t dtype,
+                       cudaStream_t stream)
 {
-    return dtype == SECURE_INFER_FP16 ? launch_rows_for<__half>(k_map, v_map, p, rows, stream)
-                                      : launch_rows_for<__nv_bfloat16>(k_map, v_map, p, rows, stream);
+    return dtype == SECURE_INFER_FP16 ? launch_rows<__half>(k_map, v_map, p, stream)
+                                      : launch_rows<__nv_bfloat16>(k_map, v_map, p, stream);
 }
 
 uint64_t attend_workspace_bytes()
