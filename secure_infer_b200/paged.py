@@ -90,25 +90,29 @@ class LayerPages:
     one type, in any order of pages, tokens and heads in memory."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
-        _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device, "K and V differ in shape, type or device")
-        _need(k.ndim == 4 and k.shape[0] > 0 and k.shape[1] == PAGE and k.shape[2] > 0 and k.shape[3] == HEAD_DIM,
-              f"a cache is [pages, {PAGE}, heads, {HEAD_DIM}], not {list(k.shape)}")
-        _need(k.dtype in _DTYPES, f"a cache holds bf16 or fp16, not {k.dtype}")
-        _need(k.is_cuda, "the cache must be on a CUDA device")
+        shape, dtype, device = k.shape, k.dtype, k.device
+        if v.shape != shape or v.dtype is not dtype or v.device != device:
+            raise ValueError("K and V differ in shape, type or device")
+        if len(shape) != 4 or shape[0] == 0 or shape[1] != PAGE or shape[2] == 0 or shape[3] != HEAD_DIM:
+            raise ValueError(f"a cache is [pages, {PAGE}, heads, {HEAD_DIM}], not {list(shape)}")
+        if dtype not in _DTYPES:
+            raise ValueError(f"a cache holds bf16 or fp16, not {dtype}")
+        if not k.is_cuda:
+            raise ValueError("the cache must be on a CUDA device")
         strides = []
         for t in (k, v):
-            s = list(t.stride())
-            if t.shape[0] == 1:
-                s[0] = PAGE * HEAD_DIM * t.shape[2]
-            if t.shape[2] == 1:
-                s[2] = HEAD_DIM
-            _need(s[3] == 1 and t.data_ptr() % 16 == 0 and all(x > 0 and x % 8 == 0 for x in s[:3]),
-                  "a head's values must be adjacent, the cache's address and strides multiples of 16 bytes")
-            strides.append(s[:3])
+            sp, st, sh, sd = t.stride()
+            if shape[0] == 1:
+                sp = PAGE * HEAD_DIM * shape[2]
+            if shape[2] == 1:
+                sh = HEAD_DIM
+            if sd != 1 or t.data_ptr() & 15 or sp <= 0 or st <= 0 or sh <= 0 or (sp | st | sh) & 7:
+                raise ValueError("a head's values must be adjacent, the cache's address and strides multiples of 16 bytes")
+            strides.append((sp, st, sh))
         self.k, self.v = k, v
-        self.pages, self.heads, self.dtype, self.device = k.shape[0], k.shape[2], k.dtype, k.device
-        self._c = _native.Pages(k.data_ptr(), v.data_ptr(), (ct.c_int64 * 3)(*strides[0]), (ct.c_int64 * 3)(*strides[1]),
-                                self.pages, self.heads, _DTYPES[k.dtype], 0)
+        self.pages, self.heads, self.dtype, self.device = shape[0], shape[2], dtype, device
+        self._strides = tuple(strides)
+        self._c = _native.Pages(k.data_ptr(), v.data_ptr(), strides[0], strides[1], self.pages, self.heads, _DTYPES[dtype], 0)
         self._ref = ct.byref(self._c)
 
 
@@ -154,11 +158,14 @@ class Rotary:
         _need(len(sections) > 0 and all(n >= 0 for n in sections) and sum(sections) == HEAD_DIM // 2,
               f"sections must be counts that add up to {HEAD_DIM // 2}")
         self.axes, self.interleaved = len(sections), bool(interleaved)
-        # Revolutions per position as a fraction of 2^64, so a position's angle is an exact product modulo one turn.
+        # Revolutions per position as a fraction of 2^64, so a position's angle is an exact product modulo one turn; the
+        # axis of each pair behind them.
         turns = [round(base ** (-i / 64) / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for i in range(HEAD_DIM // 2)]
-        self.phase = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
-        self.axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32, device=device)
-        self.device = self.phase.device
+        axis = [a for a, n in enumerate(sections) for _ in range(n)]
+        table = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns] +
+                             [axis[i] | axis[i + 1] << 32 for i in range(0, HEAD_DIM // 2, 2)], dtype=torch.int64, device=device)
+        self.phase, self.axis = table[:HEAD_DIM // 2], table[HEAD_DIM // 2:].view(torch.int32)
+        self.device = table.device
         self._phase, self._axis = self.phase.data_ptr(), self.axis.data_ptr()
 
 
@@ -304,20 +311,22 @@ class CachePages:
         _need(len(self.layers) > 0, "a cache has at least one layer")
         first = self.layers[0]
         self.pages, self.device = first.pages, first.device
-        tensors = [t for layer in self.layers for t in (layer.k, layer.v)]
-        _need(all(t.shape == first.k.shape and t.dtype == first.dtype and t.device == first.device for t in tensors),
-              "the layers' caches differ in shape, type or device")
-        self.page_bytes = first.k[0].numel() * first.k.element_size()
-        arr = (_native.PageTensor * len(tensors))()
-        for i, t in enumerate(tensors):
-            inner = sorted((s, n) for s, n in zip(t.stride()[1:], t.shape[1:]) if n > 1)
-            dense, expect = True, 1
-            for s, n in inner:
-                dense, expect = dense and s == expect, expect * n
-            stride = t.stride(0) * t.element_size() if t.shape[0] > 1 else self.page_bytes
-            _need(dense and stride >= self.page_bytes, "a page's values must fill one block of memory")
-            arr[i].base, arr[i].page_stride = t.data_ptr(), stride
-        self._tensors = arr
+        shape, size = first.k.shape, first.k.element_size()
+        self.page_bytes = PAGE * first.heads * HEAD_DIM * size
+        self._tensors = (_native.PageTensor * (2 * len(self.layers)))()
+        dense = {}   # page strides of the layouts met so far
+        for i, layer in enumerate(self.layers):
+            if layer.k.shape != shape or layer.dtype is not first.dtype or layer.device != first.device:
+                raise ValueError("the layers' caches differ in shape, type or device")
+            for j, (t, strides) in enumerate(zip((layer.k, layer.v), layer._strides)):
+                if strides not in dense:
+                    page, token, head = strides
+                    inner = (token, head) if first.heads == 1 else sorted((token, head))
+                    fills = token == HEAD_DIM if first.heads == 1 else \
+                        inner[0] == HEAD_DIM and inner[1] == HEAD_DIM * (first.heads if inner[0] == head else PAGE)
+                    _need(fills and page * size >= self.page_bytes, "a page's values must fill one block of memory")
+                    dense[strides] = page * size
+                self._tensors[2 * i + j] = (t.data_ptr(), dense[strides])
 
     def _check(self, t: PageTables) -> _native.Tables:
         if not isinstance(t, PageTables):
