@@ -179,6 +179,27 @@ def lib() -> ct.CDLL:
     return _lib
 
 
+_paged = None
+
+
+def paged_ops():
+    """Load (once) and return the extension ``_build/paged_python.so``: the
+    paged-cache calls of every layer and step (csrc/paged_python.cpp)."""
+    global _paged
+    if _paged is None:
+        import importlib.util
+
+        import torch  # noqa: F401 -- its libraries are the extension's
+        path = LIB_PATH.parent / "paged_python.so"
+        if not path.exists():
+            raise NativeLibraryMissing(f"{path} is missing; build it with `python -m secure_infer_b200.build`")
+        spec = importlib.util.spec_from_file_location("paged_python", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _paged = module
+    return _paged
+
+
 def host_pool_info() -> dict:
     """This rank's host worker pool: OpenSSL worker threads (the calling
     thread encrypts as well), the CPUs of the rank's slice and whether the

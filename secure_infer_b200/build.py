@@ -26,6 +26,11 @@ LIB = BUILD / "libsecure_infer.so"
 # cudaMemcpyAsync at run time.
 INTERPOSE = BUILD / "libsecure_infer_interpose.so"
 
+# Calls of secure_infer_b200.paged as a CPython extension (host code only); it
+# links libsecure_infer.so from its own directory and torch, which is loaded by
+# then.
+PAGED = BUILD / "paged_python.so"
+
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden,-O3",
@@ -76,7 +81,27 @@ def build(force: bool = False, verbose: bool = False) -> Path:
                f"-Wl,--version-script={script}", "-Wl,--exclude-libs,ALL"]
         print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
+    build_paged(force)
     return LIB
+
+
+def build_paged(force: bool = False) -> Path:
+    src = CSRC / "paged_python.cpp"
+    if force or _stale(PAGED, [src, ROOT / "include" / "secure_infer_paged.h", LIB]):
+        import sysconfig
+
+        import torch
+        torch_dir = Path(torch.__file__).resolve().parent
+        cxx = os.environ.get("CXX", "g++")
+        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f"-I{torch_dir / 'include'}", f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+               f"-I{sysconfig.get_paths()['include']}", f"-I{Path(NVCC).resolve().parent.parent / 'include'}", str(src),
+               "-o", str(PAGED), f"-L{BUILD}", "-lsecure_infer", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu",
+               "-lc10", "-Wl,-rpath,$ORIGIN", "-Wl,--exclude-libs,ALL"]
+        print(" ".join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
+    return PAGED
 
 
 def main():

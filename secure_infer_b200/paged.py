@@ -14,7 +14,9 @@ step for all its layers.  Calls run on the current stream and return without
 waiting; lengths, tables and page ids stay on the device.  Bad arguments raise
 ``ValueError`` before anything is launched, a refused launch ``RuntimeError``.
 As everywhere in this package there is no fallback: the work goes through
-``libsecure_infer.so``.
+``libsecure_infer.so``.  The calls of every layer (``append``, ``attend``) and
+``free`` reach it by a small extension (csrc/paged_python.cpp), which also looks
+their tensors over; the others by ctypes.
 """
 from __future__ import annotations
 
@@ -52,37 +54,12 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _stream(device) -> int:
-    return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
-
-
-def _rows(t: torch.Tensor, what: str, tokens: int, dtype, device) -> tuple[int, int, int]:
-    """Heads and strides of [tokens, heads, 128].  On the way of every call:
-    texts are only made where something is wrong."""
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != tokens or shape[2] != HEAD_DIM:
-        raise ValueError(f"{what} must be [{tokens}, heads, {HEAD_DIM}], not {list(shape)}")
-    if t.dtype is not dtype or t.device != device:
-        raise ValueError(f"{what} must be {dtype} on {device}")
-    st, sh, sd = t.stride()
-    # A single token or head has no stride of its own.
-    if tokens <= 1:
-        st = HEAD_DIM
-    if shape[1] <= 1:
-        sh = HEAD_DIM
-    if sd != 1 or st <= 0 or sh <= 0 or (st | sh) & 7 or t.data_ptr() & 15:
-        raise ValueError(f"{what}: a head's values must be adjacent, the address and strides multiples of 16 bytes")
-    return shape[1], st, sh
-
-
-def _like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
-    """A dense output of q's shape, or the given one checked."""
-    if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
-    if out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device or not out.is_contiguous() \
-            or out.data_ptr() & 15:
-        raise ValueError("out must be dense, with q's shape, type and device")
-    return out
+def _on(index: int, function, *args):
+    """function(*args) with device `index` current."""
+    if index == torch.cuda.current_device():
+        return function(*args)
+    with torch.cuda.device(index):
+        return function(*args)
 
 
 class LayerPages:
@@ -110,10 +87,10 @@ class LayerPages:
                 raise ValueError("a head's values must be adjacent, the cache's address and strides multiples of 16 bytes")
             strides.append((sp, st, sh))
         self.k, self.v = k, v
-        self.pages, self.heads, self.dtype, self.device = shape[0], shape[2], dtype, device
+        self.pages, self.heads, self.dtype, self.device, self.index = shape[0], shape[2], dtype, device, device.index
         self._strides = tuple(strides)
         self._c = _native.Pages(k.data_ptr(), v.data_ptr(), strides[0], strides[1], self.pages, self.heads, _DTYPES[dtype], 0)
-        self._ref = ct.byref(self._c)
+        self._address = ct.addressof(self._c)
 
 
 class Chunk:
@@ -142,7 +119,7 @@ class Chunk:
         self.block_table, self.cu_q, self.kv_lens, self.device = block_table, cu_q, kv_lens, device
         self._c = _native.Chunk(block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), stride, width, seqs, 0,
                                 max_q or 0)
-        self._ref = ct.byref(self._c)
+        self._address = ct.addressof(self._c)
 
 
 class Rotary:
@@ -166,17 +143,11 @@ class Rotary:
                              [axis[i] | axis[i + 1] << 32 for i in range(0, HEAD_DIM // 2, 2)], dtype=torch.int64, device=device)
         self.phase, self.axis = table[:HEAD_DIM // 2], table[HEAD_DIM // 2:].view(torch.int32)
         self.device = table.device
-        self._phase, self._axis = self.phase.data_ptr(), self.axis.data_ptr()
+        self._c = (self.phase.data_ptr(), self.axis.data_ptr(), self.axes, self.interleaved)
 
 
 def _call(name: str, device, *args) -> None:
-    function = getattr(_native.lib(), name)
-    if device.index is not None and device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            rc = function(*args)
-    else:
-        rc = function(*args)
-    if rc != 0:
+    if _on(device.index, getattr(_native.lib(), name), *args) != 0:
         raise RuntimeError(f"{name} refused its arguments or failed to launch")
 
 
@@ -189,44 +160,12 @@ def append(pages: LayerPages, chunk: Chunk, q: torch.Tensor | None, k: torch.Ten
     ``positions`` int32 ``[axes, tokens]`` or ``[tokens]``; by default the
     tokens' places in their sequences.  A token whose place lies outside its
     sequence's pages is not written."""
-    tokens, device, dtype = k.shape[0], pages.device, pages.dtype
-    if chunk.device != device:
-        raise ValueError("the chunk and the cache are on different devices")
-    heads, kt, kh = _rows(k, "k", tokens, dtype, device)
-    v_heads, vt, vh = _rows(v, "v", tokens, dtype, device)
-    if heads != pages.heads or v_heads != heads:
-        raise ValueError(f"k and v must have the cache's {pages.heads} heads")
-    q_heads = qt = qh = 0
-    q_ptr = out_ptr = None
-    if q is not None:
-        q_heads, qt, qh = _rows(q, "q", tokens, dtype, device)
-        out = _like(q, out)
-        q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
-    elif out is not None:
-        raise ValueError("out goes with q")
-    phase = axis = pos_ptr = None
-    pos_stride, axes, interleaved = 0, 1, False
-    if rotary is not None:
-        if rotary.device != device:
-            raise ValueError("rotary and the cache are on different devices")
-        phase, axis, axes, interleaved = rotary._phase, rotary._axis, rotary.axes, rotary.interleaved
-        if positions is not None:
-            _ints(positions, "positions", device, positions.ndim)
-            shape = tuple(positions.shape)
-            if shape != (axes, tokens) and not (axes == 1 and shape == (tokens,)):
-                raise ValueError(f"positions must be [{axes}, {tokens}]")
-            pos_ptr, pos_stride = positions.data_ptr(), positions.stride(0) if axes > 1 else tokens
-            if pos_stride < 0:
-                raise ValueError("positions has a negative stride")
-    elif positions is not None:
-        raise ValueError("positions go with rotary")
-    if tokens == 0:
-        return out
-    if chunk._c.tokens != tokens:
-        chunk._c.tokens = tokens
-    _call("secure_infer_paged_append", device, pages._ref, chunk._ref, q_ptr, qt, qh, q_heads, out_ptr, k.data_ptr(), kt,
-          kh, v.data_ptr(), vt, vh, phase, axis, pos_ptr, pos_stride, axes, interleaved, _stream(device))
-    return out
+    if chunk.device != pages.device or (rotary is not None and rotary.device != pages.device):
+        raise ValueError("the chunk, rotary and the cache are on different devices")
+    phase, axis, axes, interleaved = (0, 0, 1, False) if rotary is None else rotary._c
+    index = pages.index
+    return _on(index, _native.paged_ops().append, pages._address, chunk._address, index, q, k, v, phase, axis, axes,
+               interleaved, positions, out, _raw_stream(index))
 
 
 _workspaces: dict = {}
@@ -237,13 +176,13 @@ def attend_workspace(device) -> torch.Tensor:
     return torch.zeros(int(_native.lib().secure_infer_paged_attend_workspace()), dtype=torch.uint8, device=device)
 
 
-def _workspace(device, stream: int) -> torch.Tensor:
-    w = _workspaces.get((device, stream))
+def _workspace(index: int, stream: int) -> torch.Tensor:
+    w = _workspaces.get((index, stream))
     if w is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("attend's first call on a stream makes its workspace: make it before capturing, "
                                "or pass workspace=attend_workspace(device)")
-        w = _workspaces[(device, stream)] = attend_workspace(device)
+        w = _workspaces[index, stream] = attend_workspace(torch.device("cuda", index))
     return w
 
 
@@ -261,29 +200,13 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
     other keys.  A row that sees no key gives 0 and -inf.  ``workspace``:
     ``attend_workspace(device)``, by default one that the current stream
     keeps."""
-    device, tokens = pages.device, q.shape[0]
-    if chunk.device != device:
+    if chunk.device != pages.device:
         raise ValueError("the chunk and the cache are on different devices")
-    q_heads, qt, qh = _rows(q, "q", tokens, pages.dtype, device)
-    if q_heads == 0 or q_heads % pages.heads:
-        raise ValueError(f"q's heads must be a multiple of the cache's {pages.heads}")
-    if not 0 <= window < 1 << 31 or (window and not causal):
-        raise ValueError("window must be zero or positive, and goes with causal")
-    out = _like(q, out)
-    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=device) if return_lse else None
-    if tokens > 0:
-        stream = _stream(device)
-        if workspace is None:
-            workspace = _workspace(device, stream)
-        elif workspace.device != device or not workspace.is_contiguous() or workspace.data_ptr() & 255 or \
-                workspace.numel() * workspace.element_size() < _native.lib().secure_infer_paged_attend_workspace():
-            raise ValueError("workspace must come from attend_workspace of the cache's device")
-        if chunk._c.tokens != tokens:
-            chunk._c.tokens = tokens
-        _call("secure_infer_paged_attend", device, pages._ref, chunk._ref, q.data_ptr(), qt, qh, q_heads, out.data_ptr(),
-              lse.data_ptr() if return_lse else None, HEAD_DIM ** -0.5 if scale is None else scale, bool(causal), window,
-              workspace.data_ptr(), stream)
-    return (out, lse) if return_lse else out
+    index = pages.index
+    stream = _raw_stream(index)
+    return _on(index, _native.paged_ops().attend, pages._address, chunk._address, index, q, out, return_lse,
+               HEAD_DIM ** -0.5 if scale is None else scale, causal, window,
+               _workspace(index, stream) if workspace is None else workspace, stream)
 
 
 class _Tables(NamedTuple):
@@ -380,7 +303,7 @@ class CachePages:
             _need(all(0 <= i < self.pages for i in src + dst), "page outside the cache")
         src, dst = self._pair(src, dst, ("src", "dst"))
         _call("secure_infer_paged_copy", self.device, self._tensors, len(self._tensors), self.page_bytes, self.pages,
-              src.data_ptr(), dst.data_ptr(), src.shape[0], _stream(self.device))
+              src.data_ptr(), dst.data_ptr(), src.shape[0], _raw_stream(self.device.index))
 
     def fork(self, tables: PageTables, parents, children, out: PageTables | None = None):
         """Give the empty sequence ``children[i]`` the tokens of ``parents[i]``:
@@ -395,7 +318,7 @@ class CachePages:
         scratch = self._scratch(c, n)
         _call("secure_infer_paged_fork", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
               ct.byref(o), a.data_ptr(), b.data_ptr(), n, granted.data_ptr(), scratch.data_ptr(),
-              _stream(self.device))
+              _raw_stream(self.device.index))
         return out, granted
 
     def reserve(self, tables: PageTables, seqs, lens, out: PageTables | None = None):
@@ -409,17 +332,20 @@ class CachePages:
         granted = torch.empty(n, dtype=torch.int32, device=self.device)
         scratch = self._scratch(c, n)
         _call("secure_infer_paged_reserve", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), b.data_ptr(), n,
-              granted.data_ptr(), scratch.data_ptr(), _stream(self.device))
+              granted.data_ptr(), scratch.data_ptr(), _raw_stream(self.device.index))
         return out, granted
 
     def free(self, tables: PageTables, seqs, out: PageTables | None = None) -> PageTables:
         """Empty the sequences ``seqs``; a page that no other row holds becomes
         free.  Returns the new tables."""
         a = _ints(seqs, "seqs", self.device, 1)
+        if out is None and isinstance(tables, PageTables):
+            index = self.device.index
+            return PageTables(*_on(index, _native.paged_ops().free, *tables, self.pages, index, a, _raw_stream(index)))
         c, out, o = self._outputs(tables, out)
         scratch = self._scratch(c, a.shape[0])
         _call("secure_infer_paged_free", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), a.shape[0],
-              scratch.data_ptr(), _stream(self.device))
+              scratch.data_ptr(), _raw_stream(self.device.index))
         return out
 
     def compact(self, tables: PageTables, out: PageTables | None = None):
@@ -434,5 +360,5 @@ class CachePages:
         scratch = self._scratch(c, 0)
         _call("secure_infer_paged_compact", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
               ct.byref(o), moved.data_ptr(), live.data_ptr(), scratch.data_ptr(),
-              _stream(self.device))
+              _raw_stream(self.device.index))
         return out, moved, live

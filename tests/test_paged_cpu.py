@@ -152,3 +152,28 @@ def test_rotary_phases_are_exact_fractions_of_a_turn():
             got = Decimal((pos * phase) % (1 << 64)) / Decimal(1 << 64)
             off = abs(got - want)
             assert min(off, 1 - off) < Decimal("1e-9")   # 2^-53 of the phase times 2^20 positions
+
+
+def test_extension_refuses_before_any_launch():
+    """The calls of every layer look their arguments over in the extension."""
+    ops = _native.paged_ops()
+    with pytest.raises(TypeError):
+        ops.attend(1, 2)
+    pages, chunk, _ = good()
+    p, c = ct.addressof(pages), ct.addressof(chunk)
+    q = torch.zeros((3, 32, 128), dtype=torch.bfloat16)
+    for bad in (q, q[:, :, :64], q.float(), q[0], None, 7):
+        with pytest.raises(ValueError):
+            ops.attend(p, c, 0, bad, None, False, 1.0, True, 0, None, 0)
+        with pytest.raises(ValueError):
+            ops.append(p, c, 0, None, bad, bad, 0, 0, 1, False, None, None, 0)
+    t = torch.zeros((2, 2), dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.free(t, t[0], t[0], 2, 0, t[0], 0)
+
+
+def test_extension_missing_is_said(monkeypatch, tmp_path):
+    monkeypatch.setattr(_native, "_paged", None)
+    monkeypatch.setattr(_native, "LIB_PATH", tmp_path / "libsecure_infer.so")
+    with pytest.raises(_native.NativeLibraryMissing, match="paged_python"):
+        _native.paged_ops()
