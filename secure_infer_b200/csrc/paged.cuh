@@ -44,7 +44,9 @@ struct AttendParams {
     uint32_t* counters;             // three of each CTA, zero between launches
     uint32_t* status;
     Cut* cuts;                      // [grid]
-    float* slots;                   // [2 * grid] partial results
+    float* slots;                   // [2 * grid] partial results of tiles
+    float* row_slots;               // and of the kernel for few rows
+    int32_t beside;                 // the kernel for few rows runs just before in the same call
 };
 
 // Launchers (cudaError_t values).

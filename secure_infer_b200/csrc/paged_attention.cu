@@ -227,7 +227,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         }
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
         const bool split = cta1 > cta0;
-        float* slot = p.slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
+        float* slot = p.row_slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
         int lo[2], hi[2];   // keys that this thread's rows see
         int all_lo, all_hi; // keys that every row of the tile sees
         {
@@ -417,7 +417,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             // one CTA, in two steps: the last of each group of neighbours joins these into its first, the last group
             // those.  Either way in the order of the pieces.
             const int pieces = cta1 - cta0 + 1, mine = static_cast<int>(blockIdx.x) - cta0;
-            auto slot_of = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cta0 + i) + (i == 0)) * kRowSlot; };
+            auto slot_of = [&](int i) { return p.row_slots + static_cast<int64_t>(2 * (cta0 + i) + (i == 0)) * kRowSlot; };
             int group = pieces;
             if (pieces * w.rows > kJoinRows || pieces > 32) {
                 group = 2;
@@ -679,6 +679,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     volatile int* const stop = &c.stop;
     const uint32_t q_smem = smem_addr(smem_raw) + kControlBytes, ring = q_smem + 2 * kTileBytes;
     if (q_smem & 1023) {   // the swizzle needs it; shared memory would have to start elsewhere
+        wait_for_earlier_kernels();
         if (threadIdx.x == 0) atomicOr(p.status, 2u);
         return;
     }
@@ -721,7 +722,9 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tmem_fence_before();
     }
-    wait_for_earlier_kernels();
+    // Beside the kernel for few rows this one starts as that one's CTAs leave: its inputs were complete before that one
+    // read them, the two share no memory that either writes, and it waits for that one at its end instead.
+    if (!p.beside) wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
     find_share<kTileThreads>(p, 2 * rows_per_tile, kTilesCost, 0, &c.share, c.warp_sums);
     dependents_may_launch();
@@ -1211,6 +1214,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     tmem_fence_before();
     __syncthreads();
+    if (p.beside) wait_for_earlier_kernels();
     if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
@@ -1358,7 +1362,7 @@ int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const
 
 uint64_t attend_workspace_bytes()
 {
-    return kSlotOffset + static_cast<uint64_t>(2 * kMaxGrid) * kTileSlot * sizeof(float);
+    return kSlotOffset + static_cast<uint64_t>(2 * kMaxGrid) * (kTileSlot + kRowSlot) * sizeof(float);
 }
 
 void attend_workspace(void* workspace, AttendParams* p)
@@ -1367,6 +1371,7 @@ void attend_workspace(void* workspace, AttendParams* p)
     p->status = p->counters + 3 * kMaxGrid;
     p->cuts = reinterpret_cast<Cut*>(static_cast<char*>(workspace) + kCutOffset);
     p->slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotOffset);
+    p->row_slots = p->slots + static_cast<uint64_t>(2 * kMaxGrid) * kTileSlot;
 }
 
 }  // namespace paged
