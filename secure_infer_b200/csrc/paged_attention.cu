@@ -61,14 +61,19 @@ __device__ __forceinline__ void join_row(int n, Stats stats, int sums, Values va
 // reading K and V once.  One CTA per SM; a producer warp keeps three pages
 // (64 KiB each, K and V) in flight by TMA.  Each of eight warps takes 16 keys of
 // each page, with its own running maximum and sum, so no warp waits for another
-// inside the loop.  The products are m16n8k16 with
-// the keys (then the values of a head) as M and eight rows as N: a group of
-// eight query heads or fewer fills one N, where rows as M would pad them to
-// sixteen, and these instructions are slow enough here to matter (about 20
-// clocks of a quarter SM).  The results join in shared memory at the tile's
-// end, and a tile cut over several CTAs is joined by the last of them to
-// finish, in the order of the cuts, so results do not depend on the order of
-// arrival.
+// inside the loop.  The products are m16n8k16 with the keys (then the values of
+// a head) as M and eight rows as N: a group of eight query heads or fewer fills
+// one N, where rows as M would pad them to sixteen, and these instructions are
+// slow enough here to matter (about 20 clocks of a quarter SM; with the rows as
+// M a batch took 76 us that takes 64 now).  The results join in shared memory
+// at the tile's end, and a tile cut over several CTAs is joined by the last of
+// them to finish, in the order of the cuts, so results do not depend on the
+// order of arrival.
+//
+// Measured: 47 sequences of up to 8192 tokens, 7 query heads on each of 4 KV
+// heads, 64 us, 5.6 TB/s; one sequence of 131072 tokens on one KV head 23 us,
+// 2.9 TB/s (three levels of latency before the first page, two joins after the
+// last); one of 200 tokens on 8 KV heads 6.3 us.
 constexpr int kRowsWarps = 8;
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 constexpr int kRowsStages = 3;
@@ -77,13 +82,14 @@ constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 token
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
 constexpr int kRows = 8;
 constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kRows * 256 + 2 * kRowsWarps * kRows * 4;
-// Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
-// One sequence of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
+// Units up to which a tile is not cut where there is little work.  One sequence
+// of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
 constexpr int kRowsWhole = 4;
 constexpr int kRowsCost = 1;   // pages that a tile's end is worth
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
 // more in a second step.
 constexpr int kJoinRows = 160;
+// Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowSlot = kRows * (kDim + 2);
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
@@ -478,17 +484,25 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 
 // --------------------------------------------------------------- many rows
 //
-// Chunks: both products on the tcgen05 tensor cores, bound by them and by the
-// exponentials (a 128 x 128 tile takes 1024 clocks of each).  One CTA per SM
-// takes two tiles of up to 128 rows (whole tokens) that share every page.  A
-// warp loads pages by TMA through a ring of four 32 KiB buffers, a warp per tile
-// issues its products, and sixteen warps do both tiles' softmax in turn: scores
-// from tensor memory, maximum, weights back over the scores in the cache's type,
-// from where the second product reads them.  While one tile's softmax runs the
-// other's products do.  The accumulated values are only rescaled when a row's
-// maximum grew by more than 2^8 since the last time; weights up to 2^8 are as
-// exact as weights up to 1, and the sums are 32-bit.  Tensor memory: scores
-// (and weights) of the tiles at columns 0 and 128, values at 256 and 384.
+// Chunks: both products on the tcgen05 tensor cores.  One CTA per SM takes two
+// tiles of up to 128 rows (whole tokens) that share every page.  A warp loads
+// pages by TMA through a ring of four 32 KiB buffers, a warp per tile issues its
+// products, and sixteen warps do both tiles' softmax in turn: scores from tensor
+// memory, maximum, weights back over the scores in the cache's type, from where
+// the second product reads them.  While one tile's softmax runs the other's
+// products do.  The accumulated values are only rescaled when a row's maximum
+// grew by more than 2^8 since the last time; weights up to 2^8 are as exact as
+// weights up to 1, and the sums are 32-bit.  Tensor memory: scores (and weights)
+// of the tiles at columns 0 and 128, values at 256 and 384.
+//
+// For a page and both tiles the tensor cores need 2048 clocks and the special
+// function units as many, a quarter fewer as exponentials go to the multiply-add
+// units.  Measured 3380: the softmax takes 1690 a tile, of which 900 are the
+// exponentials and the rest what the warps of a quarter SM do together (loading
+// scores, agreeing on the maximum, handing weights over).  A chunk of 512 tokens
+// after 6144, 32 query heads on 8 KV heads: 69 us, 770 TFLOP/s; 4096 tokens in
+// 20480: 1.15 to 1.23 ms, 1.0 to 1.08 PFLOP/s, at an SM clock that the power
+// limit holds at 1.4 GHz.
 constexpr int kSoftWarps = 16;       // four warpgroups, each with a quarter of a page's keys
 constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, checker
 constexpr int kRing = 4;
@@ -1218,7 +1232,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// Joins the pieces of tiles that were cut over CTAs: a warp per row.
+// Joins the pieces of tiles that were cut over CTAs: a warp per row, bound by
+// latency (about 7 us with the launch for a chunk of 512 tokens after 6144).
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBlocks = kTileRows / (kJoinThreads / 32);   // for each CTA that may have ended a cut tile: a row per warp
 template <typename T>

@@ -16,7 +16,9 @@ namespace {
 // at position 10^6 as at 1, where a 32-bit product pos f would have lost it.
 // Bound by reading and writing each row once.  Eight lanes hold a row (eight
 // pairs each, 16-byte accesses), a warp four rows at a time, and computes its
-// lanes' eight angles once for all rows that it turns.
+// lanes' eight angles once for all rows that it turns.  Measured: 8000 tokens of
+// 28 query and 4 KV heads 23 us, 4.9 TB/s (27 us before rows were loaded ahead of
+// the angles); 16 tokens of 32 and 8 heads 3.7 us.
 constexpr int kAppendThreads = 128;
 constexpr int kAppendBatch = 3;
 
@@ -131,7 +133,8 @@ paged_append_kernel(const __grid_constant__ AppendParams p, int groups, int rows
 // --------------------------------------------------------------- page copy
 //
 // Bound by reading and writing every byte once: 16 KiB pieces, four 16-byte
-// loads in flight per thread.
+// loads in flight per thread.  Measured: 32 pages of 16 MiB (32 layers of 8 heads)
+// 165 us, 6.5 TB/s.
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;
 constexpr int kCopyPiece = kCopyThreads * kCopyUnroll * 16;
@@ -169,7 +172,8 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
 // cluster of CTAs does an operation in one launch, its phases apart by cluster
 // barriers.  Ranks come from prefix sums in page or request order, so pages
 // are given and moved in one order whatever the timing; the only atomics are
-// integer additions to the counts and a minimum over request numbers.
+// integer additions to the counts and a minimum over request numbers.  Measured:
+// 300 of 512 sequences freed in a table of 256 columns and 20000 pages 7.9 us.
 constexpr int kMaxCluster = 8;
 constexpr int kTableThreads = 1024;
 // Entries up to which one CTA is faster than a cluster and its barriers.
