@@ -184,7 +184,7 @@ _paged = None
 
 def paged_ops():
     """Load (once) and return the extension ``_build/paged_python.so``: the
-    paged-cache calls of every layer and step (csrc/paged_python.cpp)."""
+    paged-cache calls (csrc/paged_python.cpp)."""
     global _paged
     if _paged is None:
         import importlib.util

@@ -1,7 +1,7 @@
-// paged_python.cpp -- the calls of secure_infer_b200/paged.py that run for every
-// layer and step, as a CPython extension: it looks the tensors over, makes the
-// outputs and calls the C ABI (include/secure_infer_paged.h).  The same through
-// ctypes took 11 us of host time for an append whose kernel takes 3.
+// paged_python.cpp -- the calls of secure_infer_b200/paged.py as a CPython
+// extension: it looks the tensors over, makes the outputs and calls the C ABI
+// (include/secure_infer_paged.h).  The same through ctypes took 11 us of host
+// time for an append whose kernel takes 3.
 //
 // Handles come as the addresses of the structures that the Python objects hold,
 // the stream as its handle.  Refused arguments raise ValueError, refused
@@ -204,49 +204,179 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
-// free(block_table, lens, refs, pages, device, seqs, stream): new tables of the same shapes.
-PyObject* free_sequences(PyObject*, PyObject* const* a, Py_ssize_t n)
+struct Tables {
+    at::Tensor table, lens, refs;
+    secure_infer_tables c;
+};
+
+// block_table, lens and refs of a cache of `pages`.
+Tables tables(PyObject* const* a, int64_t pages, int64_t device)
 {
-    if (!counted(n, 7)) return nullptr;
+    Tables t{tensor(a[0], "block_table"), tensor(a[1], "lens"), tensor(a[2], "refs"), {}};
+    t.c.block_table = const_cast<int32_t*>(ints(t.table, 2, device, "block_table must be int32 [seqs, width] of the cache's device"));
+    t.c.lens = const_cast<int32_t*>(ints(t.lens, 1, device, "lens must be int32 [seqs] of the cache's device"));
+    t.c.refs = const_cast<int32_t*>(ints(t.refs, 1, device, "refs must be int32 [pages] of the cache's device"));
+    need(t.table.is_contiguous() && t.lens.is_contiguous() && t.refs.is_contiguous(), "tables must be dense");
+    need(t.table.size(0) > 0 && t.table.size(1) > 0 && t.table.size(0) <= INT32_MAX && t.table.size(1) <= INT32_MAX,
+         "block_table is empty");
+    need(t.lens.size(0) == t.table.size(0) && t.refs.size(0) == pages,
+         "lens needs an entry for each row of the block table, refs one for each page");
+    t.c.seqs = static_cast<uint32_t>(t.table.size(0));
+    t.c.width = static_cast<uint32_t>(t.table.size(1));
+    t.c.pages = static_cast<uint32_t>(pages);
+    return t;
+}
+
+// New tables of the same shapes, or the given ones.
+Tables outputs(PyObject* given, const Tables& in, int64_t pages, int64_t device)
+{
+    if (given == Py_None) {
+        Tables t{at::empty_like(in.table), at::empty_like(in.lens), at::empty_like(in.refs), in.c};
+        t.c.block_table = static_cast<int32_t*>(t.table.data_ptr());
+        t.c.lens = static_cast<int32_t*>(t.lens.data_ptr());
+        t.c.refs = static_cast<int32_t*>(t.refs.data_ptr());
+        return t;
+    }
+    need(PyTuple_Check(given) && PyTuple_GET_SIZE(given) == 3, "out must be PageTables");
+    PyObject* parts[3] = {PyTuple_GET_ITEM(given, 0), PyTuple_GET_ITEM(given, 1), PyTuple_GET_ITEM(given, 2)};
+    const Tables t = tables(parts, pages, device);
+    need(t.table.sizes() == in.table.sizes(), "out differs in shape from the tables");
+    const at::Tensor* outs[3] = {&t.table, &t.lens, &t.refs};
+    for (const at::Tensor* a : {&in.table, &in.lens, &in.refs})
+        for (const at::Tensor* b : outs) {
+            const char *x = static_cast<const char*>(a->data_ptr()), *y = static_cast<const char*>(b->data_ptr());
+            need(x + a->nbytes() <= y || y + b->nbytes() <= x, "out overlaps the tables");
+        }
+    for (int i = 0; i < 3; i++)
+        for (int j = 0; j < i; j++) {
+            const char *x = static_cast<const char*>(outs[i]->data_ptr()), *y = static_cast<const char*>(outs[j]->data_ptr());
+            need(x + outs[i]->nbytes() <= y || y + outs[j]->nbytes() <= x, "out overlaps itself");
+        }
+    return t;
+}
+
+// Entries of a list of requests, as many in both.
+uint32_t requests(const at::Tensor& a, const at::Tensor& b)
+{
+    need(a.size(0) == b.size(0), "the lists of requests differ in length");
+    need(a.size(0) <= INT32_MAX, "too many requests");
+    return static_cast<uint32_t>(a.size(0));
+}
+
+at::Tensor scratch_of(const Tables& t, uint32_t n)
+{
+    return at::empty({static_cast<int64_t>(secure_infer_paged_scratch(&t.c, n) / 4)}, t.table.options());
+}
+
+int32_t* data(const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// (block_table, lens, refs, further tensors...)
+PyObject* results(std::initializer_list<at::Tensor> tensors)
+{
+    PyObject* all = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+    Py_ssize_t i = 0;
+    for (const at::Tensor& t : tensors) {
+        PyObject* o = all != nullptr ? THPVariable_Wrap(t) : nullptr;
+        if (o == nullptr) {
+            Py_XDECREF(all);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(all, i++, o);
+    }
+    return all;
+}
+
+constexpr const char* kRequests = "requests must be int32 [n] of the cache's device";
+
+// The operations on tables: (block_table, lens, refs, pages, device, their own arguments, stream, out), where `out` is
+// None for new tables.
+
+// fork(..., tensors, count, page bytes, parents, children, ...)
+PyObject* fork_sequences(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!counted(n, 12)) return nullptr;
     return guarded([&]() -> PyObject* {
-        const at::Tensor &table = tensor(a[0], "block_table"), &lens = tensor(a[1], "lens"), &refs = tensor(a[2], "refs");
         const int64_t pages = PyLong_AsLongLong(a[3]), device = PyLong_AsLongLong(a[4]);
+        const auto* copied = address<const secure_infer_page_tensor>(a[5]);
+        const int64_t count = PyLong_AsLongLong(a[6]), bytes = PyLong_AsLongLong(a[7]);
         if (PyErr_Occurred()) return nullptr;
-        secure_infer_tables in{}, out{};
-        in.block_table = const_cast<int32_t*>(ints(table, 2, device, "block_table must be int32 [seqs, width] of the cache's device"));
-        in.lens = const_cast<int32_t*>(ints(lens, 1, device, "lens must be int32 [seqs] of the cache's device"));
-        in.refs = const_cast<int32_t*>(ints(refs, 1, device, "refs must be int32 [pages] of the cache's device"));
-        need(table.is_contiguous() && lens.is_contiguous() && refs.is_contiguous(), "tables must be dense");
-        need(table.size(0) > 0 && table.size(1) > 0 && table.size(0) <= UINT32_MAX && table.size(1) <= UINT32_MAX,
-             "block_table is empty");
-        need(lens.size(0) == table.size(0) && refs.size(0) == pages,
-             "lens needs an entry for each row of the block table, refs one for each page");
-        const at::Tensor& seqs = tensor(a[5], "seqs");
-        const int32_t* ended = ints(seqs, 1, device, "seqs must be an int32 tensor of the cache's device");
-        need(seqs.size(0) <= INT32_MAX, "too many requests");
-        in.seqs = static_cast<uint32_t>(table.size(0));
-        in.width = static_cast<uint32_t>(table.size(1));
-        in.pages = static_cast<uint32_t>(pages);
-        out = in;
-        at::Tensor t = at::empty_like(table), l = at::empty_like(lens), r = at::empty_like(refs);
-        out.block_table = static_cast<int32_t*>(t.data_ptr());
-        out.lens = static_cast<int32_t*>(l.data_ptr());
-        out.refs = static_cast<int32_t*>(r.data_ptr());
-        const uint32_t count = static_cast<uint32_t>(seqs.size(0));
-        at::Tensor scratch = at::empty({static_cast<int64_t>(secure_infer_paged_scratch(&in, count) / 4)}, table.options());
-        if (secure_infer_paged_free(&in, &out, ended, count, scratch.data_ptr(), address<void>(a[6])) != 0)
-            return failed("secure_infer_paged_free");
-        PyObject* parts[3] = {THPVariable_Wrap(std::move(t)), THPVariable_Wrap(std::move(l)), THPVariable_Wrap(std::move(r))};
-        PyObject* all = parts[0] && parts[1] && parts[2] ? PyTuple_Pack(3, parts[0], parts[1], parts[2]) : nullptr;
-        for (PyObject* o : parts) Py_XDECREF(o);
-        return all;
+        const Tables in = tables(a, pages, device), out = outputs(a[11], in, pages, device);
+        const at::Tensor &parents = tensor(a[8], "parents"), &children = tensor(a[9], "children");
+        const int32_t *p = ints(parents, 1, device, kRequests), *c = ints(children, 1, device, kRequests);
+        const uint32_t asked = requests(parents, children);
+        at::Tensor granted = at::empty({asked}, in.table.options()), scratch = scratch_of(in, asked);
+        if (secure_infer_paged_fork(copied, static_cast<uint32_t>(count), static_cast<uint64_t>(bytes), &in.c, &out.c, p, c,
+                                    asked, data(granted), scratch.data_ptr(), address<void>(a[10])) != 0)
+            return failed("secure_infer_paged_fork");
+        return results({out.table, out.lens, out.refs, granted});
     });
 }
 
+// reserve(..., seqs, lens, ...)
+PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!counted(n, 9)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int64_t pages = PyLong_AsLongLong(a[3]), device = PyLong_AsLongLong(a[4]);
+        if (PyErr_Occurred()) return nullptr;
+        const Tables in = tables(a, pages, device), out = outputs(a[8], in, pages, device);
+        const at::Tensor &seqs = tensor(a[5], "seqs"), &lens = tensor(a[6], "lens");
+        const int32_t *s = ints(seqs, 1, device, kRequests), *l = ints(lens, 1, device, kRequests);
+        const uint32_t asked = requests(seqs, lens);
+        at::Tensor granted = at::empty({asked}, in.table.options()), scratch = scratch_of(in, asked);
+        if (secure_infer_paged_reserve(&in.c, &out.c, s, l, asked, data(granted), scratch.data_ptr(), address<void>(a[7])) != 0)
+            return failed("secure_infer_paged_reserve");
+        return results({out.table, out.lens, out.refs, granted});
+    });
+}
+
+// free(..., seqs, ...), `out` may be left out
+PyObject* free_sequences(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (n != 7 && !counted(n, 8)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int64_t pages = PyLong_AsLongLong(a[3]), device = PyLong_AsLongLong(a[4]);
+        if (PyErr_Occurred()) return nullptr;
+        const Tables in = tables(a, pages, device), out = outputs(n > 7 ? a[7] : Py_None, in, pages, device);
+        const at::Tensor& seqs = tensor(a[5], "seqs");
+        const int32_t* ended = ints(seqs, 1, device, kRequests);
+        const uint32_t asked = requests(seqs, seqs);
+        at::Tensor scratch = scratch_of(in, asked);
+        if (secure_infer_paged_free(&in.c, &out.c, ended, asked, scratch.data_ptr(), address<void>(a[6])) != 0)
+            return failed("secure_infer_paged_free");
+        return results({out.table, out.lens, out.refs});
+    });
+}
+
+// compact(..., tensors, count, page bytes, ...)
+PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!counted(n, 10)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int64_t pages = PyLong_AsLongLong(a[3]), device = PyLong_AsLongLong(a[4]);
+        const auto* copied = address<const secure_infer_page_tensor>(a[5]);
+        const int64_t count = PyLong_AsLongLong(a[6]), bytes = PyLong_AsLongLong(a[7]);
+        if (PyErr_Occurred()) return nullptr;
+        const Tables in = tables(a, pages, device), out = outputs(a[9], in, pages, device);
+        at::Tensor moved = at::empty({pages}, in.table.options()), live = at::empty({1}, in.table.options());
+        at::Tensor scratch = scratch_of(in, 0);
+        if (secure_infer_paged_compact(copied, static_cast<uint32_t>(count), static_cast<uint64_t>(bytes), &in.c, &out.c,
+                                       data(moved), data(live), scratch.data_ptr(), address<void>(a[8])) != 0)
+            return failed("secure_infer_paged_compact");
+        return results({out.table, out.lens, out.refs, moved, live});
+    });
+}
+
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)); }
+
 PyMethodDef methods[] = {
-    {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
-    {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
-    {"free", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(free_sequences)), METH_FASTCALL, nullptr},
+    {"attend", fast<attend>(), METH_FASTCALL, nullptr},
+    {"append", fast<append>(), METH_FASTCALL, nullptr},
+    {"fork", fast<fork_sequences>(), METH_FASTCALL, nullptr},
+    {"reserve", fast<reserve>(), METH_FASTCALL, nullptr},
+    {"free", fast<free_sequences>(), METH_FASTCALL, nullptr},
+    {"compact", fast<compact>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "paged_python", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -14,9 +14,8 @@ step for all its layers.  Calls run on the current stream and return without
 waiting; lengths, tables and page ids stay on the device.  Bad arguments raise
 ``ValueError`` before anything is launched, a refused launch ``RuntimeError``.
 As everywhere in this package there is no fallback: the work goes through
-``libsecure_infer.so``.  The calls of every layer (``append``, ``attend``) and
-``free`` reach it by a small extension (csrc/paged_python.cpp), which also looks
-their tensors over; the others by ctypes.
+``libsecure_infer.so``, reached by a small extension (csrc/paged_python.cpp) that
+also looks the tensors over; ``copy`` alone goes by ctypes.
 """
 from __future__ import annotations
 
@@ -219,7 +218,6 @@ class PageTables(_Tables):
     """Who holds which page: ``block_table`` int32 ``[seqs, width]``, ``lens``
     int32 ``[seqs]`` tokens held, ``refs`` int32 ``[pages]`` rows that hold a
     page (0: free).  A sequence of n tokens holds ``ceil(n / 128)`` pages."""
-    _checked = None   # the C structure, once a cache has looked the tensors over
 
 
 class CachePages:
@@ -250,42 +248,14 @@ class CachePages:
                     _need(fills and page * size >= self.page_bytes, "a page's values must fill one block of memory")
                     dense[strides] = page * size
                 self._tensors[2 * i + j] = (t.data_ptr(), dense[strides])
+        self._address = ct.addressof(self._tensors)
 
-    def _check(self, t: PageTables) -> _native.Tables:
-        if not isinstance(t, PageTables):
-            raise ValueError("tables must be PageTables")
-        if t._checked is not None and t._checked[0] is self:
-            return t._checked[1]
-        for x, what, dims in ((t.block_table, "block_table", 2), (t.lens, "lens", 1), (t.refs, "refs", 1)):
-            _need(isinstance(x, torch.Tensor), f"{what} must be a tensor")
-            _ints(x, what, self.device, dims)
-            _need(x.is_contiguous(), f"{what} must be dense")
-        seqs, width = t.block_table.shape
-        _need(seqs > 0 and width > 0, "block_table is empty")
-        _need(t.lens.shape[0] == seqs and t.refs.shape[0] == self.pages,
-              "lens needs an entry for each row of the block table, refs one for each page")
-        return self._remember(t, seqs, width)
-
-    def _remember(self, t: PageTables, seqs: int, width: int) -> _native.Tables:
-        c = _native.Tables(t.block_table.data_ptr(), t.lens.data_ptr(), t.refs.data_ptr(), seqs, width, self.pages, 0)
-        t._checked = (self, c)
-        return c
-
-    def _outputs(self, t: PageTables, out: PageTables | None):
-        c = self._check(t)
-        if out is None:
-            out = PageTables(torch.empty_like(t.block_table), torch.empty_like(t.lens), torch.empty_like(t.refs))
-            return c, out, self._remember(out, c.seqs, c.width)
-        o = self._check(out)
-        _need(all(a.shape == b.shape for a, b in zip(t, out)), "out differs in shape from the tables")
-        for a in t:
-            for b in out:
-                lo, hi = max(a.data_ptr(), b.data_ptr()), min(a.data_ptr() + 4 * a.numel(), b.data_ptr() + 4 * b.numel())
-                _need(lo >= hi, "out overlaps the tables")
-        return c, out, o
-
-    def _scratch(self, c: _native.Tables, n: int) -> torch.Tensor:
-        return torch.empty(_native.lib().secure_infer_paged_scratch(ct.byref(c), n), dtype=torch.uint8, device=self.device)
+    def _run(self, name: str, tables: PageTables, out: PageTables | None, *args):
+        """The new tables and what else an operation on tables returns."""
+        _need(isinstance(tables, PageTables), "tables must be PageTables")
+        index = self.device.index
+        made = _on(index, getattr(_native.paged_ops(), name), *tables, self.pages, index, *args, _raw_stream(index), out)
+        return (PageTables(*made[:3]) if out is None else out, *made[3:])
 
     def _pair(self, a, b, names) -> tuple[torch.Tensor, torch.Tensor]:
         a, b = _ints(a, names[0], self.device, 1), _ints(b, names[1], self.device, 1)
@@ -312,14 +282,7 @@ class CachePages:
         ``[n]``: 0 where the child is not empty or named twice, an index is out
         of range, or pages ran out (requests are served in order)."""
         a, b = self._pair(parents, children, ("parents", "children"))
-        c, out, o = self._outputs(tables, out)
-        n = a.shape[0]
-        granted = torch.empty(n, dtype=torch.int32, device=self.device)
-        scratch = self._scratch(c, n)
-        _call("secure_infer_paged_fork", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
-              ct.byref(o), a.data_ptr(), b.data_ptr(), n, granted.data_ptr(), scratch.data_ptr(),
-              _raw_stream(self.device.index))
-        return out, granted
+        return self._run("fork", tables, out, self._address, len(self._tensors), self.page_bytes, a, b)
 
     def reserve(self, tables: PageTables, seqs, lens, out: PageTables | None = None):
         """Grow sequence ``seqs[i]`` to ``lens[i]`` tokens on the lowest free
@@ -327,26 +290,12 @@ class CachePages:
         would shrink or not fit the table, is named twice, its partial last page
         is shared, or pages ran out (requests are served in order)."""
         a, b = self._pair(seqs, lens, ("seqs", "lens"))
-        c, out, o = self._outputs(tables, out)
-        n = a.shape[0]
-        granted = torch.empty(n, dtype=torch.int32, device=self.device)
-        scratch = self._scratch(c, n)
-        _call("secure_infer_paged_reserve", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), b.data_ptr(), n,
-              granted.data_ptr(), scratch.data_ptr(), _raw_stream(self.device.index))
-        return out, granted
+        return self._run("reserve", tables, out, a, b)
 
     def free(self, tables: PageTables, seqs, out: PageTables | None = None) -> PageTables:
         """Empty the sequences ``seqs``; a page that no other row holds becomes
         free.  Returns the new tables."""
-        a = _ints(seqs, "seqs", self.device, 1)
-        if out is None and isinstance(tables, PageTables):
-            index = self.device.index
-            return PageTables(*_on(index, _native.paged_ops().free, *tables, self.pages, index, a, _raw_stream(index)))
-        c, out, o = self._outputs(tables, out)
-        scratch = self._scratch(c, a.shape[0])
-        _call("secure_infer_paged_free", self.device, ct.byref(c), ct.byref(o), a.data_ptr(), a.shape[0],
-              scratch.data_ptr(), _raw_stream(self.device.index))
-        return out
+        return self._run("free", tables, out, _ints(seqs, "seqs", self.device, 1))[0]
 
     def compact(self, tables: PageTables, out: PageTables | None = None):
         """Move the used pages to the lowest places, in every layer: with
@@ -354,11 +303,4 @@ class CachePages:
         the i-th free one below.  Returns the new tables, ``moved`` int32
         ``[pages]`` (where each page is now, -1 for a free one) and ``live``
         int32 ``[1]``."""
-        c, out, o = self._outputs(tables, out)
-        moved = torch.empty(self.pages, dtype=torch.int32, device=self.device)
-        live = torch.empty(1, dtype=torch.int32, device=self.device)
-        scratch = self._scratch(c, 0)
-        _call("secure_infer_paged_compact", self.device, self._tensors, len(self._tensors), self.page_bytes, ct.byref(c),
-              ct.byref(o), moved.data_ptr(), live.data_ptr(), scratch.data_ptr(),
-              _raw_stream(self.device.index))
-        return out, moved, live
+        return self._run("compact", tables, out, self._address, len(self._tensors), self.page_bytes)
