@@ -20,7 +20,7 @@ constexpr int kDim = 128;    // values of a head
 
 // What a CTA's last unit of a cut tile leaves for the join.
 struct Cut {
-    int32_t valid, cta0, rows, token0, head;
+    int32_t cta1, cta0, rows, token0, head;   // the last CTA and the first; cta1 = 0: no such tile
     int32_t n, kv, q0;
 };
 
@@ -338,15 +338,42 @@ struct Walk {
     }
 };
 
-// Units of a sequence; `largest`: of a tile.
+// Pages and cost of a tile.
+__device__ __forceinline__ int tile_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost, int tile)
+{
+    const int r = tile * rows_per_tile;
+    return tile_span(p, s, r / p.group, (min(r + rows_per_tile, s.n * p.group) - 1) / p.group).pages + cost;
+}
+
+// Up to so many tiles of a sequence are counted by one thread, more by a warp:
+// for a chunk of 4096 tokens of 4 rows a count took 4 us by one thread.
+constexpr int kOwnTiles = 4;
+
+// Units of every lane's sequence; `largest`: of a tile of theirs.  All lanes call it.
 __device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost, int& largest)
 {
+    const int lane = threadIdx.x & 31;
+    const int tiles = (s.n * p.group + rows_per_tile - 1) / rows_per_tile;
     int units = 0;
-    const int rows = s.n * p.group;
-    for (int r = 0; r < rows; r += rows_per_tile) {
-        const int u = tile_span(p, s, r / p.group, (min(r + rows_per_tile, rows) - 1) / p.group).pages + cost;
-        units += u;
-        largest = max(largest, u);
+    if (tiles <= kOwnTiles) {
+        for (int t = 0; t < tiles; ++t) {
+            const int u = tile_units(p, s, rows_per_tile, cost, t);
+            units += u;
+            largest = max(largest, u);
+        }
+    }
+    for (uint32_t many = __ballot_sync(0xffffffffu, tiles > kOwnTiles); many != 0; many &= many - 1) {
+        const int from = __ffs(many) - 1, n = __shfl_sync(0xffffffffu, tiles, from);
+        const Seq q{__shfl_sync(0xffffffffu, s.n, from), __shfl_sync(0xffffffffu, s.kv, from), 0};
+        int sum = 0, most = 0;
+        for (int t = lane; t < n; t += 32) {
+            const int u = tile_units(p, q, rows_per_tile, cost, t);
+            sum += u;
+            most = max(most, u);
+        }
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == from) units = sum, largest = max(largest, most);
     }
     return units * p.heads;
 }
@@ -420,6 +447,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
     }
 }
 
+// All lanes of a warp call it.
 __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_tile, int cost, const Share& share)
 {
     Walk w;
@@ -433,8 +461,26 @@ __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_t
     w.tiles = (w.q.n * p.group + rows_per_tile - 1) / rows_per_tile;
     w.tile = 0;
     w.tile_unit = share.seq_unit;
+    int skip = share.begin - share.seq_unit;
+    // Of a sequence of many tiles, 32 at a time.
+    for (bool past = w.tiles > kOwnTiles; past;) {
+        const int lane = threadIdx.x & 31, t = w.tile + lane;
+        int upto = t < w.tiles ? tile_units(p, w.q, rows_per_tile, cost, t) * p.heads : 0;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += up;
+        }
+        const int whole = __popc(__ballot_sync(0xffffffffu, t < w.tiles && upto <= skip));
+        if (whole > 0) {
+            const int units = __shfl_sync(0xffffffffu, upto, whole - 1);
+            skip -= units;
+            w.tile_unit += units;
+            w.tile += whole;
+        }
+        past = whole == 32;
+    }
     w.set_tile(p);
-    int skip = share.begin - share.seq_unit, units = w.span.pages + cost;
+    int units = w.span.pages + cost;
     while (skip >= units * p.heads) {
         skip -= units * p.heads;
         w.tile_unit += units * p.heads;

@@ -510,6 +510,9 @@ constexpr uint32_t kStageBytes = 32 * 32;   // 32 bytes of a softmax warp's rows
 constexpr uint32_t kTileBytes = 128 * kDim * 2;
 constexpr int kItems = 8;
 constexpr int kTileRows = 256;
+// Partial result of a pair of tiles: the values as tensor memory gives them to a warp, [8 warps' rows][32 fours of
+// values][32 rows][4], so that a warp's stores cover whole lines, then [rows] maxima and [rows] sums.  (Row by row, by
+// way of shared memory, a piece's end took 2 us more for each tile.)
 constexpr int kTileSlot = kTileRows * (kDim + 2);
 constexpr float kRescale = 8.0f;
 constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
@@ -755,8 +758,21 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             uint32_t n = 0, item = 0;
             while (w.left > 0 && !*stop) {
                 const int pages = w.take();
+                const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
+                int id = lane < pages && w.span.hi > 0 ? row[lane] : -1;
                 if (lane == 0) {
                     if (item > 0) barrier_wait(q_empty, (item - 1) & 1, stop);
+                    if (!*stop) {
+                        const int tiles = w.rows > rows_per_tile ? 2 : 1;
+                        barrier_expect(q_full, tiles * 2 * rows_per_tile * 128);
+                        for (int t = 0; t < tiles; ++t)
+                            for (int h = 0; h < 2; ++h)
+                                tma_load_rows(q_smem + t * kTileBytes + h * (kTileBytes / 2), &q_map, q_full,
+                                              w.head * p.group, w.q.q0 + w.first_token + t * tokens, h);
+                    }
+                }
+                __syncwarp();
+                auto publish = [&] {
                     Item& it = c.items[item % kItems];
                     it.span = w.span;
                     it.s = w.s;
@@ -778,30 +794,23 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     // Only the first tile of a CTA can have begun in an earlier one.
                     if (item == 0) {
                         Cut cut{};
-                        if (cta0 < static_cast<int>(blockIdx.x) && w.page + pages == w.span.pages)
-                            cut = Cut{1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
+                        if (cta0 < static_cast<int>(blockIdx.x))
+                            cut = Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
                         p.cuts[blockIdx.x] = cut;
                     }
-                    if (!*stop) {
-                        const int tiles = w.rows > rows_per_tile ? 2 : 1;
-                        barrier_expect(q_full, tiles * 2 * rows_per_tile * 128);
-                        for (int t = 0; t < tiles; ++t)
-                            for (int h = 0; h < 2; ++h)
-                                tma_load_rows(q_smem + t * kTileBytes + h * (kTileBytes / 2), &q_map, q_full,
-                                              w.head * p.group, w.q.q0 + w.first_token + t * tokens, h);
-                    }
-                }
-                __syncwarp();
-                const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
+                };
                 for (int i0 = 0; i0 < pages; i0 += 32) {
-                    const int id = i0 + lane < pages && w.span.hi > 0 ? row[i0 + lane] : -1;
+                    if (i0 > 0) id = i0 + lane < pages && w.span.hi > 0 ? row[i0 + lane] : -1;
                     for (int i = i0; i < min(pages, i0 + 32); ++i) {
                         const int page = __shfl_sync(0xffffffffu, id, i - i0);
                         for (int kv = 0; kv < 2; ++kv, ++n) {
                             const uint32_t slot = n % kRing, turns = n / kRing;
-                            if (lane != 0 || *stop || (turns > 0 && !barrier_wait(kv_empty(slot), (turns - 1) & 1, stop))) continue;
-                            barrier_expect(kv_full(slot), kTileBytes);
-                            tma_load_page(ring + slot * kTileBytes, kv ? &v_map : &k_map, kv_full(slot), 0, 0, w.head, page);
+                            if (lane == 0 && !*stop && (turns == 0 || barrier_wait(kv_empty(slot), (turns - 1) & 1, stop))) {
+                                barrier_expect(kv_full(slot), kTileBytes);
+                                tma_load_page(ring + slot * kTileBytes, kv ? &v_map : &k_map, kv_full(slot), 0, 0, w.head, page);
+                            }
+                            // The others hear of the piece once its first loads are on their way.
+                            if (lane == 0 && i == 0 && kv == 0) publish();
                         }
                     }
                     __syncwarp();
@@ -1128,7 +1137,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                                              p.table + w.s * p.table_stride, w.head, max(a, page_key),
                                              min(b + 1, page_key + pages * kPage), mm, ll, x);
                         if (split) {
-                            *reinterpret_cast<float4*>(slot + (t * 128 + rows0 + r) * kDim + lane * 4) = x;
+                            reinterpret_cast<float4*>(slot)[((t * 4 + rows0 / 32) * 32 + lane) * 32 + r] = x;
                             if (lane == 0) {
                                 slot[kTileRows * kDim + t * 128 + rows0 + r] = mm;
                                 slot[kTileRows * kDim + kTileRows + t * 128 + rows0 + r] = ll;
@@ -1172,19 +1181,12 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 tmem_load<32>(o, lanes + 256 + t * 128 + quarter * 32);
                 tmem_wait_loads();
                 if (split) {
-                    float* part = slot + (t * 128 + rows0) * kDim + quarter * 32 + (lane & 1) * 4;
+                    float4* part = reinterpret_cast<float4*>(slot) + ((t * 4 + rows0 / 32) * 32 + quarter * 8) * 32 + lane;
+                    if (lane < valid) {
 #pragma unroll
-                    for (int d = 0; d < 32; d += 8) {
-                        put(o[d], o[d + 1], o[d + 2], o[d + 3], 0);
-                        put(o[d + 4], o[d + 5], o[d + 6], o[d + 7], 1);
-                        __syncwarp();
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const int r = k * 16 + (lane >> 1);
-                            const uint4 x = get(r);
-                            if (r < valid) *reinterpret_cast<uint4*>(part + r * kDim + d) = x;
-                        }
-                        __syncwarp();
+                        for (int d = 0; d < 32; d += 4)
+                            part[d * 8] = make_float4(__uint_as_float(o[d]), __uint_as_float(o[d + 1]),
+                                                      __uint_as_float(o[d + 2]), __uint_as_float(o[d + 3]));
                     }
                 } else {
                     T* out = static_cast<T*>(p.out) + out0 * kDim + quarter * 32 + (lane & 1) * 8;
@@ -1232,37 +1234,34 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// Joins the pieces of tiles that were cut over CTAs: a warp per row, bound by
-// latency (about 7 us with the launch for a chunk of 512 tokens after 6144).
-constexpr int kJoinThreads = 256;
-constexpr int kJoinBlocks = kTileRows / (kJoinThreads / 32);   // for each CTA that may have ended a cut tile: a row per warp
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const __grid_constant__ AttendParams p)
+// Joins the pieces of tiles that were cut over CTAs, in the order of the pieces.
+// A lane takes a row, as the pieces lie, and kFours times four of its values;
+// the blocks of the CTAs that went on with a tile share its values, so a tile
+// in many pieces has more warps.  Bound by reading the pieces from L2 and by
+// latency, so all blocks are there at once: two warps each (eight, with four of
+// them on a value's pieces, had to take turns: 10 us more where every CTA ends a
+// tile).
+constexpr int kJoinThreads = 64;
+constexpr int kJoinBlocks = kTileRows / 32 * (kDim / 16) / (kJoinThreads / 32);
+template <typename T, int kFours>
+__device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cut, int r, int tile_row, int d4)
 {
-    wait_for_earlier_kernels();
-    dependents_may_launch();
-    const Cut cut = p.cuts[blockIdx.y];
-    if (!cut.valid) return;
-    const int rows_per_tile = 128 / p.group * p.group;
-    const int lane = threadIdx.x & 31;
-    const int pieces = blockIdx.y - cut.cta0 + 1;
-    const int tile_row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
-    if (tile_row >= cut.rows) return;
-    const int r = tile_row < rows_per_tile ? tile_row : 128 + tile_row - rows_per_tile;
-    // 32 pieces at a time.
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f, top = -INFINITY;
-    for (int i0 = 0; i0 < pieces; i0 += 32) {
-        auto piece = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cut.cta0 + i0 + i) + (i0 + i == 0)) * kTileSlot; };
-        float4 y;
-        float part_top, part_sum;
-        join_row(
-            min(32, pieces - i0), [&](int i) { return piece(i) + kTileRows * kDim + r; }, kTileRows,
-            [&](int i) { return piece(i) + r * kDim; }, y, part_top, part_sum);
-        const float both = fmaxf(top, part_top), f = join_weight(top, both), g = join_weight(part_top, both);
-        x = make_float4(f * x.x + g * y.x, f * x.y + g * y.y, f * x.z + g * y.z, f * x.w + g * y.w);
-        sum = f * sum + g * part_sum;
-        top = both;
+    const int pieces = cut.cta1 - cut.cta0 + 1;
+    auto piece = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cut.cta0 + i) + (i == 0)) * kTileSlot; };
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 8
+    for (int i = 0; i < pieces; ++i) top = max3_nan(top, __ldcg(piece(i) + kTileRows * kDim + r), top);
+    float4 x[kFours] = {};
+#pragma unroll (8 / kFours)
+    for (int i = 0; i < pieces; ++i) {
+        const float* at = piece(i);
+        const float f = join_weight(__ldcg(at + kTileRows * kDim + r), top);
+        sum += f * __ldcg(at + kTileRows * kDim + kTileRows + r);
+#pragma unroll
+        for (int j = 0; j < kFours; ++j) {
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(at) + ((r & ~31) + d4 + j) * 32 + (r & 31));
+            x[j] = make_float4(x[j].x + f * y.x, x[j].y + f * y.y, x[j].z + f * y.z, x[j].w + f * y.w);
+        }
     }
     const Seq s{cut.n, cut.kv, cut.q0};
     const int token = cut.token0 + tile_row / p.group, g = tile_row % p.group;
@@ -1270,10 +1269,39 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     row_keys(p, s, token, a, b);
     const float inv = 1.0f / sum;
     const int64_t at = static_cast<int64_t>(cut.q0 + token) * p.heads * p.group + cut.head * p.group + g;
-    uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-    if (b < a) packed = make_uint2(0, 0);
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
-    if (p.lse != nullptr && lane == 0) p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    uint2 y[kFours];
+#pragma unroll
+    for (int j = 0; j < kFours; ++j) {
+        y[j] = make_uint2(pack2<T>(x[j].x * inv, x[j].y * inv), pack2<T>(x[j].z * inv, x[j].w * inv));
+        if (b < a) y[j] = make_uint2(0, 0);
+    }
+    T* const out = static_cast<T*>(p.out) + at * kDim + d4 * 4;
+    if constexpr (kFours == 1) {
+        *reinterpret_cast<uint2*>(out) = y[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < kFours; j += 2)
+            reinterpret_cast<uint4*>(out)[j / 2] = make_uint4(y[j].x, y[j].y, y[j + 1].x, y[j + 1].y);
+    }
+    if (p.lse != nullptr && d4 == 0) p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const __grid_constant__ AttendParams p)
+{
+    wait_for_earlier_kernels();
+    dependents_may_launch();
+    const Cut cut = p.cuts[blockIdx.y];
+    if (cut.cta1 == 0) return;
+    const int sharers = cut.cta1 - cut.cta0, k = blockIdx.y - cut.cta0 - 1;
+    const int fours = sharers >= 4 ? 1 : sharers >= 2 ? 2 : 4;
+    const int part = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), d4 = part % 8 * 4 + k * fours;
+    const int rows_per_tile = 128 / p.group * p.group, r = part / 8 * 32 + (threadIdx.x & 31);
+    const int tile_row = r < 128 ? (r < rows_per_tile ? r : cut.rows) : (r - 128 < rows_per_tile ? rows_per_tile + r - 128 : cut.rows);
+    if (k * fours >= 4 || tile_row >= cut.rows) return;
+    if (fours == 4) join_values<T, 4>(p, cut, r, tile_row, d4);
+    else if (fours == 2) join_values<T, 2>(p, cut, r, tile_row, d4);
+    else join_values<T, 1>(p, cut, r, tile_row, d4);
 }
 
 struct Device {
