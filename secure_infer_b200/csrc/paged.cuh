@@ -46,7 +46,7 @@ struct AttendParams {
     Cut* cuts;                      // [grid]
     float* slots;                   // [2 * grid] partial results of tiles
     float* row_slots;               // and of the kernel for few rows
-    int32_t beside;                 // the kernel for few rows runs just before in the same call
+    int32_t both;                   // the call has a launch for few rows, and then one for the others, on the same SMs
 };
 
 // Launchers (cudaError_t values).
@@ -242,7 +242,8 @@ struct Seq {
     int n, kv, q0;   // new tokens, all tokens, first new token
 };
 
-__device__ __forceinline__ Seq load_seq(const AttendParams& p, int s)
+// `others`: the sequences of the call's other launch, else of this one.
+__device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool others = false)
 {
     Seq r;
     int a = p.cu[s], b = p.cu[s + 1];
@@ -252,7 +253,7 @@ __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s)
     r.n = b - a;
     r.kv = max(0, min(p.kv[s], p.width * kPage));
     const int64_t rows = static_cast<int64_t>(r.n) * p.group;
-    if (rows < p.rows_min || rows > p.rows_max) r.n = 0;
+    if ((rows < p.rows_min || rows > p.rows_max) != others) r.n = 0;
     return r;
 }
 
@@ -378,13 +379,26 @@ __device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, in
     return units * p.heads;
 }
 
-// All threads of the block take part; `warp_sums` holds two values per warp.
+// How one kind of launch cuts its tiles, and what a unit of it costs an SM.
+struct Kind {
+    int rows_per_tile, cost, whole;
+    int time;     // of a unit, in any measure that both kinds share
+    int of_16;    // sixteenths of the SMs beyond which it gets no faster
+};
+
+// All threads of the block take part; `warp_sums` holds three values per warp.
 // Where no tile has more than `whole` units a CTA gets the largest one's:
-// cutting it would cost more than the few pages that it would save.
+// cutting it would cost more than the few pages that it would save.  Where the
+// call has work of both kinds each gets SMs by the time that its units take:
+// the first CTAs of a launch work and the others leave theirs to the other
+// launch, so reading pages for few rows goes on beside the products of many: 333
+// tokens after 2167 and 15 single tokens of up to 4000 take 53 us, 62 one kind
+// after the other.
 template <int kThreads>
-__device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_tile, int cost, int whole, Share* share,
+__device__ __forceinline__ void find_share(const AttendParams& p, const Kind& kind, const Kind& other, Share* share,
                                            int32_t* warp_sums)
 {
+    const int rows_per_tile = kind.rows_per_tile, cost = kind.cost, whole = kind.whole;
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Share r;
@@ -393,12 +407,17 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
     // has a thread one pass does both.
     const bool one = p.seqs <= kThreads;
     for (int pass = one ? 1 : 0; pass < 2; ++pass) {
-        int base = 0, largest = 0;
+        int base = 0, largest = 0, others = 0;
         for (int s0 = 0; s0 < p.seqs; s0 += kThreads) {
             const int s = s0 + tid;
             Seq q{};
-            int own_largest = 0;
+            int own_largest = 0, unused = 0, beside = 0;
             if (s < p.seqs) q = load_seq(p, s);
+            if (p.both && (one || pass == 0)) {
+                Seq o{};
+                if (s < p.seqs) o = load_seq(p, s, true);
+                beside = __reduce_add_sync(0xffffffffu, seq_units(p, o, other.rows_per_tile, other.cost, unused));
+            }
             const int own = seq_units(p, q, rows_per_tile, cost, own_largest);
             int sum = own;
             for (int d = 1; d < 32; d <<= 1) {
@@ -409,6 +428,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
             if (lane == 31) {
                 warp_sums[warp] = sum;
                 warp_sums[kWarps + warp] = own_largest;
+                warp_sums[2 * kWarps + warp] = beside;
             }
             __syncthreads();
             int before = base;
@@ -418,10 +438,17 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int rows_per_t
                 if (w < warp) before += x;
                 base += x;
                 largest = max(largest, warp_sums[kWarps + w]);
+                others += warp_sums[2 * kWarps + w];
             }
             if (one || (pass == 0 && s0 + kThreads >= p.seqs)) {
                 r.total = base;
-                r.ctas = max(1, min(static_cast<int>(gridDim.x), largest <= whole ? base / max(1, largest) : base));
+                int grid = gridDim.x;
+                if (base > 0 && others > 0 && grid > 1) {
+                    const float mine = static_cast<float>(base) * kind.time, theirs = static_cast<float>(others) * other.time;
+                    const int most = max(1, grid * kind.of_16 / 16), least = grid - max(1, grid * other.of_16 / 16);
+                    grid = max(max(1, least), min(min(most, grid - 1), __float2int_rn(grid * (mine / (mine + theirs)))));
+                }
+                r.ctas = max(1, min(grid, largest <= whole ? base / max(1, largest) : base));
                 r.per = base / r.ctas;
                 r.more = base - r.per * r.ctas;
                 const int c = blockIdx.x;

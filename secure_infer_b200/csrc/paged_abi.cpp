@@ -166,10 +166,10 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
         if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
             return -1;
         p.rows_max = tiles ? kFewRows : INT_MAX;
+        p.both = tiles;
         if (launch_attend_rows(k_map, v_map, p, pages->dtype, st) != 0) return -1;
         p.rows_min = kFewRows + 1;
         p.rows_max = INT_MAX;
-        p.beside = 1;
     }
     if (!tiles) return 0;
     if (!page_map(&k_map, pages, pages->k, pages->k_stride, kPage) || !page_map(&v_map, pages, pages->v, pages->v_stride, kPage) ||

@@ -92,6 +92,13 @@ constexpr int kJoinRows = 160;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowSlot = kRows * (kDim + 2);
 
+constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
+
+// An SM takes 1.1 us of a page for few rows where fewer than 120 of 148 SMs read (58 GB/s each; 120 to 130 get nearly
+// all that memory gives), and 1.95 us of a page for a pair of tiles.
+__device__ __forceinline__ Kind rows_kind() { return {kRows, kRowsCost, kRowsWhole, 4, 14}; }
+__device__ __forceinline__ Kind tiles_kind(const AttendParams& p) { return {2 * (128 / p.group * p.group), kTilesCost, 0, 7, 16}; }
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -143,7 +150,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
     __shared__ Share share;
-    __shared__ int32_t warp_sums[2 * kRowsThreads / 32];
+    __shared__ int32_t warp_sums[3 * kRowsThreads / 32];
     __shared__ volatile int stop;   // a wait ran out
     __shared__ int irregular, last_piece, give_up;
 
@@ -171,7 +178,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     wait_for_earlier_kernels();
-    find_share<kRowsThreads>(p, kRows, kRowsCost, kRowsWhole, &share, warp_sums);
+    find_share<kRowsThreads>(p, rows_kind(), tiles_kind(p), &share, warp_sums);
     dependents_may_launch();
     Walk w = start_walk(p, kRows, kRowsCost, share);
 
@@ -515,7 +522,6 @@ constexpr int kTileRows = 256;
 // way of shared memory, a piece's end took 2 us more for each tile.)
 constexpr int kTileSlot = kTileRows * (kDim + 2);
 constexpr float kRescale = 8.0f;
-constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
 
 template <int kCols>
 __device__ __forceinline__ void tmem_load(uint32_t (&r)[kCols], uint32_t addr);
@@ -676,7 +682,7 @@ struct TilesControl {
     uint64_t checked, taken, item_full[kItems];
     Item items[kItems];
     float exchange[2][4][128];           // between a row's four threads
-    int32_t warp_sums[2 * kTileThreads / 32];
+    int32_t warp_sums[3 * kTileThreads / 32];
     Share share;
     uint32_t tmem;
     int irregular;                       // what the checker found in the piece
@@ -741,9 +747,9 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     // Beside the kernel for few rows this one starts as that one's CTAs leave: its inputs were complete before that one
     // read them, the two share no memory that either writes, and it waits for that one at its end instead.
-    if (!p.beside) wait_for_earlier_kernels();
+    if (!p.both) wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads>(p, 2 * rows_per_tile, kTilesCost, 0, &c.share, c.warp_sums);
+    find_share<kTileThreads>(p, tiles_kind(p), rows_kind(), &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
@@ -1230,7 +1236,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     tmem_fence_before();
     __syncthreads();
-    if (p.beside) wait_for_earlier_kernels();
+    if (p.both) wait_for_earlier_kernels();
     if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
