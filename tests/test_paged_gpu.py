@@ -261,6 +261,27 @@ def test_split_contexts_and_their_repetition(paged, lens, heads, kv_heads):
         assert torch.equal(out, again) and torch.equal(lse, again_lse)
 
 
+@pytest.mark.parametrize("lens", [[(1300, 1300)], [(3, 40), (700, 2000), (1, 300), (1100, 1100)]])
+@pytest.mark.parametrize("window", [0, 150])
+def test_sequences_of_many_tiles(paged, lens, window):
+    """More tiles of a sequence than a warp has lanes, before and after others."""
+    c = Case(paged, lens, 16, 1)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, window=window, return_lse=True)
+    c.check(out, lse, window=window)
+
+
+@pytest.mark.parametrize("lens", [[(300, 900)] + [(1, 3000)] * 20, [(1, 20000), (40, 50)], [(1, 5), (600, 4000), (2, 1)],
+                                  [(40 if i % 7 == 0 else 1, 40 + (i * 37) % 300) for i in range(700)]])
+def test_chunks_beside_single_tokens(paged, lens):
+    """Both kinds share the SMs, whichever has more work; repeated calls give the same bits."""
+    c = Case(paged, lens, 8, 2)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+    c.check(out, lse)
+    for _ in range(5):
+        again, again_lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, again_lse)
+
+
 def test_many_sequences(paged):
     """More sequences than a block has threads."""
     c = Case(paged, [(i % 4 != 3, 1 + (i * 37) % 300) for i in range(1500)], 4, 2)
