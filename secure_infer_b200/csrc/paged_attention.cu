@@ -506,10 +506,10 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // function units as many, a quarter fewer as exponentials go to the multiply-add
 // units.  Measured 3380: the softmax takes 1690 a tile, of which 900 are the
 // exponentials and the rest what the warps of a quarter SM do together (loading
-// scores, agreeing on the maximum, handing weights over).  A chunk of 512 tokens
-// after 6144, 32 query heads on 8 KV heads: 69 us, 770 TFLOP/s; 4096 tokens in
-// 20480: 1.15 to 1.23 ms, 1.0 to 1.08 PFLOP/s, at an SM clock that the power
-// limit holds at 1.4 GHz.
+// scores, agreeing on the maximum, handing weights over).  A piece takes 5 us to
+// its first scores and 2.5 to leave.  A chunk of 512 tokens after 6144, 32 query
+// heads on 8 KV heads: 62 us, 860 TFLOP/s; 4096 tokens in 20480: 1.18 to 1.22 ms,
+// 1.0 to 1.05 PFLOP/s, at an SM clock that the power limit holds at 1.4 GHz.
 constexpr int kSoftWarps = 16;       // four warpgroups, each with a quarter of a page's keys
 constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, checker
 constexpr int kRing = 4;
