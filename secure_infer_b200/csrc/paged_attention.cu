@@ -511,7 +511,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // heads on 8 KV heads: 62 us, 860 TFLOP/s; 4096 tokens in 20480: 1.18 to 1.22 ms,
 // 1.0 to 1.05 PFLOP/s, at an SM clock that the power limit holds at 1.4 GHz.
 constexpr int kSoftWarps = 16;       // four warpgroups, each with a quarter of a page's keys
-constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, checker
+constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, guard
 constexpr int kRing = 4;
 constexpr uint32_t kStageBytes = 32 * 32;   // 32 bytes of a softmax warp's rows, on their way to whole sectors
 constexpr uint32_t kTileBytes = 128 * kDim * 2;
@@ -656,7 +656,7 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t x2)
 
 // A CTA's piece of a tile, from the producer for the other warps.  The producer
 // is less than kItems pieces ahead of the last of them: it needs the first
-// product of the piece before, and buffers that the checker gives back, who
+// product of the piece before, and buffers that the guard gives back, who
 // waits for every softmax warp.
 struct Item {
     Span span;
@@ -685,7 +685,7 @@ struct TilesControl {
     int32_t warp_sums[3 * kTileThreads / 32];
     Share share;
     uint32_t tmem;
-    int irregular;                       // what the checker found in the piece
+    int irregular;                       // what the guard found in the piece
     int stop;                            // a wait ran out
 };
 constexpr uint32_t kControlBytes = 8192 - 1024;   // the first KiB of shared memory is the driver's
@@ -720,7 +720,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) {
             barrier_init(kv_full(i), 1);
-            barrier_init(kv_empty(i), 3);    // each tile's products and the checker
+            barrier_init(kv_empty(i), 3);    // each tile's products and the guard
         }
         barrier_init(q_full, 1);
         barrier_init(q_empty, 2);
@@ -927,7 +927,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             __syncwarp();
             barrier_wait(drained(t), 0, stop);
         } else {
-            // Checker: an infinity or NaN among values that some rows see and others do not, where weights of zero
+            // Guard: an infinity or NaN among values that some rows see and others do not, where weights of zero
             // would carry it over.
             uint32_t n = 0, item = 0;
             while (any) {
