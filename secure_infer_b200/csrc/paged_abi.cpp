@@ -80,9 +80,10 @@ bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, int64_t token_str
 }
 
 // Rows per KV head up to which a sequence goes to the kernel for few rows, in
-// tiles of eight.  Measured with 24 sequences of up to 4096 tokens and 8 KV
-// heads: 20 rows 54 us there and 59 in tiles of 128, 32 rows 100 and 53; with
-// one of 300 tokens 7.3 and 14.0, 7.7 and 14.1.
+// tiles of eight.  Measured there and in tiles of 128, us: 24 sequences of up to
+// 4096 tokens on 8 KV heads with 20 rows 54 and 55, with 24 rows 69 and 57, with
+// 32 rows 100 and 53; 8 sequences with 20 rows 27 and 33; 48 of up to 8192 on one
+// KV head with 24 rows 34 and 40; one of 300 tokens with 20 rows 7.3 and 14.0.
 constexpr uint32_t kFewRows = 24;
 
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)

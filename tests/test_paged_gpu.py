@@ -677,3 +677,32 @@ def test_refusals(paged):
     c.check(paged.attend(c.pages, c.chunk, c.q))
     empty = paged.attend(c.pages, c.chunk, q[:0])
     assert empty.shape == (0, 8, 128)
+
+
+def test_given_tables(paged):
+    """Tables to write into: refused where they overlap, else the same as new ones."""
+    c = Case(paged, [(1, 300), (1, 77)], 8, 2)
+    cache = paged.CachePages([[c.k, c.v]])
+    refs = torch.zeros(cache.pages, dtype=torch.int32, device="cuda")
+    refs[c.table[c.table >= 0].long()] = 1
+    t = paged.PageTables(c.table.contiguous(), c.chunk.kv_lens, refs)
+    fresh = lambda: paged.PageTables(*(torch.full_like(x, 55) for x in t))  # noqa: E731
+    small = torch.empty(max(2, cache.pages), dtype=torch.int32, device="cuda")
+    for out in (paged.PageTables(fresh().block_table, t.lens, fresh().refs), fresh()._replace(lens=small[:2], refs=small[:cache.pages]),
+                fresh()._replace(refs=refs[:-1]), fresh()._replace(block_table=fresh().block_table[:, 1:].contiguous()),
+                tuple(fresh())[:2], 3):
+        with pytest.raises(ValueError):
+            cache.free(t, [0], out=out)
+        with pytest.raises(ValueError):
+            cache.reserve(t, [0], [301], out=out)
+        with pytest.raises(ValueError):
+            cache.fork(t, [0], [1], out=out)
+        with pytest.raises(ValueError):
+            cache.compact(t, out=out)
+    for run in (lambda out: cache.free(t, [0], out=out), lambda out: cache.reserve(t, [1, 0], [200, 299], out=out)[0],
+                lambda out: cache.fork(t, [0], [1], out=out)[0]):
+        want, given = run(None), fresh()
+        assert run(given) is given
+        for a, b in zip(want, given):
+            assert torch.equal(a, b)
+
