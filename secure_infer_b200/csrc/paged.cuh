@@ -246,12 +246,13 @@ struct Seq {
 __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool others = false)
 {
     Seq r;
-    int a = p.cu[s], b = p.cu[s + 1];
+    // From L2, as all that may be read before this kernel has waited for the one before it.
+    int a = __ldcg(p.cu + s), b = __ldcg(p.cu + s + 1);
     a = max(0, min(a, p.tokens));
     b = max(a, min(b, p.tokens));
     r.q0 = a;
     r.n = b - a;
-    r.kv = max(0, min(p.kv[s], p.width * kPage));
+    r.kv = max(0, min(__ldcg(p.kv + s), p.width * kPage));
     const int64_t rows = static_cast<int64_t>(r.n) * p.group;
     if ((rows < p.rows_min || rows > p.rows_max) != others) r.n = 0;
     return r;
@@ -539,19 +540,19 @@ __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q
                                                int b, float& m, float& l, float4& o)
 {
     const int d = 4 * (threadIdx.x & 31);
-    const uint2 qx = *reinterpret_cast<const uint2*>(q + d);
+    const uint2 qx = __ldcg(reinterpret_cast<const uint2*>(q + d));
     const float2 q0 = unpack2<T>(qx.x), q1 = unpack2<T>(qx.y);
     m = -INFINITY;
     l = 0.0f;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int j = a; j < b; ++j) {
-        const int page = table[j / kPage];
+        const int page = __ldcg(table + j / kPage);
         float2 k0 = {0, 0}, k1 = {0, 0}, v0 = {0, 0}, v1 = {0, 0};
         if (page >= 0 && page < p.pages) {
-            const uint2 kx = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.k) + page * p.k_stride[0] +
-                                                             (j % kPage) * p.k_stride[1] + head * p.k_stride[2] + d);
-            const uint2 vx = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.v) + page * p.v_stride[0] +
-                                                             (j % kPage) * p.v_stride[1] + head * p.v_stride[2] + d);
+            const uint2 kx = __ldcg(reinterpret_cast<const uint2*>(static_cast<const T*>(p.k) + page * p.k_stride[0] +
+                                                                   (j % kPage) * p.k_stride[1] + head * p.k_stride[2] + d));
+            const uint2 vx = __ldcg(reinterpret_cast<const uint2*>(static_cast<const T*>(p.v) + page * p.v_stride[0] +
+                                                                   (j % kPage) * p.v_stride[1] + head * p.v_stride[2] + d));
             k0 = unpack2<T>(kx.x), k1 = unpack2<T>(kx.y), v0 = unpack2<T>(vx.x), v1 = unpack2<T>(vx.y);
         }
         float x = q0.x * k0.x + q0.y * k0.y + q1.x * k1.x + q1.y * k1.y;

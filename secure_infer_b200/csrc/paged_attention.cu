@@ -765,7 +765,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             while (w.left > 0 && !*stop) {
                 const int pages = w.take();
                 const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
-                int id = lane < pages && w.span.hi > 0 ? row[lane] : -1;
+                int id = lane < pages && w.span.hi > 0 ? __ldcg(row + lane) : -1;
                 if (lane == 0) {
                     if (item > 0) barrier_wait(q_empty, (item - 1) & 1, stop);
                     if (!*stop) {
@@ -806,7 +806,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                 };
                 for (int i0 = 0; i0 < pages; i0 += 32) {
-                    if (i0 > 0) id = i0 + lane < pages && w.span.hi > 0 ? row[i0 + lane] : -1;
+                    if (i0 > 0) id = i0 + lane < pages && w.span.hi > 0 ? __ldcg(row + i0 + lane) : -1;
                     for (int i = i0; i < min(pages, i0 + 32); ++i) {
                         const int page = __shfl_sync(0xffffffffu, id, i - i0);
                         for (int kv = 0; kv < 2; ++kv, ++n) {
