@@ -69,7 +69,12 @@ typedef struct {
  * whatever they hold.  workspace: secure_infer_paged_attend_workspace() bytes,
  * 256-byte aligned, zero before its first use, used by one stream at a time;
  * calls leave it ready for the next. */
+#define SECURE_INFER_ATTEND_STATE_BYTES 4096u   /* of a workspace, from its start: all that has to be zero */
 uint64_t secure_infer_paged_attend_workspace(void);
+/* The stream capture that `stream` takes part in, 0 outside of one.  A captured
+ * call uses its workspace wherever the graph is replayed, so it needs one that
+ * no other stream's calls use meanwhile. */
+uint64_t secure_infer_capture_id(void* stream);
 int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
                               int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
                               float scale, uint32_t causal, uint32_t window, void* workspace, void* stream);

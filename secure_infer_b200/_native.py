@@ -139,6 +139,7 @@ PAGED_SIGNATURES = {
     "secure_infer_paged_compact": ([P, U32, U64, P, P, P, P, P, P], I32),
 }
 HOST_SIGNATURES.update(PAGED_SIGNATURES)
+HOST_SIGNATURES["secure_infer_capture_id"] = ([P], U64)
 
 # SECURE_INFER_KIND_KV: a reload of 2n records, K packets first, V packets after.
 KIND_KV = 2

@@ -108,6 +108,17 @@ bool tensors_ok(const secure_infer_page_tensor* t, uint32_t n, uint64_t page_byt
 
 SI_EXPORT uint64_t secure_infer_paged_attend_workspace(void) { return attend_workspace_bytes(); }
 
+SI_EXPORT uint64_t secure_infer_capture_id(void* stream)
+{
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+        cudaGetLastError();   // the legacy stream beside another stream's capture
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
                                         int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out,
                                         float* lse, float scale, uint32_t causal, uint32_t window, void* workspace,

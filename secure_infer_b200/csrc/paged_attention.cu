@@ -17,7 +17,8 @@ namespace {
 
 // Workspace: counters, the status word, cuts, then partial results.
 constexpr int kMaxGrid = 256;
-constexpr uint64_t kCutOffset = 4096;
+constexpr uint64_t kCutOffset = SECURE_INFER_ATTEND_STATE_BYTES;
+static_assert((3 * kMaxGrid + 1) * sizeof(uint32_t) <= kCutOffset, "counters and the status word");
 constexpr uint64_t kSlotOffset = kCutOffset + kMaxGrid * sizeof(Cut);
 
 // One row of n <= 32 partial results, by a warp: lane l gets values 4l .. 4l+3

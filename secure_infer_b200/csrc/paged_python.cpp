@@ -367,6 +367,9 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// capture_id(stream)
+PyObject* capture_id(PyObject*, PyObject* stream) { return PyLong_FromUnsignedLongLong(secure_infer_capture_id(address<void>(stream))); }
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)); }
 
@@ -377,6 +380,7 @@ PyMethodDef methods[] = {
     {"reserve", fast<reserve>(), METH_FASTCALL, nullptr},
     {"free", fast<free_sequences>(), METH_FASTCALL, nullptr},
     {"compact", fast<compact>(), METH_FASTCALL, nullptr},
+    {"capture_id", capture_id, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "paged_python", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

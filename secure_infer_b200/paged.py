@@ -167,20 +167,31 @@ def append(pages: LayerPages, chunk: Chunk, q: torch.Tensor | None, k: torch.Ten
                interleaved, positions, out, _raw_stream(index))
 
 
-_workspaces: dict = {}
+_workspaces: dict = {}   # (device, stream): what the stream's own calls use
+_captured: dict = {}     # (device, stream): the stream's latest capture and what its calls use
+_STATE = 4096            # SECURE_INFER_ATTEND_STATE_BYTES
 
 
 def attend_workspace(device) -> torch.Tensor:
-    """A workspace for ``attend``: one per stream that calls it."""
+    """A workspace for ``attend``.  Calls that may run at the same time, on two
+    streams or in a graph beside either, need one each."""
     return torch.zeros(int(_native.lib().secure_infer_paged_attend_workspace()), dtype=torch.uint8, device=device)
 
 
 def _workspace(index: int, stream: int) -> torch.Tensor:
+    capture = _native.paged_ops().capture_id(stream)
+    if capture:
+        # The graph's calls keep theirs wherever it is replayed, so it is the graph's own: from its memory, held until the
+        # stream's next capture lest this one gives it to other tensors, cleared at every replay's first call.
+        held, w = _captured.get((index, stream), (0, None))
+        if held != capture:
+            size = int(_native.lib().secure_infer_paged_attend_workspace())
+            w = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+            w[:_STATE].zero_()
+            _captured[index, stream] = capture, w
+        return w
     w = _workspaces.get((index, stream))
     if w is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("attend's first call on a stream makes its workspace: make it before capturing, "
-                               "or pass workspace=attend_workspace(device)")
         w = _workspaces[index, stream] = attend_workspace(torch.device("cuda", index))
     return w
 
@@ -197,8 +208,8 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
     q heads, 128]``, and with ``return_lse`` the natural logarithms of the
     softmax sums, float32 ``[tokens, q heads]``, to join it with attention over
     other keys.  A row that sees no key gives 0 and -inf.  ``workspace``:
-    ``attend_workspace(device)``, by default one that the current stream
-    keeps."""
+    ``attend_workspace(device)``, by default one that the current stream keeps
+    for its calls, and while it is captured one of the graph's own."""
     if chunk.device != pages.device:
         raise ValueError("the chunk and the cache are on different devices")
     index = pages.index

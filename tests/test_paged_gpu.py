@@ -706,3 +706,55 @@ def test_given_tables(paged):
         for a, b in zip(want, given):
             assert torch.equal(a, b)
 
+
+
+# ------------------------------------------------- workspaces of captured calls
+
+@pytest.mark.parametrize("lens", [[(1, 9000)], [(100, 9000)], [(1, 4000), (300, 6000), (7, 2222)]])
+def test_graphs_beside_eager_calls(paged, lens):
+    """A graph captured on a stream that has called attend before, replayed on another while the first goes on: the two
+    cut their tiles over the same CTAs and must not count each other's pieces."""
+    a, b = Case(paged, lens, 8, 1, seed=1), Case(paged, lens, 8, 1, seed=2)
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        want_a, want_b = (paged.attend(c.pages, c.chunk, c.q) for c in (a, b))
+    first.synchronize()
+    a.check(want_a)
+    b.check(want_b)
+    out = [torch.empty_like(b.q) for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, o in zip(graphs, out):
+        with torch.cuda.graph(graph, stream=first):
+            for _ in range(3):
+                paged.attend(b.pages, b.chunk, b.q, out=o)
+    got = []
+    for i in range(40):
+        with torch.cuda.stream(second):
+            graphs[i % 2].replay()
+        with torch.cuda.stream(first):
+            graphs[1 - i % 2].replay()
+            got += [paged.attend(a.pages, a.chunk, a.q) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want_a) for x in got)
+    assert all(torch.equal(o, want_b) for o in out)
+
+
+def test_calls_of_one_capture_share_a_workspace(paged):
+    """One per capture and stream, in the graph's memory, and another for the next."""
+    c = Case(paged, [(1, 300)], 8, 2)
+    side, fork = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    used, eager = [], paged._workspace(0, side.cuda_stream)
+    for _ in range(2):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            paged.attend(c.pages, c.chunk, c.q)
+            used.append(paged._workspace(0, side.cuda_stream))
+            paged.attend(c.pages, c.chunk, c.q)
+            assert paged._workspace(0, side.cuda_stream) is used[-1]
+            fork.wait_stream(side)
+            with torch.cuda.stream(fork):
+                assert paged._workspace(0, fork.cuda_stream) is not used[-1]
+            side.wait_stream(fork)
+    assert used[0] is not used[1] and all(w is not eager for w in used)
+    assert paged._workspace(0, side.cuda_stream) is eager
