@@ -140,6 +140,8 @@ __device__ __forceinline__ bool barrier_done(uint32_t bar, uint32_t parity)
     return done != 0;
 }
 
+constexpr long long kWaitClocks = 1ll << 33;   // some seconds
+
 // Waits for the phase of parity `parity`.  The wait is bounded: some seconds
 // after its start `stop` is set and every wait of the CTA gives up, so a
 // protocol error ends the kernel instead of hanging it.  Returns whether the
@@ -150,12 +152,22 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
     const long long start = clock64();
     while (!barrier_done(bar, parity)) {
         if (*stop) return false;
-        if (clock64() - start > (1ll << 33)) {
+        if (clock64() - start > kWaitClocks) {
             *stop = 1;
             return false;
         }
     }
     return true;
+}
+
+// For copies and products that have been issued: they write memory that the CTA
+// gives back at its end, so it waits for them even after another wait ran out,
+// with a limit of its own.
+__device__ __forceinline__ void barrier_drain(uint32_t bar, uint32_t parity)
+{
+    const long long start = clock64();
+    while (!barrier_done(bar, parity))
+        if (clock64() - start > kWaitClocks) return;
 }
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int half,

@@ -185,7 +185,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
-        uint32_t unit = 0;
+        uint32_t unit = 0, issued = 0;   // units passed, and those whose copies were issued
         while (w.left > 0 && !stop) {
             const int pages = w.take();
             const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
@@ -196,6 +196,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     const int stage = unit % kRowsStages;
                     const uint32_t turn = unit / kRowsStages;
                     if (lane != 0 || stop || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, &stop))) continue;
+                    issued = unit + 1;
                     const int first = (w.span.first + w.page + i) * kPage;
                     const int qa = max(0, w.span.lo - first) / kQuarter;
                     const int qb = (min(kPage, w.span.hi - first) + kQuarter - 1) / kQuarter;
@@ -215,9 +216,9 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         }
         // Copies still in flight land before the CTA's shared memory goes away.
         if (lane == 0) {
-            for (uint32_t u = unit > kRowsStages ? unit - kRowsStages : 0; u < unit; ++u) {
-                barrier_wait(k_full(u % kRowsStages), (u / kRowsStages) & 1, &stop);
-                barrier_wait(v_full(u % kRowsStages), (u / kRowsStages) & 1, &stop);
+            for (uint32_t u = issued > kRowsStages ? issued - kRowsStages : 0; u < issued; ++u) {
+                barrier_drain(k_full(u % kRowsStages), (u / kRowsStages) & 1);
+                barrier_drain(v_full(u % kRowsStages), (u / kRowsStages) & 1);
             }
             if (stop) atomicOr(p.status, 1u);
         }
@@ -762,7 +763,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == kSoftWarps) {
             // Producer.
-            uint32_t n = 0, item = 0;
+            uint32_t n = 0, item = 0, issued = 0, q_issued = 0;   // buffers and pieces passed, and those whose copies were issued
             while (w.left > 0 && !*stop) {
                 const int pages = w.take();
                 const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
@@ -772,6 +773,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     if (!*stop) {
                         const int tiles = w.rows > rows_per_tile ? 2 : 1;
                         barrier_expect(q_full, tiles * 2 * rows_per_tile * 128);
+                        q_issued = item + 1;
                         for (int t = 0; t < tiles; ++t)
                             for (int h = 0; h < 2; ++h)
                                 tma_load_rows(q_smem + t * kTileBytes + h * (kTileBytes / 2), &q_map, q_full,
@@ -814,6 +816,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             const uint32_t slot = n % kRing, turns = n / kRing;
                             if (lane == 0 && !*stop && (turns == 0 || barrier_wait(kv_empty(slot), (turns - 1) & 1, stop))) {
                                 barrier_expect(kv_full(slot), kTileBytes);
+                                issued = n + 1;
                                 tma_load_page(ring + slot * kTileBytes, kv ? &v_map : &k_map, kv_full(slot), 0, 0, w.head, page);
                             }
                             // The others hear of the piece once its first loads are on their way.
@@ -826,7 +829,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 w.advance(p, pages);
             }
             if (lane == 0) {
-                for (uint32_t u = n > kRing ? n - kRing : 0; u < n; ++u) barrier_wait(kv_full(u % kRing), (u / kRing) & 1, stop);
+                for (uint32_t u = issued > kRing ? issued - kRing : 0; u < issued; ++u) barrier_drain(kv_full(u % kRing), (u / kRing) & 1);
+                if (q_issued > 0) barrier_drain(q_full, (q_issued - 1) & 1);
                 if (*stop) atomicOr(p.status, 1u);
             }
             __syncwarp();
@@ -926,7 +930,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             // Nothing of this warp is in flight when tensor memory is given back.
             if (elected()) commit_to(drained(t));
             __syncwarp();
-            barrier_wait(drained(t), 0, stop);
+            barrier_drain(drained(t), 0);
         } else {
             // Guard: an infinity or NaN among values that some rows see and others do not, where weights of zero
             // would carry it over.
