@@ -7,8 +7,8 @@
  * [KV heads][128], as secure_infer_h2d_reload_layer scatters it.
  *
  * Streams are cudaStream_t passed as void*; every other pointer is a device
- * pointer of the device that is current.  Nothing here waits for the device or
- * allocates.  Functions return 0, or -1 when an argument is refused (nothing is
+ * pointer of the device that is current, unless said otherwise.  Nothing here
+ * waits for the device (but secure_infer_attend_status) or allocates.  Functions return 0, or -1 when an argument is refused (nothing is
  * launched) or a launch fails.  Contents of device arrays cannot be refused:
  * page ids outside the cache read as zeros and are never written, lengths are
  * clamped to the block table, ranges of tokens to the token count.
@@ -70,11 +70,19 @@ typedef struct {
  * 256-byte aligned, zero before its first use, used by one stream at a time;
  * calls leave it ready for the next. */
 #define SECURE_INFER_ATTEND_STATE_BYTES 4096u   /* of a workspace, from its start: all that has to be zero */
+/* Waits inside the kernels have a limit of some seconds.  One that runs out ends
+ * its call with NaN in the rows that it concerns and makes the first word of the
+ * workspace non-zero, and from then on calls with this workspace give NaN in
+ * every row that sees a key. */
 uint64_t secure_infer_paged_attend_workspace(void);
 /* The stream capture that `stream` takes part in, 0 outside of one.  A captured
  * call uses its workspace wherever the graph is replayed, so it needs one that
  * no other stream's calls use meanwhile. */
 uint64_t secure_infer_capture_id(void* stream);
+/* Waits for the stream, which is the one exception here.  *status: 0, or 1 if a
+ * wait ran out in a call with this workspace; then its state is zero again and
+ * the next call computes.  -1 while the stream is captured. */
+int secure_infer_attend_status(void* workspace, uint32_t* status, void* stream);
 int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
                               int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
                               float scale, uint32_t causal, uint32_t window, void* workspace, void* stream);

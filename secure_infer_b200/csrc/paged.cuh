@@ -41,8 +41,8 @@ struct AttendParams {
     int32_t rows_min, rows_max;     // sequences with rows_min <= rows <= rows_max are this launch's
     int32_t causal, window;
     float scale_log2;               // scale * log2(e): the softmax runs in powers of two
+    uint32_t* status;               // not zero: a wait ran out, and calls give NaN until the host has read it
     uint32_t* counters;             // three of each CTA, zero between launches
-    uint32_t* status;
     Cut* cuts;                      // [grid]
     float* slots;                   // [2 * grid] partial results of tiles
     float* row_slots;               // and of the kernel for few rows
@@ -144,8 +144,8 @@ constexpr long long kWaitClocks = 1ll << 33;   // some seconds
 
 // Waits for the phase of parity `parity`.  The wait is bounded: some seconds
 // after its start `stop` is set and every wait of the CTA gives up, so a
-// protocol error ends the kernel instead of hanging it.  Returns whether the
-// phase completed.
+// protocol error ends the kernel instead of hanging it; the rows of the CTA
+// become NaN then.  Returns whether the phase completed.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* stop)
 {
     if (barrier_done(bar, parity)) return true;
@@ -158,6 +158,14 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
         }
     }
     return true;
+}
+
+// The same by a warp whose lanes may come apart.  (In the loops over pages they
+// are together and read one barrier, one flag and one clock; votes there took a
+// chunk of 512 tokens 1.2 us.)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop)
+{
+    return __all_sync(0xffffffffu, barrier_wait(bar, parity, stop));
 }
 
 // For copies and products that have been issued: they write memory that the CTA
@@ -296,6 +304,7 @@ struct Share {
     int32_t per, more, ctas, total;
     int32_t begin, units;      // of this CTA
     int32_t seq, seq_unit;     // sequence of its first unit, and that sequence's first unit
+    int32_t down;              // the status word when the kernel began
     Seq q;
 
     __device__ __forceinline__ int begin_of(int cta) const { return cta * per + min(cta, more); }
@@ -414,6 +423,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
     const int rows_per_tile = kind.rows_per_tile, cost = kind.cost, whole = kind.whole;
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int down = tid == 0 ? static_cast<int>(__ldcg(p.status)) : 0;
     Share r;
     r.begin = r.total = 0;
     // The first pass sums the units, the second finds the sequence that holds this CTA's first; where every sequence
@@ -470,6 +480,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
                 if (tid == 0) {
                     r.seq = -1;
                     r.seq_unit = 0;
+                    r.down = down;
                     *share = r;
                 }
                 __syncthreads();

@@ -119,6 +119,22 @@ SI_EXPORT uint64_t secure_infer_capture_id(void* stream)
     return status == cudaStreamCaptureStatusActive ? id : 0;
 }
 
+SI_EXPORT int secure_infer_attend_status(void* workspace, uint32_t* status, void* stream)
+{
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || status == nullptr ||
+        secure_infer_capture_id(stream) != 0)
+        return -1;
+    AttendParams p;
+    attend_workspace(workspace, &p);
+    const auto st = static_cast<cudaStream_t>(stream);
+    uint32_t word = 0;
+    if (cudaMemcpyAsync(&word, p.status, sizeof(word), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+        cudaStreamSynchronize(st) != cudaSuccess)
+        return -1;
+    *status = word != 0;
+    return word == 0 || cudaMemsetAsync(workspace, 0, SECURE_INFER_ATTEND_STATE_BYTES, st) == cudaSuccess ? 0 : -1;
+}
+
 SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
                                         int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out,
                                         float* lse, float scale, uint32_t causal, uint32_t window, void* workspace,

@@ -15,10 +15,11 @@ namespace sib {
 namespace paged {
 namespace {
 
-// Workspace: counters, the status word, cuts, then partial results.
+// Workspace: the status word, counters, cuts, then partial results.
 constexpr int kMaxGrid = 256;
+constexpr uint64_t kCounterOffset = 256;
 constexpr uint64_t kCutOffset = SECURE_INFER_ATTEND_STATE_BYTES;
-static_assert((3 * kMaxGrid + 1) * sizeof(uint32_t) <= kCutOffset, "counters and the status word");
+static_assert(kCounterOffset + 3 * kMaxGrid * sizeof(uint32_t) <= kCutOffset, "counters");
 constexpr uint64_t kSlotOffset = kCutOffset + kMaxGrid * sizeof(Cut);
 
 // One row of n <= 32 partial results, by a warp: lane l gets values 4l .. 4l+3
@@ -142,6 +143,16 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x)
 
 // Barrier of the eight computing warps.
 __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory"); }
+// And whether any of their threads says so.
+__device__ __forceinline__ bool rows_any(bool x)
+{
+    uint32_t r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.aligned.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(r)
+                 : "r"(static_cast<uint32_t>(x)), "n"(32 * kRowsWarps)
+                 : "memory");
+    return r != 0;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kRowsThreads, 1)
@@ -153,7 +164,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     __shared__ Share share;
     __shared__ int32_t warp_sums[3 * kRowsThreads / 32];
     __shared__ volatile int stop;   // a wait ran out
-    __shared__ int irregular, last_piece, give_up;
+    __shared__ int irregular, last_piece;
 
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t k_smem = smem_addr(base), v_smem = k_smem + kRowsStages * kPageTile;
@@ -186,7 +197,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
         uint32_t unit = 0, issued = 0;   // units passed, and those whose copies were issued
-        while (w.left > 0 && !stop) {
+        while (w.left > 0 && !__any_sync(0xffffffffu, stop || share.down)) {
             const int pages = w.take();
             const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
             for (int i0 = 0; i0 < pages; i0 += 32) {
@@ -220,12 +231,14 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 barrier_drain(k_full(u % kRowsStages), (u / kRowsStages) & 1);
                 barrier_drain(v_full(u % kRowsStages), (u / kRowsStages) & 1);
             }
-            if (stop) atomicOr(p.status, 1u);
         }
         return;
     }
 
     uint32_t unit = 0;
+    // A wait ran out: the rows that are left become NaN, and so do the pieces of cut tiles, which go on being counted.
+    // If it was in an earlier call, counts mean nothing and the rows of every piece are written.
+    bool failed = share.down != 0;
     while (w.left > 0) {
         const int pages = w.take();
         // The tile's rows, 256 bytes each, in 16-byte pieces swizzled against bank conflicts.
@@ -241,7 +254,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             *reinterpret_cast<uint4*>(q_bytes + r * 256 + ((piece ^ (r & 7)) << 4)) = x;
         }
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
-        const bool split = cta1 > cta0;
+        const bool split = cta1 > cta0 && !share.down;
         float* slot = p.row_slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
         int lo[2], hi[2];   // keys that this thread's rows see
         int all_lo, all_hi; // keys that every row of the tile sees
@@ -269,11 +282,12 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             ldmatrix4(q[d], q_smem + r * 256 + ((piece ^ r) << 4));
         }
 
-        for (int i = 0; i < pages; ++i, ++unit) {
+        for (int i = 0; i < pages && !failed; ++i, ++unit) {
             const int stage = unit % kRowsStages;
             const uint32_t parity = unit / kRowsStages & 1;
             const int key0 = (w.span.first + w.page + i) * kPage + warp * 16;   // of this warp's keys
-            if (!barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop)) break;
+            failed = !barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop);
+            if (failed) break;
             if (key0 < w.span.hi && key0 + 16 > w.span.lo) {
                 const uint32_t slice = stage * kPageTile + (warp >> 1) * kQuarterBytes + (warp & 1) * 16 * 128;
                 const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
@@ -358,20 +372,20 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 join_l[warp * kRows + lane * 2 + e] = l[e];
             }
         }
-        if (tid == 0) give_up = stop;
-        rows_sync();
-        if (give_up) break;
+        failed = rows_any(failed);
         const int last_stage = (unit - 1) % kRowsStages;
         const bool by_definition = irregular != 0;
         // Warp i's [8 rows][128] floats, columns swizzled by the row against bank conflicts.
         auto joined = [&](int i) { return base + last_stage * kPageTile + i * 4096; };
+        if (!failed) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int r = (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
-                *reinterpret_cast<float*>(joined(warp) + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][c];
-            }
+                for (int c = 0; c < 4; ++c) {
+                    const int r = (lane & 3) * 2 + (c & 1), d = j * 16 + (lane >> 2) + (c >> 1) * 8;
+                    *reinterpret_cast<float*>(joined(warp) + r * 512 + (d ^ ((lane & 3) << 3)) * 4) = o[j][c];
+                }
+        }
         rows_sync();
         // A warp per row.
         if (const int r = warp; r < w.rows) {
@@ -380,7 +394,11 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             row_keys(p, w.q, token, a, b);
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float top, sum;
-            if (by_definition) {
+            if (failed) {
+                top = 0.0f;
+                sum = NAN;
+                x = make_float4(NAN, NAN, NAN, NAN);
+            } else if (by_definition) {
                 const int ka = (w.span.first + w.page) * kPage;
                 row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
                                             (w.head * p.group + g) * p.q_head,
@@ -425,7 +443,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         // Reads and writes of this page's buffers come before the next copy into them.
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) barrier_arrive(empty(last_stage));
+        if (lane == 0 && !failed) barrier_arrive(empty(last_stage));
 
         if (split) {
             // Piece i of the tile is CTA cta0 + i's.  The last CTA to finish joins them; where that is much to read for
@@ -488,8 +506,8 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         rows_sync();
         w.advance(p, pages);
     }
+    if (failed && tid == 0) atomicOr(p.status, 1u);
 }
-
 
 // --------------------------------------------------------------- many rows
 //
@@ -690,9 +708,38 @@ struct TilesControl {
     int irregular;                       // what the guard found in the piece
     int stop;                            // a wait ran out
 };
-constexpr uint32_t kControlBytes = 8192 - 1024;   // the first KiB of shared memory is the driver's
+constexpr uint32_t kControlBytes = 8192 - 1024;   // operands follow at the next whole KiB, which the swizzle needs
 static_assert(sizeof(TilesControl) <= kControlBytes, "control block");
-constexpr uint32_t kTilesSmem = kControlBytes + (2 + kRing) * kTileBytes + kSoftWarps * kStageBytes;
+constexpr uint32_t kTilesSmem = kControlBytes + 1024 + (2 + kRing) * kTileBytes + kSoftWarps * kStageBytes;
+
+// After a wait that ran out, by the softmax warps: the rows of this CTA's share
+// become NaN, and so do its pieces of cut tiles.
+template <typename T>
+__device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& share)
+{
+    const int tid = threadIdx.x, cta = blockIdx.x;
+    if (tid == 0) atomicOr(p.status, 1u);
+    Walk w = start_walk(p, 2 * (128 / p.group * p.group), kTilesCost, share);
+    for (bool first = true; w.left > 0; first = false) {
+        const int pages = w.take();
+        const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
+        if (first && tid == 0)
+            p.cuts[cta] = cta0 < cta ? Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0} : Cut{};
+        if (cta1 > cta0) {
+            float* slot = p.slots + static_cast<int64_t>(2 * cta + (cta0 == cta)) * kTileSlot;
+            for (int i = tid; i < kTileSlot; i += 32 * kSoftWarps) slot[i] = NAN;
+        } else {
+            for (int i = tid; i < w.rows * 32; i += 32 * kSoftWarps) {
+                const int r = i >> 5, token = w.first_token + r / p.group;
+                const int64_t at = (static_cast<int64_t>(w.q.q0 + token) * p.heads + w.head) * p.group + r % p.group;
+                const uint32_t x = pack2<T>(NAN, NAN);
+                reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim)[i & 31] = make_uint2(x, x);
+                if (p.lse != nullptr && (i & 31) == 0) p.lse[at] = NAN;
+            }
+        }
+        w.advance(p, pages);
+    }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -702,12 +749,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     extern __shared__ __align__(16) uint8_t smem_raw[];
     TilesControl& c = *reinterpret_cast<TilesControl*>(smem_raw);
     volatile int* const stop = &c.stop;
-    const uint32_t q_smem = smem_addr(smem_raw) + kControlBytes, ring = q_smem + 2 * kTileBytes;
-    if (q_smem & 1023) {   // the swizzle needs it; shared memory would have to start elsewhere
-        wait_for_earlier_kernels();
-        if (threadIdx.x == 0) atomicOr(p.status, 2u);
-        return;
-    }
+    const uint32_t q_smem = (smem_addr(smem_raw) + kControlBytes + 1023) & ~1023u, ring = q_smem + 2 * kTileBytes;
     auto kv_full = [&](int i) { return smem_addr(&c.kv_full[i]); };
     auto kv_empty = [&](int i) { return smem_addr(&c.kv_empty[i]); };
     const uint32_t q_full = smem_addr(&c.q_full), q_empty = smem_addr(&c.q_empty);
@@ -756,7 +798,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
     Walk w = start_walk(p, 2 * rows_per_tile, kTilesCost, c.share);
-    const bool any = w.left > 0;
+    const bool any = w.left > 0 && c.share.down == 0;
 
     // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.
     if (warp >= kSoftWarps) {
@@ -764,7 +806,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         if (warp == kSoftWarps) {
             // Producer.
             uint32_t n = 0, item = 0, issued = 0, q_issued = 0;   // buffers and pieces passed, and those whose copies were issued
-            while (w.left > 0 && !*stop) {
+            while (any && w.left > 0 && !__any_sync(0xffffffffu, *stop)) {
                 const int pages = w.take();
                 const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
                 int id = lane < pages && w.span.hi > 0 ? __ldcg(row + lane) : -1;
@@ -831,7 +873,6 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             if (lane == 0) {
                 for (uint32_t u = issued > kRing ? issued - kRing : 0; u < issued; ++u) barrier_drain(kv_full(u % kRing), (u / kRing) & 1);
                 if (q_issued > 0) barrier_drain(q_full, (q_issued - 1) & 1);
-                if (*stop) atomicOr(p.status, 1u);
             }
             __syncwarp();
         } else if (warp < kSoftWarps + 3) {
@@ -855,7 +896,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             };
             bool ok = true;
             while (ok && any) {
-                ok = barrier_wait(item_full(item), (item / kItems) & 1, stop) && barrier_wait(q_full, item & 1, stop);
+                ok = warp_wait(item_full(item), (item / kItems) & 1, stop) && warp_wait(q_full, item & 1, stop);
                 if (!ok) break;
                 const Item& w = c.items[item % kItems];
                 const int pages = w.pages;
@@ -936,7 +977,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             // would carry it over.
             uint32_t n = 0, item = 0;
             while (any) {
-                if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
+                if (!warp_wait(item_full(item), (item / kItems) & 1, stop)) break;
                 const Item w = c.items[item % kItems];
                 const int pages = w.pages, lo_all = w.lo_all, hi_all = w.hi_all;
                 uint32_t odd = 0;
@@ -977,8 +1018,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         }
     } else {
         // Softmax: a row by four threads, each with a quarter of a page's keys, the tiles in turn: while one tile's
-        // products run all warps are at the other.  After a wait that ran out the loops run on without waiting, so
-        // the four keep meeting.
+        // products run all warps are at the other.  After a wait that ran out the loops run on without waiting to the
+        // piece's end, so the four keep meeting, and leave it together.
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
         const int quarter = warp >> 2, rows0 = (warp & 3) * 32, row = rows0 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
@@ -998,7 +1039,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         uint32_t seen[2] = {0, 0}, done[2] = {0, 0}, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
         while (any) {
-            if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
+            ok = ok && warp_wait(item_full(item), (item / kItems) & 1, stop);
+            if (meet_or(!ok)) break;
             const Item& w = c.items[item % kItems];
             const int pages = w.pages, tiles = w.rows > rows_per_tile ? 2 : 1;
             const int lo_all = w.lo_all, hi_all = w.hi_all, page_key = w.first_key;
@@ -1123,13 +1165,14 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     if (lane == 0) barrier_arrive(p_ready(t));
                 }
             }
-            ok = ok && barrier_wait(checked, item & 1, stop);
-            const bool split = w.slot >= 0, by_definition = *static_cast<volatile int*>(&c.irregular) != 0;
+            ok = ok && warp_wait(checked, item & 1, stop);
+            ok = !meet_or(!ok);   // the four go the same way
+            const bool split = w.slot >= 0, by_definition = ok && *static_cast<volatile int*>(&c.irregular) != 0;
             float* slot = p.slots + static_cast<int64_t>(w.slot) * kTileSlot;
             const uint32_t stage = ring + kRing * kTileBytes + warp * kStageBytes;
 #pragma unroll 1
             for (int t = 0; t < tiles; ++t) {
-                ok = ok && barrier_wait(o_full(t), (t ? done[1] : done[0]) & 1, stop);
+                ok = ok && warp_wait(o_full(t), (t ? done[1] : done[0]) & 1, stop);
                 if (t) ++done[1];
                 else ++done[0];
                 tmem_fence_after();
@@ -1241,6 +1284,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     tmem_fence_before();
     __syncthreads();
+    if (warp < kSoftWarps && (*stop || c.share.down)) fail_tiles<T>(p, c.share);
     if (p.both) wait_for_earlier_kernels();
     if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
@@ -1421,8 +1465,8 @@ uint64_t attend_workspace_bytes()
 
 void attend_workspace(void* workspace, AttendParams* p)
 {
-    p->counters = static_cast<uint32_t*>(workspace);
-    p->status = p->counters + 3 * kMaxGrid;
+    p->status = static_cast<uint32_t*>(workspace);
+    p->counters = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kCounterOffset);
     p->cuts = reinterpret_cast<Cut*>(static_cast<char*>(workspace) + kCutOffset);
     p->slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotOffset);
     p->row_slots = p->slots + static_cast<uint64_t>(2 * kMaxGrid) * kTileSlot;

@@ -219,6 +219,23 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
                _workspace(index, stream) if workspace is None else workspace, stream)
 
 
+def attend_status(workspace: torch.Tensor | None = None) -> int:
+    """0, or 1 if a wait inside ``attend`` ran out in a call with ``workspace``
+    (by default the one that the current stream keeps).  Such a call leaves NaN
+    in its rows, and so does every later one with this workspace until this has
+    reported it.  Waits for the current stream."""
+    _need(workspace is None or workspace.is_cuda, "workspace must come from attend_workspace")
+    index = torch.cuda.current_device() if workspace is None else workspace.device.index
+    stream = _raw_stream(index)
+    if workspace is None:
+        workspace = _workspaces.get((index, stream))
+        if workspace is None:
+            return 0
+    status = ct.c_uint32()
+    _call("secure_infer_attend_status", workspace.device, workspace.data_ptr(), ct.addressof(status), stream)
+    return status.value
+
+
 class _Tables(NamedTuple):
     block_table: torch.Tensor
     lens: torch.Tensor

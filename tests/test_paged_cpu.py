@@ -177,3 +177,12 @@ def test_extension_missing_is_said(monkeypatch, tmp_path):
     monkeypatch.setattr(_native, "LIB_PATH", tmp_path / "libsecure_infer.so")
     with pytest.raises(_native.NativeLibraryMissing, match="paged_python"):
         _native.paged_ops()
+
+
+def test_status_refuses(lib):
+    word = ct.c_uint32(7)
+    call = lib.secure_infer_attend_status
+    assert call(None, ct.byref(word), None) == -1
+    assert call(A + 16, ct.byref(word), None) == -1
+    assert call(A, None, None) == -1
+    assert word.value == 7

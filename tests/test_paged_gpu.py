@@ -758,3 +758,45 @@ def test_calls_of_one_capture_share_a_workspace(paged):
             side.wait_stream(fork)
     assert used[0] is not used[1] and all(w is not eager for w in used)
     assert paged._workspace(0, side.cuda_stream) is eager
+
+
+# ------------------------------------------------- a workspace that is down
+
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(1, 300), (3, 40)], 8, 2), ([(1, 20000)], 8, 1), ([(200, 500)], 28, 4),
+                                                 ([(100, 9000)], 8, 1), ([(1, 3000), (300, 2000), (0, 5), (2, 700)], 16, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_workspace_that_is_down_gives_nan_until_its_status_is_read(paged, lens, heads, kv_heads, dtype):
+    """The host writes the status that a wait leaves when it runs out (and counts that were left behind); no wait runs
+    out here."""
+    c = Case(paged, lens, heads, kv_heads, dtype)
+    workspace = paged.attend_workspace("cuda:0")
+    out, lse = torch.zeros_like(c.q), None
+    state = workspace.view(torch.int32)
+    state[0] = 1
+    state[64:200] = 3
+    for _ in range(2):
+        out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True, out=out, workspace=workspace)
+        assert torch.isnan(out).all() and torch.isnan(lse).all()
+    assert paged.attend_status(workspace) == 1
+    assert paged.attend_status(workspace) == 0 and not workspace[:4096].any()
+    for _ in range(2):
+        out, lse = paged.attend(c.pages, c.chunk, c.q, return_lse=True, workspace=workspace)
+        c.check(out, lse)
+    assert paged.attend_status(workspace) == 0 and not workspace[:4096].any()
+
+
+def test_status_of_the_streams_own_workspace(paged):
+    c = Case(paged, [(1, 300)], 8, 2)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert paged.attend_status() == 0
+        paged.attend(c.pages, c.chunk, c.q)
+        paged._workspaces[0, side.cuda_stream][0] = 1
+        assert torch.isnan(paged.attend(c.pages, c.chunk, c.q)).all()
+        assert paged.attend_status() == 1 and paged.attend_status() == 0
+        c.check(paged.attend(c.pages, c.chunk, c.q))
+    with pytest.raises(ValueError):
+        paged.attend_status(torch.zeros(8192, dtype=torch.uint8))
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+        with pytest.raises(RuntimeError):
+            paged.attend_status(paged._workspaces[0, side.cuda_stream])
