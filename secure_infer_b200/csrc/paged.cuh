@@ -140,21 +140,28 @@ __device__ __forceinline__ bool barrier_done(uint32_t bar, uint32_t parity)
     return done != 0;
 }
 
-constexpr long long kWaitClocks = 1ll << 33;   // some seconds
+constexpr long long kWaitClocks = 1ll << 32;   // some seconds
 
-// Waits for the phase of parity `parity`.  The wait is bounded: some seconds
-// after its start `stop` is set and every wait of the CTA gives up, so a
-// protocol error ends the kernel instead of hanging it; the rows of the CTA
-// become NaN then.  Returns whether the phase completed.
+// Waits for the phase of parity `parity`.  The wait is bounded: where nothing has
+// happened for some seconds stop[0] is set and every wait of the CTA gives up, so
+// a protocol error ends the kernel instead of hanging it; the rows of the CTA
+// become NaN then.  stop[1] goes up while warps are at work that may take longer
+// than that, and the others wait on.  Returns whether the phase completed.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* stop)
 {
     if (barrier_done(bar, parity)) return true;
-    const long long start = clock64();
+    long long start = clock64();
+    int work = -1;
     while (!barrier_done(bar, parity)) {
         if (*stop) return false;
         if (clock64() - start > kWaitClocks) {
-            *stop = 1;
-            return false;
+            const int now = stop[1] & INT32_MAX;
+            if (now == work) {
+                *stop = 1;
+                return false;
+            }
+            work = now;
+            start = clock64();
         }
     }
     return true;
@@ -175,7 +182,7 @@ __device__ __forceinline__ void barrier_drain(uint32_t bar, uint32_t parity)
 {
     const long long start = clock64();
     while (!barrier_done(bar, parity))
-        if (clock64() - start > kWaitClocks) return;
+        if (clock64() - start > 2 * kWaitClocks) return;
 }
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int half,
@@ -557,10 +564,12 @@ __device__ __forceinline__ void row_keys(const AttendParams& p, const Seq& s, in
 // One row over keys [a, b) by one warp, straight from the pages: lane l holds
 // values 4l .. 4l+3.  Only rows of a tile in which some row must not see an
 // infinite or NaN value that another one does see come here: in a matrix
-// product zero times such a value would be NaN.
+// product zero times such a value would be NaN.  A key takes about 430
+// clocks, the rows of a long piece longer than the other warps' waits last, so
+// it counts its way in *work.
 template <typename T>
 __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q, const int32_t* table, int head, int a,
-                                               int b, float& m, float& l, float4& o)
+                                               int b, float& m, float& l, float4& o, volatile int* work)
 {
     const int d = 4 * (threadIdx.x & 31);
     const uint2 qx = __ldcg(reinterpret_cast<const uint2*>(q + d));
@@ -569,6 +578,7 @@ __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q
     l = 0.0f;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int j = a; j < b; ++j) {
+        if (((j - a) & 1023) == 0 && d == 0) atomicAdd(const_cast<int*>(work), 1);
         const int page = __ldcg(table + j / kPage);
         float2 k0 = {0, 0}, k1 = {0, 0}, v0 = {0, 0}, v1 = {0, 0};
         if (page >= 0 && page < p.pages) {

@@ -163,7 +163,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
     __shared__ Share share;
     __shared__ int32_t warp_sums[3 * kRowsThreads / 32];
-    __shared__ volatile int stop;   // a wait ran out
+    __shared__ volatile int stop[2];   // a wait ran out, and work that lets waits go on
     __shared__ int irregular, last_piece;
 
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -183,7 +183,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             barrier_init(v_full(s), 1);
             barrier_init(empty(s), kRowsWarps);
         }
-        stop = 0;
+        stop[0] = stop[1] = 0;
         irregular = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
@@ -197,7 +197,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
         uint32_t unit = 0, issued = 0;   // units passed, and those whose copies were issued
-        while (w.left > 0 && !__any_sync(0xffffffffu, stop || share.down)) {
+        while (w.left > 0 && !__any_sync(0xffffffffu, stop[0] || share.down)) {
             const int pages = w.take();
             const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
             for (int i0 = 0; i0 < pages; i0 += 32) {
@@ -206,7 +206,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     const int page = __shfl_sync(0xffffffffu, id, i - i0);
                     const int stage = unit % kRowsStages;
                     const uint32_t turn = unit / kRowsStages;
-                    if (lane != 0 || stop || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, &stop))) continue;
+                    if (lane != 0 || stop[0] || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, stop))) continue;
                     issued = unit + 1;
                     const int first = (w.span.first + w.page + i) * kPage;
                     const int qa = max(0, w.span.lo - first) / kQuarter;
@@ -286,7 +286,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             const int stage = unit % kRowsStages;
             const uint32_t parity = unit / kRowsStages & 1;
             const int key0 = (w.span.first + w.page + i) * kPage + warp * 16;   // of this warp's keys
-            failed = !barrier_wait(k_full(stage), parity, &stop) || !barrier_wait(v_full(stage), parity, &stop);
+            failed = !barrier_wait(k_full(stage), parity, stop) || !barrier_wait(v_full(stage), parity, stop);
             if (failed) break;
             if (key0 < w.span.hi && key0 + 16 > w.span.lo) {
                 const uint32_t slice = stage * kPageTile + (warp >> 1) * kQuarterBytes + (warp & 1) * 16 * 128;
@@ -403,7 +403,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
                                             (w.head * p.group + g) * p.q_head,
                                      p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, ka + pages * kPage), top,
-                                     sum, x);
+                                     sum, x, stop + 1);
             } else {
                 const int stat = (lane & (kRowsWarps - 1)) * kRows + r;
                 const float mi = join_m[stat];
@@ -706,7 +706,7 @@ struct TilesControl {
     Share share;
     uint32_t tmem;
     int irregular;                       // what the guard found in the piece
-    int stop;                            // a wait ran out
+    int stop[2];                         // a wait ran out, and work that lets waits go on
 };
 constexpr uint32_t kControlBytes = 8192 - 1024;   // operands follow at the next whole KiB, which the swizzle needs
 static_assert(sizeof(TilesControl) <= kControlBytes, "control block");
@@ -748,7 +748,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     TilesControl& c = *reinterpret_cast<TilesControl*>(smem_raw);
-    volatile int* const stop = &c.stop;
+    volatile int* const stop = c.stop;
     const uint32_t q_smem = (smem_addr(smem_raw) + kControlBytes + 1023) & ~1023u, ring = q_smem + 2 * kTileBytes;
     auto kv_full = [&](int i) { return smem_addr(&c.kv_full[i]); };
     auto kv_empty = [&](int i) { return smem_addr(&c.kv_empty[i]); };
@@ -777,7 +777,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         barrier_init(checked, 1);
         barrier_init(taken, kSoftWarps);
         for (int i = 0; i < kItems; ++i) barrier_init(item_full(i), 1);
-        c.stop = 0;
+        c.stop[0] = c.stop[1] = 0;
         c.irregular = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
@@ -1189,7 +1189,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q0 + t * tokens + tok) * p.q_token +
                                                     (w.head * p.group + head) * p.q_head,
                                              p.table + w.s * p.table_stride, w.head, max(a, page_key),
-                                             min(b + 1, page_key + pages * kPage), mm, ll, x);
+                                             min(b + 1, page_key + pages * kPage), mm, ll, x, stop + 1);
                         if (split) {
                             reinterpret_cast<float4*>(slot)[((t * 4 + rows0 / 32) * 32 + lane) * 32 + r] = x;
                             if (lane == 0) {

@@ -800,3 +800,14 @@ def test_status_of_the_streams_own_workspace(paged):
     with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
         with pytest.raises(RuntimeError):
             paged.attend_status(paged._workspaces[0, side.cuda_stream])
+
+
+@pytest.mark.parametrize("lens", [[(5, 30000)], [(150, 20000)]])
+def test_values_that_do_not_leak_after_long_contexts(paged, lens):
+    """Rows taken key by key over a long context, while the kernel's other warps wait for them."""
+    c = Case(paged, lens, 8, 1, seed=4)
+    n, kv = lens[0]
+    c.set_row(0, kv - n // 2, 0, v=math.inf)
+    workspace = paged.attend_workspace("cuda:0")
+    c.check(paged.attend(c.pages, c.chunk, c.q, workspace=workspace))
+    assert paged.attend_status(workspace) == 0
