@@ -136,14 +136,15 @@ int secure_infer_paged_copy(const secure_infer_page_tensor* tensors, uint32_t n_
  * parents[i].  It shares the full pages and gets a copy of a partial last one,
  * in the lowest free page; requests are served in order, and granted[i] = 0
  * where the child is not empty or given twice, an index is out of range, or no
- * page is left. */
+ * page is left for it. */
 int secure_infer_paged_fork(const secure_infer_page_tensor* tensors, uint32_t n_tensors, uint64_t page_bytes,
                             const secure_infer_tables* in, const secure_infer_tables* out, const int32_t* parents,
                             const int32_t* children, uint32_t n, int32_t* granted, void* scratch, void* stream);
 
 /* reserve: sequence seqs[i] grows to new_lens[i] tokens, on the lowest free
  * pages in order; granted[i] = 0 where it would shrink, does not fit the table,
- * is given twice, its partial last page is shared, or no page is left. */
+ * is given twice, its partial last page is shared, or fewer pages are left than
+ * it needs (later requests may still have them). */
 int secure_infer_paged_reserve(const secure_infer_tables* in, const secure_infer_tables* out, const int32_t* seqs,
                                const int32_t* new_lens, uint32_t n, int32_t* granted, void* scratch, void* stream);
 

@@ -241,6 +241,7 @@ template <int kOp, int kCluster>
 __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __grid_constant__ TableParams p)
 {
     __shared__ int sums[33];
+    __shared__ int needs[kOp == kFork || kOp == kReserve ? kTableThreads + 1 : 1];
     wait_for_earlier_kernels();
     const int tid = threadIdx.x, cta = blockIdx.x, lane = tid & 31;
     const int all = cta * kTableThreads + tid, stride = kCluster * kTableThreads;
@@ -275,7 +276,8 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
             if (c < cta) free_before += k;
             free_all += k;
         }
-        // Every CTA walks the requests, CTA 0 writes what it finds.
+        // Every CTA walks the requests, CTA 0 writes what it finds.  Where a block of them asks for more than is left one
+        // thread goes through them, as a request that finds too few pages leaves them to the next: 1024 take it 13 us.
         int needed = 0;
         for (int i0 = 0; i0 < p.n; i0 += kTableThreads) {
             const int i = i0 + tid;
@@ -303,10 +305,30 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
                 }
             }
             int total;
-            const int place = needed + block_prefix(need, sums, total);
+            int place = block_prefix(need, sums, total);
+            // (Sums of needs this large might pass 32 bits.)
+            if (__syncthreads_or(need > 1 << 20) || total > free_all - needed) {
+                needs[tid] = need;
+                __syncthreads();
+                if (tid == 0) {
+                    const int left = free_all - needed;
+                    int taken = 0;
+                    for (int k = 0; k < min(kTableThreads, p.n - i0); ++k) {
+                        const int want = needs[k];
+                        const bool fits = want <= left - taken;
+                        needs[k] = fits ? taken : -1;
+                        taken += fits ? want : 0;
+                    }
+                    needs[kTableThreads] = taken;
+                }
+                __syncthreads();
+                place = needs[tid];
+                ok = ok && place >= 0;
+                total = needs[kTableThreads];
+            }
+            place += needed;
             needed += total;
             if (cta == 0 && i < p.n) {
-                ok = ok && (need == 0 || place + need <= free_all);
                 p.granted[i] = ok;
                 s.place[i] = place;
                 if (ok) s.row_of[to] = i;
@@ -325,7 +347,7 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
                 else s.first[rank] = i;
             }
         }
-        if (kOp == kFork && cta == 0 && tid == 0) *s.copies = min(needed, free_all);
+        if (kOp == kFork && cta == 0 && tid == 0) *s.copies = needed;
         cluster_barrier<kCluster>();
     }
     if (kOp == kFree) {

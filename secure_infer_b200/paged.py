@@ -316,7 +316,8 @@ class CachePages:
         """Grow sequence ``seqs[i]`` to ``lens[i]`` tokens on the lowest free
         pages.  Returns the new tables and ``granted`` int32 ``[n]``: 0 where it
         would shrink or not fit the table, is named twice, its partial last page
-        is shared, or pages ran out (requests are served in order)."""
+        is shared, or fewer pages are left than it needs (requests are served in
+        order, and later ones may still have those)."""
         a, b = self._pair(seqs, lens, ("seqs", "lens"))
         return self._run("reserve", tables, out, a, b)
 

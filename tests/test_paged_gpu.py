@@ -811,3 +811,50 @@ def test_values_that_do_not_leak_after_long_contexts(paged, lens):
     workspace = paged.attend_workspace("cuda:0")
     c.check(paged.attend(c.pages, c.chunk, c.q, workspace=workspace))
     assert paged.attend_status(workspace) == 0
+
+
+# ------------------------------------------- requests that find too few pages
+
+def test_reserve_goes_on_after_a_request_that_does_not_fit(paged):
+    """Five free pages: ten do not fit, the two that the next one asks for do, then three, then none is left."""
+    data = torch.zeros((1, 2, 8, 128, 1, 128), dtype=torch.bfloat16, device="cuda")
+    cache = paged.CachePages([[d[0], d[1]] for d in data])
+    t = paged.PageTables(torch.full((6, 12), -1, dtype=torch.int32, device="cuda"), torch.zeros(6, dtype=torch.int32, device="cuda"),
+                         torch.tensor([0, 1, 0, 0, 1, 0, 1, 0], dtype=torch.int32, device="cuda"))
+    new, granted = cache.reserve(t, [0, 1, 2, 3, 4, 5], [1280, 256, 513, 384, 1, 0])
+    assert granted.tolist() == [0, 1, 0, 1, 0, 1]
+    assert new.lens.tolist() == [0, 256, 0, 384, 0, 0]
+    assert new.block_table[1, :3].tolist() == [0, 2, -1] and new.block_table[3, :4].tolist() == [3, 5, 7, -1]
+    assert (new.block_table[[0, 2, 4, 5]] == -1).all() and new.refs.tolist() == [1] * 8
+
+
+@pytest.mark.parametrize("seqs,width,pages", [(40, 8, 60), (700, 9, 900), (3000, 5, 2500), (2500, 40, 20000)])
+def test_reserve_with_few_pages(paged, seqs, width, pages):
+    """Every request that fits into what the ones before it left is granted, and no other."""
+    t, data, cache = model_of(paged, seqs, width, pages, seqs + 4, share=False)
+    table, lens, refs = (x.cpu().clone() for x in t)
+    r = torch.Generator().manual_seed(seqs)
+    order = torch.randperm(seqs, generator=r).tolist()
+    asks = [(s, min(width * 128, int(lens[s]) + int(torch.randint(0, width * 128, (1,), generator=r)))) for s in order]
+    asks[seqs // 2:seqs // 2] = [(order[0], width * 128), (-1, 3), (seqs, 3)]
+    new, granted = cache.reserve(t, [s for s, _ in asks], [n for _, n in asks])
+    free, want, seen = [p for p in range(pages) if refs[p] == 0], [], set()
+    some_after_a_refusal = False
+    for s, n in asks:
+        ok = 0 <= s < seqs and s not in seen
+        seen.add(s)
+        if ok:
+            a, b = -(-int(lens[s]) // 128), -(-n // 128)
+            ok = b - a <= len(free)
+            if ok and b > a:
+                some_after_a_refusal |= 0 in want
+                table[s, a:b] = torch.tensor(free[:b - a], dtype=torch.int32)
+                refs[free[:b - a]] = 1
+                del free[:b - a]
+        if ok:
+            lens[s] = n
+        want.append(int(ok))
+    assert some_after_a_refusal
+    assert granted.tolist() == want
+    assert torch.equal(new.block_table.cpu(), table) and torch.equal(new.lens.cpu(), lens) and torch.equal(new.refs.cpu(), refs)
+    assert consistent(new)
