@@ -180,7 +180,8 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     p.rows_min = 1;
     p.rows_max = INT_MAX;
     p.causal = causal != 0;
-    p.window = static_cast<int32_t>(window);
+    // As many tokens as a table can hold hide nothing, and positions less such a window might pass 32 bits.
+    p.window = window >= static_cast<uint64_t>(chunk->table_width) * kPage ? 0 : static_cast<int32_t>(window);
     p.scale_log2 = scale * 1.4426950408889634f;
     // Hidden scores are -inf before they are scaled, so the scale is never zero; at 1e-30 all weights are 1.
     if (p.scale_log2 > -1e-30f && p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;

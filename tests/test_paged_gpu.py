@@ -858,3 +858,12 @@ def test_reserve_with_few_pages(paged, seqs, width, pages):
     assert granted.tolist() == want
     assert torch.equal(new.block_table.cpu(), table) and torch.equal(new.lens.cpu(), lens) and torch.equal(new.refs.cpu(), refs)
     assert consistent(new)
+
+
+@pytest.mark.parametrize("lens", [[(10, 4)], [(200, 50), (3, 1), (1, 300)], [(300, 120)]])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 100000])
+def test_windows_that_hide_nothing(paged, lens, window):
+    """The largest windows, with rows at positions before the sequence's first."""
+    c = Case(paged, lens, 8, 2, seed=6)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, window=window, return_lse=True)
+    c.check(out, lse)
