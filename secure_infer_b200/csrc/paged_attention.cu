@@ -656,7 +656,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
 // 2^x of a pair on the multiply-add units, for x <= 126: x = n + f with n the
 // nearest integer, 2^f by the polynomial of degree 4 with the least largest
 // relative error on [-1/2, 1/2] (2.7e-6, by Remez's exchange), n added to the
-// exponent.  Below -126 it stays at 2^-126.  NaN does not survive.
+// exponent.  Below -126 it stays at 2^-126, which beside a largest weight of 2^-8
+// or more is nothing.  NaN does not survive.
 __device__ __forceinline__ float2 exp2_poly(uint64_t x2)
 {
     constexpr float kRound = 12582912.0f;   // 1.5 2^23: the sum's last bits are n
@@ -1087,7 +1088,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         const float top = max3_nan(tops[0], tops[1], tops[1]);
                         // Weights may cover scores once the row's other threads have read theirs.
                         tmem_fence_before();
-                        fresh = meet_or(!((top - m) * scale <= kRescale) && top != -INFINITY);
+                        // (A row that has only met scores of minus infinity is not for the polynomial either.)
+                        fresh = meet_or(!((top - m) * scale <= kRescale));
                         tmem_fence_after();
                         if (!fresh) {
                             tmem_store(w_at, w2);

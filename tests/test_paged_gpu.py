@@ -867,3 +867,26 @@ def test_windows_that_hide_nothing(paged, lens, window):
     c = Case(paged, lens, 8, 2, seed=6)
     out, lse = paged.attend(c.pages, c.chunk, c.q, window=window, return_lse=True)
     c.check(out, lse)
+
+
+@pytest.mark.parametrize("lens", [[(1, 300)], [(5, 700)], [(40, 1000)], [(200, 1000)], [(500, 2000)]])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (64, 32)])
+def test_rows_whose_scores_are_all_minus_infinity(paged, lens, heads, kv_heads):
+    """A query that meets keys of minus infinity alone has no softmax: NaN, as 0 / 0 is, and not an average of values.
+    Rows that see one finite score have all their weight there."""
+    c = Case(paged, lens, heads, kv_heads, seed=7)
+    n, kv = lens[0]
+    c.q[:, :, 0] = 1.0                                    # so that a key's minus infinity is its score's
+    c.rows[0][0][:, ::2, 0] = -math.inf
+    for i in range(0, kv, 128):
+        c.k[c.table[0, i // 128], :min(128, kv - i), ::2, 0] = -math.inf
+    odd = torch.arange(heads, device="cuda") // 2 % 2 == 1
+    out = paged.attend(c.pages, c.chunk, c.q)
+    assert torch.isnan(out[:, ~odd]).all()
+    want, _, bound = c.expected()
+    assert ((out.double() - want).abs() <= bound)[:, odd].all()
+    for h in range(0, kv_heads, 2):
+        c.set_row(0, 200, h, k=0.0)                       # one finite score, on a page after the first
+    out, seen = paged.attend(c.pages, c.chunk, c.q)[:, ~odd], torch.arange(kv - n, kv, device="cuda") >= 200
+    assert torch.isnan(out[~seen]).all()
+    assert torch.equal(out[seen], c.rows[0][1][200, ::2].repeat_interleave(2, 0).expand_as(out[seen]))
