@@ -910,6 +910,18 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                     if (lane == 0) barrier_arrive(q_empty);
                 } else {
+                    // Rows that are not used become zero: the warps rescale 32 rows together, and with others' queries,
+                    // or what shared memory held, beside them, the roundings of the used ones would follow those.
+                    const int used = min(rows_per_tile, w.rows - t * rows_per_tile);
+                    if (used < 128) {
+                        for (int x = lane; x < (128 - used) * 16; x += 32) {
+                            const uint32_t at = q_smem + t * kTileBytes + (x & 8 ? kTileBytes / 2 : 0) +
+                                                (used + (x >> 4)) * 128 + (x & 7) * 16;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
                     ok = ok && barrier_wait(kv_full(n % kRing), (n / kRing) & 1, stop);
                     if (!ok) break;
                     tmem_fence_after();

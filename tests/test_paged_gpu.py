@@ -890,3 +890,31 @@ def test_rows_whose_scores_are_all_minus_infinity(paged, lens, heads, kv_heads):
     out, seen = paged.attend(c.pages, c.chunk, c.q)[:, ~odd], torch.arange(kv - n, kv, device="cuda") >= 200
     assert torch.isnan(out[~seen]).all()
     assert torch.equal(out[seen], c.rows[0][1][200, ::2].repeat_interleave(2, 0).expand_as(out[seen]))
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads", [([(600, 3000)], 28, 4), ([(300, 2500), (100, 1500)], 40, 8)])
+def test_results_do_not_depend_on_what_shared_memory_held(paged, lens, heads, kv_heads):
+    """Groups that do not fill a tile's 128 rows: after calls that leave finite values or NaN in shared memory, the same
+    bits."""
+    c = Case(paged, lens, heads, kv_heads, seed=8)
+    before = Case(paged, [(1, 700)] * 80, 16, 8)
+    got = []
+    for value in (0.5, math.nan, 2.0, math.nan):
+        before.k.fill_(value)
+        before.v.fill_(value)
+        paged.attend(before.pages, before.chunk, before.q)
+        got.append(paged.attend(c.pages, c.chunk, c.q))
+    c.check(got[0])
+    assert all(torch.equal(g, got[0]) for g in got)
+
+
+@pytest.mark.parametrize("lens", [[(500, 2500)], [(100, 1500), (250, 2000)]])
+def test_results_do_not_depend_on_tokens_of_nobody(paged, lens):
+    """Queries past the chunk's last token, as a padded step has them."""
+    c = Case(paged, lens, 32, 8, seed=9)
+    got = []
+    for value in (0.0, math.nan, 50.0):
+        q = torch.cat((c.q, torch.full((64, 32, 128), value, dtype=c.dtype, device="cuda")))
+        got.append(paged.attend(c.pages, c.chunk, q)[:c.cu[-1]])
+    c.check(got[0])
+    assert all(torch.equal(g, got[0]) for g in got)
