@@ -66,7 +66,8 @@ typedef struct {
  * causal: the token at position p sees keys 0..p (else all of its sequence),
  * and with window > 0 only the last `window` of them.  A row that sees no key
  * gives zeros and -inf.  Keys that a row does not see take no part in it,
- * whatever they hold.  workspace: secure_infer_paged_attend_workspace() bytes,
+ * whatever they hold.  workspace: secure_infer_paged_attend_workspace() bytes
+ * (41 MB on a device of 148 SMs; it is asked with that device current),
  * 256-byte aligned, zero before its first use, used by one stream at a time;
  * calls leave it ready for the next. */
 #define SECURE_INFER_ATTEND_STATE_BYTES 4096u   /* of a workspace, from its start: all that has to be zero */

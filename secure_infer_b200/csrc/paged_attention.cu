@@ -9,6 +9,7 @@
 #include "paged.cuh"
 #include "gcm_kernels.cuh"
 
+#include <atomic>
 #include <mutex>
 
 namespace sib {
@@ -16,7 +17,7 @@ namespace paged {
 namespace {
 
 // Workspace: the status word, counters, cuts, then partial results.
-constexpr int kMaxGrid = 256;
+constexpr int kMaxGrid = 256;   // CTAs; a device with fewer SMs has as many
 constexpr uint64_t kCounterOffset = 256;
 constexpr uint64_t kCutOffset = SECURE_INFER_ATTEND_STATE_BYTES;
 static_assert(kCounterOffset + 3 * kMaxGrid * sizeof(uint32_t) <= kCutOffset, "counters");
@@ -1373,8 +1374,20 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     else join_values<T, 1>(p, cut, r, tile_row, d4);
 }
 
+// CTAs of a launch on the current device.
+int attend_grid()
+{
+    static std::atomic<int> grids[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return kMaxGrid;
+    std::atomic<int>& grid = grids[dev & 63];
+    if ((n = grid.load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return kMaxGrid;
+    grid.store(n = n < kMaxGrid ? n : kMaxGrid, std::memory_order_relaxed);
+    return n;
+}
+
 struct Device {
-    int sms = 0;
     bool rows_set[2] = {};
     bool tiles_set[2] = {};
 };
@@ -1386,11 +1399,10 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
 {
     int dev = 0;
     cudaGetDevice(&dev);
-    int sms;
+    const int grid = attend_grid();
     {
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
-        if (d.sms == 0) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
         bool& set = d.rows_set[std::is_same<T, __half>::value];
         if (!set) {
             const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T>,
@@ -1398,10 +1410,9 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
             if (e != cudaSuccess) return e;
             set = true;
         }
-        sms = d.sms;
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(sms < kMaxGrid ? sms : kMaxGrid);
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kRowsThreads);
     cfg.dynamicSmemBytes = kRowsSmem;
     cfg.stream = stream;
@@ -1420,11 +1431,10 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
 {
     int dev = 0;
     cudaGetDevice(&dev);
-    int sms;
+    const int grid = attend_grid();
     {
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
-        if (d.sms == 0) cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
         bool& set = d.tiles_set[std::is_same<T, __half>::value];
         if (!set) {
             const cudaError_t e = cudaFuncSetAttribute(paged_attend_tiles_kernel<T>,
@@ -1432,10 +1442,9 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
             if (e != cudaSuccess) return e;
             set = true;
         }
-        sms = d.sms < kMaxGrid ? d.sms : kMaxGrid;
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(sms);
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kTileThreads);
     cfg.dynamicSmemBytes = kTilesSmem;
     cfg.stream = stream;
@@ -1449,7 +1458,7 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
         const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attend_tiles_kernel<T>, q_map, k_map, v_map, p);
         if (e != cudaSuccess) return e;
     }
-    cfg.gridDim = dim3(kJoinBlocks, sms);
+    cfg.gridDim = dim3(kJoinBlocks, grid);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     ProfileScope prof(kKernAttendJoin, stream);
@@ -1474,7 +1483,7 @@ int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const
 
 uint64_t attend_workspace_bytes()
 {
-    return kSlotOffset + static_cast<uint64_t>(2 * kMaxGrid) * (kTileSlot + kRowSlot) * sizeof(float);
+    return kSlotOffset + static_cast<uint64_t>(2 * attend_grid()) * (kTileSlot + kRowSlot) * sizeof(float);
 }
 
 void attend_workspace(void* workspace, AttendParams* p)
@@ -1483,7 +1492,7 @@ void attend_workspace(void* workspace, AttendParams* p)
     p->counters = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kCounterOffset);
     p->cuts = reinterpret_cast<Cut*>(static_cast<char*>(workspace) + kCutOffset);
     p->slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotOffset);
-    p->row_slots = p->slots + static_cast<uint64_t>(2 * kMaxGrid) * kTileSlot;
+    p->row_slots = p->slots + static_cast<uint64_t>(2 * attend_grid()) * kTileSlot;
 }
 
 }  // namespace paged

@@ -172,10 +172,25 @@ _captured: dict = {}     # (device, stream): the stream's latest capture and wha
 _STATE = 4096            # SECURE_INFER_ATTEND_STATE_BYTES
 
 
+def _workspace_bytes(index: int) -> int:
+    return int(_on(index, _native.lib().secure_infer_paged_attend_workspace))
+
+
 def attend_workspace(device) -> torch.Tensor:
-    """A workspace for ``attend``.  Calls that may run at the same time, on two
-    streams or in a graph beside either, need one each."""
-    return torch.zeros(int(_native.lib().secure_infer_paged_attend_workspace()), dtype=torch.uint8, device=device)
+    """A workspace for ``attend`` (41 MB on a B200).  Calls that may run at the
+    same time, on two streams or in a graph beside either, need one each."""
+    device = torch.device(device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch.zeros(_workspace_bytes(index), dtype=torch.uint8, device=torch.device("cuda", index))
+
+
+def release_workspaces(stream: torch.cuda.Stream | None = None) -> None:
+    """Give up the workspaces that ``attend`` keeps, of all streams or of one:
+    before a stream is destroyed, since its handle may come back as another's.
+    The next call makes a new one."""
+    for kept in (_workspaces, _captured):
+        for key in [k for k in kept if stream is None or k == (stream.device.index, stream.cuda_stream)]:
+            del kept[key]
 
 
 def _workspace(index: int, stream: int) -> torch.Tensor:
@@ -185,8 +200,7 @@ def _workspace(index: int, stream: int) -> torch.Tensor:
         # stream's next capture lest this one gives it to other tensors, cleared at every replay's first call.
         held, w = _captured.get((index, stream), (0, None))
         if held != capture:
-            size = int(_native.lib().secure_infer_paged_attend_workspace())
-            w = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+            w = torch.empty(_workspace_bytes(index), dtype=torch.uint8, device=torch.device("cuda", index))
             w[:_STATE].zero_()
             _captured[index, stream] = capture, w
         return w

@@ -918,3 +918,30 @@ def test_results_do_not_depend_on_tokens_of_nobody(paged, lens):
         got.append(paged.attend(c.pages, c.chunk, q)[:c.cu[-1]])
     c.check(got[0])
     assert all(torch.equal(g, got[0]) for g in got)
+
+
+def test_workspaces_are_of_the_devices_size_and_can_be_given_up(paged):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    workspace = paged.attend_workspace("cuda")
+    assert workspace.device == torch.device("cuda", 0)
+    assert 0 < workspace.nbytes - 4 * 2 * sms * (256 + 8) * 130 < 16384   # two partial results a CTA, counters and cuts
+    c = Case(paged, [(1, 20000), (300, 5000)], 8, 1)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with torch.cuda.stream(side):
+            out = paged.attend(c.pages, c.chunk, c.q)
+        side.synchronize()
+        c.check(out)
+        assert (0, side.cuda_stream) in paged._workspaces
+        paged.release_workspaces(side)
+        assert (0, side.cuda_stream) not in paged._workspaces
+    paged.attend(c.pages, c.chunk, c.q)
+    paged.release_workspaces()
+    assert not paged._workspaces and not paged._captured
+    # Nothing is written past a workspace of the size that is asked for.
+    n = workspace.nbytes
+    guarded = torch.full((n + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+    guarded[:n].zero_()
+    c.check(paged.attend(c.pages, c.chunk, c.q, workspace=guarded[:n]))
+    assert (guarded[n:] == 0x5A).all()
