@@ -146,7 +146,9 @@ constexpr long long kWaitClocks = 1ll << 32;   // some seconds
 // happened for some seconds stop[0] is set and every wait of the CTA gives up, so
 // a protocol error ends the kernel instead of hanging it; the rows of the CTA
 // become NaN then.  stop[1] goes up while warps are at work that may take longer
-// than that, and the others wait on.  Returns whether the phase completed.
+// than that, and the others wait on.  Returns whether the phase completed: the
+// lanes of a warp are together and read one barrier, one flag and one clock, so
+// they get one answer.  (Votes on it took a chunk of 512 tokens 1.2 us.)
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* stop)
 {
     if (barrier_done(bar, parity)) return true;
@@ -165,14 +167,6 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
         }
     }
     return true;
-}
-
-// The same by a warp whose lanes may come apart.  (In the loops over pages they
-// are together and read one barrier, one flag and one clock; votes there took a
-// chunk of 512 tokens 1.2 us.)
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop)
-{
-    return __all_sync(0xffffffffu, barrier_wait(bar, parity, stop));
 }
 
 // For copies and products that have been issued: they write memory that the CTA

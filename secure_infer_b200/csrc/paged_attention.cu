@@ -898,7 +898,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             };
             bool ok = true;
             while (ok && any) {
-                ok = warp_wait(item_full(item), (item / kItems) & 1, stop) && warp_wait(q_full, item & 1, stop);
+                ok = barrier_wait(item_full(item), (item / kItems) & 1, stop) && barrier_wait(q_full, item & 1, stop);
                 if (!ok) break;
                 const Item& w = c.items[item % kItems];
                 const int pages = w.pages;
@@ -911,15 +911,13 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     }
                     if (lane == 0) barrier_arrive(q_empty);
                 } else {
-                    // Rows that are not used become zero: the warps rescale 32 rows together, and with others' queries,
-                    // or what shared memory held, beside them, the roundings of the used ones would follow those.
-                    const int used = min(rows_per_tile, w.rows - t * rows_per_tile);
-                    if (used < 128) {
-                        for (int x = lane; x < (128 - used) * 16; x += 32) {
-                            const uint32_t at = q_smem + t * kTileBytes + (x & 8 ? kTileBytes / 2 : 0) +
-                                                (used + (x >> 4)) * 128 + (x & 7) * 16;
+                    // Unused rows beside used ones become zero: 32 rows are rescaled together, and the roundings of the
+                    // used ones would follow others' queries, or what shared memory held.
+                    if (const int used = min(rows_per_tile, w.rows - t * rows_per_tile); used & 31) {
+                        const uint32_t end = q_smem + t * kTileBytes + (lane & 8 ? kTileBytes / 2 : 0) + ((used | 31) + 1) * 128;
+#pragma unroll 4
+                        for (uint32_t at = end - ((used | 31) + 1 - used - (lane >> 4)) * 128 + (lane & 7) * 16; at < end; at += 256)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
-                        }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
@@ -991,7 +989,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             // would carry it over.
             uint32_t n = 0, item = 0;
             while (any) {
-                if (!warp_wait(item_full(item), (item / kItems) & 1, stop)) break;
+                if (!barrier_wait(item_full(item), (item / kItems) & 1, stop)) break;
                 const Item w = c.items[item % kItems];
                 const int pages = w.pages, lo_all = w.lo_all, hi_all = w.hi_all;
                 uint32_t odd = 0;
@@ -1053,7 +1051,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
         uint32_t seen[2] = {0, 0}, done[2] = {0, 0}, item = 0;   // completions of s_full and o_full taken
         bool ok = true;
         while (any) {
-            ok = ok && warp_wait(item_full(item), (item / kItems) & 1, stop);
+            ok = ok && barrier_wait(item_full(item), (item / kItems) & 1, stop);
             if (meet_or(!ok)) break;
             const Item& w = c.items[item % kItems];
             const int pages = w.pages, tiles = w.rows > rows_per_tile ? 2 : 1;
@@ -1180,14 +1178,14 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     if (lane == 0) barrier_arrive(p_ready(t));
                 }
             }
-            ok = ok && warp_wait(checked, item & 1, stop);
+            ok = ok && barrier_wait(checked, item & 1, stop);
             ok = !meet_or(!ok);   // the four go the same way
             const bool split = w.slot >= 0, by_definition = ok && *static_cast<volatile int*>(&c.irregular) != 0;
             float* slot = p.slots + static_cast<int64_t>(w.slot) * kTileSlot;
             const uint32_t stage = ring + kRing * kTileBytes + warp * kStageBytes;
 #pragma unroll 1
             for (int t = 0; t < tiles; ++t) {
-                ok = ok && warp_wait(o_full(t), (t ? done[1] : done[0]) & 1, stop);
+                ok = ok && barrier_wait(o_full(t), (t ? done[1] : done[0]) & 1, stop);
                 if (t) ++done[1];
                 else ++done[0];
                 tmem_fence_after();
