@@ -27,6 +27,19 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
     return fn;
 }
 
+// The encoder wants the device's context, which a host thread only has once it has called the runtime.
+template <class... Args>
+bool encoded(Args... args)
+{
+    const auto encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    CUresult e = encode(args...);
+    if (int device = 0; e == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess &&
+                        cudaSetDevice(device) == cudaSuccess)
+        e = encode(args...);
+    return e == CUDA_SUCCESS;
+}
+
 bool aligned16(const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool stride_ok(int64_t elements) { return elements > 0 && elements % 8 == 0 && elements < (int64_t(1) << 38); }
 
@@ -56,11 +69,8 @@ bool page_map(CUtensorMap* map, const secure_infer_pages* p, const void* base, c
                                  static_cast<cuuint64_t>(stride[0]) * 2};
     const cuuint32_t box[5] = {64, tokens, 2, 1, 1}, step[5] = {1, 1, 1, 1, 1};
     const auto type = p->dtype == SECURE_INFER_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const auto encode = tensor_map_encoder();
-    return encode != nullptr &&
-           encode(map, type, 5, const_cast<void*>(base), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded(map, type, 5, const_cast<void*>(base), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // Queries as [half of a head][token][query head][64 values], in boxes of a KV
@@ -72,11 +82,8 @@ bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, int64_t token_str
     const cuuint64_t bytes[3] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2, 128};
     const cuuint32_t box[4] = {64, group, 128 / group, 1}, step[4] = {1, 1, 1, 1};
     const auto type = dtype == SECURE_INFER_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const auto encode = tensor_map_encoder();
-    return encode != nullptr &&
-           encode(map, type, 4, const_cast<void*>(q), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return encoded(map, type, 4, const_cast<void*>(q), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // Rows per KV head up to which a sequence goes to the kernel for few rows, in

@@ -945,3 +945,31 @@ def test_workspaces_are_of_the_devices_size_and_can_be_given_up(paged):
     guarded[:n].zero_()
     c.check(paged.attend(c.pages, c.chunk, c.q, workspace=guarded[:n]))
     assert (guarded[n:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("through", ["python", "c"])
+def test_a_host_thread_may_begin_with_attend(paged, through):
+    """A thread that has called nothing else of CUDA."""
+    import threading
+    from secure_infer_b200 import _native
+    c = Case(paged, [(1, 900), (200, 600)], 8, 2)
+    want = paged.attend(c.pages, c.chunk, c.q)
+    out, workspace = torch.empty_like(c.q), paged.attend_workspace("cuda:0")
+    chunk = _native.Chunk.from_buffer_copy(c.chunk._c)
+    chunk.tokens = c.q.shape[0]
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        if through == "python":
+            got.append(paged.attend(c.pages, c.chunk, c.q, out=out, workspace=workspace) is not None)
+        else:
+            got.append(_native.lib().secure_infer_paged_attend(
+                c.pages._address, _native.ct.addressof(chunk), c.q.data_ptr(), c.q.stride(0), c.q.stride(1), 8, out.data_ptr(),
+                None, 128 ** -0.5, 1, 0, workspace.data_ptr(), None) == 0)
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert got == [True] and torch.equal(out, want)
