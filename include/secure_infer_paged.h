@@ -68,7 +68,8 @@ typedef struct {
  * gives zeros and -inf.  Keys that a row does not see take no part in it,
  * whatever they hold.  workspace: secure_infer_paged_attend_workspace() bytes
  * (41 MB on a device of 148 SMs; it is asked with that device current),
- * 256-byte aligned, zero before its first use, used by one stream at a time;
+ * 256-byte aligned, zero before its first use, used by one stream at a time
+ * (host threads that share the stream may share it too);
  * calls leave it ready for the next. */
 #define SECURE_INFER_ATTEND_STATE_BYTES 4096u   /* of a workspace, from its start: all that has to be zero */
 /* Waits inside the kernels have a limit of some seconds.  One that runs out ends

@@ -194,6 +194,9 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     if (p.scale_log2 > -1e-30f && p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
     attend_workspace(workspace, &p);
     const auto st = static_cast<cudaStream_t>(stream);
+    // One call's launches follow one another on the stream: they hand the workspace on.
+    static std::mutex launches;
+    const std::lock_guard<std::mutex> lock(launches);
     // Up to kFewRows rows per KV head a sequence is bound by reading K and V once, which the kernel for few rows does
     // with less latency; more rows are worth tiles of 128.
     const bool tiles = max_rows > kFewRows && group <= 128;

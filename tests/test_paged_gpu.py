@@ -973,3 +973,34 @@ def test_a_host_thread_may_begin_with_attend(paged, through):
     thread.join()
     torch.cuda.synchronize()
     assert got == [True] and torch.equal(out, want)
+
+
+def test_host_threads_that_share_a_stream_and_a_workspace(paged):
+    """Each call is up to three launches that hand the workspace on; two threads' calls do not come between."""
+    import threading
+    from secure_infer_b200 import _native
+    cases = [Case(paged, lens, 8, 1, seed=i) for i, lens in enumerate(([(300, 4000), (1, 900), (2, 70)], [(200, 6000), (1, 2500)]))]
+    workspace, stream = paged.attend_workspace("cuda:0"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    want = [paged.attend(c.pages, c.chunk, c.q) for c in cases]
+    outs = [[torch.empty_like(c.q) for _ in range(60)] for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(c, outs):
+        chunk = _native.Chunk.from_buffer_copy(c.chunk._c)
+        chunk.tokens = c.q.shape[0]
+        for o in outs:   # ctypes lets the other thread run during the call
+            bad.append(_native.lib().secure_infer_paged_attend(
+                c.pages._address, _native.ct.addressof(chunk), c.q.data_ptr(), c.q.stride(0), c.q.stride(1), 8, o.data_ptr(),
+                None, 128 ** -0.5, 1, 0, workspace.data_ptr(), stream.cuda_stream))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    stream.synchronize()
+    assert bad == [0] * 120
+    for w, got in zip(want, outs):
+        assert all(torch.equal(o, w) for o in got)
