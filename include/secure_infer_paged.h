@@ -81,6 +81,10 @@ uint64_t secure_infer_paged_attend_workspace(void);
  * call uses its workspace wherever the graph is replayed, so it needs one that
  * no other stream's calls use meanwhile. */
 uint64_t secure_infer_capture_id(void* stream);
+/* 1 where a call of this size is not refused, 0 where it has more than 2^31 - 1
+ * units of work (a page for a tile of rows and a KV head), by the longest context
+ * that the table's width can hold. */
+int secure_infer_attend_fits(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads);
 /* Waits for the stream, which is the one exception here.  *status: 0, or 1 if a
  * wait ran out in a call with this workspace; then its state is zero again and
  * the next call computes.  -1 while the stream is captured. */

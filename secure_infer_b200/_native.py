@@ -140,6 +140,7 @@ PAGED_SIGNATURES = {
 }
 HOST_SIGNATURES.update(PAGED_SIGNATURES)
 HOST_SIGNATURES["secure_infer_capture_id"] = ([P], U64)
+HOST_SIGNATURES["secure_infer_attend_fits"] = ([P, P, U32], I32)
 HOST_SIGNATURES["secure_infer_attend_status"] = ([P, P, P], I32)
 
 # SECURE_INFER_KIND_KV: a reload of 2n records, K packets first, V packets after.

@@ -93,6 +93,38 @@ bool rows_map(CUtensorMap* map, uint32_t dtype, const void* q, int64_t token_str
 // KV head with 24 rows 34 and 40; one of 300 tokens with 20 rows 7.3 and 14.0.
 constexpr uint32_t kFewRows = 24;
 
+// How a call is launched, and the most units of work that its launches may have
+// (a page for a tile and a KV head, and what a tile costs besides, in the
+// longest context that the table can hold).
+struct Work {
+    uint32_t group;
+    bool tiles;         // sequences of more than kFewRows rows go to the kernel for many
+    uint64_t rows_units, tiles_units;
+
+    // Units are counted in 32 bits.
+    bool fits() const { return rows_units <= INT_MAX && tiles_units <= INT_MAX; }
+};
+
+Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, uint32_t q_heads)
+{
+    Work w{q_heads / pages.heads, false, 0, 0};
+    const uint32_t max_q = chunk.max_q == 0 || chunk.max_q > chunk.tokens ? chunk.tokens : chunk.max_q;
+    const uint64_t max_rows = static_cast<uint64_t>(max_q) * w.group, rows = static_cast<uint64_t>(chunk.tokens) * w.group;
+    // Up to kFewRows rows per KV head a sequence is bound by reading K and V once, which the kernel for few rows does
+    // with less latency; more rows are worth tiles of 128.
+    w.tiles = max_rows > kFewRows && w.group <= 128;
+    const auto units = [&](uint64_t tiles, uint64_t cost) -> uint64_t {
+        return tiles * pages.heads > INT_MAX ? UINT64_MAX : tiles * pages.heads * (chunk.table_width + cost);
+    };
+    if (max_rows > INT_MAX) w.rows_units = UINT64_MAX;
+    else if (!w.tiles) w.rows_units = units(rows / 8 + chunk.seqs, 1);
+    else {
+        w.rows_units = chunk.seqs > 1 ? units(uint64_t(chunk.seqs) * (kFewRows / 8), 1) : 0;
+        w.tiles_units = units(rows / (2 * (128 / w.group * w.group)) + chunk.seqs, 2);
+    }
+    return w;
+}
+
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)
 {
     return in != nullptr && out != nullptr && in->block_table != nullptr && in->lens != nullptr && in->refs != nullptr &&
@@ -142,6 +174,12 @@ SI_EXPORT int secure_infer_attend_status(void* workspace, uint32_t* status, void
     return word == 0 || cudaMemsetAsync(workspace, 0, SECURE_INFER_ATTEND_STATE_BYTES, st) == cudaSuccess ? 0 : -1;
 }
 
+SI_EXPORT int secure_infer_attend_fits(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads)
+{
+    return pages_ok(pages) && chunk_ok(chunk) && q_heads > 0 && q_heads <= (1u << 16) && q_heads % pages->heads == 0 &&
+           work_of(*pages, *chunk, q_heads).fits();
+}
+
 SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
                                         int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out,
                                         float* lse, float scale, uint32_t causal, uint32_t window, void* workspace,
@@ -153,13 +191,9 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
         return -1;
     if (chunk->tokens == 0) return 0;
     if (!aligned16(q) || !aligned16(out) || !stride_ok(q_token_stride) || !stride_ok(q_head_stride)) return -1;
-    const uint32_t group = q_heads / pages->heads;
-    const uint32_t max_q = chunk->max_q == 0 || chunk->max_q > chunk->tokens ? chunk->tokens : chunk->max_q;
-    const uint64_t max_rows = static_cast<uint64_t>(max_q) * group;
-    if (max_rows > INT_MAX) return -1;
-    // Units of work (a page for eight rows and a KV head) are counted in 32 bits.
-    const uint64_t tiles8 = (static_cast<uint64_t>(chunk->tokens) * group / 8 + chunk->seqs) * pages->heads;
-    if (tiles8 > INT_MAX || tiles8 * (chunk->table_width + 1) > INT_MAX) return -1;
+    const Work work = work_of(*pages, *chunk, q_heads);
+    if (!work.fits()) return -1;
+    const uint32_t group = work.group;
 
     AttendParams p;
     std::memset(&p, 0, sizeof(p));
@@ -197,9 +231,7 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     // One call's launches follow one another on the stream: they hand the workspace on.
     static std::mutex launches;
     const std::lock_guard<std::mutex> lock(launches);
-    // Up to kFewRows rows per KV head a sequence is bound by reading K and V once, which the kernel for few rows does
-    // with less latency; more rows are worth tiles of 128.
-    const bool tiles = max_rows > kFewRows && group <= 128;
+    const bool tiles = work.tiles;
     CUtensorMap q_map, k_map, v_map;
     if (!tiles || chunk->seqs > 1) {
         if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))

@@ -138,8 +138,11 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
             if (secure_infer_paged_attend(pages, &chunk, r.data, r.token, r.head, static_cast<uint32_t>(r.heads),
                                           out.data_ptr(), want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
                                           static_cast<float>(scale), causal, static_cast<uint32_t>(window),
-                                          workspace.data_ptr(), address<void>(a[10])) != 0)
+                                          workspace.data_ptr(), address<void>(a[10])) != 0) {
+                need(secure_infer_attend_fits(pages, &chunk, static_cast<uint32_t>(r.heads)),
+                     "more work than one call takes: fewer tokens, or a narrower block table");
                 return failed("secure_infer_paged_attend");
+            }
         }
         if (!want_lse) return THPVariable_Wrap(std::move(out));
         PyObject* first = THPVariable_Wrap(std::move(out));

@@ -186,3 +186,26 @@ def test_status_refuses(lib):
     assert call(A + 16, ct.byref(word), None) == -1
     assert call(A, None, None) == -1
     assert word.value == 7
+
+
+def test_attend_fits_by_what_is_launched(lib):
+    """Units of work are a page for a tile: of 256 rows where there are more than a few, of eight otherwise."""
+    pages, chunk, _ = good()
+
+    def fits(tokens, max_q, width, seqs=1, heads=32, kv_heads=8):
+        pages.heads, chunk.tokens, chunk.max_q, chunk.seqs = kv_heads, tokens, max_q, seqs
+        chunk.table_width = chunk.table_stride = width
+        return lib.secure_infer_attend_fits(ct.byref(pages), ct.byref(chunk), heads)
+
+    assert fits(2, 1, 4, 2)
+    assert fits(65536, 0, 8192, heads=64)                  # a long prompt in a table for a million tokens
+    assert fits(65536, 0, 8192, 64, heads=64)
+    assert fits(2048, 0, 1 << 20) and fits(2048, 0, 1 << 22)
+    assert not fits(2048, 0, 1 << 22, heads=64, kv_heads=64)
+    assert not fits(1 << 20, 1, 1 << 12, 1 << 20)          # a million single tokens
+    assert fits(1 << 12, 1, 1 << 12, 1 << 12)
+    assert not fits(1 << 28, 0, 4, heads=4096)             # rows beyond 32 bits
+    assert not fits(4, 1, 1 << 24)                         # wider than a table may be
+    assert not fits(4, 1, 4, heads=33)
+    assert not lib.secure_infer_attend_fits(None, ct.byref(chunk), 32)
+    assert not lib.secure_infer_attend_fits(ct.byref(pages), None, 32)

@@ -1004,3 +1004,16 @@ def test_host_threads_that_share_a_stream_and_a_workspace(paged):
     assert bad == [0] * 120
     for w, got in zip(want, outs):
         assert all(torch.equal(o, w) for o in got)
+
+
+def test_wide_tables(paged):
+    """A table for a hundred million tokens costs nothing by itself; work beyond 32 bits is a refused argument."""
+    c = Case(paged, [(2048, 2100)], 8, 8)
+    want = paged.attend(c.pages, c.chunk, c.q)
+    table = torch.full((1, 1 << 20), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table
+    assert torch.equal(paged.attend(c.pages, paged.Chunk(table, c.chunk.cu_q, c.chunk.kv_lens), c.q), want)
+    many = Case(paged, [(2048, 2048)], 64, 64)
+    table = torch.full((1, 1 << 22), -1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="more work"):
+        paged.attend(many.pages, paged.Chunk(table, many.chunk.cu_q, many.chunk.kv_lens), many.q)
