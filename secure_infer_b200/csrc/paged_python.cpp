@@ -85,18 +85,18 @@ PyObject* failed(const char* name)
     return nullptr;
 }
 
-// Exceptions of the body become Python's.
+// Exceptions of the body become Python's, torch's own as they do elsewhere in torch.
 template <class Body>
 PyObject* guarded(Body body)
 {
+    HANDLE_TH_ERRORS
     try {
         return body();
     } catch (const Refused& r) {
         PyErr_SetString(PyExc_ValueError, r.why.c_str());
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
     }
-    return nullptr;
+    END_HANDLE_TH_ERRORS
 }
 
 bool counted(Py_ssize_t n, Py_ssize_t want)

@@ -1017,3 +1017,24 @@ def test_wide_tables(paged):
     table = torch.full((1, 1 << 22), -1, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="more work"):
         paged.attend(many.pages, paged.Chunk(table, many.chunk.cu_q, many.chunk.kv_lens), many.q)
+
+
+def test_memory_that_runs_out_is_torchs_error(paged):
+    """A caller that makes room and tries again catches torch.OutOfMemoryError."""
+    c = Case(paged, [(300, 300)], 64, 1)
+    k = torch.zeros((300, 1, 128), dtype=c.dtype, device="cuda")
+    want = paged.attend(c.pages, c.chunk, c.q)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction(torch.cuda.memory_reserved() / total)
+    try:
+        kept = []
+        with pytest.raises(torch.OutOfMemoryError):
+            for _ in range(1000):
+                kept.append(paged.attend(c.pages, c.chunk, c.q))
+        with pytest.raises(torch.OutOfMemoryError):
+            paged.append(c.pages, c.chunk, c.q, k, k)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.equal(paged.attend(c.pages, c.chunk, c.q), want)
