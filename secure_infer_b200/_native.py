@@ -185,6 +185,15 @@ def lib() -> ct.CDLL:
 _paged = None
 
 
+def paged_made_for() -> str:
+    """What ``paged_python.so`` depends on besides its sources: this Python and
+    this torch."""
+    import platform
+
+    import torch
+    return f"python {platform.python_version()}, torch {torch.__version__}"
+
+
 def paged_ops():
     """Load (once) and return the extension ``_build/paged_python.so``: the
     paged-cache calls (csrc/paged_python.cpp)."""
@@ -192,10 +201,13 @@ def paged_ops():
     if _paged is None:
         import importlib.util
 
-        import torch  # noqa: F401 -- its libraries are the extension's
         path = LIB_PATH.parent / "paged_python.so"
         if not path.exists():
             raise NativeLibraryMissing(f"{path} is missing; build it with `python -m secure_infer_b200.build`")
+        stamp, made_for = path.with_suffix(".torch"), paged_made_for()   # torch's libraries, loaded now, are the extension's
+        if stamp.exists() and stamp.read_text() != made_for:
+            raise NativeLibraryMissing(f"{path} was built for {stamp.read_text()}, this is {made_for}; build it again with "
+                                       "`python -m secure_infer_b200.build`")
         spec = importlib.util.spec_from_file_location("paged_python", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)

@@ -4,7 +4,9 @@ Every CUDA source is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``); host sources go through nvcc's
 host compiler.  The CUDA runtime is linked statically (nvcc's default), so the
 library works next to any torch build; OpenSSL libcrypto is linked for the
-host-side AES-GCM record path.
+host-side AES-GCM record path.  The extension behind secure_infer_b200.paged is
+built for the torch that is importable, again when that is another one, and left
+out where there is none: the C ABI needs no torch.
 
     python -m secure_infer_b200.build [--force]
 """
@@ -27,8 +29,8 @@ LIB = BUILD / "libsecure_infer.so"
 INTERPOSE = BUILD / "libsecure_infer_interpose.so"
 
 # Calls of secure_infer_b200.paged as a CPython extension (host code only); it
-# links libsecure_infer.so from its own directory and torch, which is loaded by
-# then.
+# links libsecure_infer.so from its own directory, whatever LD_LIBRARY_PATH says
+# (hence an RPATH), and torch, which is loaded by then.
 PAGED = BUILD / "paged_python.so"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -85,12 +87,19 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
-def build_paged(force: bool = False) -> Path:
-    src = CSRC / "paged_python.cpp"
-    if force or _stale(PAGED, [src, ROOT / "include" / "secure_infer_paged.h", LIB]):
+def build_paged(force: bool = False) -> Path | None:
+    """The extension, or None where torch cannot be imported."""
+    try:
+        import torch
+    except ImportError as e:
+        print(f"{PAGED.name}: not built, secure_infer_b200.paged will be missing ({e})", file=sys.stderr)
+        return None
+    from secure_infer_b200 import _native
+    src, stamp, made_for = CSRC / "paged_python.cpp", PAGED.with_suffix(".torch"), _native.paged_made_for()
+    if force or _stale(PAGED, [src, ROOT / "include" / "secure_infer_paged.h", LIB, Path(__file__)]) or \
+            not stamp.exists() or stamp.read_text() != made_for:
         import sysconfig
 
-        import torch
         torch_dir = Path(torch.__file__).resolve().parent
         cxx = os.environ.get("CXX", "g++")
         cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
@@ -98,9 +107,10 @@ def build_paged(force: bool = False) -> Path:
                f"-I{torch_dir / 'include'}", f"-I{torch_dir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
                f"-I{sysconfig.get_paths()['include']}", f"-I{Path(NVCC).resolve().parent.parent / 'include'}", str(src),
                "-o", str(PAGED), f"-L{BUILD}", "-lsecure_infer", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu",
-               "-lc10", "-Wl,-rpath,$ORIGIN", "-Wl,--exclude-libs,ALL"]
+               "-lc10", "-Wl,-rpath,$ORIGIN", "-Wl,--disable-new-dtags", "-Wl,--exclude-libs,ALL"]
         print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)
+        stamp.write_text(made_for)
     return PAGED
 
 
