@@ -74,9 +74,9 @@ __device__ __forceinline__ void join_row(int n, Stats stats, int sums, Values va
 // order of arrival.
 //
 // Measured: 47 sequences of up to 8192 tokens, 7 query heads on each of 4 KV
-// heads, 64 us, 5.6 TB/s; one sequence of 131072 tokens on one KV head 23 us,
+// heads, 65 us, 5.5 TB/s; one sequence of 131072 tokens on one KV head 23 us,
 // 2.9 TB/s (three levels of latency before the first page, two joins after the
-// last); one of 200 tokens on 8 KV heads 6.3 us.
+// last); one of 200 tokens on 8 KV heads 6.7 us.
 constexpr int kRowsWarps = 8;
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 constexpr int kRowsStages = 3;
@@ -529,8 +529,10 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 // exponentials and the rest what the warps of a quarter SM do together (loading
 // scores, agreeing on the maximum, handing weights over).  A piece takes 5 us to
 // its first scores and 2.5 to leave.  A chunk of 512 tokens after 6144, 32 query
-// heads on 8 KV heads: 62 us, 860 TFLOP/s; 4096 tokens in 20480: 1.18 to 1.22 ms,
-// 1.0 to 1.05 PFLOP/s, at an SM clock that the power limit holds at 1.4 GHz.
+// heads on 8 KV heads: 63 us with the pages in L2 (850 TFLOP/s), 70 without (768);
+// 4096 tokens in 20480: 1.13 to 1.22 ms, 1.0 to 1.09 PFLOP/s, which is the
+// products' part of the page loop (2048 of 3380 clocks) at the SM clock of 1.4 GHz
+// that such a call runs at.
 constexpr int kSoftWarps = 16;       // four warpgroups, each with a quarter of a page's keys
 constexpr int kTileThreads = 32 * (kSoftWarps + 4);   // and producer, products of two tiles, guard
 constexpr int kRing = 4;

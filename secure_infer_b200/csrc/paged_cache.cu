@@ -14,13 +14,15 @@ namespace {
 // 2^64 / 2 pi: (x, y) -> (x cos a - y sin a, y cos a + x sin a).  The product
 // pos f_i modulo 2^64 is the exact fraction of a turn, so the angle is as good
 // at position 10^6 as at 1, where a 32-bit product pos f would have lost it.
-// Bound by reading and writing each row once.  Eight lanes hold a row (eight
-// pairs each, 16-byte accesses), a warp four rows at a time, and computes its
-// lanes' eight angles once for all rows that it turns.  Measured: 8000 tokens of
-// 28 query and 4 KV heads 23 us, 4.9 TB/s (27 us before rows were loaded ahead of
-// the angles); 16 tokens of 32 and 8 heads 3.7 us.
+// It cannot do without reading and writing each row once.  Eight lanes hold a row
+// (eight pairs each, 16-byte accesses), a warp four rows at a time, and computes
+// its lanes' eight angles once for all rows that it turns.  Measured: 6237 tokens
+// of 28 query and 4 KV heads 23 us, 4.9 TB/s, where the copy rate would take 17.6
+// (27 us before rows were loaded ahead of the angles).  Memory is not what bounds
+// it: 1560 blocks are one and a half times what fits at 72 registers, and issue is
+// half busy.  16 tokens of 32 and 8 heads: 3.7 us.
 constexpr int kAppendThreads = 128;
-// Twelve rows of a warp on their way at once: 23.0 us for the 8000 tokens; with 16, 20, 24 or 36 rows 26.7, 24.6, 27.1
+// Twelve rows of a warp on their way at once: 23.0 us for the 6237 tokens; with 16, 20, 24 or 36 rows 26.7, 24.6, 27.1
 // and 27.0 (fewer warps for their registers), with twelve in 64 registers of a thread instead of 72 26.5.
 constexpr int kAppendBatch = 3;
 
@@ -175,7 +177,9 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_co
 // barriers.  Ranks come from prefix sums in page or request order, so pages
 // are given and moved in one order whatever the timing; the only atomics are
 // integer additions to the counts and a minimum over request numbers.  Measured:
-// 300 of 512 sequences freed in a table of 256 columns and 20000 pages 7.9 us.
+// 300 of 512 sequences freed in a table of 256 columns and 20000 pages 7.9 us, one
+// token reserved for each of 256 sequences (64 columns, 20000 pages) 7.7, of 1024
+// 11.4.
 constexpr int kMaxCluster = 8;
 constexpr int kTableThreads = 1024;
 // Entries up to which one CTA is faster than a cluster and its barriers.

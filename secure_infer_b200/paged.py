@@ -11,8 +11,9 @@ A layer's cache is K and V of ``[pages, 128, KV heads, 128]`` in bf16 or fp16,
 as ``NativeTransfer`` and ``LayerwiseReloader`` fill it.  Handles
 (``LayerPages``, ``CachePages``, ``Rotary``) are made once, a ``Chunk`` once per
 step for all its layers.  Calls run on the current stream and return without
-waiting; lengths, tables and page ids stay on the device.  Bad arguments raise
-``ValueError`` before anything is launched, a refused launch ``RuntimeError``.
+waiting; lengths, tables and page ids stay on the device (those given as lists are
+copied there first, which does wait).  Bad arguments raise ``ValueError`` before
+anything is launched, a refused launch ``RuntimeError``.  Outputs carry no gradient.
 As everywhere in this package there is no fallback: the work goes through
 ``libsecure_infer.so``, reached by a small extension (csrc/paged_python.cpp) that
 also looks the tensors over; ``copy`` alone goes by ctypes.
@@ -221,7 +222,8 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
     ``window`` of them; otherwise all of its sequence.  Returns ``[tokens,
     q heads, 128]``, and with ``return_lse`` the natural logarithms of the
     softmax sums, float32 ``[tokens, q heads]``, to join it with attention over
-    other keys.  A row that sees no key gives 0 and -inf.  ``workspace``:
+    other keys.  A row that sees no key gives 0 and -inf; rows of tokens past
+    the chunk's last are left as they were.  ``workspace``:
     ``attend_workspace(device)``, by default one that the current stream keeps
     for its calls, and while it is captured one of the graph's own."""
     if chunk.device != pages.device:
