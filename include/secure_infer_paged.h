@@ -66,7 +66,9 @@ typedef struct {
  * causal: the token at position p sees keys 0..p (else all of its sequence),
  * and with window > 0 only the last `window` of them.  A row that sees no key
  * gives zeros and -inf.  Keys that a row does not see take no part in it,
- * whatever they hold.  Rows of tokens that belong to nobody are not written.  workspace: secure_infer_paged_attend_workspace() bytes
+ * whatever they hold; an infinite value that it sees makes it infinite, or NaN
+ * where the key's weight rounds to zero.  Rows of tokens that belong to nobody are
+ * not written.  workspace: secure_infer_paged_attend_workspace() bytes
  * (41 MB on a device of 148 SMs; it is asked with that device current),
  * 256-byte aligned, zero before its first use, used by one stream at a time
  * (host threads that share the stream may share it too);
