@@ -95,6 +95,60 @@ int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infe
                               int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
                               float scale, uint32_t causal, uint32_t window, void* workspace, void* stream);
 
+/* The same with more of it.  sinks, with a window: the first `sinks` tokens of a
+ * sequence stay visible behind it, so the token at position p sees the keys j <= p
+ * with j > p - window or j < sinks; what lies between is not read, and its pages
+ * may be given back (secure_infer_trim).
+ *
+ * plan, from secure_infer_shared_prefix of this chunk: groups of sequences attend
+ * the pages that they have in common once for all of their rows, which gives what
+ * the call without it gives, up to the order of sums.  Not with a window.  parts:
+ * secure_infer_attend_parts() bytes, 16-byte aligned, for this call alone; may
+ * be null where there is no token.  options may be null. */
+typedef struct {
+    const int32_t* plan;
+    float* parts;
+    uint32_t groups;
+    uint32_t sinks;
+} secure_infer_attend_options;
+int secure_infer_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
+                        int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
+                        float scale, uint32_t causal, uint32_t window, const secure_infer_attend_options* options,
+                        void* workspace, void* stream);
+uint64_t secure_infer_attend_parts(uint32_t tokens, uint32_t q_heads);
+/* secure_infer_attend_fits of a call with a plan for so many groups. */
+int secure_infer_attend_fits_shared(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads,
+                                    uint32_t groups);
+
+/* What the sequences of a chunk have in common.  Group g is the sequences
+ * [cu_seqs[g], cu_seqs[g+1]), 1 <= groups <= seqs; cu_seqs may be null for one
+ * group of all.  Common are the pages from the first on that every sequence of the
+ * group with new tokens names in the same places, as far as all their tokens lie
+ * before the new ones of each.  plan: secure_infer_shared_prefix_ints() int32,
+ * 16-byte aligned: the common tokens of each sequence [seqs], then the kernels'
+ * own.  It goes with the chunk's contents when this runs: lengths and tables that
+ * change (other than by more tokens behind the common ones) need another. */
+uint64_t secure_infer_shared_prefix_ints(uint32_t seqs, uint32_t groups);
+int secure_infer_shared_prefix(const secure_infer_chunk* chunk, const int32_t* cu_seqs, uint32_t groups, int32_t* plan,
+                               void* stream);
+
+/* Attention over all keys from attention over n sets of them that have none in
+ * common, 1 <= n <= SECURE_INFER_JOIN_PARTS: lse = log sum e^lse_i and out = sum
+ * e^(lse_i - lse) out_i.  A part with lse_i = -inf counts for nothing, whatever
+ * its out_i holds; where all are, out is 0 and lse -inf.  A part's out:
+ * [tokens][heads][128] of `dtype` with its strides (token, head) in elements,
+ * multiples of 16 bytes; its lse: [tokens][heads] with strides.  out, lse: dense;
+ * out may be one part's own where that is dense. */
+#define SECURE_INFER_JOIN_PARTS 8u
+typedef struct {
+    const void* out;
+    const float* lse;
+    int64_t out_stride[2];
+    int64_t lse_stride[2];
+} secure_infer_attend_part;
+int secure_infer_attend_join(const secure_infer_attend_part* parts, uint32_t n, uint32_t tokens, uint32_t heads,
+                             uint32_t dtype, void* out, float* lse, void* stream);
+
 /* Rotary positions and the chunk's way into its pages.  q (may be null), k and
  * v: [tokens][heads][128] with their strides (token, head).  Pair i of a head
  * (elements i and i + 64, or 2i and 2i + 1 where `interleaved`) turns by
@@ -111,7 +165,7 @@ int secure_infer_paged_append(const secure_infer_pages* pages, const secure_infe
 
 /* Tables of a cache: block_table [seqs][width], tokens held per sequence, and
  * how many rows hold each page (0: free).  A sequence of n tokens holds
- * ceil(n / 128) pages. */
+ * ceil(n / 128) pages, less those that secure_infer_trim took (-1). */
 typedef struct {
     int32_t* block_table;
     int32_t* lens;
@@ -159,6 +213,13 @@ int secure_infer_paged_reserve(const secure_infer_tables* in, const secure_infer
 /* free: the sequences give up their pages and become empty. */
 int secure_infer_paged_free(const secure_infer_tables* in, const secure_infer_tables* out, const int32_t* seqs,
                             uint32_t n, void* scratch, void* stream);
+
+/* trim: the sequences give up the pages that no later token sees when it is
+ * attended with this window and these sinks: those behind the first `sinks`
+ * tokens that lie wholly before the window of the token at position lens.
+ * window >= 1.  Their entries become -1, lengths stay. */
+int secure_infer_trim(const secure_infer_tables* in, const secure_infer_tables* out, const int32_t* seqs, uint32_t n,
+                      uint32_t window, uint32_t sinks, void* scratch, void* stream);
 
 /* compact: with `live` pages in use, the i-th used page at or above `live`
  * moves to the i-th free page below it.  moved[p]: where page p is now, -1 for

@@ -126,6 +126,16 @@ class PageTensor(ct.Structure):
     _fields_ = [("base", P), ("page_stride", ct.c_int64)]
 
 
+class AttendOptions(ct.Structure):
+    """secure_infer_attend_options (include/secure_infer_paged.h)."""
+    _fields_ = [("plan", P), ("parts", P), ("groups", U32), ("sinks", U32)]
+
+
+class AttendPart(ct.Structure):
+    """secure_infer_attend_part (include/secure_infer_paged.h)."""
+    _fields_ = [("out", P), ("lse", P), ("out_stride", ct.c_int64 * 2), ("lse_stride", ct.c_int64 * 2)]
+
+
 # Operators on the paged cache.  Structures go by reference.
 PAGED_SIGNATURES = {
     "secure_infer_paged_attend_workspace": ([], U64),
@@ -142,6 +152,13 @@ HOST_SIGNATURES.update(PAGED_SIGNATURES)
 HOST_SIGNATURES["secure_infer_capture_id"] = ([P], U64)
 HOST_SIGNATURES["secure_infer_attend_fits"] = ([P, P, U32], I32)
 HOST_SIGNATURES["secure_infer_attend_status"] = ([P, P, P], I32)
+HOST_SIGNATURES["secure_infer_attend"] = ([P, P, P, I64, I64, U32, P, P, ct.c_float, U32, U32, P, P, P], I32)
+HOST_SIGNATURES["secure_infer_attend_parts"] = ([U32, U32], U64)
+HOST_SIGNATURES["secure_infer_attend_fits_shared"] = ([P, P, U32, U32], I32)
+HOST_SIGNATURES["secure_infer_attend_join"] = ([P, U32, U32, U32, U32, P, P, P], I32)
+HOST_SIGNATURES["secure_infer_shared_prefix_ints"] = ([U32, U32], U64)
+HOST_SIGNATURES["secure_infer_shared_prefix"] = ([P, P, U32, P, P], I32)
+HOST_SIGNATURES["secure_infer_trim"] = ([P, P, P, U32, U32, U32, P, P], I32)
 
 # SECURE_INFER_KIND_KV: a reload of 2n records, K packets first, V packets after.
 KIND_KV = 2

@@ -37,8 +37,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden,-O3",
           f"-I{CSRC}", f"-I{ROOT / 'include'}"]
-SOURCES = ["gcm_kernels.cu", "plugin_abi.cpp", "host_runtime.cpp", "paged_attention.cu", "paged_cache.cu",
-           "paged_abi.cpp"]
+SOURCES = ["gcm_kernels.cu", "plugin_abi.cpp", "host_runtime.cpp", "paged_attention.cu", "paged_join.cu",
+           "paged_cache.cu", "paged_abi.cpp"]
 HEADERS = ["gcm_device.cuh", "gcm_kernels.cuh", "host_runtime.h", "bitsliced_aes.cuh", "bitsliced_sbox.cuh",
            "paged.cuh"]
 

@@ -21,7 +21,23 @@ constexpr int kDim = 128;    // values of a head
 // What a CTA's last unit of a cut tile leaves for the join.
 struct Cut {
     int32_t cta1, cta0, rows, token0, head;   // the last CTA and the first; cta1 = 0: no such tile
-    int32_t n, kv, q0;
+    int32_t n, kv, q0, part;
+};
+
+// What rows see.  The kernels are made for each, so that the usual call does not
+// pay for the others.
+enum Mode : int {
+    kPlain,    // the causal order with or without a window, or every key
+    kSinks,    // behind a window the first tokens as well
+    kShared    // groups of sequences whose first pages are the same: these are attended once for all of a group's rows
+};
+
+// A group of sequences with a common prefix, as secure_infer_shared_prefix
+// leaves it behind the sequences' own prefixes.
+struct Group {
+    int32_t lead;      // the sequence whose block table is read
+    int32_t q0, n;     // the group's new tokens
+    int32_t tokens;    // keys in common, whole pages; 0: none
 };
 
 struct AttendParams {
@@ -47,16 +63,44 @@ struct AttendParams {
     float* slots;                   // [2 * grid] partial results of tiles
     float* row_slots;               // and of the kernel for few rows
     int32_t both;                   // the call has a launch for few rows, and then one for the others, on the same SMs
+    int32_t sinks;                  // kSinks: the first tokens that stay visible
+    const int32_t* prefix;          // kShared: [seqs] keys in common with the sequence's group
+    const Group* shared;            // [groups]
+    int32_t groups;
+    float* parts;                   // [2][rows of the output][128] sums over the group's and over a sequence's own keys, then
+                                    // [2][rows] maxima and sums of weights
 };
 
 // Launchers (cudaError_t values).
-int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, uint32_t dtype,
-                       cudaStream_t stream);
+int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, Mode mode,
+                       uint32_t dtype, cudaStream_t stream);
 // q_map: boxes of [128 / group tokens][group heads][64 values].
 int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
-                        const AttendParams& p, uint32_t dtype, cudaStream_t stream);
+                        const AttendParams& p, Mode mode, uint32_t dtype, cudaStream_t stream);
 uint64_t attend_workspace_bytes();
 void attend_workspace(void* workspace, AttendParams* p);   // its counters, status word and slots
+
+struct PrefixParams {
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* cu;
+    const int32_t* kv;
+    const int32_t* groups;          // where each begins among the sequences, and the last one's end; null: one of all
+    int32_t width, seqs;
+    int32_t* prefix;
+    Group* shared;
+};
+int launch_shared_prefix(const PrefixParams& p, uint32_t groups, cudaStream_t stream);
+// kShared: makes p.parts into results, after the kernels that leave them.
+int launch_attend_parts(const AttendParams& p, uint32_t dtype, cudaStream_t stream);
+
+struct JoinParams {
+    secure_infer_attend_part part[SECURE_INFER_JOIN_PARTS];
+    int32_t n, tokens, heads;
+    void* out;
+    float* lse;
+};
+int launch_join(const JoinParams& p, uint32_t dtype, cudaStream_t stream);
 
 struct AppendParams {
     const void* q;
@@ -91,16 +135,17 @@ struct CopyParams {
 int launch_page_copy(const secure_infer_page_tensor* tensors, uint32_t n_tensors, uint64_t page_bytes, uint32_t pages,
                      const int32_t* src, const int32_t* dst, const int32_t* count, uint32_t n, cudaStream_t stream);
 
-enum TableOp : int32_t { kFork, kReserve, kFree, kCompact };
+enum TableOp : int32_t { kFork, kReserve, kFree, kCompact, kTrim };
 struct TableParams {
     secure_infer_tables in, out;
-    const int32_t* a;               // fork: parents; reserve, free: sequences
+    const int32_t* a;               // fork: parents; reserve, free, trim: sequences
     const int32_t* b;               // fork: children; reserve: new lengths
     int32_t* granted;
     int32_t* moved;
     int32_t* live;
     int32_t* scratch;
     int32_t n;
+    int32_t window, sinks;          // trim
 };
 int launch_tables(TableOp op, const TableParams& p, cudaStream_t stream);
 uint64_t table_scratch_ints(uint32_t seqs, uint32_t pages, uint32_t n);
@@ -248,6 +293,22 @@ __device__ __forceinline__ bool zero_sum_odd(uint32_t sum)
     return x.x != x.x || x.y != x.y;
 }
 
+// The sequence of a token, by a warp: the last s with cu[s] <= token, 32 probes at
+// a time.
+__device__ __forceinline__ int find_seq(const int32_t* cu, int seqs, int token)
+{
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = seqs;   // cu[lo] <= token, and the answer lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const uint32_t below = __ballot_sync(0xffffffffu, at < hi && cu[at] <= token);
+        const int k = below == 0 ? 0 : 31 - __clz(below);
+        lo += k * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
 // ------------------------------------------------- attention's work, in order
 //
 // A sequence's rows are (new token, query head of the group), flattened, so one
@@ -259,14 +320,42 @@ __device__ __forceinline__ bool zero_sum_odd(uint32_t sum)
 // What a tile takes besides its pages (its queries, its end) counts as `cost`
 // units more, before its pages.  Units are counted in 32 bits; the host refuses
 // more.
+//
+// Where groups share a prefix, their common keys are sequences of their own
+// behind the call's: all new tokens of the group over the prefix, which every
+// one of them sees.  What a sequence's rows see besides begins after it.
 struct Seq {
     int n, kv, q0;   // new tokens, all tokens, first new token
+    // kShared: its first key, which part of its rows this is (0: over a group's keys, 1: over its own, -1: whole), and
+    // its row of the block table.
+    int begin, part, row;
 };
 
+template <int M>
+__device__ __forceinline__ int seq_count(const AttendParams& p)
+{
+    return M == kShared ? p.seqs + p.groups : p.seqs;
+}
+
 // `others`: the sequences of the call's other launch, else of this one.
+template <int M>
 __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool others = false)
 {
     Seq r;
+    r.begin = 0;
+    r.part = -1;
+    r.row = s;
+    if (M == kShared && s >= p.seqs) {
+        const int4 g = __ldcg(reinterpret_cast<const int4*>(p.shared) + (s - p.seqs));
+        r.row = max(0, min(g.x, p.seqs - 1));
+        r.q0 = max(0, min(g.y, p.tokens));
+        r.kv = max(0, min(g.w, p.width * kPage));
+        r.n = r.kv > 0 ? max(0, min(g.z, p.tokens - r.q0)) : 0;
+        r.part = 0;
+        const int64_t rows = static_cast<int64_t>(r.n) * p.group;
+        if ((rows < p.rows_min || rows > p.rows_max) != others) r.n = 0;
+        return r;
+    }
     // From L2, as all that may be read before this kernel has waited for the one before it.
     int a = __ldcg(p.cu + s), b = __ldcg(p.cu + s + 1);
     a = max(0, min(a, p.tokens));
@@ -274,6 +363,10 @@ __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool other
     r.q0 = a;
     r.n = b - a;
     r.kv = max(0, min(__ldcg(p.kv + s), p.width * kPage));
+    if (M == kShared) {
+        r.begin = max(0, min(__ldcg(p.prefix + s), r.kv));
+        r.part = r.begin > 0 ? 1 : -1;
+    }
     const int64_t rows = static_cast<int64_t>(r.n) * p.group;
     if ((rows < p.rows_min || rows > p.rows_max) != others) r.n = 0;
     return r;
@@ -281,20 +374,43 @@ __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool other
 
 struct Span {
     int first, pages;   // page range of a tile
-    int lo, hi;         // keys that any row of it sees: [lo, hi)
+    int lo, hi;         // keys that any row of it sees: [lo, hi), and with sinks min(sinks, hi) before them
+    int jump, skip;     // kSinks: from the tile's page `jump` on, `skip` pages behind the sinks are left out
+
+    // Number in its sequence of the tile's page i.
+    template <int M>
+    __device__ __forceinline__ int page(int i) const
+    {
+        return first + i + (M == kSinks && i >= jump ? skip : 0);
+    }
 };
 
+template <int M>
+__device__ __forceinline__ bool in_order(const AttendParams& p, const Seq& s)
+{
+    return p.causal && !(M == kShared && s.part == 0);
+}
+
+template <int M>
 __device__ __forceinline__ Span tile_span(const AttendParams& p, const Seq& s, int first_token, int last_token)
 {
     Span r;
-    r.hi = p.causal ? min(s.kv, s.kv - s.n + last_token + 1) : s.kv;
-    r.lo = p.window ? max(0, s.kv - s.n + first_token - p.window + 1) : 0;
+    r.hi = in_order<M>(p, s) ? min(s.kv, s.kv - s.n + last_token + 1) : s.kv;
+    if (M == kShared) r.lo = s.begin;
+    else r.lo = p.window ? max(0, s.kv - s.n + first_token - p.window + 1) : 0;
+    r.jump = r.skip = 0;
     if (r.hi <= r.lo) {
         r.lo = r.hi = r.first = 0;
         r.pages = 1;
     } else {
         r.first = r.lo / kPage;
         r.pages = (r.hi + kPage - 1) / kPage - r.first;
+        if (M == kSinks) {
+            r.jump = min((min(p.sinks, r.hi) + kPage - 1) / kPage, r.first);
+            r.skip = r.first - r.jump;
+            r.pages += r.jump;
+            r.first = 0;
+        }
     }
     return r;
 }
@@ -316,6 +432,7 @@ struct Share {
     }
 };
 
+template <int M>
 struct Walk {
     int rows_per_tile, cost;
     int s, tile, tiles, head;
@@ -333,8 +450,10 @@ struct Walk {
         rows = min(rows_per_tile, q.n * p.group - r0);
         first_token = r0 / p.group;
         last_token = (r0 + rows - 1) / p.group;
-        span = tile_span(p, q, first_token, last_token);
+        span = tile_span<M>(p, q, first_token, last_token);
     }
+    // Its row of the block table.
+    __device__ __forceinline__ int row() const { return M == kShared ? q.row : s; }
     // After `taken` units: the next head, tile or sequence.
     __device__ __forceinline__ void advance(const AttendParams& p, int taken)
     {
@@ -351,11 +470,11 @@ struct Walk {
         }
         tile = 0;
         do {
-            if (++s >= p.seqs) {   // only if lengths changed under the kernel
+            if (++s >= seq_count<M>(p)) {   // only if lengths changed under the kernel
                 left = 0;
                 return;
             }
-            q = load_seq(p, s);
+            q = load_seq<M>(p, s);
         } while (q.n == 0);
         tiles = (q.n * p.group + rows_per_tile - 1) / rows_per_tile;
         set_tile(p);
@@ -363,10 +482,11 @@ struct Walk {
 };
 
 // Pages and cost of a tile.
+template <int M>
 __device__ __forceinline__ int tile_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost, int tile)
 {
     const int r = tile * rows_per_tile;
-    return tile_span(p, s, r / p.group, (min(r + rows_per_tile, s.n * p.group) - 1) / p.group).pages + cost;
+    return tile_span<M>(p, s, r / p.group, (min(r + rows_per_tile, s.n * p.group) - 1) / p.group).pages + cost;
 }
 
 // Up to so many tiles of a sequence are counted by one thread, more by a warp:
@@ -374,6 +494,7 @@ __device__ __forceinline__ int tile_units(const AttendParams& p, const Seq& s, i
 constexpr int kOwnTiles = 4;
 
 // Units of every lane's sequence; `largest`: of a tile of theirs.  All lanes call it.
+template <int M>
 __device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, int rows_per_tile, int cost, int& largest)
 {
     const int lane = threadIdx.x & 31;
@@ -381,17 +502,21 @@ __device__ __forceinline__ int seq_units(const AttendParams& p, const Seq& s, in
     int units = 0;
     if (tiles <= kOwnTiles) {
         for (int t = 0; t < tiles; ++t) {
-            const int u = tile_units(p, s, rows_per_tile, cost, t);
+            const int u = tile_units<M>(p, s, rows_per_tile, cost, t);
             units += u;
             largest = max(largest, u);
         }
     }
     for (uint32_t many = __ballot_sync(0xffffffffu, tiles > kOwnTiles); many != 0; many &= many - 1) {
         const int from = __ffs(many) - 1, n = __shfl_sync(0xffffffffu, tiles, from);
-        const Seq q{__shfl_sync(0xffffffffu, s.n, from), __shfl_sync(0xffffffffu, s.kv, from), 0};
+        Seq q{__shfl_sync(0xffffffffu, s.n, from), __shfl_sync(0xffffffffu, s.kv, from), 0, 0, -1, 0};
+        if (M == kShared) {
+            q.begin = __shfl_sync(0xffffffffu, s.begin, from);
+            q.part = __shfl_sync(0xffffffffu, s.part, from);
+        }
         int sum = 0, most = 0;
         for (int t = lane; t < n; t += 32) {
-            const int u = tile_units(p, q, rows_per_tile, cost, t);
+            const int u = tile_units<M>(p, q, rows_per_tile, cost, t);
             sum += u;
             most = max(most, u);
         }
@@ -417,32 +542,32 @@ struct Kind {
 // launch, so reading pages for few rows goes on beside the products of many: 333
 // tokens after 2167 and 15 single tokens of up to 4000 take 53 us, 62 one kind
 // after the other.
-template <int kThreads>
+template <int kThreads, int M>
 __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& kind, const Kind& other, Share* share,
                                            int32_t* warp_sums)
 {
     const int rows_per_tile = kind.rows_per_tile, cost = kind.cost, whole = kind.whole;
     constexpr int kWarps = kThreads / 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seqs = seq_count<M>(p);
     const int down = tid == 0 ? static_cast<int>(__ldcg(p.status)) : 0;
     Share r;
     r.begin = r.total = 0;
     // The first pass sums the units, the second finds the sequence that holds this CTA's first; where every sequence
     // has a thread one pass does both.
-    const bool one = p.seqs <= kThreads;
+    const bool one = seqs <= kThreads;
     for (int pass = one ? 1 : 0; pass < 2; ++pass) {
         int base = 0, largest = 0, others = 0;
-        for (int s0 = 0; s0 < p.seqs; s0 += kThreads) {
+        for (int s0 = 0; s0 < seqs; s0 += kThreads) {
             const int s = s0 + tid;
             Seq q{};
             int own_largest = 0, unused = 0, beside = 0;
-            if (s < p.seqs) q = load_seq(p, s);
+            if (s < seqs) q = load_seq<M>(p, s);
             if (p.both && (one || pass == 0)) {
                 Seq o{};
-                if (s < p.seqs) o = load_seq(p, s, true);
-                beside = __reduce_add_sync(0xffffffffu, seq_units(p, o, other.rows_per_tile, other.cost, unused));
+                if (s < seqs) o = load_seq<M>(p, s, true);
+                beside = __reduce_add_sync(0xffffffffu, seq_units<M>(p, o, other.rows_per_tile, other.cost, unused));
             }
-            const int own = seq_units(p, q, rows_per_tile, cost, own_largest);
+            const int own = seq_units<M>(p, q, rows_per_tile, cost, own_largest);
             int sum = own;
             for (int d = 1; d < 32; d <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, sum, d);
@@ -464,7 +589,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
                 largest = max(largest, warp_sums[kWarps + w]);
                 others += warp_sums[2 * kWarps + w];
             }
-            if (one || (pass == 0 && s0 + kThreads >= p.seqs)) {
+            if (one || (pass == 0 && s0 + kThreads >= seqs)) {
                 r.total = base;
                 int grid = gridDim.x;
                 if (base > 0 && others > 0 && grid > 1) {
@@ -500,9 +625,10 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
 }
 
 // All lanes of a warp call it.
-__device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_tile, int cost, const Share& share)
+template <int M>
+__device__ __forceinline__ Walk<M> start_walk(const AttendParams& p, int rows_per_tile, int cost, const Share& share)
 {
-    Walk w;
+    Walk<M> w;
     w.rows_per_tile = rows_per_tile;
     w.cost = cost;
     w.left = 0;
@@ -517,7 +643,7 @@ __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_t
     // Of a sequence of many tiles, 32 at a time.
     for (bool past = w.tiles > kOwnTiles; past;) {
         const int lane = threadIdx.x & 31, t = w.tile + lane;
-        int upto = t < w.tiles ? tile_units(p, w.q, rows_per_tile, cost, t) * p.heads : 0;
+        int upto = t < w.tiles ? tile_units<M>(p, w.q, rows_per_tile, cost, t) * p.heads : 0;
         for (int d = 1; d < 32; d <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += up;
@@ -548,22 +674,49 @@ __device__ __forceinline__ Walk start_walk(const AttendParams& p, int rows_per_t
     return w;
 }
 
-// Keys that row r of the tile sees: [lo, hi].
+// Keys that row r of the tile sees: [lo, hi], and with sinks those before
+// min(sinks, hi + 1).
+template <int M>
 __device__ __forceinline__ void row_keys(const AttendParams& p, const Seq& s, int token, int& lo, int& hi)
 {
-    hi = p.causal ? min(s.kv, s.kv - s.n + token + 1) - 1 : s.kv - 1;
-    lo = p.window ? max(0, s.kv - s.n + token - p.window + 1) : 0;
+    hi = in_order<M>(p, s) ? min(s.kv, s.kv - s.n + token + 1) - 1 : s.kv - 1;
+    if (M == kShared) lo = s.begin;
+    else lo = p.window ? max(0, s.kv - s.n + token - p.window + 1) : 0;
 }
 
-// One row over keys [a, b) by one warp, straight from the pages: lane l holds
+// Keys that a row sees on `pages` of its tile's pages from page `from` on: [a, b),
+// and with sinks [sa, sb) before them.
+struct PieceKeys {
+    int sa, sb, a, b;
+};
+template <int M>
+__device__ __forceinline__ PieceKeys piece_keys(const AttendParams& p, const Span& span, int from, int pages, int lo, int hi)
+{
+    PieceKeys k{0, 0, 0, 0};
+    if (M != kSinks) {
+        const int first = span.page<M>(from) * kPage;
+        k.a = max(lo, first);
+        k.b = min(hi + 1, first + pages * kPage);
+        return k;
+    }
+    // With pages left out the piece is what lies before them and what lies behind.
+    const int end = from + pages;
+    k.sa = from * kPage;
+    k.sb = min(min(min(p.sinks, lo), hi + 1), (span.skip > 0 ? min(end, span.jump) : end) * kPage);
+    k.a = max(lo, (span.skip > 0 ? max(from, span.jump) + span.skip : from) * kPage);
+    k.b = min(hi + 1, (end + span.skip) * kPage);
+    return k;
+}
+
+// One row over the keys `in` by one warp, straight from the pages: lane l holds
 // values 4l .. 4l+3.  Only rows of a tile in which some row must not see an
 // infinite or NaN value that another one does see come here: in a matrix
 // product zero times such a value would be NaN.  A key takes about 430
 // clocks, the rows of a long piece longer than the other warps' waits last, so
 // it counts its way in *work.
-template <typename T>
-__device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q, const int32_t* table, int head, int a,
-                                               int b, float& m, float& l, float4& o, volatile int* work)
+template <typename T, int M>
+__device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q, const int32_t* table, int head,
+                                               PieceKeys in, float& m, float& l, float4& o, volatile int* work)
 {
     const int d = 4 * (threadIdx.x & 31);
     const uint2 qx = __ldcg(reinterpret_cast<const uint2*>(q + d));
@@ -571,8 +724,10 @@ __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q
     m = -INFINITY;
     l = 0.0f;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int j = a; j < b; ++j) {
-        if (((j - a) & 1023) == 0 && d == 0) atomicAdd(const_cast<int*>(work), 1);
+    const int sinks = M == kSinks ? max(0, in.sb - in.sa) : 0, keys = sinks + max(0, in.b - in.a);
+    for (int i = 0; i < keys; ++i) {
+        if ((i & 1023) == 0 && d == 0) atomicAdd(const_cast<int*>(work), 1);
+        const int j = i < sinks ? in.sa + i : in.a + i - sinks;
         const int page = __ldcg(table + j / kPage);
         float2 k0 = {0, 0}, k1 = {0, 0}, v0 = {0, 0}, v1 = {0, 0};
         if (page >= 0 && page < p.pages) {
@@ -594,6 +749,26 @@ __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q
         o.z = o.z * f + e * v1.x;
         o.w = o.w * f + e * v1.y;
     }
+}
+
+// One row's result, by a warp: values 4 lane .. 4 lane + 3 of the sum x, the
+// maximum and the sum of weights; `none`: it sees no key.  Where a group's common
+// keys are attended elsewhere it goes to the parts, as it is.
+template <typename T, int M>
+__device__ __forceinline__ void put_row(const AttendParams& p, int part, int64_t at, float4 x, float top, float sum, bool none)
+{
+    const int lane = threadIdx.x & 31;
+    if (M == kShared && part >= 0) {
+        const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads * p.group, to = part * rows + at;
+        *reinterpret_cast<float4*>(p.parts + to * kDim + lane * 4) = x;
+        if (lane == 0) *reinterpret_cast<float2*>(p.parts + 2 * rows * kDim + 2 * to) = make_float2(top, sum);
+        return;
+    }
+    const float inv = 1.0f / sum;
+    uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+    if (none) packed = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
+    if (p.lse != nullptr && lane == 0) p.lse[at] = none ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Weight of a partial result with maximum m in a whole with maximum top.

@@ -105,22 +105,24 @@ struct Work {
     bool fits() const { return rows_units <= INT_MAX && tiles_units <= INT_MAX; }
 };
 
-Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, uint32_t q_heads)
+// `groups` of sequences share a prefix: all their rows make tiles of it.
+Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, uint32_t q_heads, uint32_t groups = 0)
 {
     Work w{q_heads / pages.heads, false, 0, 0};
     const uint32_t max_q = chunk.max_q == 0 || chunk.max_q > chunk.tokens ? chunk.tokens : chunk.max_q;
     const uint64_t max_rows = static_cast<uint64_t>(max_q) * w.group, rows = static_cast<uint64_t>(chunk.tokens) * w.group;
     // Up to kFewRows rows per KV head a sequence is bound by reading K and V once, which the kernel for few rows does
     // with less latency; more rows are worth tiles of 128.
-    w.tiles = max_rows > kFewRows && w.group <= 128;
+    w.tiles = (groups > 0 ? rows : max_rows) > kFewRows && w.group <= 128;
     const auto units = [&](uint64_t tiles, uint64_t cost) -> uint64_t {
         return tiles * pages.heads > INT_MAX ? UINT64_MAX : tiles * pages.heads * (chunk.table_width + cost);
     };
-    if (max_rows > INT_MAX) w.rows_units = UINT64_MAX;
-    else if (!w.tiles) w.rows_units = units(rows / 8 + chunk.seqs, 1);
+    const uint64_t seqs = uint64_t(chunk.seqs) + groups, all = groups > 0 ? 2 * rows : rows;
+    if (max_rows > INT_MAX || (groups > 0 && rows > INT_MAX)) w.rows_units = UINT64_MAX;
+    else if (!w.tiles) w.rows_units = units(all / 8 + seqs, 1);
     else {
-        w.rows_units = chunk.seqs > 1 ? units(uint64_t(chunk.seqs) * (kFewRows / 8), 1) : 0;
-        w.tiles_units = units(rows / (2 * (128 / w.group * w.group)) + chunk.seqs, 2);
+        w.rows_units = seqs > 1 ? units(seqs * (kFewRows / 8), 1) : 0;
+        w.tiles_units = units(all / (2 * (128 / w.group * w.group)) + seqs, 2);
     }
     return w;
 }
@@ -176,8 +178,63 @@ SI_EXPORT int secure_infer_attend_status(void* workspace, uint32_t* status, void
 
 SI_EXPORT int secure_infer_attend_fits(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads)
 {
+    return secure_infer_attend_fits_shared(pages, chunk, q_heads, 0);
+}
+
+SI_EXPORT int secure_infer_attend_fits_shared(const secure_infer_pages* pages, const secure_infer_chunk* chunk,
+                                              uint32_t q_heads, uint32_t groups)
+{
     return pages_ok(pages) && chunk_ok(chunk) && q_heads > 0 && q_heads <= (1u << 16) && q_heads % pages->heads == 0 &&
-           work_of(*pages, *chunk, q_heads).fits();
+           groups <= chunk->seqs && work_of(*pages, *chunk, q_heads, groups).fits();
+}
+
+SI_EXPORT uint64_t secure_infer_attend_parts(uint32_t tokens, uint32_t q_heads)
+{
+    return static_cast<uint64_t>(tokens) * q_heads * 2 * (kDim + 2) * sizeof(float);
+}
+
+// The sequences' prefixes, then the groups, which are read 16 bytes at a time.
+static uint64_t group_offset(uint32_t seqs) { return (static_cast<uint64_t>(seqs) + 3) / 4 * 4; }
+
+SI_EXPORT uint64_t secure_infer_shared_prefix_ints(uint32_t seqs, uint32_t groups)
+{
+    return group_offset(seqs) + static_cast<uint64_t>(groups) * (sizeof(Group) / sizeof(int32_t));
+}
+
+SI_EXPORT int secure_infer_shared_prefix(const secure_infer_chunk* chunk, const int32_t* cu_seqs, uint32_t groups,
+                                         int32_t* plan, void* stream)
+{
+    if (!chunk_ok(chunk) || groups == 0 || groups > chunk->seqs || (cu_seqs == nullptr && groups != 1) || !aligned16(plan))
+        return -1;
+    const PrefixParams p{chunk->block_table, chunk->table_stride, chunk->cu_q, chunk->kv_lens, cu_seqs,
+                         static_cast<int32_t>(chunk->table_width), static_cast<int32_t>(chunk->seqs), plan,
+                         reinterpret_cast<Group*>(plan + group_offset(chunk->seqs))};
+    return launch_shared_prefix(p, groups, static_cast<cudaStream_t>(stream)) == 0 ? 0 : -1;
+}
+
+SI_EXPORT int secure_infer_attend_join(const secure_infer_attend_part* parts, uint32_t n, uint32_t tokens, uint32_t heads,
+                                       uint32_t dtype, void* out, float* lse, void* stream)
+{
+    if (parts == nullptr || n == 0 || n > SECURE_INFER_JOIN_PARTS || tokens > (1u << 28) || heads == 0 ||
+        heads > (1u << 16) || dtype > SECURE_INFER_FP16)
+        return -1;
+    if (tokens == 0) return 0;
+    if (!aligned16(out) || lse == nullptr || static_cast<uint64_t>(tokens) * heads > (uint64_t(1) << 34)) return -1;
+    JoinParams p;
+    std::memset(&p, 0, sizeof(p));
+    for (uint32_t i = 0; i < n; ++i) {
+        const secure_infer_attend_part& a = parts[i];
+        if (!aligned16(a.out) || a.lse == nullptr || !stride_ok(a.out_stride[0]) || !stride_ok(a.out_stride[1]) ||
+            a.lse_stride[0] < 0 || a.lse_stride[1] < 0)
+            return -1;
+        p.part[i] = a;
+    }
+    p.n = static_cast<int32_t>(n);
+    p.tokens = static_cast<int32_t>(tokens);
+    p.heads = static_cast<int32_t>(heads);
+    p.out = out;
+    p.lse = lse;
+    return launch_join(p, dtype, static_cast<cudaStream_t>(stream)) == 0 ? 0 : -1;
 }
 
 SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
@@ -185,13 +242,29 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
                                         float* lse, float scale, uint32_t causal, uint32_t window, void* workspace,
                                         void* stream)
 {
+    return secure_infer_attend(pages, chunk, q, q_token_stride, q_head_stride, q_heads, out, lse, scale, causal, window,
+                               nullptr, workspace, stream);
+}
+
+SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
+                                  int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
+                                  float scale, uint32_t causal, uint32_t window,
+                                  const secure_infer_attend_options* options, void* workspace, void* stream)
+{
+    const uint32_t sinks = options != nullptr ? options->sinks : 0;
+    const uint32_t groups = options != nullptr && options->plan != nullptr ? options->groups : 0;
     if (!pages_ok(pages) || !chunk_ok(chunk) || q_heads == 0 || q_heads > (1u << 16) ||
         q_heads % pages->heads != 0 || (window != 0 && !causal) || window > INT_MAX || workspace == nullptr ||
-        (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+        (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || sinks > INT_MAX || (sinks != 0 && window == 0))
+        return -1;
+    if (options != nullptr && options->plan != nullptr &&
+        (!aligned16(options->plan) || groups == 0 || groups > chunk->seqs || window != 0))
         return -1;
     if (chunk->tokens == 0) return 0;
-    if (!aligned16(q) || !aligned16(out) || !stride_ok(q_token_stride) || !stride_ok(q_head_stride)) return -1;
-    const Work work = work_of(*pages, *chunk, q_heads);
+    if (!aligned16(q) || !aligned16(out) || !stride_ok(q_token_stride) || !stride_ok(q_head_stride) ||
+        (groups > 0 && !aligned16(options->parts)))
+        return -1;
+    const Work work = work_of(*pages, *chunk, q_heads, groups);
     if (!work.fits()) return -1;
     const uint32_t group = work.group;
 
@@ -222,7 +295,17 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     p.rows_max = INT_MAX;
     p.causal = causal != 0;
     // As many tokens as a table can hold hide nothing, and positions less such a window might pass 32 bits.
-    p.window = window >= static_cast<uint64_t>(chunk->table_width) * kPage ? 0 : static_cast<int32_t>(window);
+    const uint64_t most = static_cast<uint64_t>(chunk->table_width) * kPage;
+    p.window = window >= most || sinks >= most ? 0 : static_cast<int32_t>(window);
+    p.sinks = p.window != 0 ? static_cast<int32_t>(sinks) : 0;
+    Mode mode = p.sinks > 0 ? kSinks : kPlain;
+    if (groups > 0) {
+        mode = kShared;
+        p.prefix = options->plan;
+        p.shared = reinterpret_cast<const Group*>(options->plan + group_offset(chunk->seqs));
+        p.groups = static_cast<int32_t>(groups);
+        p.parts = options->parts;
+    }
     p.scale_log2 = scale * 1.4426950408889634f;
     // Hidden scores are -inf before they are scaled, so the scale is never zero; at 1e-30 all weights are 1.
     if (p.scale_log2 > -1e-30f && p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
@@ -233,20 +316,21 @@ SI_EXPORT int secure_infer_paged_attend(const secure_infer_pages* pages, const s
     const std::lock_guard<std::mutex> lock(launches);
     const bool tiles = work.tiles;
     CUtensorMap q_map, k_map, v_map;
-    if (!tiles || chunk->seqs > 1) {
+    if (!tiles || chunk->seqs > 1) {   // (groups go with several sequences)
         if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
             return -1;
         p.rows_max = tiles ? kFewRows : INT_MAX;
         p.both = tiles;
-        if (launch_attend_rows(k_map, v_map, p, pages->dtype, st) != 0) return -1;
+        if (launch_attend_rows(k_map, v_map, p, mode, pages->dtype, st) != 0) return -1;
         p.rows_min = kFewRows + 1;
         p.rows_max = INT_MAX;
     }
-    if (!tiles) return 0;
+    if (!tiles) return groups > 0 && launch_attend_parts(p, pages->dtype, st) != 0 ? -1 : 0;
     if (!page_map(&k_map, pages, pages->k, pages->k_stride, kPage) || !page_map(&v_map, pages, pages->v, pages->v_stride, kPage) ||
         !rows_map(&q_map, pages->dtype, q, q_token_stride, q_head_stride, chunk->tokens, q_heads, group))
         return -1;
-    return launch_attend_tiles(q_map, k_map, v_map, p, pages->dtype, st) == 0 ? 0 : -1;
+    if (launch_attend_tiles(q_map, k_map, v_map, p, mode, pages->dtype, st) != 0) return -1;
+    return groups > 0 && launch_attend_parts(p, pages->dtype, st) != 0 ? -1 : 0;
 }
 
 SI_EXPORT int secure_infer_paged_append(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
@@ -329,7 +413,7 @@ SI_EXPORT int secure_infer_paged_fork(const secure_infer_page_tensor* tensors, u
         (n > 0 && (parents == nullptr || children == nullptr || granted == nullptr)))
         return -1;
     const TableParams p{*in, *out, parents, children, granted, nullptr, nullptr, static_cast<int32_t*>(scratch),
-                        static_cast<int32_t>(n)};
+                        static_cast<int32_t>(n), 0, 0};
     if (launch_tables(kFork, p, static_cast<cudaStream_t>(stream)) != 0) return -1;
     const CopyList list = table_copy_list(p.scratch, in->pages);
     return launch_page_copy(tensors, n_tensors, page_bytes, in->pages, list.src, list.dst, list.count,
@@ -346,7 +430,7 @@ SI_EXPORT int secure_infer_paged_reserve(const secure_infer_tables* in, const se
         (n > 0 && (seqs == nullptr || new_lens == nullptr || granted == nullptr)))
         return -1;
     const TableParams p{*in, *out, seqs, new_lens, granted, nullptr, nullptr, static_cast<int32_t*>(scratch),
-                        static_cast<int32_t>(n)};
+                        static_cast<int32_t>(n), 0, 0};
     return launch_tables(kReserve, p, static_cast<cudaStream_t>(stream)) == 0 ? 0 : -1;
 }
 
@@ -355,8 +439,19 @@ SI_EXPORT int secure_infer_paged_free(const secure_infer_tables* in, const secur
 {
     if (!tables_ok(in, out) || n > INT_MAX || scratch == nullptr || (n > 0 && seqs == nullptr)) return -1;
     const TableParams p{*in, *out, seqs, nullptr, nullptr, nullptr, nullptr, static_cast<int32_t*>(scratch),
-                        static_cast<int32_t>(n)};
+                        static_cast<int32_t>(n), 0, 0};
     return launch_tables(kFree, p, static_cast<cudaStream_t>(stream)) == 0 ? 0 : -1;
+}
+
+SI_EXPORT int secure_infer_trim(const secure_infer_tables* in, const secure_infer_tables* out, const int32_t* seqs, uint32_t n,
+                                uint32_t window, uint32_t sinks, void* scratch, void* stream)
+{
+    if (!tables_ok(in, out) || n > INT_MAX || scratch == nullptr || (n > 0 && seqs == nullptr) || window == 0 ||
+        window > INT_MAX || sinks > INT_MAX - kPage)
+        return -1;
+    const TableParams p{*in, *out, seqs, nullptr, nullptr, nullptr, nullptr, static_cast<int32_t*>(scratch),
+                        static_cast<int32_t>(n), static_cast<int32_t>(window), static_cast<int32_t>(sinks)};
+    return launch_tables(kTrim, p, static_cast<cudaStream_t>(stream)) == 0 ? 0 : -1;
 }
 
 SI_EXPORT int secure_infer_paged_compact(const secure_infer_page_tensor* tensors, uint32_t n_tensors,
@@ -367,7 +462,7 @@ SI_EXPORT int secure_infer_paged_compact(const secure_infer_page_tensor* tensors
     if (!tensors_ok(tensors, n_tensors, page_bytes) || !tables_ok(in, out) || moved == nullptr || live == nullptr ||
         scratch == nullptr)
         return -1;
-    const TableParams p{*in, *out, nullptr, nullptr, nullptr, moved, live, static_cast<int32_t*>(scratch), 0};
+    const TableParams p{*in, *out, nullptr, nullptr, nullptr, moved, live, static_cast<int32_t*>(scratch), 0, 0, 0};
     if (launch_tables(kCompact, p, static_cast<cudaStream_t>(stream)) != 0) return -1;
     const CopyList list = table_copy_list(p.scratch, in->pages);
     return launch_page_copy(tensors, n_tensors, page_bytes, in->pages, list.src, list.dst, list.count, in->pages / 2 + 1,

@@ -155,7 +155,7 @@ __device__ __forceinline__ bool rows_any(bool x)
     return r != 0;
 }
 
-template <typename T>
+template <typename T, int M>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                          const __grid_constant__ AttendParams p)
@@ -191,27 +191,31 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     wait_for_earlier_kernels();
-    find_share<kRowsThreads>(p, rows_kind(), tiles_kind(p), &share, warp_sums);
+    find_share<kRowsThreads, M>(p, rows_kind(), tiles_kind(p), &share, warp_sums);
     dependents_may_launch();
-    Walk w = start_walk(p, kRows, kRowsCost, share);
+    Walk<M> w = start_walk<M>(p, kRows, kRowsCost, share);
 
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
         uint32_t unit = 0, issued = 0;   // units passed, and those whose copies were issued
         while (w.left > 0 && !__any_sync(0xffffffffu, stop[0] || share.down)) {
             const int pages = w.take();
-            const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
+            const int32_t* row = p.table + w.row() * p.table_stride;
             for (int i0 = 0; i0 < pages; i0 += 32) {
-                const int id = i0 + lane < pages && w.span.hi > 0 ? row[i0 + lane] : -1;
+                const int id = i0 + lane < pages && w.span.hi > 0 ? row[w.span.page<M>(w.page + i0 + lane)] : -1;
                 for (int i = i0; i < min(pages, i0 + 32); ++i, ++unit) {
                     const int page = __shfl_sync(0xffffffffu, id, i - i0);
                     const int stage = unit % kRowsStages;
                     const uint32_t turn = unit / kRowsStages;
                     if (lane != 0 || stop[0] || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, stop))) continue;
                     issued = unit + 1;
-                    const int first = (w.span.first + w.page + i) * kPage;
-                    const int qa = max(0, w.span.lo - first) / kQuarter;
-                    const int qb = (min(kPage, w.span.hi - first) + kQuarter - 1) / kQuarter;
+                    const int first = w.span.page<M>(w.page + i) * kPage;
+                    int qa = max(0, w.span.lo - first) / kQuarter;
+                    int qb = (min(kPage, w.span.hi - first) + kQuarter - 1) / kQuarter;
+                    if (M == kSinks && first < p.sinks) {   // from its start; to the sinks' end where no window reaches it
+                        qa = 0;
+                        if (w.span.lo >= first + kPage) qb = (min(kPage, min(p.sinks, w.span.hi) - first) + kQuarter - 1) / kQuarter;
+                    }
                     const uint32_t bytes = qb > qa ? (qb - qa) * kQuarterBytes : 0;
                     barrier_expect(k_full(stage), bytes);
                     for (int t = qa; t < qb; ++t)
@@ -261,13 +265,13 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         int all_lo, all_hi; // keys that every row of the tile sees
         {
             int unused;
-            row_keys(p, w.q, w.last_token, all_lo, unused);
-            row_keys(p, w.q, w.first_token, unused, all_hi);
+            row_keys<M>(p, w.q, w.last_token, all_lo, unused);
+            row_keys<M>(p, w.q, w.first_token, unused, all_hi);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = (lane & 3) * 2 + e;
-            row_keys(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[e], hi[e]);
+            row_keys<M>(p, w.q, min(w.last_token, (r0 + r) / p.group), lo[e], hi[e]);
         }
         // Sums of values: o[j] holds values 16 j + lane / 4 (+ 8) of rows 2 (lane % 4) (+ 1).
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[8][4];
@@ -286,12 +290,12 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         for (int i = 0; i < pages && !failed; ++i, ++unit) {
             const int stage = unit % kRowsStages;
             const uint32_t parity = unit / kRowsStages & 1;
-            const int key0 = (w.span.first + w.page + i) * kPage + warp * 16;   // of this warp's keys
+            const int key0 = w.span.page<M>(w.page + i) * kPage + warp * 16;   // of this warp's keys
             failed = !barrier_wait(k_full(stage), parity, stop) || !barrier_wait(v_full(stage), parity, stop);
             if (failed) break;
-            if (key0 < w.span.hi && key0 + 16 > w.span.lo) {
+            if (key0 < w.span.hi && (key0 + 16 > w.span.lo || (M == kSinks && key0 < p.sinks))) {
                 const uint32_t slice = stage * kPageTile + (warp >> 1) * kQuarterBytes + (warp & 1) * 16 * 128;
-                const bool whole = key0 >= all_lo && key0 + 15 <= all_hi;
+                const bool whole = (key0 >= all_lo || (M == kSinks && key0 + 16 <= p.sinks)) && key0 + 15 <= all_hi;
                 float s[2][4] = {};   // two chains of products
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {   // 16 values of the head at a time
@@ -306,7 +310,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     x[c] = (s[0][c] + s[1][c]) * p.scale_log2;
                     if (!whole) {
                         const int key = key0 + (lane >> 2) + (c >> 1) * 8;
-                        if (key < lo[c & 1] || key > hi[c & 1]) x[c] = -INFINITY;
+                        if ((key < lo[c & 1] && !(M == kSinks && key < p.sinks)) || key > hi[c & 1]) x[c] = -INFINITY;
                     }
                     top[c & 1] = fmaxf(top[c & 1], x[c]);
                 }
@@ -340,7 +344,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = key0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
-                    if (key >= w.span.lo && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
+                    if ((key >= w.span.lo || (M == kSinks && key < p.sinks)) && key < w.span.hi) keep[j >> 1] |= (j & 1) ? 0xffff0000u : 0x0000ffffu;
                 }
                 uint32_t odd = 0;
 #pragma unroll
@@ -392,7 +396,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (const int r = warp; r < w.rows) {
             const int token = (r0 + r) / p.group, g = (r0 + r) - token * p.group;
             int a, b;
-            row_keys(p, w.q, token, a, b);
+            row_keys<M>(p, w.q, token, a, b);
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float top, sum;
             if (failed) {
@@ -400,11 +404,10 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 sum = NAN;
                 x = make_float4(NAN, NAN, NAN, NAN);
             } else if (by_definition) {
-                const int ka = (w.span.first + w.page) * kPage;
-                row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
-                                            (w.head * p.group + g) * p.q_head,
-                                     p.table + w.s * p.table_stride, w.head, max(a, ka), min(b + 1, ka + pages * kPage), top,
-                                     sum, x, stop + 1);
+                row_by_definition<T, M>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
+                                               (w.head * p.group + g) * p.q_head,
+                                        p.table + w.row() * p.table_stride, w.head,
+                                        piece_keys<M>(p, w.span, w.page, pages, a, b), top, sum, x, stop + 1);
             } else {
                 const int stat = (lane & (kRowsWarps - 1)) * kRows + r;
                 const float mi = join_m[stat];
@@ -432,13 +435,8 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     slot[kRows * kDim + kRows + r] = sum;
                 }
             } else {
-                const float inv = 1.0f / sum;
                 const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + g;
-                uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-                if (b < a) packed = make_uint2(0, 0);
-                *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
-                if (p.lse != nullptr && lane == 0)
-                    p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+                put_row<T, M>(p, w.q.part, at, x, top, sum, b < a);
             }
         }
         // Reads and writes of this page's buffers come before the next copy into them.
@@ -483,14 +481,9 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                     } else {
                         const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
                         int a, b;
-                        row_keys(p, w.q, token, a, b);
-                        const float inv = 1.0f / sum;
+                        row_keys<M>(p, w.q, token, a, b);
                         const int64_t at = static_cast<int64_t>(w.q.q0 + token) * p.heads * p.group + w.head * p.group + g;
-                        uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-                        if (b < a) packed = make_uint2(0, 0);
-                        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
-                        if (p.lse != nullptr && lane == 0)
-                            p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+                        put_row<T, M>(p, w.q.part, at, x, top, sum, b < a);
                     }
                 }
                 if (final) break;
@@ -684,19 +677,28 @@ __device__ __forceinline__ float2 exp2_poly(uint64_t x2)
 // waits for every softmax warp.
 struct Item {
     Span span;
-    int s, head, pages, rows;
-    int first_key;               // of the piece
+    int s, head, pages, rows;    // s: row of the block table
+    int page, first_key;         // of the piece: the first of the tile's pages, its first key
     int pos, last_pos, last_key; // of the tile's first and last token, and of the sequence
     int lo_all, hi_all;          // keys that every row sees
     int q0;                      // the tile's first token among all
     int slot;                    // where a part of a cut tile goes, -1: the tile is whole
     int more;                    // another piece follows
+    int begin, part;             // kShared: as a Seq's
 
-    // Keys that the row at position p sees: [lo, hi].
+    // First key of the piece's page i.
+    template <int M>
+    __device__ __forceinline__ int key(int i) const
+    {
+        return M == kSinks ? span.page<M>(page + i) * kPage : first_key + i * kPage;
+    }
+    // Keys that the row at position p sees: [lo, hi], and with sinks those before min(sinks, hi + 1).
+    template <int M>
     __device__ __forceinline__ void keys(const AttendParams& a, int p, int& lo, int& hi) const
     {
-        hi = a.causal ? min(last_key, p) : last_key;
-        lo = a.window ? max(0, p - a.window + 1) : 0;
+        hi = a.causal && !(M == kShared && part == 0) ? min(last_key, p) : last_key;
+        if (M == kShared) lo = begin;
+        else lo = a.window ? max(0, p - a.window + 1) : 0;
     }
 };
 
@@ -718,17 +720,17 @@ constexpr uint32_t kTilesSmem = kControlBytes + 1024 + (2 + kRing) * kTileBytes 
 
 // After a wait that ran out, by the softmax warps: the rows of this CTA's share
 // become NaN, and so do its pieces of cut tiles.
-template <typename T>
+template <typename T, int M>
 __device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& share)
 {
     const int tid = threadIdx.x, cta = blockIdx.x;
     if (tid == 0) atomicOr(p.status, 1u);
-    Walk w = start_walk(p, 2 * (128 / p.group * p.group), kTilesCost, share);
+    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), kTilesCost, share);
     for (bool first = true; w.left > 0; first = false) {
         const int pages = w.take();
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
         if (first && tid == 0)
-            p.cuts[cta] = cta0 < cta ? Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0} : Cut{};
+            p.cuts[cta] = cta0 < cta ? Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0, w.q.part} : Cut{};
         if (cta1 > cta0) {
             float* slot = p.slots + static_cast<int64_t>(2 * cta + (cta0 == cta)) * kTileSlot;
             for (int i = tid; i < kTileSlot; i += 32 * kSoftWarps) slot[i] = NAN;
@@ -736,16 +738,14 @@ __device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& shar
             for (int i = tid; i < w.rows * 32; i += 32 * kSoftWarps) {
                 const int r = i >> 5, token = w.first_token + r / p.group;
                 const int64_t at = (static_cast<int64_t>(w.q.q0 + token) * p.heads + w.head) * p.group + r % p.group;
-                const uint32_t x = pack2<T>(NAN, NAN);
-                reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim)[i & 31] = make_uint2(x, x);
-                if (p.lse != nullptr && (i & 31) == 0) p.lse[at] = NAN;
+                put_row<T, M>(p, w.q.part, at, make_float4(NAN, NAN, NAN, NAN), 0.0f, NAN, false);
             }
         }
         w.advance(p, pages);
     }
 }
 
-template <typename T>
+template <typename T, int M>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                           const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttendParams p)
@@ -797,11 +797,11 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     // read them, the two share no memory that either writes, and it waits for that one at its end instead.
     if (!p.both) wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads>(p, tiles_kind(p), rows_kind(), &c.share, c.warp_sums);
+    find_share<kTileThreads, M>(p, tiles_kind(p), rows_kind(), &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
-    Walk w = start_walk(p, 2 * rows_per_tile, kTilesCost, c.share);
+    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, kTilesCost, c.share);
     const bool any = w.left > 0 && c.share.down == 0;
 
     // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.
@@ -812,8 +812,8 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             uint32_t n = 0, item = 0, issued = 0, q_issued = 0;   // buffers and pieces passed, and those whose copies were issued
             while (any && w.left > 0 && !__any_sync(0xffffffffu, *stop)) {
                 const int pages = w.take();
-                const int32_t* row = p.table + w.s * p.table_stride + w.span.first + w.page;
-                int id = lane < pages && w.span.hi > 0 ? __ldcg(row + lane) : -1;
+                const int32_t* row = p.table + w.row() * p.table_stride;
+                int id = lane < pages && w.span.hi > 0 ? __ldcg(row + w.span.page<M>(w.page + lane)) : -1;
                 if (lane == 0) {
                     if (item > 0) barrier_wait(q_empty, (item - 1) & 1, stop);
                     if (!*stop) {
@@ -830,17 +830,20 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 auto publish = [&] {
                     Item& it = c.items[item % kItems];
                     it.span = w.span;
-                    it.s = w.s;
+                    it.s = w.row();
                     it.head = w.head;
                     it.pages = pages;
                     it.rows = w.rows;
-                    it.first_key = (w.span.first + w.page) * kPage;
+                    it.page = w.page;
+                    it.first_key = w.span.page<M>(w.page) * kPage;
+                    it.begin = w.q.begin;
+                    it.part = w.q.part;
                     it.pos = w.q.kv - w.q.n + w.first_token;
                     it.last_pos = it.pos + w.last_token - w.first_token;
                     it.last_key = w.q.kv - 1;
                     int unused;
-                    it.keys(p, it.last_pos, it.lo_all, unused);
-                    it.keys(p, it.pos, unused, it.hi_all);
+                    it.keys<M>(p, it.last_pos, it.lo_all, unused);
+                    it.keys<M>(p, it.pos, unused, it.hi_all);
                     it.q0 = w.q.q0 + w.first_token;
                     const int cta0 = c.share.owner(w.tile_unit), cta1 = c.share.owner(w.tile_unit + w.span.pages - 1);
                     it.slot = cta1 > cta0 ? 2 * static_cast<int>(blockIdx.x) + (cta0 == static_cast<int>(blockIdx.x)) : -1;
@@ -850,12 +853,12 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     if (item == 0) {
                         Cut cut{};
                         if (cta0 < static_cast<int>(blockIdx.x))
-                            cut = Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0};
+                            cut = Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0, w.q.part};
                         p.cuts[blockIdx.x] = cut;
                     }
                 };
                 for (int i0 = 0; i0 < pages; i0 += 32) {
-                    if (i0 > 0) id = i0 + lane < pages && w.span.hi > 0 ? __ldcg(row + i0 + lane) : -1;
+                    if (i0 > 0) id = i0 + lane < pages && w.span.hi > 0 ? __ldcg(row + w.span.page<M>(w.page + i0 + lane)) : -1;
                     for (int i = i0; i < min(pages, i0 + 32); ++i) {
                         const int page = __shfl_sync(0xffffffffu, id, i - i0);
                         for (int kv = 0; kv < 2; ++kv, ++n) {
@@ -938,12 +941,24 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         ok = barrier_wait(kv_full(v_slot), (n / kRing) & 1, stop);
                         // Values of keys that no row sees were never written or belong to others: weights of zero do
                         // not silence a NaN there, so within the 16-key steps that are multiplied they become zero.
-                        const int key0 = w.first_key + i * kPage;
-                        const int lo = max(0, min(kPage, w.span.lo - key0)), hi = max(0, min(kPage, w.span.hi - key0));
+                        const int key0 = w.key<M>(i);
+                        int lo = max(0, min(kPage, w.span.lo - key0)), hi = max(0, min(kPage, w.span.hi - key0));
+                        int gap0 = 0, gap1 = 0;   // between the sinks and the window
+                        if (M == kSinks) {
+                            const int sinks = max(0, min(kPage, min(p.sinks, w.span.hi) - key0));
+                            if (sinks > 0 && hi <= lo) {
+                                hi = sinks;
+                            } else if (sinks > 0 && sinks < lo) {
+                                gap0 = sinks;
+                                gap1 = lo;
+                            }
+                            if (sinks > 0) lo = 0;
+                        }
                         const int step0 = lo >> 4, step1 = hi > lo ? (hi + 15) >> 4 : step0;
-                        if (lo & 15 || hi & 15) {
-                            for (int side = 0; side < 2; ++side) {
-                                const int a = side ? hi : step0 * 16, b = side ? min(kPage, step1 * 16) : lo;
+                        if (lo & 15 || hi & 15 || (M == kSinks && gap1 > 0)) {
+                            for (int side = 0; side < (M == kSinks ? 3 : 2); ++side) {
+                                const int a = side == 0 ? step0 * 16 : side == 1 ? hi : gap0;
+                                const int b = side == 0 ? lo : side == 1 ? min(kPage, step1 * 16) : gap1;
                                 for (int x = lane; x < (b - a) * 16; x += 32) {
                                     const uint32_t at = ring + v_slot * kTileBytes + (x & 8 ? kTileBytes / 2 : 0) +
                                                         (a + (x >> 4)) * 128 + (x & 7) * 16;
@@ -996,13 +1011,15 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 const int pages = w.pages, lo_all = w.lo_all, hi_all = w.hi_all;
                 uint32_t odd = 0;
                 for (int i = 0; i < pages; ++i) {
-                    const int key0 = w.first_key + i * kPage;
+                    const int key0 = w.key<M>(i);
                     for (int kv = 0; kv < 2; ++kv, ++n) {
                         const uint32_t slot = n % kRing;
                         if (!barrier_wait(kv_full(slot), (n / kRing) & 1, stop)) break;
                         if (kv == 1 && w.pos != w.last_pos && (key0 < lo_all || key0 + kPage - 1 > hi_all)) {
                             // Two keys at a time: left of what all rows see, then right of it.
-                            const int a = max(0, w.span.lo - key0), b = min(kPage, w.span.hi - key0);
+                            // (Every row sees the sinks up to its own position.)
+                            const int a = max(0, (M == kSinks ? max(w.span.lo, min(p.sinks, hi_all + 1)) : w.span.lo) - key0);
+                            const int b = min(kPage, w.span.hi - key0);
                             for (int side = 0; side < 2; ++side) {
                                 const int k0 = side ? max(a, hi_all + 1 - key0) : a, k1 = side ? b : min(b, lo_all - key0);
                                 const uint32_t at = ring + slot * kTileBytes + (lane & 8 ? kTileBytes / 2 : 0) + (lane & 7) * 16;
@@ -1057,12 +1074,12 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             if (meet_or(!ok)) break;
             const Item& w = c.items[item % kItems];
             const int pages = w.pages, tiles = w.rows > rows_per_tile ? 2 : 1;
-            const int lo_all = w.lo_all, hi_all = w.hi_all, page_key = w.first_key;
+            const int lo_all = w.lo_all, hi_all = w.hi_all;
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
             for (int i = 0; i < pages; ++i) {
                 // By the whole page and both tiles, so that all threads agree.
-                const int page0 = page_key + i * kPage;
-                const bool masked = page0 < lo_all || page0 + kPage - 1 > hi_all;
+                const int page0 = w.key<M>(i);
+                const bool masked = (page0 < lo_all && !(M == kSinks && page0 + kPage <= p.sinks)) || page0 + kPage - 1 > hi_all;
 #pragma unroll 1
                 for (int t = 0; t < tiles; ++t) {
                     ok = ok && barrier_wait(s_full(t), (t ? seen[1] : seen[0]) & 1, stop);
@@ -1122,9 +1139,13 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                         if (masked) {
                             // Bits of the keys from lo to hi.
                             int lo, hi;
-                            w.keys(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
+                            w.keys<M>(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
                             const int a = max(0, lo - page0 - quarter * 32), b = min(31, hi - page0 - quarter * 32);
-                            const uint32_t keep = b < a ? 0 : (~0u << a) & (~0u >> (31 - b));
+                            uint32_t keep = b < a ? 0 : (~0u << a) & (~0u >> (31 - b));
+                            if (M == kSinks) {
+                                const int c = min(32, min(p.sinks, hi + 1) - page0 - quarter * 32);
+                                if (c > 0) keep |= ~0u >> (32 - c);
+                            }
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 if (!(keep >> j & 1)) s[j] = 0xff800000u;
@@ -1198,13 +1219,13 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     for (int r = quarter; r < min(32, valid); r += 4) {
                         const int tok = (rows0 + r) / p.group, head = (rows0 + r) % p.group;
                         int a, b;
-                        w.keys(p, w.pos + t * tokens + tok, a, b);
+                        w.keys<M>(p, w.pos + t * tokens + tok, a, b);
                         float mm, ll;
                         float4 x;
-                        row_by_definition<T>(p, static_cast<const T*>(p.q) + (w.q0 + t * tokens + tok) * p.q_token +
-                                                    (w.head * p.group + head) * p.q_head,
-                                             p.table + w.s * p.table_stride, w.head, max(a, page_key),
-                                             min(b + 1, page_key + pages * kPage), mm, ll, x, stop + 1);
+                        row_by_definition<T, M>(p, static_cast<const T*>(p.q) + (w.q0 + t * tokens + tok) * p.q_token +
+                                                       (w.head * p.group + head) * p.q_head,
+                                                p.table + w.s * p.table_stride, w.head,
+                                                piece_keys<M>(p, w.span, w.page, pages, a, b), mm, ll, x, stop + 1);
                         if (split) {
                             reinterpret_cast<float4*>(slot)[((t * 4 + rows0 / 32) * 32 + lane) * 32 + r] = x;
                             if (lane == 0) {
@@ -1212,13 +1233,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                                 slot[kTileRows * kDim + kTileRows + t * 128 + rows0 + r] = ll;
                             }
                         } else {
-                            const float inv = 1.0f / ll;
-                            const int64_t at = out0 + tok * p.heads * p.group + head;
-                            uint2 packed = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
-                            if (b < a) packed = make_uint2(0, 0);
-                            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * kDim + lane * 4) = packed;
-                            if (p.lse != nullptr && lane == 0)
-                                p.lse[at] = b >= a ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
+                            put_row<T, M>(p, w.part, out0 + tok * p.heads * p.group + head, x, mm, ll, b < a);
                         }
                     }
                     continue;
@@ -1229,7 +1244,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                 const float l = (parts[0] + parts[128]) + (parts[256] + parts[384]);
                 meet_or(false);   // read before the next piece's maxima come
                 int lo, hi;
-                w.keys(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
+                w.keys<M>(p, min(w.pos + t * tokens + token, w.last_pos), lo, hi);
                 const float inv = 1.0f / l;
                 // Rows leave through a warp's own piece of shared memory, 32 bytes of each at a time, so that a store
                 // covers whole sectors: sixteen rows by two lanes.
@@ -1257,6 +1272,17 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                             part[d * 8] = make_float4(__uint_as_float(o[d]), __uint_as_float(o[d + 1]),
                                                       __uint_as_float(o[d + 2]), __uint_as_float(o[d + 3]));
                     }
+                } else if (M == kShared && w.part >= 0) {
+                    if (lane < valid) {
+                        const int64_t all = static_cast<int64_t>(p.tokens) * p.heads * p.group, to = w.part * all + out0 + rel;
+                        float4* part = reinterpret_cast<float4*>(p.parts + to * kDim + quarter * 32);
+#pragma unroll
+                        for (int d = 0; d < 32; d += 4)
+                            part[d / 4] = make_float4(__uint_as_float(o[d]), __uint_as_float(o[d + 1]),
+                                                      __uint_as_float(o[d + 2]), __uint_as_float(o[d + 3]));
+                        if (quarter == 0)
+                            *reinterpret_cast<float2*>(p.parts + 2 * all * kDim + 2 * to) = make_float2((t ? m1 : m0) * scale, l);
+                    }
                 } else {
                     T* out = static_cast<T*>(p.out) + out0 * kDim + quarter * 32 + (lane & 1) * 8;
 #pragma unroll
@@ -1283,7 +1309,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     if (split) {
                         slot[kTileRows * kDim + t * 128 + row] = top;
                         slot[kTileRows * kDim + kTileRows + t * 128 + row] = l;
-                    } else if (p.lse != nullptr) {
+                    } else if (p.lse != nullptr && !(M == kShared && w.part >= 0)) {
                         p.lse[out0 + rel] = hi >= lo ? (top + log2f(l)) * 0.6931471805599453f : -INFINITY;
                     }
                 }
@@ -1299,7 +1325,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     }
     tmem_fence_before();
     __syncthreads();
-    if (warp < kSoftWarps && (*stop || c.share.down)) fail_tiles<T>(p, c.share);
+    if (warp < kSoftWarps && (*stop || c.share.down)) fail_tiles<T, M>(p, c.share);
     if (p.both) wait_for_earlier_kernels();
     if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
@@ -1313,7 +1339,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 // tile).
 constexpr int kJoinThreads = 64;
 constexpr int kJoinBlocks = kTileRows / 32 * (kDim / 16) / (kJoinThreads / 32);
-template <typename T, int kFours>
+template <typename T, int M, int kFours>
 __device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cut, int r, int tile_row, int d4)
 {
     const int pieces = cut.cta1 - cut.cta0 + 1;
@@ -1333,12 +1359,19 @@ __device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cu
             x[j] = make_float4(x[j].x + f * y.x, x[j].y + f * y.y, x[j].z + f * y.z, x[j].w + f * y.w);
         }
     }
-    const Seq s{cut.n, cut.kv, cut.q0};
+    const Seq s{cut.n, cut.kv, cut.q0, 0, cut.part, 0};
     const int token = cut.token0 + tile_row / p.group, g = tile_row % p.group;
-    int a, b;
-    row_keys(p, s, token, a, b);
-    const float inv = 1.0f / sum;
     const int64_t at = static_cast<int64_t>(cut.q0 + token) * p.heads * p.group + cut.head * p.group + g;
+    if (M == kShared && cut.part >= 0) {
+        const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads * p.group, to = cut.part * rows + at;
+#pragma unroll
+        for (int j = 0; j < kFours; ++j) reinterpret_cast<float4*>(p.parts + to * kDim)[d4 + j] = x[j];
+        if (d4 == 0) *reinterpret_cast<float2*>(p.parts + 2 * rows * kDim + 2 * to) = make_float2(top, sum);
+        return;
+    }
+    int a, b;
+    row_keys<M>(p, s, token, a, b);
+    const float inv = 1.0f / sum;
     uint2 y[kFours];
 #pragma unroll
     for (int j = 0; j < kFours; ++j) {
@@ -1356,7 +1389,7 @@ __device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cu
     if (p.lse != nullptr && d4 == 0) p.lse[at] = b >= a ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
-template <typename T>
+template <typename T, int M>
 __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const __grid_constant__ AttendParams p)
 {
     wait_for_earlier_kernels();
@@ -1369,9 +1402,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     const int rows_per_tile = 128 / p.group * p.group, r = part / 8 * 32 + (threadIdx.x & 31);
     const int tile_row = r < 128 ? (r < rows_per_tile ? r : cut.rows) : (r - 128 < rows_per_tile ? rows_per_tile + r - 128 : cut.rows);
     if (k * fours >= 4 || tile_row >= cut.rows) return;
-    if (fours == 4) join_values<T, 4>(p, cut, r, tile_row, d4);
-    else if (fours == 2) join_values<T, 2>(p, cut, r, tile_row, d4);
-    else join_values<T, 1>(p, cut, r, tile_row, d4);
+    if (fours == 4) join_values<T, M, 4>(p, cut, r, tile_row, d4);
+    else if (fours == 2) join_values<T, M, 2>(p, cut, r, tile_row, d4);
+    else join_values<T, M, 1>(p, cut, r, tile_row, d4);
 }
 
 // CTAs of a launch on the current device.
@@ -1388,13 +1421,13 @@ int attend_grid()
 }
 
 struct Device {
-    bool rows_set[2] = {};
-    bool tiles_set[2] = {};
+    bool rows_set[3][2] = {};
+    bool tiles_set[3][2] = {};
 };
 std::mutex g_mu;
 Device g_devices[64];
 
-template <typename T>
+template <typename T, int M>
 int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, cudaStream_t stream)
 {
     int dev = 0;
@@ -1403,9 +1436,9 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
     {
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
-        bool& set = d.rows_set[std::is_same<T, __half>::value];
+        bool& set = d.rows_set[M][std::is_same<T, __half>::value];
         if (!set) {
-            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T>,
+            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, M>,
                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
             if (e != cudaSuccess) return e;
             set = true;
@@ -1422,10 +1455,10 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     ProfileScope prof(kKernAttendRows, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T>, k_map, v_map, p);
+    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, M>, k_map, v_map, p);
 }
 
-template <typename T>
+template <typename T, int M>
 int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p,
                  cudaStream_t stream)
 {
@@ -1435,11 +1468,16 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
     {
         std::lock_guard<std::mutex> lock(g_mu);
         Device& d = g_devices[dev & 63];
-        bool& set = d.tiles_set[std::is_same<T, __half>::value];
+        bool& set = d.tiles_set[M][std::is_same<T, __half>::value];
         if (!set) {
-            const cudaError_t e = cudaFuncSetAttribute(paged_attend_tiles_kernel<T>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kTilesSmem);
+            cudaError_t e = cudaFuncSetAttribute(paged_attend_tiles_kernel<T, M>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kTilesSmem);
             if (e != cudaSuccess) return e;
+            // The softmax warps' registers come from what the block was launched with, or they would wait for ever.
+            cudaFuncAttributes made;
+            e = cudaFuncGetAttributes(&made, paged_attend_tiles_kernel<T, M>);
+            if (e != cudaSuccess) return e;
+            if (made.numRegs * kTileThreads < 32 * (104 * kSoftWarps + 64 * 4)) return cudaErrorLaunchOutOfResources;
             set = true;
         }
     }
@@ -1455,30 +1493,46 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
     cfg.numAttrs = 1;
     {
         ProfileScope prof(kKernAttendTiles, stream);
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attend_tiles_kernel<T>, q_map, k_map, v_map, p);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attend_tiles_kernel<T, M>, q_map, k_map, v_map, p);
         if (e != cudaSuccess) return e;
     }
     cfg.gridDim = dim3(kJoinBlocks, grid);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     ProfileScope prof(kKernAttendJoin, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_join_kernel<T>, p);
+    return cudaLaunchKernelEx(&cfg, paged_attend_join_kernel<T, M>, p);
+}
+
+// f(type, mode) for the call's type and mode.
+template <class F>
+int by_type_and_mode(uint32_t dtype, Mode mode, F f)
+{
+    const auto by_mode = [&](auto type) {
+        switch (mode) {
+            case kSinks: return f(type, std::integral_constant<int, kSinks>{});
+            case kShared: return f(type, std::integral_constant<int, kShared>{});
+            default: return f(type, std::integral_constant<int, kPlain>{});
+        }
+    };
+    return dtype == SECURE_INFER_FP16 ? by_mode(__half{}) : by_mode(__nv_bfloat16{});
 }
 
 }  // namespace
 
 int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
-                        const AttendParams& p, uint32_t dtype, cudaStream_t stream)
+                        const AttendParams& p, Mode mode, uint32_t dtype, cudaStream_t stream)
 {
-    return dtype == SECURE_INFER_FP16 ? launch_tiles<__half>(q_map, k_map, v_map, p, stream)
-                                      : launch_tiles<__nv_bfloat16>(q_map, k_map, v_map, p, stream);
+    return by_type_and_mode(dtype, mode, [&](auto type, auto m) {
+        return launch_tiles<decltype(type), decltype(m)::value>(q_map, k_map, v_map, p, stream);
+    });
 }
 
-int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, uint32_t dtype,
-                       cudaStream_t stream)
+int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, Mode mode,
+                       uint32_t dtype, cudaStream_t stream)
 {
-    return dtype == SECURE_INFER_FP16 ? launch_rows<__half>(k_map, v_map, p, stream)
-                                      : launch_rows<__nv_bfloat16>(k_map, v_map, p, stream);
+    return by_type_and_mode(dtype, mode, [&](auto type, auto m) {
+        return launch_rows<decltype(type), decltype(m)::value>(k_map, v_map, p, stream);
+    });
 }
 
 uint64_t attend_workspace_bytes()

@@ -26,21 +26,6 @@ constexpr int kAppendThreads = 128;
 // and 27.0 (fewer warps for their registers), with twelve in 64 registers of a thread instead of 72 26.5.
 constexpr int kAppendBatch = 3;
 
-__device__ __forceinline__ int find_seq(const int32_t* cu, int seqs, int token)
-{
-    // The last s with cu[s] <= token: 32 probes at a time.
-    const int lane = threadIdx.x & 31;
-    int lo = 0, hi = seqs;   // cu[lo] <= token, and the answer lies in [lo, hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const uint32_t below = __ballot_sync(0xffffffffu, at < hi && cu[at] <= token);
-        const int k = below == 0 ? 0 : 31 - __clz(below);
-        lo += k * step;
-        hi = min(hi, lo + step);
-    }
-    return lo;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads)
 paged_append_kernel(const __grid_constant__ AppendParams p, int groups, int rows_per_warp)
@@ -260,7 +245,7 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
         if (kOp != kCompact) p.out.refs[i] = r;
         found += kOp == kCompact ? r > 0 : r == 0;
     }
-    if (kOp != kFree) {
+    if (kOp != kFree && kOp != kTrim) {
         int total;
         block_prefix(found, sums, total);
         if (tid == 0) s.counts[cta] = total;
@@ -354,7 +339,7 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
         if (kOp == kFork && cta == 0 && tid == 0) *s.copies = needed;
         cluster_barrier<kCluster>();
     }
-    if (kOp == kFree) {
+    if (kOp == kFree || kOp == kTrim) {
         for (int i = all; i < p.n; i += stride)
             if (p.a[i] >= 0 && p.a[i] < seqs) s.row_of[p.a[i]] = i;
         cluster_barrier<kCluster>();
@@ -422,6 +407,18 @@ __global__ void __launch_bounds__(kTableThreads, 1) page_tables_kernel(const __g
             const int i = __ldcg(&s.row_of[r]);
             if (i < 0) {
                 for (int c = lane; c < width; c += 32) out[c] = in[c];
+                now = p.in.lens[r];
+            } else if (kOp == kTrim) {
+                // Pages from the sinks' end to the window of the token at `len`, which sees len - window + 1 and what follows.
+                const int kept = (p.sinks + kPage - 1) / kPage, gone = min(used, max(0, len - p.window + 1) / kPage);
+                for (int c = lane; c < width; c += 32) {
+                    int page = in[c];
+                    if (c >= kept && c < gone) {
+                        if (page >= 0 && page < pages) atomicSub(&p.out.refs[page], 1);
+                        page = -1;
+                    }
+                    out[c] = page;
+                }
                 now = p.in.lens[r];
             } else if (kOp == kFree) {
                 now = 0;
@@ -583,6 +580,7 @@ int launch_tables(TableOp op, const TableParams& p, cudaStream_t stream)
         case kFork: return launch_op<kFork>(p, stream);
         case kReserve: return launch_op<kReserve>(p, stream);
         case kFree: return launch_op<kFree>(p, stream);
+        case kTrim: return launch_op<kTrim>(p, stream);
         default: return launch_op<kCompact>(p, stream);
     }
 }

@@ -106,10 +106,21 @@ bool counted(Py_ssize_t n, Py_ssize_t want)
     return false;
 }
 
-// attend(pages, chunk, device, q, out, return_lse, scale, causal, window, workspace, stream)
+PyObject* pair(at::Tensor a, at::Tensor b)
+{
+    PyObject* first = THPVariable_Wrap(std::move(a));
+    PyObject* second = THPVariable_Wrap(std::move(b));
+    PyObject* both = first != nullptr && second != nullptr ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return both;
+}
+
+// attend(pages, chunk, device, q, out, return_lse, scale, causal, window, workspace, stream), and perhaps (sinks, plan
+// of a shared prefix or None, its groups)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    if (!counted(n, 11)) return nullptr;
+    if (n != 11 && !counted(n, 14)) return nullptr;
     return guarded([&]() -> PyObject* {
         const auto* pages = address<const secure_infer_pages>(a[0]);
         secure_infer_chunk chunk = *address<const secure_infer_chunk>(a[1]);
@@ -124,6 +135,24 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
         if (PyErr_Occurred()) return nullptr;
         need(window >= 0 && window < int64_t(1) << 31 && (window == 0 || causal),
              "window must be zero or positive, and goes with causal");
+        secure_infer_attend_options options{};
+        at::Tensor parts;
+        if (n > 11) {
+            const int64_t sinks = PyLong_AsLongLong(a[11]), groups = PyLong_AsLongLong(a[13]);
+            if (PyErr_Occurred()) return nullptr;
+            need(sinks >= 0 && sinks < int64_t(1) << 31 && (sinks == 0 || window > 0),
+                 "sinks must be zero or positive, and go with a window");
+            options.sinks = static_cast<uint32_t>(sinks);
+            if (a[12] != Py_None) {
+                need(window == 0, "a shared prefix does not go with a window");
+                need(groups > 0 && groups <= chunk.seqs, "a shared prefix has one group for each sequence at most");
+                const at::Tensor& plan = tensor(a[12], "the shared prefix's plan");
+                options.groups = static_cast<uint32_t>(groups);
+                options.plan = ints(plan, 1, device, "the shared prefix must be on the cache's device");
+                need(static_cast<uint64_t>(plan.numel()) >= secure_infer_shared_prefix_ints(chunk.seqs, options.groups) &&
+                         aligned(plan), "the shared prefix is another chunk's");
+            }
+        }
         at::Tensor out = output(a[4], q), lse;
         const bool want_lse = PyObject_IsTrue(a[5]);
         if (want_lse) lse = at::empty({tokens, r.heads}, q.options().dtype(at::kFloat));
@@ -135,22 +164,76 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
                  "workspace must come from attend_workspace of the cache's device");
             need(tokens <= UINT32_MAX, "too many tokens");
             chunk.tokens = static_cast<uint32_t>(tokens);
-            if (secure_infer_paged_attend(pages, &chunk, r.data, r.token, r.head, static_cast<uint32_t>(r.heads),
-                                          out.data_ptr(), want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
-                                          static_cast<float>(scale), causal, static_cast<uint32_t>(window),
-                                          workspace.data_ptr(), address<void>(a[10])) != 0) {
-                need(secure_infer_attend_fits(pages, &chunk, static_cast<uint32_t>(r.heads)),
-                     "more work than one call takes: fewer tokens, or a narrower block table");
-                return failed("secure_infer_paged_attend");
+            const char* most = "more work than one call takes: fewer tokens, or a narrower block table";
+            if (options.groups > 0) {
+                // Memory for partial results only for what will be launched.
+                need(secure_infer_attend_fits_shared(pages, &chunk, static_cast<uint32_t>(r.heads), options.groups), most);
+                const uint64_t bytes = secure_infer_attend_parts(chunk.tokens, static_cast<uint32_t>(r.heads));
+                parts = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+                options.parts = static_cast<float*>(parts.data_ptr());
+            }
+            if (secure_infer_attend(pages, &chunk, r.data, r.token, r.head, static_cast<uint32_t>(r.heads), out.data_ptr(),
+                                    want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, static_cast<float>(scale),
+                                    causal, static_cast<uint32_t>(window), &options, workspace.data_ptr(),
+                                    address<void>(a[10])) != 0) {
+                need(secure_infer_attend_fits(pages, &chunk, static_cast<uint32_t>(r.heads)), most);
+                return failed("secure_infer_attend");
             }
         }
-        if (!want_lse) return THPVariable_Wrap(std::move(out));
-        PyObject* first = THPVariable_Wrap(std::move(out));
-        PyObject* second = THPVariable_Wrap(std::move(lse));
-        PyObject* both = first != nullptr && second != nullptr ? PyTuple_Pack(2, first, second) : nullptr;
-        Py_XDECREF(first);
-        Py_XDECREF(second);
-        return both;
+        return want_lse ? pair(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
+    });
+}
+
+// join(outs, lses, device, out, stream)
+PyObject* join(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!counted(n, 5)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        need(PyTuple_Check(a[0]) && PyTuple_Check(a[1]), "outs and lses must be tuples of tensors");
+        const Py_ssize_t count = PyTuple_GET_SIZE(a[0]);
+        need(count > 0 && count <= static_cast<Py_ssize_t>(SECURE_INFER_JOIN_PARTS) && PyTuple_GET_SIZE(a[1]) == count,
+             "outs and lses must be one to eight tensors each, as many of both");
+        const int64_t device = PyLong_AsLongLong(a[2]);
+        if (PyErr_Occurred()) return nullptr;
+        const at::Tensor& like = tensor(PyTuple_GET_ITEM(a[0], 0), "an output");
+        const at::ScalarType type = like.scalar_type();
+        need(type == at::kHalf || type == at::kBFloat16, "outputs are bf16 or fp16");
+        const int64_t tokens = like.dim() > 0 ? like.size(0) : 0;
+        secure_infer_attend_part parts[SECURE_INFER_JOIN_PARTS];
+        int64_t heads = 0;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            const at::Tensor& o = tensor(PyTuple_GET_ITEM(a[0], i), "an output");
+            need(o.dim() == 3 && o.sizes() == like.sizes() && o.scalar_type() == type && o.is_cuda() && o.get_device() == device,
+                 "the outputs differ in shape, type or device");
+            const Rows r = rows(o, "an output", tokens, type, device);
+            const at::Tensor& l = tensor(PyTuple_GET_ITEM(a[1], i), "a logarithm of sums");
+            need(l.dim() == 2 && l.size(0) == tokens && l.size(1) == r.heads && l.scalar_type() == at::kFloat && l.is_cuda() &&
+                     l.get_device() == device && l.stride(0) >= 0 && l.stride(1) >= 0,
+                 "lses must be float32 [tokens, heads] of the outputs' device");
+            heads = r.heads;
+            parts[i] = {r.data, static_cast<const float*>(l.data_ptr()), {r.token, r.head}, {l.stride(0), l.stride(1)}};
+        }
+        need(heads > 0 && heads <= 1 << 16 && tokens <= 1 << 28 && tokens * heads <= int64_t(1) << 34, "more rows than one call takes");
+        at::Tensor out = output(a[3], like);
+        // Rows are read before they are written, so a part may be written over, but not by its neighbours.
+        const char* begin = static_cast<const char*>(out.data_ptr());
+        for (Py_ssize_t i = 0; i < count && a[3] != Py_None && tokens > 0; ++i) {
+            const char* from = static_cast<const char*>(parts[i].out);
+            const int64_t span = ((tokens - 1) * parts[i].out_stride[0] + (heads - 1) * parts[i].out_stride[1] + kDim) * 2;
+            const bool same = from == begin && (heads == 1 || parts[i].out_stride[1] == kDim) &&
+                              (tokens == 1 || parts[i].out_stride[0] == heads * kDim);
+            need(same || from + span <= begin || begin + out.nbytes() <= from, "out overlaps a part");
+            const char* sums = reinterpret_cast<const char*>(parts[i].lse);
+            const int64_t end = ((tokens - 1) * parts[i].lse_stride[0] + (heads - 1) * parts[i].lse_stride[1] + 1) * 4;
+            need(sums + end <= begin || begin + out.nbytes() <= sums, "out overlaps a part");
+        }
+        at::Tensor lse = at::empty({tokens, heads}, like.options().dtype(at::kFloat));
+        if (secure_infer_attend_join(parts, static_cast<uint32_t>(count), static_cast<uint32_t>(tokens),
+                                     static_cast<uint32_t>(heads),
+                                     type == at::kHalf ? SECURE_INFER_FP16 : SECURE_INFER_BF16, out.data_ptr(),
+                                     static_cast<float*>(lse.data_ptr()), address<void>(a[4])) != 0)
+            return failed("secure_infer_attend_join");
+        return pair(std::move(out), std::move(lse));
     });
 }
 
@@ -351,6 +434,28 @@ PyObject* free_sequences(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// trim(..., seqs, window, sinks, ...)
+PyObject* trim(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    if (!counted(n, 10)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const int64_t pages = PyLong_AsLongLong(a[3]), device = PyLong_AsLongLong(a[4]);
+        const int64_t window = PyLong_AsLongLong(a[6]), sinks = PyLong_AsLongLong(a[7]);
+        if (PyErr_Occurred()) return nullptr;
+        need(window > 0 && window < int64_t(1) << 31, "window must be positive");
+        need(sinks >= 0 && sinks < (int64_t(1) << 31) - 256, "sinks must be zero or positive");
+        const Tables in = tables(a, pages, device), out = outputs(a[9], in, pages, device);
+        const at::Tensor& seqs = tensor(a[5], "seqs");
+        const int32_t* named = ints(seqs, 1, device, kRequests);
+        const uint32_t asked = requests(seqs, seqs);
+        at::Tensor scratch = scratch_of(in, asked);
+        if (secure_infer_trim(&in.c, &out.c, named, asked, static_cast<uint32_t>(window), static_cast<uint32_t>(sinks),
+                              scratch.data_ptr(), address<void>(a[8])) != 0)
+            return failed("secure_infer_trim");
+        return results({out.table, out.lens, out.refs});
+    });
+}
+
 // compact(..., tensors, count, page bytes, ...)
 PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
@@ -379,6 +484,8 @@ PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void 
 PyMethodDef methods[] = {
     {"attend", fast<attend>(), METH_FASTCALL, nullptr},
     {"append", fast<append>(), METH_FASTCALL, nullptr},
+    {"join", fast<join>(), METH_FASTCALL, nullptr},
+    {"trim", fast<trim>(), METH_FASTCALL, nullptr},
     {"fork", fast<fork_sequences>(), METH_FASTCALL, nullptr},
     {"reserve", fast<reserve>(), METH_FASTCALL, nullptr},
     {"free", fast<free_sequences>(), METH_FASTCALL, nullptr},

@@ -3,14 +3,17 @@
 * ``append``  -- rotary positions (one or several axes) of a step's new queries
   and keys, and the new keys' and values' way into their pages;
 * ``attend``  -- attention of the new tokens over the pages, from single tokens
-  to long chunks, ragged over sequences;
-* ``CachePages`` -- copies, forks, reserves, frees and compacts pages of all
-  layers.
+  to long chunks, ragged over sequences; behind a sliding window the first tokens
+  may stay visible, and the prefix that sequences share (``SharedPrefix``) is
+  attended once for all of them;
+* ``join``    -- attention over parts of the keys made into attention over all;
+* ``CachePages`` -- copies, forks, reserves, trims, frees and compacts pages of
+  all layers.
 
 A layer's cache is K and V of ``[pages, 128, KV heads, 128]`` in bf16 or fp16,
 as ``NativeTransfer`` and ``LayerwiseReloader`` fill it.  Handles
-(``LayerPages``, ``CachePages``, ``Rotary``) are made once, a ``Chunk`` once per
-step for all its layers.  Calls run on the current stream and return without
+(``LayerPages``, ``CachePages``, ``Rotary``) are made once, a ``Chunk`` and a
+``SharedPrefix`` once per step for all its layers.  Calls run on the current stream and return without
 waiting; lengths, tables and page ids stay on the device (those given as lists are
 copied there first, which does wait).  Bad arguments raise ``ValueError`` before
 anything is launched, a refused launch ``RuntimeError``.  Outputs carry no gradient.
@@ -122,6 +125,41 @@ class Chunk:
         self._address = ct.addressof(self._c)
 
 
+class SharedPrefix:
+    """What groups of a chunk's sequences have in common, as ``fork`` leaves
+    them: ``attend`` with it reads those pages once for all rows of a group.
+
+    ``cu_seqs`` int32 ``[groups + 1]``: group ``g`` is the sequences ``cu_seqs[g]
+    .. cu_seqs[g + 1] - 1``; by default all sequences are one group.  Common are
+    the pages from the first on that the block table names in the same places for
+    every sequence of the group that has new tokens, as far as they lie before
+    the new tokens of each.  ``tokens`` int32 ``[seqs]``: how many tokens of each
+    sequence that is, 0 for those of no group or of a group that shares nothing.
+
+    Found on the device, on the current stream, from what the chunk's tensors
+    hold at that time.  ``update`` finds it again where they have changed, as a
+    captured graph does that holds this call."""
+
+    def __init__(self, chunk: Chunk, cu_seqs: torch.Tensor | None = None):
+        _need(isinstance(chunk, Chunk), "chunk must be a Chunk")
+        seqs = chunk._c.seqs
+        if cu_seqs is not None:
+            cu_seqs = _ints(cu_seqs, "cu_seqs", chunk.device, 1)
+            _need(2 <= cu_seqs.shape[0] <= seqs + 1, "cu_seqs needs groups + 1 entries, of one group at least and one for each "
+                  "sequence at most")
+        self.chunk, self.cu_seqs, self.device = chunk, cu_seqs, chunk.device
+        self.groups = 1 if cu_seqs is None else cu_seqs.shape[0] - 1
+        self._plan = torch.empty(_native.lib().secure_infer_shared_prefix_ints(seqs, self.groups), dtype=torch.int32,
+                                 device=chunk.device)
+        self.tokens = self._plan[:seqs]
+        self.update()
+
+    def update(self) -> None:
+        _call("secure_infer_shared_prefix", self.device, self.chunk._address,
+              None if self.cu_seqs is None else self.cu_seqs.data_ptr(), self.groups, self._plan.data_ptr(),
+              _raw_stream(self.device.index))
+
+
 class Rotary:
     """Rotary positions of 128-value heads: pair ``i`` turns by ``position *
     base ** (-i / 64)`` radians.  ``sections``: how many of the 64 pairs, in
@@ -212,14 +250,17 @@ def _workspace(index: int, stream: int) -> torch.Tensor:
 
 
 def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | None = None, causal: bool = True,
-           window: int = 0, return_lse: bool = False, out: torch.Tensor | None = None,
-           workspace: torch.Tensor | None = None):
+           window: int = 0, sinks: int = 0, shared: SharedPrefix | None = None, return_lse: bool = False,
+           out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """Attention of the chunk's queries ``[tokens, q heads, 128]`` over the
     pages: query head ``h`` reads KV head ``h // (q heads / KV heads)``.
 
     ``scale``: of the scores, 128 ** -0.5 by default.  ``causal``: the token at
     position ``p`` sees keys ``0 .. p``, with ``window`` only the last
-    ``window`` of them; otherwise all of its sequence.  Returns ``[tokens,
+    ``window`` of them and, behind these, the sequence's first ``sinks``;
+    otherwise all of its sequence.  ``shared``, of this chunk and without a
+    window: what its groups have in common is attended once for all of a group's
+    rows, which gives the same up to the order of sums.  Returns ``[tokens,
     q heads, 128]``, and with ``return_lse`` the natural logarithms of the
     softmax sums, float32 ``[tokens, q heads]``, to join it with attention over
     other keys.  A row that sees no key gives 0 and -inf; rows of tokens past
@@ -230,9 +271,28 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
         raise ValueError("the chunk and the cache are on different devices")
     index = pages.index
     stream = _raw_stream(index)
+    more = ()
+    if sinks or shared is not None:
+        if shared is not None and shared.chunk is not chunk:
+            raise ValueError("the shared prefix is another chunk's")
+        more = (sinks, None, 0) if shared is None else (sinks, shared._plan, shared.groups)
     return _on(index, _native.paged_ops().attend, pages._address, chunk._address, index, q, out, return_lse,
                HEAD_DIM ** -0.5 if scale is None else scale, causal, window,
-               _workspace(index, stream) if workspace is None else workspace, stream)
+               _workspace(index, stream) if workspace is None else workspace, stream, *more)
+
+
+def join(outs, lses, *, out: torch.Tensor | None = None):
+    """Attention over all keys from attention over sets of them that have none
+    in common: up to eight ``outs`` ``[tokens, heads, 128]`` of one type and their
+    ``lses`` float32 ``[tokens, heads]``, as ``attend`` returns them with
+    ``return_lse``.  Returns ``out`` (given: it may be one of ``outs``) and the
+    logarithms of all sums.  A part whose logarithm is -inf counts for nothing,
+    whatever it holds; a row that sees no key of any gives 0 and -inf."""
+    outs, lses = tuple(outs), tuple(lses)
+    if not outs or not isinstance(outs[0], torch.Tensor) or not outs[0].is_cuda:
+        raise ValueError("outs must be tensors on a CUDA device")
+    index = outs[0].device.index
+    return _on(index, _native.paged_ops().join, outs, lses, index, out, _raw_stream(index))
 
 
 def attend_status(workspace: torch.Tensor | None = None) -> int:
@@ -261,7 +321,8 @@ class _Tables(NamedTuple):
 class PageTables(_Tables):
     """Who holds which page: ``block_table`` int32 ``[seqs, width]``, ``lens``
     int32 ``[seqs]`` tokens held, ``refs`` int32 ``[pages]`` rows that hold a
-    page (0: free).  A sequence of n tokens holds ``ceil(n / 128)`` pages."""
+    page (0: free).  A sequence of n tokens holds ``ceil(n / 128)`` pages, less
+    those that ``trim`` took, whose entries are -1."""
 
 
 class CachePages:
@@ -341,6 +402,14 @@ class CachePages:
         """Empty the sequences ``seqs``; a page that no other row holds becomes
         free.  Returns the new tables."""
         return self._run("free", tables, out, _ints(seqs, "seqs", self.device, 1))[0]
+
+    def trim(self, tables: PageTables, seqs, window: int, sinks: int = 0, out: PageTables | None = None) -> PageTables:
+        """Give back the pages of the sequences ``seqs`` that no later token sees
+        when it is attended with ``window`` and ``sinks``: those behind the first
+        ``sinks`` tokens that lie wholly before the window of the token at
+        position ``lens`` (so tokens up to ``lens`` have been attended).  Lengths
+        stay.  Returns the new tables."""
+        return self._run("trim", tables, out, _ints(seqs, "seqs", self.device, 1), window, sinks)[0]
 
     def compact(self, tables: PageTables, out: PageTables | None = None):
         """Move the used pages to the lowest places, in every layer: with
