@@ -1182,8 +1182,11 @@ std::shared_ptr<Prepared> take_prepared(uint32_t layer, const void* const* srcs,
                                         const secure_infer_codec* codec)
 {
     std::unique_lock<std::mutex> lock(g_prep.mu);
-    if (g_prep.entries.empty()) return nullptr;
+    // An entry that was being encrypted when its scope was invalidated is still here, and announces nothing any more.
     const uint64_t gen = g_generation.load();
+    if (std::none_of(g_prep.entries.begin(), g_prep.entries.end(),
+                     [gen](const std::shared_ptr<Prepared>& e) { return e->generation == gen; }))
+        return nullptr;
     auto it = std::find_if(g_prep.entries.begin(), g_prep.entries.end(), [&](const std::shared_ptr<Prepared>& e) {
         return e->layer == layer && e->count == count && e->srcs.size() == n && e->generation == gen &&
                same_codec(*e, codec) && std::equal(e->srcs.begin(), e->srcs.end(), srcs);
