@@ -102,23 +102,25 @@ int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infe
  *
  * plan, from secure_infer_shared_prefix of this chunk: groups of sequences attend
  * the pages that they have in common once for all of their rows, which gives what
- * the call without it gives, up to the order of sums.  Not with a window.  parts:
- * secure_infer_attend_parts() bytes, 16-byte aligned, for this call alone; may
- * be null where there is no token.  options may be null. */
+ * the call without it gives, up to the order of sums.  Not with a window.  It is
+ * done where it saves time, which is judged on the host by the sizes alone:
+ * max_common says that no group has more tokens in common (0: as many as the
+ * table holds).  parts: secure_infer_attend_parts() bytes, 16-byte aligned, for
+ * this call alone; null where that is 0.  options may be null. */
 typedef struct {
     const int32_t* plan;
     float* parts;
     uint32_t groups;
+    uint32_t max_common;
     uint32_t sinks;
+    uint32_t reserved;
 } secure_infer_attend_options;
 int secure_infer_attend(const secure_infer_pages* pages, const secure_infer_chunk* chunk, const void* q,
                         int64_t q_token_stride, int64_t q_head_stride, uint32_t q_heads, void* out, float* lse,
                         float scale, uint32_t causal, uint32_t window, const secure_infer_attend_options* options,
                         void* workspace, void* stream);
-uint64_t secure_infer_attend_parts(uint32_t tokens, uint32_t q_heads);
-/* secure_infer_attend_fits of a call with a plan for so many groups. */
-int secure_infer_attend_fits_shared(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads,
-                                    uint32_t groups);
+uint64_t secure_infer_attend_parts(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads,
+                                   const secure_infer_attend_options* options);
 
 /* What the sequences of a chunk have in common.  Group g is the sequences
  * [cu_seqs[g], cu_seqs[g+1]), 1 <= groups <= seqs; cu_seqs may be null for one

@@ -128,7 +128,7 @@ class PageTensor(ct.Structure):
 
 class AttendOptions(ct.Structure):
     """secure_infer_attend_options (include/secure_infer_paged.h)."""
-    _fields_ = [("plan", P), ("parts", P), ("groups", U32), ("sinks", U32)]
+    _fields_ = [("plan", P), ("parts", P), ("groups", U32), ("max_common", U32), ("sinks", U32), ("reserved", U32)]
 
 
 class AttendPart(ct.Structure):
@@ -153,8 +153,7 @@ HOST_SIGNATURES["secure_infer_capture_id"] = ([P], U64)
 HOST_SIGNATURES["secure_infer_attend_fits"] = ([P, P, U32], I32)
 HOST_SIGNATURES["secure_infer_attend_status"] = ([P, P, P], I32)
 HOST_SIGNATURES["secure_infer_attend"] = ([P, P, P, I64, I64, U32, P, P, ct.c_float, U32, U32, P, P, P], I32)
-HOST_SIGNATURES["secure_infer_attend_parts"] = ([U32, U32], U64)
-HOST_SIGNATURES["secure_infer_attend_fits_shared"] = ([P, P, U32, U32], I32)
+HOST_SIGNATURES["secure_infer_attend_parts"] = ([P, P, U32, P], U64)
 HOST_SIGNATURES["secure_infer_attend_join"] = ([P, U32, U32, U32, U32, P, P, P], I32)
 HOST_SIGNATURES["secure_infer_shared_prefix_ints"] = ([U32, U32], U64)
 HOST_SIGNATURES["secure_infer_shared_prefix"] = ([P, P, U32, P, P], I32)

@@ -127,6 +127,34 @@ Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, u
     return w;
 }
 
+// Whether a call attends what its groups have in common for all their rows at
+// once, by what that saves if the common pages are `pages`, all that the table or
+// the caller says they may be.  A page takes an SM 4 units of time (1.1 us) for
+// eight rows in the kernel for few rows, as long for 128 rows in tiles and 7 for
+// 256.  It costs the joining of the parts (0.17 units a row) and, in a call that has
+// no tiles otherwise, the tiles' kernel and its own join.
+constexpr int64_t kShareCost = 1500, kShareTilesCost = 13000;
+int64_t page_time(uint64_t rows)
+{
+    return static_cast<int64_t>(rows <= kFewRows ? 4 * ((rows + 7) / 8) : rows <= 128 ? 4 : 7 * ((rows + 255) / 256));
+}
+// -> the groups that the call's options name, or 0.
+uint32_t shared_groups(const secure_infer_pages& pages, const secure_infer_chunk& chunk, uint32_t q_heads,
+                       const secure_infer_attend_options* options)
+{
+    if (options == nullptr || options->plan == nullptr || chunk.tokens == 0 || options->groups == 0) return 0;
+    const uint32_t groups = options->groups, most = static_cast<uint32_t>((uint64_t(options->max_common) + kPage - 1) / kPage);
+    const uint32_t common = most == 0 || most > chunk.table_width ? chunk.table_width : most;
+    const uint64_t group = q_heads / pages.heads, tokens = chunk.tokens, seqs = chunk.seqs < tokens ? chunk.seqs : tokens;
+    const int64_t apart = static_cast<int64_t>(seqs) * page_time((tokens + seqs - 1) / seqs * group);
+    const int64_t together = groups * page_time((tokens + groups - 1) / groups * group);
+    const uint64_t largest = (chunk.max_q == 0 || chunk.max_q > tokens ? tokens : chunk.max_q) * group;
+    const int64_t cost = largest > kFewRows || group > 128 ? kShareCost : kShareTilesCost;
+    const double saved = static_cast<double>(apart - together) * common * pages.heads;
+    const bool worth = saved > static_cast<double>(cost) + static_cast<double>(tokens * q_heads) / 6;
+    return worth && work_of(pages, chunk, q_heads, groups).fits() ? groups : 0;
+}
+
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)
 {
     return in != nullptr && out != nullptr && in->block_table != nullptr && in->lens != nullptr && in->refs != nullptr &&
@@ -176,24 +204,24 @@ SI_EXPORT int secure_infer_attend_status(void* workspace, uint32_t* status, void
     return word == 0 || cudaMemsetAsync(workspace, 0, SECURE_INFER_ATTEND_STATE_BYTES, st) == cudaSuccess ? 0 : -1;
 }
 
+static bool call_ok(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads)
+{
+    return pages_ok(pages) && chunk_ok(chunk) && q_heads > 0 && q_heads <= (1u << 16) && q_heads % pages->heads == 0;
+}
+
 SI_EXPORT int secure_infer_attend_fits(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads)
 {
-    return secure_infer_attend_fits_shared(pages, chunk, q_heads, 0);
+    return call_ok(pages, chunk, q_heads) && work_of(*pages, *chunk, q_heads).fits();
 }
 
-SI_EXPORT int secure_infer_attend_fits_shared(const secure_infer_pages* pages, const secure_infer_chunk* chunk,
-                                              uint32_t q_heads, uint32_t groups)
+SI_EXPORT uint64_t secure_infer_attend_parts(const secure_infer_pages* pages, const secure_infer_chunk* chunk,
+                                             uint32_t q_heads, const secure_infer_attend_options* options)
 {
-    return pages_ok(pages) && chunk_ok(chunk) && q_heads > 0 && q_heads <= (1u << 16) && q_heads % pages->heads == 0 &&
-           groups <= chunk->seqs && work_of(*pages, *chunk, q_heads, groups).fits();
+    if (!call_ok(pages, chunk, q_heads) || shared_groups(*pages, *chunk, q_heads, options) == 0) return 0;
+    return static_cast<uint64_t>(chunk->tokens) * q_heads * 2 * (kDim + 2) * sizeof(float);
 }
 
-SI_EXPORT uint64_t secure_infer_attend_parts(uint32_t tokens, uint32_t q_heads)
-{
-    return static_cast<uint64_t>(tokens) * q_heads * 2 * (kDim + 2) * sizeof(float);
-}
-
-// The sequences' prefixes, then the groups, which are read 16 bytes at a time.
+// The sequences' common tokens, then the groups, which are read 16 bytes at a time.
 static uint64_t group_offset(uint32_t seqs) { return (static_cast<uint64_t>(seqs) + 3) / 4 * 4; }
 
 SI_EXPORT uint64_t secure_infer_shared_prefix_ints(uint32_t seqs, uint32_t groups)
@@ -252,15 +280,14 @@ SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_
                                   const secure_infer_attend_options* options, void* workspace, void* stream)
 {
     const uint32_t sinks = options != nullptr ? options->sinks : 0;
-    const uint32_t groups = options != nullptr && options->plan != nullptr ? options->groups : 0;
-    if (!pages_ok(pages) || !chunk_ok(chunk) || q_heads == 0 || q_heads > (1u << 16) ||
-        q_heads % pages->heads != 0 || (window != 0 && !causal) || window > INT_MAX || workspace == nullptr ||
+    if (!call_ok(pages, chunk, q_heads) || (window != 0 && !causal) || window > INT_MAX || workspace == nullptr ||
         (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || sinks > INT_MAX || (sinks != 0 && window == 0))
         return -1;
     if (options != nullptr && options->plan != nullptr &&
-        (!aligned16(options->plan) || groups == 0 || groups > chunk->seqs || window != 0))
+        (!aligned16(options->plan) || options->groups == 0 || options->groups > chunk->seqs || window != 0))
         return -1;
     if (chunk->tokens == 0) return 0;
+    const uint32_t groups = shared_groups(*pages, *chunk, q_heads, options);
     if (!aligned16(q) || !aligned16(out) || !stride_ok(q_token_stride) || !stride_ok(q_head_stride) ||
         (groups > 0 && !aligned16(options->parts)))
         return -1;

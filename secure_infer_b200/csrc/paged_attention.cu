@@ -95,12 +95,19 @@ constexpr int kJoinRows = 160;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowSlot = kRows * (kDim + 2);
 
-constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
+// Pages that a pair of tiles' beginning and end are worth.  Measured: 8.6 us, where a page takes 2.0; the usual call keeps
+// the 2 that its results' order of sums goes by.
+template <int M>
+constexpr int kTilesCost = M == kPlain ? 2 : 4;
 
 // An SM takes 1.1 us of a page for few rows where fewer than 120 of 148 SMs read (58 GB/s each; 120 to 130 get nearly
 // all that memory gives), and 1.95 us of a page for a pair of tiles.
 __device__ __forceinline__ Kind rows_kind() { return {kRows, kRowsCost, kRowsWhole, 4, 14}; }
-__device__ __forceinline__ Kind tiles_kind(const AttendParams& p) { return {2 * (128 / p.group * p.group), kTilesCost, 0, 7, 16}; }
+template <int M>
+__device__ __forceinline__ Kind tiles_kind(const AttendParams& p)
+{
+    return {2 * (128 / p.group * p.group), kTilesCost<M>, 0, 7, 16};
+}
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -191,7 +198,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     wait_for_earlier_kernels();
-    find_share<kRowsThreads, M>(p, rows_kind(), tiles_kind(p), &share, warp_sums);
+    find_share<kRowsThreads, M>(p, rows_kind(), tiles_kind<M>(p), &share, warp_sums);
     dependents_may_launch();
     Walk<M> w = start_walk<M>(p, kRows, kRowsCost, share);
 
@@ -725,7 +732,7 @@ __device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& shar
 {
     const int tid = threadIdx.x, cta = blockIdx.x;
     if (tid == 0) atomicOr(p.status, 1u);
-    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), kTilesCost, share);
+    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), kTilesCost<M>, share);
     for (bool first = true; w.left > 0; first = false) {
         const int pages = w.take();
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
@@ -797,11 +804,11 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     // read them, the two share no memory that either writes, and it waits for that one at its end instead.
     if (!p.both) wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads, M>(p, tiles_kind(p), rows_kind(), &c.share, c.warp_sums);
+    find_share<kTileThreads, M>(p, tiles_kind<M>(p), rows_kind(), &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
-    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, kTilesCost, c.share);
+    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, kTilesCost<M>, c.share);
     const bool any = w.left > 0 && c.share.down == 0;
 
     // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.

@@ -11,6 +11,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 
+#include <algorithm>
 #include <string>
 
 #include "../../include/secure_infer_paged.h"
@@ -117,10 +118,10 @@ PyObject* pair(at::Tensor a, at::Tensor b)
 }
 
 // attend(pages, chunk, device, q, out, return_lse, scale, causal, window, workspace, stream), and perhaps (sinks, plan
-// of a shared prefix or None, its groups)
+// of a shared prefix or None, its groups, most tokens in common)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    if (n != 11 && !counted(n, 14)) return nullptr;
+    if (n != 11 && !counted(n, 15)) return nullptr;
     return guarded([&]() -> PyObject* {
         const auto* pages = address<const secure_infer_pages>(a[0]);
         secure_infer_chunk chunk = *address<const secure_infer_chunk>(a[1]);
@@ -138,7 +139,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
         secure_infer_attend_options options{};
         at::Tensor parts;
         if (n > 11) {
-            const int64_t sinks = PyLong_AsLongLong(a[11]), groups = PyLong_AsLongLong(a[13]);
+            const int64_t sinks = PyLong_AsLongLong(a[11]), groups = PyLong_AsLongLong(a[13]), most = PyLong_AsLongLong(a[14]);
             if (PyErr_Occurred()) return nullptr;
             need(sinks >= 0 && sinks < int64_t(1) << 31 && (sinks == 0 || window > 0),
                  "sinks must be zero or positive, and go with a window");
@@ -148,6 +149,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
                 need(groups > 0 && groups <= chunk.seqs, "a shared prefix has one group for each sequence at most");
                 const at::Tensor& plan = tensor(a[12], "the shared prefix's plan");
                 options.groups = static_cast<uint32_t>(groups);
+                options.max_common = static_cast<uint32_t>(std::min<int64_t>(std::max<int64_t>(most, 0), UINT32_MAX));
                 options.plan = ints(plan, 1, device, "the shared prefix must be on the cache's device");
                 need(static_cast<uint64_t>(plan.numel()) >= secure_infer_shared_prefix_ints(chunk.seqs, options.groups) &&
                          aligned(plan), "the shared prefix is another chunk's");
@@ -164,11 +166,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
                  "workspace must come from attend_workspace of the cache's device");
             need(tokens <= UINT32_MAX, "too many tokens");
             chunk.tokens = static_cast<uint32_t>(tokens);
-            const char* most = "more work than one call takes: fewer tokens, or a narrower block table";
-            if (options.groups > 0) {
-                // Memory for partial results only for what will be launched.
-                need(secure_infer_attend_fits_shared(pages, &chunk, static_cast<uint32_t>(r.heads), options.groups), most);
-                const uint64_t bytes = secure_infer_attend_parts(chunk.tokens, static_cast<uint32_t>(r.heads));
+            if (const uint64_t bytes = options.groups > 0 ? secure_infer_attend_parts(pages, &chunk, r.heads, &options) : 0; bytes > 0) {
                 parts = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
                 options.parts = static_cast<float*>(parts.data_ptr());
             }
@@ -176,7 +174,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
                                     want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, static_cast<float>(scale),
                                     causal, static_cast<uint32_t>(window), &options, workspace.data_ptr(),
                                     address<void>(a[10])) != 0) {
-                need(secure_infer_attend_fits(pages, &chunk, static_cast<uint32_t>(r.heads)), most);
+                need(secure_infer_attend_fits(pages, &chunk, static_cast<uint32_t>(r.heads)),
+                     "more work than one call takes: fewer tokens, or a narrower block table");
                 return failed("secure_infer_attend");
             }
         }

@@ -138,16 +138,23 @@ class SharedPrefix:
 
     Found on the device, on the current stream, from what the chunk's tensors
     hold at that time.  ``update`` finds it again where they have changed, as a
-    captured graph does that holds this call."""
+    captured graph does that holds this call.
 
-    def __init__(self, chunk: Chunk, cu_seqs: torch.Tensor | None = None):
+    Whether ``attend`` goes by it is a matter of time, and judged on the host by
+    the numbers of sequences, groups, tokens and heads, and by ``max_common``: no
+    group has more tokens in common (by default as many as the block table is wide
+    for; given, it keeps short prefixes in wide tables from costing more than they
+    save)."""
+
+    def __init__(self, chunk: Chunk, cu_seqs: torch.Tensor | None = None, max_common: int | None = None):
         _need(isinstance(chunk, Chunk), "chunk must be a Chunk")
         seqs = chunk._c.seqs
         if cu_seqs is not None:
             cu_seqs = _ints(cu_seqs, "cu_seqs", chunk.device, 1)
             _need(2 <= cu_seqs.shape[0] <= seqs + 1, "cu_seqs needs groups + 1 entries, of one group at least and one for each "
                   "sequence at most")
-        self.chunk, self.cu_seqs, self.device = chunk, cu_seqs, chunk.device
+        _need(max_common is None or max_common > 0, "max_common must be positive")
+        self.chunk, self.cu_seqs, self.device, self.max_common = chunk, cu_seqs, chunk.device, max_common or 0
         self.groups = 1 if cu_seqs is None else cu_seqs.shape[0] - 1
         self._plan = torch.empty(_native.lib().secure_infer_shared_prefix_ints(seqs, self.groups), dtype=torch.int32,
                                  device=chunk.device)
@@ -275,7 +282,7 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
     if sinks or shared is not None:
         if shared is not None and shared.chunk is not chunk:
             raise ValueError("the shared prefix is another chunk's")
-        more = (sinks, None, 0) if shared is None else (sinks, shared._plan, shared.groups)
+        more = (sinks, None, 0, 0) if shared is None else (sinks, shared._plan, shared.groups, shared.max_common)
     return _on(index, _native.paged_ops().attend, pages._address, chunk._address, index, q, out, return_lse,
                HEAD_DIM ** -0.5 if scale is None else scale, causal, window,
                _workspace(index, stream) if workspace is None else workspace, stream, *more)

@@ -29,7 +29,7 @@ def good():
 def test_every_declaration_is_exported_and_bound(lib):
     text = (ROOT / "include" / "secure_infer_paged.h").read_text()
     names = set(re.findall(r"^(?:int|uint64_t) (secure_infer_\w+)\(", text, re.M))
-    assert {"secure_infer_attend", "secure_infer_attend_parts", "secure_infer_attend_join", "secure_infer_attend_fits_shared",
+    assert {"secure_infer_attend", "secure_infer_attend_parts", "secure_infer_attend_join",
             "secure_infer_shared_prefix", "secure_infer_shared_prefix_ints", "secure_infer_trim"} <= names
     assert names <= set(_native.HOST_SIGNATURES) and all(hasattr(lib, n) for n in names)
 
@@ -42,18 +42,19 @@ def test_structures_match_the_header():
 
 
 @pytest.mark.parametrize("window,causal,options", [
-    (0, 1, (None, None, 0, 4)),           # sinks without a window
-    (8, 0, (None, None, 0, 4)),           # a window without the causal order
-    (8, 1, (None, None, 0, 1 << 31)),
-    (8, 1, (A, A, 1, 0)),                 # a shared prefix with a window
-    (0, 1, (A, A, 0, 0)),                 # no group
-    (0, 1, (A, A, 3, 0)),                 # more groups than sequences
-    (0, 1, (A + 4, A, 1, 0)),
-    (0, 1, (A, None, 1, 0)),
-    (0, 1, (A, A + 8, 1, 0)),
+    (0, 1, (None, None, 0, 0, 4)),        # sinks without a window
+    (8, 0, (None, None, 0, 0, 4)),        # a window without the causal order
+    (8, 1, (None, None, 0, 0, 1 << 31)),
+    (8, 1, (A, A, 1, 0, 0)),              # a shared prefix with a window
+    (0, 1, (A, A, 0, 0, 0)),              # no group
+    (0, 1, (A, A, 65, 0, 0)),             # more groups than sequences
+    (0, 1, (A + 4, A, 1, 0, 0)),
+    (0, 1, (A, None, 1, 0, 0)),
+    (0, 1, (A, A + 8, 1, 0, 0)),
 ])
 def test_attend_refuses(lib, window, causal, options):
     pages, chunk = good()
+    chunk.seqs, chunk.tokens, chunk.table_width, chunk.table_stride = 64, 64, 1000, 1000
     o = _native.AttendOptions(*options)
     assert lib.secure_infer_attend(ct.byref(pages), ct.byref(chunk), A, 4096, 128, 32, A, None, 1.0, causal, window, ct.byref(o),
                                    A, None) == -1
@@ -63,18 +64,28 @@ def test_attend_refuses(lib, window, causal, options):
                                        A, None) == 0
 
 
-def test_units_of_shared_calls(lib):
+def test_what_is_shared_by_its_sizes(lib):
+    """Memory for parts is asked for where the groups' pages are attended together: by what that saves."""
     pages, chunk = good()
 
-    def fits(tokens, max_q, width, seqs, groups, heads=32):
-        chunk.tokens, chunk.max_q, chunk.seqs, chunk.table_width, chunk.table_stride = tokens, max_q, seqs, width, width
-        return lib.secure_infer_attend_fits_shared(ct.byref(pages), ct.byref(chunk), heads, groups)
+    def parts(seqs, q, width, groups=1, heads=32, kv_heads=8, common=0, max_q=None):
+        pages.heads, chunk.tokens, chunk.max_q, chunk.seqs = kv_heads, seqs * q, q if max_q is None else max_q, seqs
+        chunk.table_width = chunk.table_stride = width
+        o = _native.AttendOptions(A, None, groups, common, 0)
+        got = lib.secure_infer_attend_parts(ct.byref(pages), ct.byref(chunk), heads, ct.byref(o))
+        assert got in (0, seqs * q * heads * 2 * 130 * 4)
+        return got > 0
 
-    assert fits(64, 1, 1024, 64, 1) and fits(64, 1, 1024, 64, 64)
-    assert not fits(64, 1, 1024, 64, 65)
-    assert fits(1 << 14, 1, 1 << 10, 1 << 14, 1) and not fits(1 << 17, 1, 1 << 10, 1 << 17, 1)
-    assert not fits(1 << 28, 1, 4, 2, 1, heads=4096)
-    assert lib.secure_infer_attend_parts(1 << 28, 1 << 16) == (1 << 44) * 2 * 130 * 4
+    assert parts(48, 1, 72) and not parts(2, 1, 6) and not parts(8, 1, 6)
+    assert parts(24, 5, 240, 4, 8, 1) and not parts(24, 5, 240, 24, 8, 1)      # groups of one save nothing
+    assert not parts(5, 300, 52, heads=28, kv_heads=4)                          # chunks that fill tiles of their own
+    assert parts(48, 1, 4096) and not parts(48, 1, 4096, common=128) and parts(48, 1, 4096, common=1 << 20)
+    assert not parts(1 << 17, 1, 1 << 12) and parts(1 << 14, 1, 1 << 10)        # units beyond 32 bits: sequence by sequence
+    assert not parts(1, 1, 4096) and not parts(4, 0, 4096)
+    o = _native.AttendOptions(None, None, 0, 0, 4)
+    assert lib.secure_infer_attend_parts(ct.byref(pages), ct.byref(chunk), 32, ct.byref(o)) == 0
+    assert lib.secure_infer_attend_parts(ct.byref(pages), ct.byref(chunk), 32, None) == 0
+    assert lib.secure_infer_attend_parts(None, ct.byref(chunk), 32, ct.byref(o)) == 0
     assert lib.secure_infer_shared_prefix_ints(5, 2) == 8 + 8
 
 
@@ -129,7 +140,7 @@ def test_extension_and_python_refuse():
     with pytest.raises(TypeError):
         ops.attend(p, c, 0, q, None, False, 1.0, True, 0, None, 0, 4)
     with pytest.raises(ValueError):
-        ops.attend(p, c, 0, q, None, False, 1.0, True, 0, None, 0, 4, None, 0)
+        ops.attend(p, c, 0, q, None, False, 1.0, True, 0, None, 0, 4, None, 0, 0)
     lse = torch.zeros((3, 32))
     for bad in (((q, q), (lse,)), ((), ()), ((q,) * 9, (lse,) * 9), ((q, q), (lse, lse)), ((q, 3), (lse, lse)), ([q], [lse])):
         with pytest.raises(ValueError):

@@ -215,6 +215,16 @@ def test_rows_whose_sinks_are_minus_infinity(paged):
 
 # ------------------------------------------------------------ shared prefixes
 
+def together(pages, chunk, q, shared):
+    """Whether a call attends what groups have in common together."""
+    from secure_infer_b200 import _native
+    ct = _native.ct
+    c = _native.Chunk.from_buffer_copy(chunk._c)
+    c.tokens = q.shape[0]
+    o = _native.AttendOptions(shared._plan.data_ptr(), None, shared.groups, shared.max_common)
+    return _native.lib().secure_infer_attend_parts(pages._address, ct.addressof(c), q.shape[1], ct.addressof(o)) > 0
+
+
 class Family(Seen):
     """Groups of sequences whose first pages are the same.  groups: (sequences, pages in common)."""
 
@@ -229,7 +239,10 @@ class Family(Seen):
                     x[:128 * pages] = y[:128 * pages]
             s0 += n
             self.bounds.append(s0)
-        self.chunk.block_table.copy_(self.table)
+        # In a wide table groups are attended together however small they are.
+        table = torch.full((len(lens), 1 << 16), -1, dtype=torch.int32, device="cuda")
+        table[:, :self.table.shape[1]] = self.table.cuda()
+        self.chunk = paged.Chunk(table, self.chunk.cu_q, self.chunk.kv_lens, max_q=max(n for n, _ in lens))
         self.shared = paged.SharedPrefix(self.chunk, ints(self.bounds))
 
     def tokens(self):
@@ -245,8 +258,16 @@ class Family(Seen):
                 common[s] = 128 * next((i for i in range(most) if not same[i]), most)
         return common
 
+    def saves(self):
+        """Whether rows of a page are fewer tiles together than apart."""
+        time = lambda rows: 4 * -(-rows // 8) if rows <= 24 else 4 if rows <= 128 else 7 * -(-rows // 256)  # noqa: E731
+        tokens, groups = self.cu[-1], self.shared.groups
+        seqs = min(len(self.lens), tokens)
+        return seqs * time(-(-tokens // seqs) * self.group) > groups * time(-(-tokens // groups) * self.group)
+
     def run(self, paged, **kw):
         assert self.shared.tokens.tolist() == self.tokens()
+        assert together(self.pages, self.chunk, self.q, self.shared) or not self.saves()
         return paged.attend(self.pages, self.chunk, self.q, shared=self.shared, return_lse=True, **kw)
 
 
@@ -319,6 +340,8 @@ def test_groups_of_many_sequences(paged, seqs):
 def test_long_prefixes_repeat(paged, lens, groups, heads):
     """Prefixes and own keys that are cut over many CTAs: the same bits whoever finishes last."""
     c = Family(paged, lens, groups, heads, 1)
+    out, lse = paged.attend(c.pages, c.chunk, c.q, shared=c.shared, return_lse=True)
+    c.check(out, lse)
     out, lse = c.run(paged)
     c.check(out, lse)
     for _ in range(10):
@@ -358,6 +381,22 @@ def test_scores_of_minus_infinity_in_a_shared_prefix(paged):
         assert torch.isnan(out[:n, :2]).all() and torch.isfinite(out[n:]).all() and torch.isfinite(out[:, 2:]).all()
 
 
+@pytest.mark.parametrize("lens,groups,shares", [([(1, 5200 + 9 * i) for i in range(30)], [(30, 40)], True),
+                                                ([(5, 9000)] * 8 + [(5, 9100)] * 8, [(8, 70), (8, 70)], True),
+                                                ([(1, 300), (1, 310)], [(2, 2)], False), ([(300, 900), (280, 900)], [(2, 4)], False)])
+def test_sharing_where_it_saves_time(paged, lens, groups, shares):
+    """Narrow tables, and wide ones with a bound on what is common, leave the choice to the sizes."""
+    c = Family(paged, lens, groups, 32, 8, seed=8)
+    narrow = paged.Chunk(c.chunk.block_table[:, :c.table.shape[1]], c.chunk.cu_q, c.chunk.kv_lens, max_q=c.chunk._c.max_q)
+    for chunk, most in ((narrow, None), (c.chunk, 128 * max(n for _, n in groups))):
+        shared = paged.SharedPrefix(chunk, ints(c.bounds), max_common=most)
+        assert shared.tokens.tolist() == c.tokens() and together(c.pages, chunk, c.q, shared) == shares
+        out, lse = paged.attend(c.pages, chunk, c.q, shared=shared, return_lse=True)
+        c.check(out, lse)
+        if not shares:
+            assert torch.equal(out, paged.attend(c.pages, chunk, c.q))
+
+
 def test_tokens_of_nobody_stay_with_a_shared_prefix(paged):
     c = Family(paged, [(1, 300), (1, 290), (40, 400)], [(3, 2)], 8, 2)
     q = torch.cat((c.q, torch.full((9, 8, 128), math.nan, dtype=c.dtype, device="cuda")))
@@ -381,7 +420,7 @@ def test_plans_follow_the_chunk_in_a_graph(paged):
         if step == 2:   # another table: one page is common
             c.table[2, 1:4] = c.table[1, 1:4] = c.table[0, 1:4]
             c.table[2, 1] = c.table[2, 4]
-            c.chunk.block_table.copy_(c.table)
+            c.chunk.block_table[:, :c.table.shape[1]].copy_(c.table)
             for which, cache in enumerate((c.k, c.v)):
                 for i in range(4):
                     c.rows[2][which][128 * i:128 * (i + 1)] = cache[c.table[2, i].item()]
@@ -653,6 +692,7 @@ def test_refusals(paged):
         lambda: attend(shared=c.shared, window=8, sinks=2),
         lambda: paged.attend(c.pages, other, c.q, shared=c.shared),
         lambda: paged.SharedPrefix(c.chunk, ints([0])),
+        lambda: paged.SharedPrefix(c.chunk, max_common=0),
         lambda: paged.SharedPrefix(c.chunk, ints([0, 1, 2, 2])),
         lambda: paged.SharedPrefix(c.chunk, torch.tensor([0, 2], device="cuda")),
         lambda: paged.SharedPrefix(c.chunk, torch.tensor([0, 2], dtype=torch.int32)),
@@ -691,15 +731,19 @@ def test_offsets_past_two_gigabytes(paged):
         pytest.skip("needs 25 GB")
     pages = 20000
     k, v = (torch.zeros((pages, 128, 8, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
-    c = Family(paged, [(1, 500), (130, 500), (2, 500)], [(3, 2)], 32, 8, spare=0)
-    where = {p: q for p, q in zip(sorted(set(c.table[c.table >= 0].tolist())), range(pages - 1, 0, -1211))}
-    table = c.table.clone()
-    for p, q in where.items():
-        k[q], v[q] = c.k[p], c.v[p]
-        table[c.table == p] = q
-    layer, chunk = paged.LayerPages(k, v), paged.Chunk(table.cuda(), c.chunk.cu_q, c.chunk.kv_lens)
-    c.check(paged.attend(layer, chunk, c.q, shared=paged.SharedPrefix(chunk)))
-    c.check(paged.attend(layer, chunk, c.q, window=100, sinks=3), window=100, sinks=3)
+    for lens in ([(1, 500), (130, 500), (2, 500)], [(1, 500), (4, 510), (2, 500)]):
+        c = Family(paged, lens, [(3, 2)], 32, 8, spare=0)
+        where = {p: q for p, q in zip(sorted(set(c.table[c.table >= 0].tolist())), range(pages - 1, 0, -1211))}
+        table = c.chunk.block_table.clone()
+        for p, q in where.items():
+            k[q], v[q] = c.k[p], c.v[p]
+            table[c.chunk.block_table == p] = q
+        layer, chunk = paged.LayerPages(k, v), paged.Chunk(table, c.chunk.cu_q, c.chunk.kv_lens)
+        whole = paged.SharedPrefix(chunk)
+        assert together(layer, chunk, c.q, whole) == c.saves()
+        c.check(paged.attend(layer, chunk, c.q, shared=whole))
+        c.check(paged.attend(layer, chunk, c.q, window=100, sinks=3), window=100, sinks=3)
+    assert c.saves()
     outs = [torch.full((70000, 128, 128), float(i), dtype=torch.bfloat16, device="cuda") for i in range(2)]
     lses = [torch.zeros((70000, 128), device="cuda") for _ in range(2)]
     outs[1][-1, -1] = 3.0
