@@ -337,9 +337,9 @@ __device__ __forceinline__ int seq_count(const AttendParams& p)
     return M == kShared ? p.seqs + p.groups : p.seqs;
 }
 
-// `others`: the sequences of the call's other launch, else of this one.
+// A sequence of either launch.
 template <int M>
-__device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool others = false)
+__device__ __forceinline__ Seq load_any(const AttendParams& p, int s)
 {
     Seq r;
     r.begin = 0;
@@ -352,8 +352,6 @@ __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool other
         r.kv = max(0, min(g.w, p.width * kPage));
         r.n = r.kv > 0 ? max(0, min(g.z, p.tokens - r.q0)) : 0;
         r.part = 0;
-        const int64_t rows = static_cast<int64_t>(r.n) * p.group;
-        if ((rows < p.rows_min || rows > p.rows_max) != others) r.n = 0;
         return r;
     }
     // From L2, as all that may be read before this kernel has waited for the one before it.
@@ -367,8 +365,21 @@ __device__ __forceinline__ Seq load_seq(const AttendParams& p, int s, bool other
         r.begin = max(0, min(__ldcg(p.prefix + s), r.kv));
         r.part = r.begin > 0 ? 1 : -1;
     }
-    const int64_t rows = static_cast<int64_t>(r.n) * p.group;
-    if ((rows < p.rows_min || rows > p.rows_max) != others) r.n = 0;
+    return r;
+}
+
+// Whether this launch takes it.
+__device__ __forceinline__ bool is_mine(const AttendParams& p, const Seq& s)
+{
+    const int64_t rows = static_cast<int64_t>(s.n) * p.group;
+    return rows >= p.rows_min && rows <= p.rows_max;
+}
+
+template <int M>
+__device__ __forceinline__ Seq load_seq(const AttendParams& p, int s)
+{
+    Seq r = load_any<M>(p, s);
+    if (!is_mine(p, r)) r.n = 0;
     return r;
 }
 
@@ -422,6 +433,7 @@ struct Share {
     int32_t begin, units;      // of this CTA
     int32_t seq, seq_unit;     // sequence of its first unit, and that sequence's first unit
     int32_t down;              // the status word when the kernel began
+    int32_t others;            // CTAs of the call's other launch that have one, if that is the one for many rows
     Seq q;
 
     __device__ __forceinline__ int begin_of(int cta) const { return cta * per + min(cta, more); }
@@ -532,6 +544,7 @@ struct Kind {
     int rows_per_tile, cost, whole;
     int time;     // of a unit, in any measure that both kinds share
     int of_16;    // sixteenths of the SMs beyond which it gets no faster
+    int later;    // how much later than the other kind's its first page is there, in the measure of time
 };
 
 // All threads of the block take part; `warp_sums` holds three values per warp.
@@ -542,7 +555,35 @@ struct Kind {
 // launch, so reading pages for few rows goes on beside the products of many: 333
 // tokens after 2167 and 15 single tokens of up to 4000 take 53 us, 62 one kind
 // after the other.
-template <int kThreads, int M>
+// SMs for `units` of a kind beside `others` of the other.
+template <int M>
+__device__ __forceinline__ int sms_of(const Kind& kind, int units, const Kind& other, int others)
+{
+    const int grid = gridDim.x;
+    if (units == 0 || others == 0 || grid == 1) return grid;
+    const float mine = static_cast<float>(units) * kind.time, theirs = static_cast<float>(others) * other.time;
+    if (M == kPlain) {
+        const int most = max(1, grid * kind.of_16 / 16), least = grid - max(1, grid * other.of_16 / 16);
+        return max(max(1, least), min(min(most, grid - 1), __float2int_rn(grid * (mine / (mine + theirs)))));
+    }
+    // Both end together where few / x = many / (grid - x) + later, a quadratic equation.  One count serves both kinds, or a
+    // CTA might have to wait for the other launch's.
+    const bool first = kind.later == 0;
+    const float few = first ? mine : theirs, many = first ? theirs : mine, later = first ? other.later : kind.later;
+    const float b = few + many + later * grid;
+    const float x = 2.0f * few * grid / (b + sqrtf(fmaxf(0.0f, b * b - 4.0f * later * few * grid)));
+    // The whole number on either side with the earlier end.
+    const int most = max(1, min(grid * (first ? kind : other).of_16 / 16, grid - 1)), low = max(1, min(most, __float2int_rd(x)));
+    const int high = min(most, low + 1);
+    const auto end = [&](int r) { return fmaxf(few / r, many / (grid - r) + later); };
+    const int rows = end(high) < end(low) ? high : low;
+    return first ? rows : grid - rows;
+}
+
+// kIdle: the launch before has left in p.status[1] how many CTAs of this one have
+// work.  The others would count it again when the first launch's CTAs leave, at
+// the call's end: 4 us, where there are more CTAs than fit.
+template <int kThreads, int M, bool kIdle>
 __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& kind, const Kind& other, Share* share,
                                            int32_t* warp_sums)
 {
@@ -550,6 +591,11 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seqs = seq_count<M>(p);
     const int down = tid == 0 ? static_cast<int>(__ldcg(p.status)) : 0;
+    bool leave = false;
+    if (kIdle && tid == 0 && p.both) {
+        const uint32_t busy = __ldcg(p.status + 1);
+        leave = busy != 0 && blockIdx.x >= busy;
+    }
     Share r;
     r.begin = r.total = 0;
     // The first pass sums the units, the second finds the sequence that holds this CTA's first; where every sequence
@@ -561,10 +607,22 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
             const int s = s0 + tid;
             Seq q{};
             int own_largest = 0, unused = 0, beside = 0;
-            if (s < seqs) q = load_seq<M>(p, s);
+            if (s < seqs) q = load_any<M>(p, s);
+            if (kIdle && (one || pass == 0) && s0 == 0 && __syncthreads_or(leave)) {
+                // The kernel before has counted both kinds, and leaves this CTA none.
+                if (tid == 0) {
+                    *share = Share{};
+                    share->ctas = 1;
+                    share->seq = -1;
+                    share->down = down;
+                }
+                __syncthreads();
+                return;
+            }
+            Seq o = q;
+            if (is_mine(p, q)) o.n = 0;
+            else q.n = 0;
             if (p.both && (one || pass == 0)) {
-                Seq o{};
-                if (s < seqs) o = load_seq<M>(p, s, true);
                 beside = __reduce_add_sync(0xffffffffu, seq_units<M>(p, o, other.rows_per_tile, other.cost, unused));
             }
             const int own = seq_units<M>(p, q, rows_per_tile, cost, own_largest);
@@ -580,24 +638,18 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
                 warp_sums[2 * kWarps + warp] = beside;
             }
             __syncthreads();
-            int before = base;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const int x = warp_sums[w];
-                if (w < warp) before += x;
-                base += x;
-                largest = max(largest, warp_sums[kWarps + w]);
-                others += warp_sums[2 * kWarps + w];
-            }
+            // A lane per warp.
+            static_assert(kWarps <= 32, "a warp sums the warps");
+            const bool has = lane < kWarps;
+            const int x = has ? warp_sums[lane] : 0;
+            const int before = base + __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+            base += __reduce_add_sync(0xffffffffu, x);
+            largest = max(largest, __reduce_max_sync(0xffffffffu, has ? warp_sums[kWarps + lane] : 0));
+            others += __reduce_add_sync(0xffffffffu, has ? warp_sums[2 * kWarps + lane] : 0);
             if (one || (pass == 0 && s0 + kThreads >= seqs)) {
                 r.total = base;
-                int grid = gridDim.x;
-                if (base > 0 && others > 0 && grid > 1) {
-                    const float mine = static_cast<float>(base) * kind.time, theirs = static_cast<float>(others) * other.time;
-                    const int most = max(1, grid * kind.of_16 / 16), least = grid - max(1, grid * other.of_16 / 16);
-                    grid = max(max(1, least), min(min(most, grid - 1), __float2int_rn(grid * (mine / (mine + theirs)))));
-                }
-                r.ctas = max(1, min(grid, largest <= whole ? base / max(1, largest) : base));
+                r.ctas = max(1, min(sms_of<M>(kind, base, other, others), largest <= whole ? base / max(1, largest) : base));
+                r.others = max(1, min(sms_of<M>(other, others, kind, base), others));
                 r.per = base / r.ctas;
                 r.more = base - r.per * r.ctas;
                 const int c = blockIdx.x;

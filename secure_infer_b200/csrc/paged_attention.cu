@@ -85,28 +85,32 @@ constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 token
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
 constexpr int kRows = 8;
 constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kRows * 256 + 2 * kRowsWarps * kRows * 4;
-// Units up to which a tile is not cut where there is little work.  One sequence
-// of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
+// Units up to which a tile is not cut where there is little work, with a cost of 1.
+// One sequence of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
 constexpr int kRowsWhole = 4;
-constexpr int kRowsCost = 1;   // pages that a tile's end is worth
+// Pages that a tile's beginning and end are worth.  Measured: its queries 0.7 us, its end 1.1, where a page takes 1.1 to
+// 1.4; the usual call keeps the 1 that its results' order of sums goes by.
+template <int M>
+constexpr int kRowsCost = M == kPlain ? 1 : 2;
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
 // more in a second step.
 constexpr int kJoinRows = 160;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowSlot = kRows * (kDim + 2);
 
-// Pages that a pair of tiles' beginning and end are worth.  Measured: 8.6 us, where a page takes 2.0; the usual call keeps
-// the 2 that its results' order of sums goes by.
-template <int M>
-constexpr int kTilesCost = M == kPlain ? 2 : 4;
+constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
 
 // An SM takes 1.1 us of a page for few rows where fewer than 120 of 148 SMs read (58 GB/s each; 120 to 130 get nearly
-// all that memory gives), and 1.95 us of a page for a pair of tiles.
-__device__ __forceinline__ Kind rows_kind() { return {kRows, kRowsCost, kRowsWhole, 4, 14}; }
+// all that memory gives), and 1.95 us of a page for a pair of tiles, whose kernel begins 5.5 us later.
+template <int M>
+__device__ __forceinline__ Kind rows_kind()
+{
+    return {kRows, kRowsCost<M>, kRowsWhole - 1 + kRowsCost<M>, 4, 14, 0};
+}
 template <int M>
 __device__ __forceinline__ Kind tiles_kind(const AttendParams& p)
 {
-    return {2 * (128 / p.group * p.group), kTilesCost<M>, 0, 7, 16};
+    return {2 * (128 / p.group * p.group), kTilesCost, 0, 7, 16, 20};
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
@@ -198,9 +202,13 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     wait_for_earlier_kernels();
-    find_share<kRowsThreads, M>(p, rows_kind(), tiles_kind<M>(p), &share, warp_sums);
+    find_share<kRowsThreads, M, false>(p, rows_kind<M>(), tiles_kind<M>(p), &share, warp_sums);
+    if (M != kPlain && p.both && blockIdx.x == 0 && tid == 0) {
+        atomicExch(p.status + 1, static_cast<uint32_t>(share.others));
+        __threadfence();
+    }
     dependents_may_launch();
-    Walk<M> w = start_walk<M>(p, kRows, kRowsCost, share);
+    Walk<M> w = start_walk<M>(p, kRows, kRowsCost<M>, share);
 
     if (warp == kRowsWarps) {
         // Producer: the quarters of each page that hold keys any row sees.
@@ -732,7 +740,7 @@ __device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& shar
 {
     const int tid = threadIdx.x, cta = blockIdx.x;
     if (tid == 0) atomicOr(p.status, 1u);
-    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), kTilesCost<M>, share);
+    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), kTilesCost, share);
     for (bool first = true; w.left > 0; first = false) {
         const int pages = w.take();
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
@@ -804,11 +812,11 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     // read them, the two share no memory that either writes, and it waits for that one at its end instead.
     if (!p.both) wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads, M>(p, tiles_kind<M>(p), rows_kind(), &c.share, c.warp_sums);
+    find_share<kTileThreads, M, M != kPlain>(p, tiles_kind<M>(p), rows_kind<M>(), &c.share, c.warp_sums);
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
-    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, kTilesCost<M>, c.share);
+    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, kTilesCost, c.share);
     const bool any = w.left > 0 && c.share.down == 0;
 
     // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.
@@ -1352,18 +1360,57 @@ __device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cu
     const int pieces = cut.cta1 - cut.cta0 + 1;
     auto piece = [&](int i) { return p.slots + static_cast<int64_t>(2 * (cut.cta0 + i) + (i == 0)) * kTileSlot; };
     float top = -INFINITY, sum = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < pieces; ++i) top = max3_nan(top, __ldcg(piece(i) + kTileRows * kDim + r), top);
     float4 x[kFours] = {};
+    if (M == kPlain) {
+#pragma unroll 8
+        for (int i = 0; i < pieces; ++i) top = max3_nan(top, __ldcg(piece(i) + kTileRows * kDim + r), top);
 #pragma unroll (8 / kFours)
-    for (int i = 0; i < pieces; ++i) {
-        const float* at = piece(i);
-        const float f = join_weight(__ldcg(at + kTileRows * kDim + r), top);
-        sum += f * __ldcg(at + kTileRows * kDim + kTileRows + r);
+        for (int i = 0; i < pieces; ++i) {
+            const float* at = piece(i);
+            const float f = join_weight(__ldcg(at + kTileRows * kDim + r), top);
+            sum += f * __ldcg(at + kTileRows * kDim + kTileRows + r);
 #pragma unroll
-        for (int j = 0; j < kFours; ++j) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(at) + ((r & ~31) + d4 + j) * 32 + (r & 31));
-            x[j] = make_float4(x[j].x + f * y.x, x[j].y + f * y.y, x[j].z + f * y.z, x[j].w + f * y.w);
+            for (int j = 0; j < kFours; ++j) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(at) + ((r & ~31) + d4 + j) * 32 + (r & 31));
+                x[j] = make_float4(x[j].x + f * y.x, x[j].y + f * y.y, x[j].z + f * y.z, x[j].w + f * y.w);
+            }
+        }
+    } else {
+        // In one pass by the running maximum: everything of some pieces is on its way at once, as a prefix may be cut
+        // into as many pieces as there are SMs.
+        constexpr int kBatch = 8 / kFours;
+        for (int i0 = 0; i0 < pieces; i0 += kBatch) {
+            float m[kBatch], l[kBatch];
+            float4 y[kBatch][kFours];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                m[i] = -INFINITY;
+                l[i] = 0.0f;
+                if (i0 + i >= pieces) continue;
+                const float* at = piece(i0 + i);
+                m[i] = __ldcg(at + kTileRows * kDim + r);
+                l[i] = __ldcg(at + kTileRows * kDim + kTileRows + r);
+#pragma unroll
+                for (int j = 0; j < kFours; ++j)
+                    y[i][j] = __ldcg(reinterpret_cast<const float4*>(at) + ((r & ~31) + d4 + j) * 32 + (r & 31));
+            }
+            float now = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) now = max3_nan(now, m[i], now);
+            const float back = join_weight(top, now);
+            sum *= back;
+#pragma unroll
+            for (int j = 0; j < kFours; ++j) x[j] = make_float4(x[j].x * back, x[j].y * back, x[j].z * back, x[j].w * back);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (i0 + i >= pieces) break;
+                const float f = join_weight(m[i], now);
+                sum += f * l[i];
+#pragma unroll
+                for (int j = 0; j < kFours; ++j)
+                    x[j] = make_float4(x[j].x + f * y[i][j].x, x[j].y + f * y[i][j].y, x[j].z + f * y[i][j].z, x[j].w + f * y[i][j].w);
+            }
+            top = now;
         }
     }
     const Seq s{cut.n, cut.kv, cut.q0, 0, cut.part, 0};
@@ -1399,8 +1446,10 @@ __device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cu
 template <typename T, int M>
 __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const __grid_constant__ AttendParams p)
 {
+    if (M == kShared) dependents_may_launch();   // what joins the parts finds its rows meanwhile
     wait_for_earlier_kernels();
-    dependents_may_launch();
+    if (M != kShared) dependents_may_launch();
+    if (M != kPlain && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.status[1] = 0;
     const Cut cut = p.cuts[blockIdx.y];
     if (cut.cta1 == 0) return;
     const int sharers = cut.cta1 - cut.cta0, k = blockIdx.y - cut.cta0 - 1;

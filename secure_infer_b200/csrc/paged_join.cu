@@ -85,18 +85,20 @@ __global__ void __launch_bounds__(kPrefixThreads) shared_prefix_kernel(const __g
 
 // ------------------------------------------------- a group's keys and a row's own
 //
-// A warp per row of the output.  Both partial results are on their way before the
-// row's sequence is known; rows of sequences that share nothing are whole already.
+// A warp per row of the output, which finds its sequence while the kernels before
+// go on; rows of sequences that share nothing are whole already.
 constexpr int kPartsWarps = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kPartsWarps) attend_parts_kernel(const __grid_constant__ AttendParams p)
 {
     const int lane = threadIdx.x & 31, token = blockIdx.x, head = blockIdx.y * kPartsWarps + (threadIdx.x >> 5);
+    const int heads = p.heads * p.group;
+    // What the call was given was complete before its first kernel read it.
+    const Seq q = load_seq<kShared>(p, find_seq(p.cu, p.seqs, token));
     wait_for_earlier_kernels();
     dependents_may_launch();
-    const int heads = p.heads * p.group;
-    if (head >= heads) return;
+    if (head >= heads || q.part != 1 || token < q.q0 || token >= q.q0 + q.n) return;
     const int64_t rows = static_cast<int64_t>(p.tokens) * heads, at = static_cast<int64_t>(token) * heads + head;
     float4 x[2];
     float2 stat[2];
@@ -105,9 +107,6 @@ __global__ void __launch_bounds__(32 * kPartsWarps) attend_parts_kernel(const __
         x[i] = __ldcg(reinterpret_cast<const float4*>(p.parts + (i * rows + at) * kDim) + lane);
         stat[i] = __ldcg(reinterpret_cast<const float2*>(p.parts + 2 * rows * kDim) + i * rows + at);
     }
-    const int s = find_seq(p.cu, p.seqs, token);
-    const Seq q = load_seq<kShared>(p, s);
-    if (q.part != 1 || token < q.q0 || token >= q.q0 + q.n) return;
     const float top = fmaxf(stat[0].x, stat[1].x), f0 = join_weight(stat[0].x, top), f1 = join_weight(stat[1].x, top);
     const float4 sum = make_float4(f0 * x[0].x + f1 * x[1].x, f0 * x[0].y + f1 * x[1].y, f0 * x[0].z + f1 * x[1].z,
                                    f0 * x[0].w + f1 * x[1].w);
