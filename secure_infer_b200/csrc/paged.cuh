@@ -67,6 +67,7 @@ struct AttendParams {
     const int32_t* prefix;          // kShared: [seqs] keys in common with the sequence's group
     const Group* shared;            // [groups]
     int32_t groups;
+    int32_t tiles_cost;             // pages that the beginning and the end of a pair of tiles are worth
     float* parts;                   // [2][rows of the output][128] sums over the group's and over a sequence's own keys, then
                                     // [2][rows] maxima and sums of weights
 };

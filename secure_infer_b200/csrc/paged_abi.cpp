@@ -132,8 +132,12 @@ Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, u
 // the caller says they may be.  A page takes an SM 4 units of time (1.1 us) for
 // eight rows in the kernel for few rows, as long for 128 rows in tiles and 7 for
 // 256.  It costs the joining of the parts (0.17 units a row) and, in a call that has
-// no tiles otherwise, the tiles' kernel and its own join.
-constexpr int64_t kShareCost = 1500, kShareTilesCost = 13000;
+// no tiles otherwise, the tiles' kernel and its own join.  Together and apart, us:
+// single tokens of 8 KV heads of 4 rows, 2 sequences with 512, 2048 and 8192 tokens in
+// common 10.2 and 8.4, 11.9 and 9.8, 14.4 and 16.5; 8 sequences with 2048, 8192 and
+// 30000 (tiles) 22.0 and 16.4, 25.7 and 32.4, 50.7 and 87; 8 chunks of up to 40
+// tokens of 4 rows with 2048, 8192, 30000 41 and 37, 65 and 71, 146 and 202.
+constexpr int64_t kShareCost = 1000, kShareTilesCost = 12000;
 int64_t page_time(uint64_t rows)
 {
     return static_cast<int64_t>(rows <= kFewRows ? 4 * ((rows + 7) / 8) : rows <= 128 ? 4 : 7 * ((rows + 255) / 256));
@@ -149,7 +153,7 @@ uint32_t shared_groups(const secure_infer_pages& pages, const secure_infer_chunk
     const int64_t apart = static_cast<int64_t>(seqs) * page_time((tokens + seqs - 1) / seqs * group);
     const int64_t together = groups * page_time((tokens + groups - 1) / groups * group);
     const uint64_t largest = (chunk.max_q == 0 || chunk.max_q > tokens ? tokens : chunk.max_q) * group;
-    const int64_t cost = largest > kFewRows || group > 128 ? kShareCost : kShareTilesCost;
+    const int64_t cost = largest > kFewRows || group > 128 || tokens * group <= kFewRows ? kShareCost : kShareTilesCost;
     const double saved = static_cast<double>(apart - together) * common * pages.heads;
     const bool worth = saved > static_cast<double>(cost) + static_cast<double>(tokens * q_heads) / 6;
     return worth && work_of(pages, chunk, q_heads, groups).fits() ? groups : 0;
@@ -332,6 +336,11 @@ SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_
         p.shared = reinterpret_cast<const Group*>(options->plan + group_offset(chunk->seqs));
         p.groups = static_cast<int32_t>(groups);
         p.parts = options->parts;
+        // Partial results are twice as long: a pair of tiles takes 4.5 us besides its pages, where sequences fill both. Eight
+        // chunks of up to 40 tokens of 7 rows on 30000: 194 us with 2, 131 with 4; four times six drafts of 5 of 8 rows on
+        // up to 30000, one tile each: 35.2 and 37.1.
+        const uint64_t seqs = chunk->seqs < chunk->tokens ? chunk->seqs : chunk->tokens;
+        p.tiles_cost = uint64_t(chunk->tokens) * group > 128 * seqs ? 4 : 2;
     }
     p.scale_log2 = scale * 1.4426950408889634f;
     // Hidden scores are -inf before they are scaled, so the scale is never zero; at 1e-30 all weights are 1.

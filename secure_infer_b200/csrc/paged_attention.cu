@@ -98,7 +98,12 @@ constexpr int kJoinRows = 160;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowSlot = kRows * (kDim + 2);
 
-constexpr int kTilesCost = 2;   // pages that a pair of tiles' beginning and end are worth
+// Pages that a pair of tiles' beginning and end are worth.
+template <int M>
+__device__ __forceinline__ int tiles_cost(const AttendParams& p)
+{
+    return M == kShared ? p.tiles_cost : 2;
+}
 
 // An SM takes 1.1 us of a page for few rows where fewer than 120 of 148 SMs read (58 GB/s each; 120 to 130 get nearly
 // all that memory gives), and 1.95 us of a page for a pair of tiles, whose kernel begins 5.5 us later.
@@ -110,7 +115,7 @@ __device__ __forceinline__ Kind rows_kind()
 template <int M>
 __device__ __forceinline__ Kind tiles_kind(const AttendParams& p)
 {
-    return {2 * (128 / p.group * p.group), kTilesCost, 0, 7, 16, 20};
+    return {2 * (128 / p.group * p.group), tiles_cost<M>(p), 0, 7, 16, 20};
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
@@ -740,7 +745,7 @@ __device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& shar
 {
     const int tid = threadIdx.x, cta = blockIdx.x;
     if (tid == 0) atomicOr(p.status, 1u);
-    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), kTilesCost, share);
+    Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), tiles_cost<M>(p), share);
     for (bool first = true; w.left > 0; first = false) {
         const int pages = w.take();
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
@@ -816,7 +821,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
-    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, kTilesCost, c.share);
+    Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, tiles_cost<M>(p), c.share);
     const bool any = w.left > 0 && c.share.down == 0;
 
     // 640 threads at 96 registers: 104 for the four softmax warpgroups and 64 for the fifth make the same sum.
@@ -1288,16 +1293,26 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                                                       __uint_as_float(o[d + 2]), __uint_as_float(o[d + 3]));
                     }
                 } else if (M == kShared && w.part >= 0) {
-                    if (lane < valid) {
-                        const int64_t all = static_cast<int64_t>(p.tokens) * p.heads * p.group, to = w.part * all + out0 + rel;
-                        float4* part = reinterpret_cast<float4*>(p.parts + to * kDim + quarter * 32);
+                    // The same with 32-bit values (straight from the registers, sixteen bytes of 32 rows a store, a tile's
+                    // took 3.4 us).
+                    const int64_t all = static_cast<int64_t>(p.tokens) * p.heads * p.group, first = w.part * all + out0;
+                    float* part = p.parts + first * kDim + quarter * 32 + (lane & 1) * 4;
 #pragma unroll
-                        for (int d = 0; d < 32; d += 4)
-                            part[d / 4] = make_float4(__uint_as_float(o[d]), __uint_as_float(o[d + 1]),
-                                                      __uint_as_float(o[d + 2]), __uint_as_float(o[d + 3]));
-                        if (quarter == 0)
-                            *reinterpret_cast<float2*>(p.parts + 2 * all * kDim + 2 * to) = make_float2((t ? m1 : m0) * scale, l);
+                    for (int d = 0; d < 32; d += 8) {
+                        put(o[d], o[d + 1], o[d + 2], o[d + 3], 0);
+                        put(o[d + 4], o[d + 5], o[d + 6], o[d + 7], 1);
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int r = k * 16 + (lane >> 1);
+                            const int64_t to = __shfl_sync(0xffffffffu, rel, r);
+                            const uint4 y = get(r);
+                            if (r < valid) *reinterpret_cast<uint4*>(part + to * kDim + d) = y;
+                        }
+                        __syncwarp();
                     }
+                    if (quarter == 0 && lane < valid)
+                        *reinterpret_cast<float2*>(p.parts + 2 * all * kDim + 2 * (first + rel)) = make_float2((t ? m1 : m0) * scale, l);
                 } else {
                     T* out = static_cast<T*>(p.out) + out0 * kDim + quarter * 32 + (lane & 1) * 8;
 #pragma unroll
