@@ -1982,7 +1982,7 @@ const char* kernel_kind_name(uint32_t kind)
                                             "paged_attend_rows_kernel", "paged_attend_tiles_kernel",
                                             "paged_attend_join_kernel", "paged_append_kernel", "page_copy_kernel",
                                             "page_tables_kernel", "shared_prefix_kernel", "attend_parts_kernel",
-                                            "join_parts_kernel"};
+                                            "join_parts_kernel", "paged_attend_both_kernel"};
     return kind < kKernKinds ? names[kind] : nullptr;
 }
 

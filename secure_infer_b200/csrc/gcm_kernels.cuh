@@ -165,7 +165,8 @@ int launch_layer_verify_inline(const LayerHeader& h, const LayerRec* rec, cudaSt
 enum KernelKind : uint32_t {
     kKernLayerCtr = 0, kKernLayerVerify, kKernLayerEncrypt, kKernEncode, kKernSegment, kKernCtr, kKernSchedule,
     kKernAuthGate, kKernLayerVerifyInline, kKernLayerCtrBitsliced, kKernAttendRows, kKernAttendTiles, kKernAttendJoin,
-    kKernAppend, kKernPageCopy, kKernTables, kKernSharedPrefix, kKernAttendParts, kKernJoinParts, kKernKinds
+    kKernAppend, kKernPageCopy, kKernTables, kKernSharedPrefix, kKernAttendParts, kKernJoinParts,
+    kKernAttendBoth, kKernKinds
 };
 // Brackets one launch with timing events while the profile is enabled.
 class ProfileScope {

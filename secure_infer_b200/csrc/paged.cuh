@@ -78,6 +78,11 @@ int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const
 // q_map: boxes of [128 / group tokens][group heads][64 values].
 int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
                         const AttendParams& p, Mode mode, uint32_t dtype, cudaStream_t stream);
+// Both kinds of sequences in one launch, not for kPlain.  quarters: the maps of the rows' kernel; few and many: the
+// call with the limits of either kind's rows.
+int launch_attend_both(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                       const CUtensorMap& k_quarters, const CUtensorMap& v_quarters, const AttendParams& few,
+                       const AttendParams& many, Mode mode, uint32_t dtype, cudaStream_t stream);
 uint64_t attend_workspace_bytes();
 void attend_workspace(void* workspace, AttendParams* p);   // its counters, status word and slots
 
@@ -434,7 +439,6 @@ struct Share {
     int32_t begin, units;      // of this CTA
     int32_t seq, seq_unit;     // sequence of its first unit, and that sequence's first unit
     int32_t down;              // the status word when the kernel began
-    int32_t others;            // CTAs of the call's other launch that have one, if that is the one for many rows
     Seq q;
 
     __device__ __forceinline__ int begin_of(int cta) const { return cta * per + min(cta, more); }
@@ -545,7 +549,7 @@ struct Kind {
     int rows_per_tile, cost, whole;
     int time;     // of a unit, in any measure that both kinds share
     int of_16;    // sixteenths of the SMs beyond which it gets no faster
-    int later;    // how much later than the other kind's its first page is there, in the measure of time
+    int later;    // in one launch: how much later than the other kind's its first scores are there, in the measure of time
 };
 
 // All threads of the block take part; `warp_sums` holds three values per warp.
@@ -556,35 +560,33 @@ struct Kind {
 // launch, so reading pages for few rows goes on beside the products of many: 333
 // tokens after 2167 and 15 single tokens of up to 4000 take 53 us, 62 one kind
 // after the other.
-// SMs for `units` of a kind beside `others` of the other.
-template <int M>
+// SMs for `units` of a kind beside `others` of the other, in launches of their own.
 __device__ __forceinline__ int sms_of(const Kind& kind, int units, const Kind& other, int others)
 {
     const int grid = gridDim.x;
     if (units == 0 || others == 0 || grid == 1) return grid;
     const float mine = static_cast<float>(units) * kind.time, theirs = static_cast<float>(others) * other.time;
-    if (M == kPlain) {
-        const int most = max(1, grid * kind.of_16 / 16), least = grid - max(1, grid * other.of_16 / 16);
-        return max(max(1, least), min(min(most, grid - 1), __float2int_rn(grid * (mine / (mine + theirs)))));
-    }
-    // Both end together where few / x = many / (grid - x) + later, a quadratic equation.  One count serves both kinds, or a
-    // CTA might have to wait for the other launch's.
-    const bool first = kind.later == 0;
-    const float few = first ? mine : theirs, many = first ? theirs : mine, later = first ? other.later : kind.later;
-    const float b = few + many + later * grid;
-    const float x = 2.0f * few * grid / (b + sqrtf(fmaxf(0.0f, b * b - 4.0f * later * few * grid)));
-    // The whole number on either side with the earlier end.
-    const int most = max(1, min(grid * (first ? kind : other).of_16 / 16, grid - 1)), low = max(1, min(most, __float2int_rd(x)));
-    const int high = min(most, low + 1);
-    const auto end = [&](int r) { return fmaxf(few / r, many / (grid - r) + later); };
-    const int rows = end(high) < end(low) ? high : low;
-    return first ? rows : grid - rows;
+    const int most = max(1, grid * kind.of_16 / 16), least = grid - max(1, grid * other.of_16 / 16);
+    return max(max(1, least), min(min(most, grid - 1), __float2int_rn(grid * (mine / (mine + theirs)))));
 }
 
-// kIdle: the launch before has left in p.status[1] how many CTAs of this one have
-// work.  The others would count it again when the first launch's CTAs leave, at
-// the call's end: 4 us, where there are more CTAs than fit.
-template <int kThreads, int M, bool kIdle>
+// SMs for units of few rows beside units of many in one launch: both end together
+// where few / x = many / (grid - x) + later, a quadratic equation.
+__device__ __forceinline__ int sms_for_few(const Kind& few, int units, const Kind& many, int others)
+{
+    const int grid = gridDim.x;
+    if (units == 0 || others == 0 || grid == 1) return units == 0 ? 0 : grid;
+    const float u = static_cast<float>(units) * few.time, v = static_cast<float>(others) * many.time;
+    const float later = many.later, b = u + v + later * grid;
+    const float x = 2.0f * u * grid / (b + sqrtf(fmaxf(0.0f, b * b - 4.0f * later * u * grid)));
+    // The whole number on either side with the earlier end.
+    const int most = max(1, min(grid * few.of_16 / 16, grid - 1)), low = max(1, min(most, __float2int_rd(x)));
+    const int high = min(most, low + 1);
+    const auto end = [&](int r) { return fmaxf(u / r, v / (grid - r) + later); };
+    return end(high) < end(low) ? high : low;
+}
+
+template <int kThreads, int M>
 __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& kind, const Kind& other, Share* share,
                                            int32_t* warp_sums)
 {
@@ -592,11 +594,6 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
     constexpr int kWarps = kThreads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seqs = seq_count<M>(p);
     const int down = tid == 0 ? static_cast<int>(__ldcg(p.status)) : 0;
-    bool leave = false;
-    if (kIdle && tid == 0 && p.both) {
-        const uint32_t busy = __ldcg(p.status + 1);
-        leave = busy != 0 && blockIdx.x >= busy;
-    }
     Share r;
     r.begin = r.total = 0;
     // The first pass sums the units, the second finds the sequence that holds this CTA's first; where every sequence
@@ -609,17 +606,6 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
             Seq q{};
             int own_largest = 0, unused = 0, beside = 0;
             if (s < seqs) q = load_any<M>(p, s);
-            if (kIdle && (one || pass == 0) && s0 == 0 && __syncthreads_or(leave)) {
-                // The kernel before has counted both kinds, and leaves this CTA none.
-                if (tid == 0) {
-                    *share = Share{};
-                    share->ctas = 1;
-                    share->seq = -1;
-                    share->down = down;
-                }
-                __syncthreads();
-                return;
-            }
             Seq o = q;
             if (is_mine(p, q)) o.n = 0;
             else q.n = 0;
@@ -649,8 +635,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
             others += __reduce_add_sync(0xffffffffu, has ? warp_sums[2 * kWarps + lane] : 0);
             if (one || (pass == 0 && s0 + kThreads >= seqs)) {
                 r.total = base;
-                r.ctas = max(1, min(sms_of<M>(kind, base, other, others), largest <= whole ? base / max(1, largest) : base));
-                r.others = max(1, min(sms_of<M>(other, others, kind, base), others));
+                r.ctas = max(1, min(sms_of(kind, base, other, others), largest <= whole ? base / max(1, largest) : base));
                 r.per = base / r.ctas;
                 r.more = base - r.per * r.ctas;
                 const int c = blockIdx.x;
@@ -675,6 +660,87 @@ __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& ki
             __syncthreads();
         }
     }
+}
+
+// The same for one launch of both kinds: its first CTAs take the tiles of few rows,
+// its last ones those of many, counted from the end.  -> whether this one takes
+// the former.  few and many: the call as either kind sees it.
+template <int kThreads, int M>
+__device__ __forceinline__ bool find_share_of_both(const AttendParams& few, const Kind& few_kind, const AttendParams& many,
+                                                   const Kind& many_kind, Share* share, int32_t* warp_sums, int& cta)
+{
+    constexpr int kWarps = kThreads / 32;
+    static_assert(kWarps <= 32, "a warp sums the warps");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seqs = seq_count<M>(few);
+    const int down = tid == 0 ? static_cast<int>(__ldcg(few.status)) : 0;
+    Share r;
+    r.begin = r.total = r.units = 0;
+    bool first_kind = true;
+    cta = blockIdx.x;
+    const bool one = seqs <= kThreads;
+    for (int pass = one ? 1 : 0; pass < 2; ++pass) {
+        int base = 0, all_few = 0, all_many = 0, largest = 0;
+        for (int s0 = 0; s0 < seqs; s0 += kThreads) {
+            const int s = s0 + tid;
+            Seq q{};
+            int own_largest = 0, unused = 0;
+            if (s < seqs) q = load_any<M>(few, s);
+            Seq f = q, m = q;
+            if (!is_mine(few, q)) f.n = 0;
+            if (!is_mine(many, q)) m.n = 0;
+            const int few_units = seq_units<M>(few, f, few_kind.rows_per_tile, few_kind.cost, own_largest);
+            const int many_units = seq_units<M>(many, m, many_kind.rows_per_tile, many_kind.cost, unused);
+            const int few_sum = __reduce_add_sync(0xffffffffu, few_units), many_sum = __reduce_add_sync(0xffffffffu, many_units);
+            own_largest = __reduce_max_sync(0xffffffffu, own_largest);
+            if (lane == 0) {
+                warp_sums[warp] = few_sum;
+                warp_sums[kWarps + warp] = own_largest;
+                warp_sums[2 * kWarps + warp] = many_sum;
+            }
+            __syncthreads();
+            const bool has = lane < kWarps;
+            const int x = has ? warp_sums[lane] : 0, y = has ? warp_sums[2 * kWarps + lane] : 0;
+            all_few += __reduce_add_sync(0xffffffffu, x);
+            all_many += __reduce_add_sync(0xffffffffu, y);
+            largest = max(largest, __reduce_max_sync(0xffffffffu, has ? warp_sums[kWarps + lane] : 0));
+            if (one || (pass == 0 && s0 + kThreads >= seqs)) {
+                const int sms = sms_for_few(few_kind, all_few, many_kind, all_many), grid = gridDim.x;
+                const int few_ctas = min(sms, largest <= few_kind.whole ? all_few / max(1, largest) : all_few);
+                first_kind = static_cast<int>(blockIdx.x) < few_ctas;
+                cta = first_kind ? blockIdx.x : grid - 1 - blockIdx.x;
+                r.total = first_kind ? all_few : all_many;
+                r.ctas = first_kind ? few_ctas : max(1, min(grid - sms, all_many));
+                r.per = r.total / r.ctas;
+                r.more = r.total - r.per * r.ctas;
+                r.begin = r.begin_of(cta);
+                r.units = cta < r.ctas ? r.per + (cta < r.more) : 0;
+                if (tid == 0) {
+                    r.seq = -1;
+                    r.seq_unit = 0;
+                    r.down = down;
+                    *share = r;
+                }
+                __syncthreads();
+            }
+            if (pass == 1) {
+                const int own = first_kind ? few_units : many_units, z = first_kind ? x : y;
+                int sum = own;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, sum, d);
+                    if (lane >= d) sum += up;
+                }
+                const int first = base + __reduce_add_sync(0xffffffffu, lane < warp ? z : 0) + sum - own;
+                if (r.units > 0 && own > 0 && r.begin >= first && r.begin < first + own) {
+                    share->seq = s;
+                    share->seq_unit = first;
+                    share->q = q;
+                }
+                base += __reduce_add_sync(0xffffffffu, z);
+            }
+            __syncthreads();
+        }
+    }
+    return first_kind;
 }
 
 // All lanes of a warp call it.
@@ -768,8 +834,8 @@ __device__ __forceinline__ PieceKeys piece_keys(const AttendParams& p, const Spa
 // clocks, the rows of a long piece longer than the other warps' waits last, so
 // it counts its way in *work.
 template <typename T, int M>
-__device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q, const int32_t* table, int head,
-                                               PieceKeys in, float& m, float& l, float4& o, volatile int* work)
+__device__ __forceinline__ void row_by_definition_here(const AttendParams& p, const T* q, const int32_t* table, int head,
+                                                       PieceKeys in, float& m, float& l, float4& o, volatile int* work)
 {
     const int d = 4 * (threadIdx.x & 31);
     const uint2 qx = __ldcg(reinterpret_cast<const uint2*>(q + d));
@@ -802,6 +868,13 @@ __device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q
         o.z = o.z * f + e * v1.x;
         o.w = o.w * f + e * v1.y;
     }
+}
+
+template <typename T, int M>
+__device__ __noinline__ void row_by_definition(const AttendParams& p, const T* q, const int32_t* table, int head,
+                                               PieceKeys in, float& m, float& l, float4& o, volatile int* work)
+{
+    row_by_definition_here<T, M>(p, q, table, head, in, m, l, o, work);
 }
 
 // One row's result, by a warp: values 4 lane .. 4 lane + 3 of the sum x, the

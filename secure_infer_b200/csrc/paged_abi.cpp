@@ -351,21 +351,27 @@ SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_
     static std::mutex launches;
     const std::lock_guard<std::mutex> lock(launches);
     const bool tiles = work.tiles;
-    CUtensorMap q_map, k_map, v_map;
-    if (!tiles || chunk->seqs > 1) {   // (groups go with several sequences)
-        if (!page_map(&k_map, pages, pages->k, pages->k_stride, 32) || !page_map(&v_map, pages, pages->v, pages->v_stride, 32))
-            return -1;
-        p.rows_max = tiles ? kFewRows : INT_MAX;
-        p.both = tiles;
-        if (launch_attend_rows(k_map, v_map, p, mode, pages->dtype, st) != 0) return -1;
-        p.rows_min = kFewRows + 1;
-        p.rows_max = INT_MAX;
-    }
-    if (!tiles) return groups > 0 && launch_attend_parts(p, pages->dtype, st) != 0 ? -1 : 0;
-    if (!page_map(&k_map, pages, pages->k, pages->k_stride, kPage) || !page_map(&v_map, pages, pages->v, pages->v_stride, kPage) ||
-        !rows_map(&q_map, pages->dtype, q, q_token_stride, q_head_stride, chunk->tokens, q_heads, group))
+    CUtensorMap q_map, k_map, v_map, k_quarters, v_quarters;
+    const bool some_rows = !tiles || chunk->seqs > 1;   // (groups go with several sequences)
+    if (some_rows && (!page_map(&k_quarters, pages, pages->k, pages->k_stride, 32) ||
+                      !page_map(&v_quarters, pages, pages->v, pages->v_stride, 32)))
         return -1;
-    if (launch_attend_tiles(q_map, k_map, v_map, p, mode, pages->dtype, st) != 0) return -1;
+    if (tiles && (!page_map(&k_map, pages, pages->k, pages->k_stride, kPage) ||
+                  !page_map(&v_map, pages, pages->v, pages->v_stride, kPage) ||
+                  !rows_map(&q_map, pages->dtype, q, q_token_stride, q_head_stride, chunk->tokens, q_heads, group)))
+        return -1;
+    AttendParams few = p;
+    if (tiles) {
+        few.rows_max = kFewRows;
+        if (some_rows) p.rows_min = kFewRows + 1;
+    }
+    if (tiles && some_rows && mode != kPlain) {
+        if (launch_attend_both(q_map, k_map, v_map, k_quarters, v_quarters, few, p, mode, pages->dtype, st) != 0) return -1;
+    } else {
+        few.both = p.both = tiles && some_rows;
+        if (some_rows && launch_attend_rows(k_quarters, v_quarters, few, mode, pages->dtype, st) != 0) return -1;
+        if (tiles && launch_attend_tiles(q_map, k_map, v_map, p, mode, pages->dtype, st) != 0) return -1;
+    }
     return groups > 0 && launch_attend_parts(p, pages->dtype, st) != 0 ? -1 : 0;
 }
 

@@ -84,7 +84,7 @@ constexpr int kQuarter = 32;                              // tokens of one TMA b
 constexpr uint32_t kQuarterBytes = kQuarter * kDim * 2;   // [2 halves][32 tokens][64 values]
 constexpr uint32_t kPageTile = 4 * kQuarterBytes;         // K or V of one page and head
 constexpr int kRows = 8;
-constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + kRows * 256 + 2 * kRowsWarps * kRows * 4;
+constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + 2 * kRows * 256 + 2 * kRowsWarps * kRows * 4;
 // Units up to which a tile is not cut where there is little work, with a cost of 1.
 // One sequence of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
 constexpr int kRowsWhole = 4;
@@ -115,7 +115,7 @@ __device__ __forceinline__ Kind rows_kind()
 template <int M>
 __device__ __forceinline__ Kind tiles_kind(const AttendParams& p)
 {
-    return {2 * (128 / p.group * p.group), tiles_cost<M>(p), 0, 7, 16, 20};
+    return {2 * (128 / p.group * p.group), tiles_cost<M>(p), 0, 7, 16, 7};
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
@@ -171,30 +171,20 @@ __device__ __forceinline__ bool rows_any(bool x)
     return r != 0;
 }
 
-template <typename T, int M>
-__global__ void __launch_bounds__(kRowsThreads, 1)
-paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                         const __grid_constant__ AttendParams p)
-{
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[3 * kRowsStages];   // K full, V full, empty
-    __shared__ Share share;
-    __shared__ int32_t warp_sums[3 * kRowsThreads / 32];
-    __shared__ volatile int stop[2];   // a wait ran out, and work that lets waits go on
-    __shared__ int irregular, last_piece;
+struct RowsControl {
+    uint64_t bars[3 * kRowsStages];   // K full, V full, empty
+    Share share;
+    int32_t warp_sums[3 * kRowsThreads / 32];
+    int stop[2];                      // a wait ran out, and work that lets waits go on
+    int irregular, last_piece;
 
-    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t k_smem = smem_addr(base), v_smem = k_smem + kRowsStages * kPageTile;
-    const uint32_t q_smem = v_smem + kRowsStages * kPageTile;
-    uint8_t* q_bytes = base + 2 * kRowsStages * kPageTile;
-    float* join_m = reinterpret_cast<float*>(q_bytes + kRows * 256);
-    float* join_l = join_m + kRowsWarps * kRows;
+    __device__ __forceinline__ uint32_t k_full(int s) const { return smem_addr(&bars[s]); }
+    __device__ __forceinline__ uint32_t v_full(int s) const { return smem_addr(&bars[kRowsStages + s]); }
+    __device__ __forceinline__ uint32_t empty(int s) const { return smem_addr(&bars[2 * kRowsStages + s]); }
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto k_full = [&](int s) { return smem_addr(&bars[s]); };
-    auto v_full = [&](int s) { return smem_addr(&bars[kRowsStages + s]); };
-    auto empty = [&](int s) { return smem_addr(&bars[2 * kRowsStages + s]); };
-    if (tid == 0) {
+    // By one thread, before a barrier of the block.
+    __device__ __forceinline__ void init(const CUtensorMap& k_map, const CUtensorMap& v_map)
+    {
         for (int s = 0; s < kRowsStages; ++s) {
             barrier_init(k_full(s), 1);
             barrier_init(v_full(s), 1);
@@ -206,81 +196,116 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
-    wait_for_earlier_kernels();
-    find_share<kRowsThreads, M, false>(p, rows_kind<M>(), tiles_kind<M>(p), &share, warp_sums);
-    if (M != kPlain && p.both && blockIdx.x == 0 && tid == 0) {
-        atomicExch(p.status + 1, static_cast<uint32_t>(share.others));
-        __threadfence();
-    }
-    dependents_may_launch();
-    Walk<M> w = start_walk<M>(p, kRows, kRowsCost<M>, share);
+};
 
-    if (warp == kRowsWarps) {
-        // Producer: the quarters of each page that hold keys any row sees.
-        uint32_t unit = 0, issued = 0;   // units passed, and those whose copies were issued
-        while (w.left > 0 && !__any_sync(0xffffffffu, stop[0] || share.down)) {
-            const int pages = w.take();
-            const int32_t* row = p.table + w.row() * p.table_stride;
-            for (int i0 = 0; i0 < pages; i0 += 32) {
-                const int id = i0 + lane < pages && w.span.hi > 0 ? row[w.span.page<M>(w.page + i0 + lane)] : -1;
-                for (int i = i0; i < min(pages, i0 + 32); ++i, ++unit) {
-                    const int page = __shfl_sync(0xffffffffu, id, i - i0);
-                    const int stage = unit % kRowsStages;
-                    const uint32_t turn = unit / kRowsStages;
-                    if (lane != 0 || stop[0] || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, stop))) continue;
-                    issued = unit + 1;
-                    const int first = w.span.page<M>(w.page + i) * kPage;
-                    int qa = max(0, w.span.lo - first) / kQuarter;
-                    int qb = (min(kPage, w.span.hi - first) + kQuarter - 1) / kQuarter;
-                    if (M == kSinks && first < p.sinks) {   // from its start; to the sinks' end where no window reaches it
-                        qa = 0;
-                        if (w.span.lo >= first + kPage) qb = (min(kPage, min(p.sinks, w.span.hi) - first) + kQuarter - 1) / kQuarter;
-                    }
-                    const uint32_t bytes = qb > qa ? (qb - qa) * kQuarterBytes : 0;
-                    barrier_expect(k_full(stage), bytes);
-                    for (int t = qa; t < qb; ++t)
-                        tma_load_page(k_smem + stage * kPageTile + t * kQuarterBytes, &k_map, k_full(stage),
-                                      t * kQuarter, 0, w.head, page);
-                    barrier_expect(v_full(stage), bytes);
-                    for (int t = qa; t < qb; ++t)
-                        tma_load_page(v_smem + stage * kPageTile + t * kQuarterBytes, &v_map, v_full(stage),
-                                      t * kQuarter, 0, w.head, page);
+// A CTA's shared memory (kRowsSmem bytes) for pages, queries and what the warps join.
+struct RowsMemory {
+    uint8_t* base;
+    uint32_t k, v;
+
+    __device__ __forceinline__ explicit RowsMemory(uint8_t* memory)
+    {
+        base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(memory) + 1023) & ~uintptr_t(1023));
+        k = smem_addr(base);
+        v = k + kRowsStages * kPageTile;
+    }
+};
+
+// The producer, a warp: the quarters of each page that hold keys any row sees.
+template <int M>
+__device__ __forceinline__ void load_rows_pages(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p,
+                                                RowsControl& c, const Share& share, uint8_t* memory, Walk<M> w)
+{
+    const RowsMemory at(memory);
+    const uint32_t k_smem = at.k, v_smem = at.v;
+    const int lane = threadIdx.x & 31;
+    auto k_full = [&](int s) { return c.k_full(s); };
+    auto v_full = [&](int s) { return c.v_full(s); };
+    auto empty = [&](int s) { return c.empty(s); };
+    volatile int* const stop = c.stop;
+    uint32_t unit = 0, issued = 0;   // units passed, and those whose copies were issued
+    while (w.left > 0 && !__any_sync(0xffffffffu, stop[0] || share.down)) {
+        const int pages = w.take();
+        const int32_t* row = p.table + w.row() * p.table_stride;
+        for (int i0 = 0; i0 < pages; i0 += 32) {
+            const int id = i0 + lane < pages && w.span.hi > 0 ? row[w.span.page<M>(w.page + i0 + lane)] : -1;
+            for (int i = i0; i < min(pages, i0 + 32); ++i, ++unit) {
+                const int page = __shfl_sync(0xffffffffu, id, i - i0);
+                const int stage = unit % kRowsStages;
+                const uint32_t turn = unit / kRowsStages;
+                if (lane != 0 || stop[0] || (turn > 0 && !barrier_wait(empty(stage), (turn - 1) & 1, stop))) continue;
+                issued = unit + 1;
+                const int first = w.span.page<M>(w.page + i) * kPage;
+                int qa = max(0, w.span.lo - first) / kQuarter;
+                int qb = (min(kPage, w.span.hi - first) + kQuarter - 1) / kQuarter;
+                if (M == kSinks && first < p.sinks) {   // from its start; to the sinks' end where no window reaches it
+                    qa = 0;
+                    if (w.span.lo >= first + kPage) qb = (min(kPage, min(p.sinks, w.span.hi) - first) + kQuarter - 1) / kQuarter;
                 }
-                __syncwarp();
+                const uint32_t bytes = qb > qa ? (qb - qa) * kQuarterBytes : 0;
+                barrier_expect(k_full(stage), bytes);
+                for (int t = qa; t < qb; ++t)
+                    tma_load_page(k_smem + stage * kPageTile + t * kQuarterBytes, &k_map, k_full(stage),
+                                  t * kQuarter, 0, w.head, page);
+                barrier_expect(v_full(stage), bytes);
+                for (int t = qa; t < qb; ++t)
+                    tma_load_page(v_smem + stage * kPageTile + t * kQuarterBytes, &v_map, v_full(stage),
+                                  t * kQuarter, 0, w.head, page);
             }
-            w.advance(p, pages);
+            __syncwarp();
         }
-        // Copies still in flight land before the CTA's shared memory goes away.
-        if (lane == 0) {
-            for (uint32_t u = issued > kRowsStages ? issued - kRowsStages : 0; u < issued; ++u) {
-                barrier_drain(k_full(u % kRowsStages), (u / kRowsStages) & 1);
-                barrier_drain(v_full(u % kRowsStages), (u / kRowsStages) & 1);
-            }
-        }
-        return;
+        w.advance(p, pages);
     }
+    // Copies still in flight land before the CTA's shared memory goes away.
+    if (lane == 0) {
+        for (uint32_t u = issued > kRowsStages ? issued - kRowsStages : 0; u < issued; ++u) {
+            barrier_drain(k_full(u % kRowsStages), (u / kRowsStages) & 1);
+            barrier_drain(v_full(u % kRowsStages), (u / kRowsStages) & 1);
+        }
+    }
+}
 
+// The work of CTA `cta` of those for few rows, by kRowsWarps warps.
+template <typename T, int M>
+__device__ __forceinline__ void attend_rows(const AttendParams& p, RowsControl& c, const Share& share, uint8_t* memory, int cta,
+                                            Walk<M> w)
+{
+    const RowsMemory at(memory);
+    uint8_t* const base = at.base;
+    const uint32_t k_smem = at.k, v_smem = at.v, q_smem = v_smem + kRowsStages * kPageTile;
+    float* join_m = reinterpret_cast<float*>(base + 2 * kRowsStages * kPageTile + 2 * kRows * 256);
+    float* join_l = join_m + kRowsWarps * kRows;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto k_full = [&](int s) { return c.k_full(s); };
+    auto v_full = [&](int s) { return c.v_full(s); };
+    auto empty = [&](int s) { return c.empty(s); };
+    volatile int* const stop = c.stop;
+    volatile int& irregular = c.irregular;
+    volatile int& last_piece = c.last_piece;
     uint32_t unit = 0;
     // A wait ran out: the rows that are left become NaN, and so do the pieces of cut tiles, which go on being counted.
     // If it was in an earlier call, counts mean nothing and the rows of every piece are written.
     bool failed = share.down != 0;
+    // A tile's rows, 256 bytes each, in 16-byte pieces swizzled against bank conflicts, into one of two buffers.
+    uint32_t turn = 0;
+    auto fetch = [&](const Walk<M>& t, uint32_t to) {
+        static_assert(kRows * 16 <= 32 * kRowsWarps, "a piece a thread");
+        const int r = tid >> 4, piece = tid & 15;
+        if (t.left <= 0 || r >= kRows) return;
+        const int row = t.tile * kRows + min(r, t.rows - 1), token = row / p.group, g = row % p.group;
+        const T* from = static_cast<const T*>(p.q) + (t.q.q0 + token) * p.q_token + (t.head * p.group + g) * p.q_head + piece * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_smem + to * kRows * 256 + r * 256 + ((piece ^ (r & 7)) << 4)),
+                     "l"(from), "r"(r < t.rows ? 16 : 0)   // rows that are not used are zero
+                     : "memory");
+    };
+    fetch(w, 0);
     while (w.left > 0) {
         const int pages = w.take();
-        // The tile's rows, 256 bytes each, in 16-byte pieces swizzled against bank conflicts.
         const int r0 = w.tile * kRows;
-        for (int c = tid; c < kRows * 16; c += 32 * kRowsWarps) {
-            const int r = c >> 4, piece = c & 15;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (r < w.rows) {
-                const int token = (r0 + r) / p.group, g = (r0 + r) % p.group;
-                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
-                                                    (w.head * p.group + g) * p.q_head + piece * 8);
-            }
-            *reinterpret_cast<uint4*>(q_bytes + r * 256 + ((piece ^ (r & 7)) << 4)) = x;
-        }
         const int cta0 = share.owner(w.tile_unit), cta1 = share.owner(w.tile_unit + w.span.pages - 1);
         const bool split = cta1 > cta0 && !share.down;
-        float* slot = p.row_slots + static_cast<int64_t>(2 * blockIdx.x + (static_cast<int>(blockIdx.x) == cta0)) * kRowSlot;
+        float* slot = p.row_slots + static_cast<int64_t>(2 * cta + (cta == cta0)) * kRowSlot;
         int lo[2], hi[2];   // keys that this thread's rows see
         int all_lo, all_hi; // keys that every row of the tile sees
         {
@@ -299,12 +324,20 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[j][c] = 0.0f;
+        asm volatile("cp.async.wait_all;" ::: "memory");
         rows_sync();
         uint32_t q[4][4];   // 32 values of the rows each
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             const int r = lane & 7, piece = d * 4 + (lane >> 3);
-            ldmatrix4(q[d], q_smem + r * 256 + ((piece ^ r) << 4));
+            ldmatrix4(q[d], q_smem + turn * kRows * 256 + r * 256 + ((piece ^ r) << 4));
+        }
+        // The next tile's are on their way meanwhile: 0.7 us of a tile.
+        turn ^= 1;
+        {
+            Walk<M> next = w;
+            next.advance(p, pages);
+            fetch(next, turn);
         }
 
         for (int i = 0; i < pages && !failed; ++i, ++unit) {
@@ -424,10 +457,12 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 sum = NAN;
                 x = make_float4(NAN, NAN, NAN, NAN);
             } else if (by_definition) {
-                row_by_definition<T, M>(p, static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token +
-                                               (w.head * p.group + g) * p.q_head,
-                                        p.table + w.row() * p.table_stride, w.head,
-                                        piece_keys<M>(p, w.span, w.page, pages, a, b), top, sum, x, stop + 1);
+                const T* q = static_cast<const T*>(p.q) + (w.q.q0 + token) * p.q_token + (w.head * p.group + g) * p.q_head;
+                const int32_t* table = p.table + w.row() * p.table_stride;
+                const PieceKeys keys = piece_keys<M>(p, w.span, w.page, pages, a, b);
+                // (A call from warps whose registers were raised finds none for its results.)
+                if (M == kPlain) row_by_definition<T, M>(p, q, table, w.head, keys, top, sum, x, stop + 1);
+                else row_by_definition_here<T, M>(p, q, table, w.head, keys, top, sum, x, stop + 1);
             } else {
                 const int stat = (lane & (kRowsWarps - 1)) * kRows + r;
                 const float mi = join_m[stat];
@@ -468,7 +503,7 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             // Piece i of the tile is CTA cta0 + i's.  The last CTA to finish joins them; where that is much to read for
             // one CTA, in two steps: the last of each group of neighbours joins these into its first, the last group
             // those.  Either way in the order of the pieces.
-            const int pieces = cta1 - cta0 + 1, mine = static_cast<int>(blockIdx.x) - cta0;
+            const int pieces = cta1 - cta0 + 1, mine = cta - cta0;
             auto slot_of = [&](int i) { return p.row_slots + static_cast<int64_t>(2 * (cta0 + i) + (i == 0)) * kRowSlot; };
             int group = pieces;
             if (pieces * w.rows > kJoinRows || pieces > 32) {
@@ -521,6 +556,22 @@ paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         w.advance(p, pages);
     }
     if (failed && tid == 0) atomicOr(p.status, 1u);
+}
+
+template <typename T, int M>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+paged_attend_rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                         const __grid_constant__ AttendParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ RowsControl c;
+    if (threadIdx.x == 0) c.init(k_map, v_map);
+    wait_for_earlier_kernels();
+    find_share<kRowsThreads, M>(p, rows_kind<M>(), tiles_kind<M>(p), &c.share, c.warp_sums);
+    dependents_may_launch();
+    const Walk<M> w = start_walk<M>(p, kRows, kRowsCost<M>, c.share);
+    if (threadIdx.x >= 32 * kRowsWarps) load_rows_pages<M>(k_map, v_map, p, c, c.share, smem_raw, w);
+    else attend_rows<T, M>(p, c, c.share, smem_raw, blockIdx.x, w);
 }
 
 // --------------------------------------------------------------- many rows
@@ -732,6 +783,7 @@ struct TilesControl {
     Share share;
     uint32_t tmem;
     int irregular;                       // what the guard found in the piece
+    int cta;                             // number of the CTA among those of this kind
     int stop[2];                         // a wait ran out, and work that lets waits go on
 };
 constexpr uint32_t kControlBytes = 8192 - 1024;   // operands follow at the next whole KiB, which the swizzle needs
@@ -741,9 +793,9 @@ constexpr uint32_t kTilesSmem = kControlBytes + 1024 + (2 + kRing) * kTileBytes 
 // After a wait that ran out, by the softmax warps: the rows of this CTA's share
 // become NaN, and so do its pieces of cut tiles.
 template <typename T, int M>
-__device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& share)
+__device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& share, int cta)
 {
-    const int tid = threadIdx.x, cta = blockIdx.x;
+    const int tid = threadIdx.x;
     if (tid == 0) atomicOr(p.status, 1u);
     Walk<M> w = start_walk<M>(p, 2 * (128 / p.group * p.group), tiles_cost<M>(p), share);
     for (bool first = true; w.left > 0; first = false) {
@@ -765,13 +817,50 @@ __device__ __noinline__ void fail_tiles(const AttendParams& p, const Share& shar
     }
 }
 
-template <typename T, int M>
-__global__ void __launch_bounds__(kTileThreads, 1)
-paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttendParams p)
+// By one thread, before a barrier of the block.
+__device__ __forceinline__ void init_tiles(TilesControl& c, const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map)
 {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    TilesControl& c = *reinterpret_cast<TilesControl*>(smem_raw);
+    for (int i = 0; i < kRing; ++i) {
+        barrier_init(smem_addr(&c.kv_full[i]), 1);
+        barrier_init(smem_addr(&c.kv_empty[i]), 3);    // each tile's products and the guard
+    }
+    barrier_init(smem_addr(&c.q_full), 1);
+    barrier_init(smem_addr(&c.q_empty), 2);
+    for (int w = 0; w < 2; ++w) {
+        barrier_init(smem_addr(&c.s_full[w]), 1);
+        barrier_init(smem_addr(&c.p_ready[w]), kSoftWarps);
+        barrier_init(smem_addr(&c.o_full[w]), 1);
+        barrier_init(smem_addr(&c.drained[w]), 1);
+    }
+    barrier_init(smem_addr(&c.checked), 1);
+    barrier_init(smem_addr(&c.taken), kSoftWarps);
+    for (int i = 0; i < kItems; ++i) barrier_init(smem_addr(&c.item_full[i]), 1);
+    c.stop[0] = c.stop[1] = 0;
+    c.irregular = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+}
+
+// By a warp: all of tensor memory.
+__device__ __forceinline__ void take_tensor_memory(TilesControl& c)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&c.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    tmem_fence_before();
+}
+__device__ __forceinline__ void return_tensor_memory(uint32_t tmem)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// The work of CTA c.cta of those for many rows, by all kTileThreads threads.  (The number is read where it is needed: the
+// softmax warps have no register for it.)
+template <typename T, int M>
+__device__ __forceinline__ void tiles_of_cta(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                                             const AttendParams& p, TilesControl& c, uint8_t* smem_raw)
+{
     volatile int* const stop = c.stop;
     const uint32_t q_smem = (smem_addr(smem_raw) + kControlBytes + 1023) & ~1023u, ring = q_smem + 2 * kTileBytes;
     auto kv_full = [&](int i) { return smem_addr(&c.kv_full[i]); };
@@ -785,40 +874,7 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
     const uint32_t checked = smem_addr(&c.checked), taken = smem_addr(&c.taken);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) {
-        for (int i = 0; i < kRing; ++i) {
-            barrier_init(kv_full(i), 1);
-            barrier_init(kv_empty(i), 3);    // each tile's products and the guard
-        }
-        barrier_init(q_full, 1);
-        barrier_init(q_empty, 2);
-        for (int w = 0; w < 2; ++w) {
-            barrier_init(s_full(w), 1);
-            barrier_init(p_ready(w), kSoftWarps);
-            barrier_init(o_full(w), 1);
-            barrier_init(drained(w), 1);
-        }
-        barrier_init(checked, 1);
-        barrier_init(taken, kSoftWarps);
-        for (int i = 0; i < kItems; ++i) barrier_init(item_full(i), 1);
-        c.stop[0] = c.stop[1] = 0;
-        c.irregular = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
-    }
-    if (warp == kSoftWarps + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&c.tmem)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-        tmem_fence_before();
-    }
-    // Beside the kernel for few rows this one starts as that one's CTAs leave: its inputs were complete before that one
-    // read them, the two share no memory that either writes, and it waits for that one at its end instead.
-    if (!p.both) wait_for_earlier_kernels();
     const int tokens = 128 / p.group, rows_per_tile = tokens * p.group;   // of one of the two tiles
-    find_share<kTileThreads, M, M != kPlain>(p, tiles_kind<M>(p), rows_kind<M>(), &c.share, c.warp_sums);
-    dependents_may_launch();
     tmem_fence_after();
     const uint32_t tmem = c.tmem;
     Walk<M> w = start_walk<M>(p, 2 * rows_per_tile, tiles_cost<M>(p), c.share);
@@ -866,15 +922,16 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
                     it.keys<M>(p, it.pos, unused, it.hi_all);
                     it.q0 = w.q.q0 + w.first_token;
                     const int cta0 = c.share.owner(w.tile_unit), cta1 = c.share.owner(w.tile_unit + w.span.pages - 1);
-                    it.slot = cta1 > cta0 ? 2 * static_cast<int>(blockIdx.x) + (cta0 == static_cast<int>(blockIdx.x)) : -1;
+                    const int cta = *static_cast<volatile int*>(&c.cta);
+                    it.slot = cta1 > cta0 ? 2 * cta + (cta0 == cta) : -1;
                     it.more = w.left > pages + w.cost;
                     barrier_arrive(item_full(item));
                     // Only the first tile of a CTA can have begun in an earlier one.
                     if (item == 0) {
                         Cut cut{};
-                        if (cta0 < static_cast<int>(blockIdx.x))
+                        if (cta0 < cta)
                             cut = Cut{cta1, cta0, w.rows, w.first_token, w.head, w.q.n, w.q.kv, w.q.q0, w.q.part};
-                        p.cuts[blockIdx.x] = cut;
+                        p.cuts[cta] = cut;
                     }
                 };
                 for (int i0 = 0; i0 < pages; i0 += 32) {
@@ -1351,14 +1408,87 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
             if (lane == 0) barrier_arrive(taken);
             if (last) break;
         }
-        if (tid == 0 && !any) p.cuts[blockIdx.x] = Cut{};
+        if (tid == 0 && !any) p.cuts[*static_cast<volatile int*>(&c.cta)] = Cut{};
     }
     tmem_fence_before();
     __syncthreads();
-    if (warp < kSoftWarps && (*stop || c.share.down)) fail_tiles<T, M>(p, c.share);
-    if (p.both) wait_for_earlier_kernels();
-    if (warp == kSoftWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp < kSoftWarps && (*stop || c.share.down)) fail_tiles<T, M>(p, c.share, *static_cast<volatile int*>(&c.cta));
 }
+
+template <typename T, int M>
+__global__ void __launch_bounds__(kTileThreads, 1)
+paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ AttendParams p)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    TilesControl& c = *reinterpret_cast<TilesControl*>(smem_raw);
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        init_tiles(c, q_map, k_map, v_map);
+        c.cta = blockIdx.x;
+    }
+    if (warp == kSoftWarps + 1) take_tensor_memory(c);
+    // Beside the kernel for few rows this one starts as that one's CTAs leave: its inputs were complete before that one
+    // read them, the two share no memory that either writes, and it waits for that one at its end instead.
+    if (!p.both) wait_for_earlier_kernels();
+    find_share<kTileThreads, M>(p, tiles_kind<M>(p), rows_kind<M>(), &c.share, c.warp_sums);
+    dependents_may_launch();
+    tiles_of_cta<T, M>(q_map, k_map, v_map, p, c, smem_raw);
+    if (p.both) wait_for_earlier_kernels();
+    if (warp == kSoftWarps + 1) return_tensor_memory(c.tmem);
+}
+
+// ---------------------------------------------------------------- both kinds
+//
+// Sequences of few rows beside chunks, or beside the prefixes that they share: one
+// launch, in which a CTA does the one or the other.  As two launches the second's
+// CTAs started 3.6 us later, where the first's had counted the work and left.
+template <typename T, int M>
+__global__ void __launch_bounds__(kTileThreads, 1)
+paged_attend_both_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap k_quarters,
+                         const __grid_constant__ CUtensorMap v_quarters, const __grid_constant__ AttendParams few,
+                         const __grid_constant__ AttendParams many)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ RowsControl rows;
+    TilesControl& c = *reinterpret_cast<TilesControl*>(smem_raw);
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        init_tiles(c, q_map, k_map, v_map);
+        rows.init(k_quarters, v_quarters);
+        c.cta = gridDim.x - 1 - blockIdx.x;   // if it takes tiles
+    }
+    if (warp == kSoftWarps + 1) take_tensor_memory(c);
+    wait_for_earlier_kernels();
+    int cta;
+    const bool first_kind = find_share_of_both<kTileThreads, M>(few, rows_kind<M>(), many, tiles_kind<M>(many), &c.share,
+                                                                 c.warp_sums, cta);
+    dependents_may_launch();
+    if (first_kind) {
+        // No tile is cut at this CTA, by its number among those for many rows.
+        if (threadIdx.x == 0) many.cuts[gridDim.x - 1 - blockIdx.x] = Cut{};
+        if (warp == kSoftWarps + 1) {
+            tmem_fence_after();
+            return_tensor_memory(c.tmem);
+        }
+        const Walk<M> w = start_walk<M>(few, kRows, kRowsCost<M>, c.share);
+        // 640 threads at 96 registers: 176 for the eight computing warps, 80 for the producer's warpgroup, 24 for the others.
+        if (warp >= kRowsWarps + 4) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        } else if (warp >= kRowsWarps) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+            if (warp == kRowsWarps) load_rows_pages<M>(k_quarters, v_quarters, few, rows, c.share, smem_raw + kControlBytes, w);
+        } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+            attend_rows<T, M>(few, rows, c.share, smem_raw + kControlBytes, cta, w);
+        }
+        return;
+    }
+    tiles_of_cta<T, M>(q_map, k_map, v_map, many, c, smem_raw);
+    if (warp == kSoftWarps + 1) return_tensor_memory(c.tmem);
+}
+static_assert(kControlBytes + kRowsSmem <= kTilesSmem, "either kind's memory");
 
 // Joins the pieces of tiles that were cut over CTAs, in the order of the pieces.
 // A lane takes a row, as the pieces lie, and kFours times four of its values;
@@ -1464,7 +1594,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     if (M == kShared) dependents_may_launch();   // what joins the parts finds its rows meanwhile
     wait_for_earlier_kernels();
     if (M != kShared) dependents_may_launch();
-    if (M != kPlain && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.status[1] = 0;
     const Cut cut = p.cuts[blockIdx.y];
     if (cut.cta1 == 0) return;
     const int sharers = cut.cta1 - cut.cta0, k = blockIdx.y - cut.cta0 - 1;
@@ -1491,87 +1620,85 @@ int attend_grid()
     return n;
 }
 
-struct Device {
-    bool rows_set[3][2] = {};
-    bool tiles_set[3][2] = {};
-};
-std::mutex g_mu;
-Device g_devices[64];
-
-template <typename T, int M>
-int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, cudaStream_t stream)
+// A launch on the current device of one block per SM, or of `grid`, that may begin before the kernels ahead end.
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, uint32_t shared, KernelKind kind, cudaStream_t stream,
+                   const Args&... args)
 {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const int grid = attend_grid();
-    {
-        std::lock_guard<std::mutex> lock(g_mu);
-        Device& d = g_devices[dev & 63];
-        bool& set = d.rows_set[M][std::is_same<T, __half>::value];
-        if (!set) {
-            const cudaError_t e = cudaFuncSetAttribute(paged_attend_rows_kernel<T, M>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
-            if (e != cudaSuccess) return e;
-            set = true;
-        }
-    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kRowsThreads);
-    cfg.dynamicSmemBytes = kRowsSmem;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    ProfileScope prof(kKernAttendRows, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_rows_kernel<T, M>, k_map, v_map, p);
+    ProfileScope prof(kind, stream);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+std::mutex g_mu;
+
+// Before a kernel's first launch on the current device: its shared memory, and whether its block has the registers that
+// its warps take over from one another, without which they would wait for ever.
+template <class Kernel>
+cudaError_t prepare(Kernel kernel, bool (&set)[64], uint32_t shared, int threads, int registers)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (set[dev & 63]) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (e != cudaSuccess) return e;
+    cudaFuncAttributes made;
+    e = cudaFuncGetAttributes(&made, kernel);
+    if (e != cudaSuccess) return e;
+    if (made.numRegs * threads < registers) return cudaErrorLaunchOutOfResources;
+    set[dev & 63] = true;
+    return cudaSuccess;
+}
+constexpr int kTilesRegisters = 32 * (104 * kSoftWarps + 64 * 4);
+constexpr int kBothRegisters = 32 * (176 * kRowsWarps + 80 * 4 + 24 * (kTileThreads / 32 - kRowsWarps - 4));
+static_assert(kBothRegisters <= kTilesRegisters, "the tiles' split is the larger one");
+
+template <typename T, int M>
+int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, cudaStream_t stream)
+{
+    static bool set[64];
+    const cudaError_t e = prepare(paged_attend_rows_kernel<T, M>, set, kRowsSmem, kRowsThreads, 0);
+    if (e != cudaSuccess) return e;
+    return launch(paged_attend_rows_kernel<T, M>, dim3(attend_grid()), kRowsThreads, kRowsSmem, kKernAttendRows, stream, k_map,
+                  v_map, p);
 }
 
 template <typename T, int M>
 int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p,
                  cudaStream_t stream)
 {
-    int dev = 0;
-    cudaGetDevice(&dev);
+    static bool set[64];
+    cudaError_t e = prepare(paged_attend_tiles_kernel<T, M>, set, kTilesSmem, kTileThreads, kTilesRegisters);
+    if (e != cudaSuccess) return e;
     const int grid = attend_grid();
-    {
-        std::lock_guard<std::mutex> lock(g_mu);
-        Device& d = g_devices[dev & 63];
-        bool& set = d.tiles_set[M][std::is_same<T, __half>::value];
-        if (!set) {
-            cudaError_t e = cudaFuncSetAttribute(paged_attend_tiles_kernel<T, M>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kTilesSmem);
-            if (e != cudaSuccess) return e;
-            // The softmax warps' registers come from what the block was launched with, or they would wait for ever.
-            cudaFuncAttributes made;
-            e = cudaFuncGetAttributes(&made, paged_attend_tiles_kernel<T, M>);
-            if (e != cudaSuccess) return e;
-            if (made.numRegs * kTileThreads < 32 * (104 * kSoftWarps + 64 * 4)) return cudaErrorLaunchOutOfResources;
-            set = true;
-        }
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kTileThreads);
-    cfg.dynamicSmemBytes = kTilesSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    {
-        ProfileScope prof(kKernAttendTiles, stream);
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attend_tiles_kernel<T, M>, q_map, k_map, v_map, p);
-        if (e != cudaSuccess) return e;
-    }
-    cfg.gridDim = dim3(kJoinBlocks, grid);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.dynamicSmemBytes = 0;
-    ProfileScope prof(kKernAttendJoin, stream);
-    return cudaLaunchKernelEx(&cfg, paged_attend_join_kernel<T, M>, p);
+    e = launch(paged_attend_tiles_kernel<T, M>, dim3(grid), kTileThreads, kTilesSmem, kKernAttendTiles, stream, q_map, k_map,
+               v_map, p);
+    if (e != cudaSuccess) return e;
+    return launch(paged_attend_join_kernel<T, M>, dim3(kJoinBlocks, grid), kJoinThreads, 0, kKernAttendJoin, stream, p);
+}
+
+template <typename T, int M>
+int launch_both(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const CUtensorMap& k_quarters,
+                const CUtensorMap& v_quarters, const AttendParams& few, const AttendParams& many, cudaStream_t stream)
+{
+    static bool set[64];
+    cudaError_t e = prepare(paged_attend_both_kernel<T, M>, set, kTilesSmem, kTileThreads, kTilesRegisters);
+    if (e != cudaSuccess) return e;
+    const int grid = attend_grid();
+    e = launch(paged_attend_both_kernel<T, M>, dim3(grid), kTileThreads, kTilesSmem, kKernAttendBoth, stream, q_map, k_map, v_map,
+               k_quarters, v_quarters, few, many);
+    if (e != cudaSuccess) return e;
+    return launch(paged_attend_join_kernel<T, M>, dim3(kJoinBlocks, grid), kJoinThreads, 0, kKernAttendJoin, stream, many);
 }
 
 // f(type, mode) for the call's type and mode.
@@ -1604,6 +1731,17 @@ int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const
     return by_type_and_mode(dtype, mode, [&](auto type, auto m) {
         return launch_rows<decltype(type), decltype(m)::value>(k_map, v_map, p, stream);
     });
+}
+
+int launch_attend_both(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                       const CUtensorMap& k_quarters, const CUtensorMap& v_quarters, const AttendParams& few,
+                       const AttendParams& many, Mode mode, uint32_t dtype, cudaStream_t stream)
+{
+    const auto with = [&](auto type) -> int {
+        return mode == kSinks ? launch_both<decltype(type), kSinks>(q_map, k_map, v_map, k_quarters, v_quarters, few, many, stream)
+                              : launch_both<decltype(type), kShared>(q_map, k_map, v_map, k_quarters, v_quarters, few, many, stream);
+    };
+    return dtype == SECURE_INFER_FP16 ? with(__half{}) : with(__nv_bfloat16{});
 }
 
 uint64_t attend_workspace_bytes()
