@@ -6,7 +6,9 @@ a small stack of attention layers with random weights: each layer appends its
 keys and values to the paged cache and attends as soon as its prefix is
 authentic.  The request is then forked into several answers that share the
 prompt's pages, each is continued token by token, some end and give up their
-pages, the cache is compacted, and the others go on.
+pages, the cache is compacted, and the others go on.  What the answers share is
+found once a step (``SharedPrefix``), and attended once for all of them where that
+saves time.
 
     python examples/parallel_answers.py [--layers 4] [--answers 4] [--steps 6]
 
@@ -36,13 +38,13 @@ class Layer:
         self.qkv = torch.randn((HEADS * DIM, (HEADS + 2 * KV_HEADS) * DIM), generator=g, device="cuda").mul_(0.03).bfloat16()
         self.out = torch.randn((HEADS * DIM, HEADS * DIM), generator=g, device="cuda").mul_(0.03).bfloat16()
 
-    def __call__(self, x, pages, chunk, rotary, ready=None):
+    def __call__(self, x, pages, chunk, rotary, ready=None, shared=None):
         qkv = (x @ self.qkv).unflatten(1, (-1, DIM))
         q, k, v = qkv.split((HEADS, KV_HEADS, KV_HEADS), 1)
         q = paged.append(pages, chunk, q, k, v, rotary=rotary)
         if ready is not None:
             ready()   # the layer's reloaded prefix is authentic and ordered before what follows
-        self.attended = paged.attend(pages, chunk, q)
+        self.attended = paged.attend(pages, chunk, q, shared=shared)
         self.query = q
         return x + self.attended.flatten(1) @ self.out
 
@@ -97,8 +99,9 @@ def run(layers=4, prefix_blocks=6, chunk_tokens=75, answers=4, steps=6, check=Fa
             tables, granted = cache.reserve(tables, ints(alive), tables.lens[rows] + 1)
             assert granted.all()
             chunk = paged.Chunk(tables.block_table[rows], ints(list(range(len(alive) + 1))), tables.lens[rows], max_q=1)
+            shared = paged.SharedPrefix(chunk)
             for i, layer in enumerate(stack):
-                x = layer(x, cache.layers[i], chunk, rotary)
+                x = layer(x, cache.layers[i], chunk, rotary, shared=shared)
         say(f"{steps} tokens for each answer; lengths {tables.lens.tolist()}")
         off = 0.0
         if check:

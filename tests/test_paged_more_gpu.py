@@ -673,6 +673,52 @@ def test_attention_after_a_trim(paged):
     assert most <= 2 * (1 + 4) and int(t.lens.sum()) > 2500
 
 
+@pytest.mark.parametrize("answers,prompt,dtype", [(2, 300, torch.bfloat16), (24, 2300, torch.float16), (40, 5000, torch.bfloat16)])
+def test_answers_from_a_prompt_to_their_end(paged, answers, prompt, dtype):
+    """Reserve, append, fork, and then token by token: append, find what is shared, attend with it, and the same from
+    two parts joined.  All that the answers have in common is found, and every way gives one result."""
+    heads, kv_heads, pages = 32, 8, 60 + 2 * answers
+    g = torch.Generator(device="cuda").manual_seed(answers)
+    cache = paged.CachePages([[torch.full((pages, 128, kv_heads, 128), math.nan, dtype=dtype, device="cuda") for _ in range(2)]])
+    layer, rotary = cache.layers[0], paged.Rotary(base=500000.0, device="cuda:0")
+    t = paged.PageTables(torch.full((answers, 50), -1, dtype=torch.int32, device="cuda"), ints([0] * answers), ints([0] * pages))
+    t, granted = cache.reserve(t, [0], [prompt])
+    assert granted.tolist() == [1]
+    rand = lambda n, h: torch.randn((n, h, 128), generator=g, device="cuda").to(dtype)  # noqa: E731
+    first = paged.Chunk(t.block_table[:1], ints([0, prompt]), t.lens[:1])
+    paged.append(layer, first, None, rand(prompt, kv_heads), rand(prompt, kv_heads), rotary=rotary)
+    t, granted = cache.fork(t, [0] * (answers - 1), list(range(1, answers)))
+    assert granted.all()
+    for step in range(3):
+        t, granted = cache.reserve(t, list(range(answers)), [prompt + step + 1] * answers)
+        assert granted.all()
+        chunk = paged.Chunk(t.block_table, ints(list(range(answers + 1))), t.lens, max_q=1)
+        q = paged.append(layer, chunk, 2 * rand(answers, heads), rand(answers, kv_heads), rand(answers, kv_heads), rotary=rotary)
+        shared, common = paged.SharedPrefix(chunk), prompt // 128 * 128
+        assert shared.tokens.tolist() == [common] * answers
+        apart, apart_lse = paged.attend(layer, chunk, q, return_lse=True)
+        out, lse = paged.attend(layer, chunk, q, shared=shared, return_lse=True)
+        head = paged.Chunk(t.block_table, chunk.cu_q, ints([common] * answers), max_q=1)
+        rest = paged.Chunk(t.block_table[:, common // 128:], chunk.cu_q, t.lens - common, max_q=1)
+        parts = [paged.attend(layer, head, q, causal=False, return_lse=True), paged.attend(layer, rest, q, return_lse=True)]
+        joined, joined_lse = paged.join(*zip(*parts))
+        rows = t.block_table.long()
+        k, v = (x[rows].flatten(1, 2)[:, :prompt + step + 1].double().repeat_interleave(heads // kv_heads, 2) for x in (layer.k, layer.v))
+        x = torch.einsum("shd,skhd->shk", q.double(), k) * 128 ** -0.5
+        w = torch.softmax(x, -1)
+        want, mass = torch.einsum("shk,skhd->shd", w, v), torch.einsum("shk,skhd->shd", w, v.abs())
+        tail = (prompt + 3) * 2.0 ** -25 * v.abs().amax() if dtype == torch.float16 else 0.0
+        bound = EPS[dtype] * want.abs() + (EPS[dtype] + 2e-4) * mass + tail + 1e-7
+        for got, got_lse in ((apart, apart_lse), (out, lse)):
+            assert ((got.double() - want).abs() <= bound).all()
+            assert (got_lse.double() - torch.logsumexp(x, -1)).abs().max() <= 3e-4
+        # The parts were rounded once more.
+        assert ((joined.double() - want).abs() <= bound + EPS[dtype] * sum(p[0].double().abs() for p in parts)).all()
+        assert (joined_lse.double() - torch.logsumexp(x, -1)).abs().max() <= 3e-4
+    t = cache.free(t, list(range(answers)))
+    assert not t.refs.any()
+
+
 # ----------------------------------------------------------------- refusals
 
 def test_refusals(paged):
