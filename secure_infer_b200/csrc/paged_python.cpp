@@ -312,11 +312,24 @@ Tables tables(PyObject* const* a, int64_t pages, int64_t device)
     return t;
 }
 
+// Part of a dense tensor from element `first` on, in a shape.
+at::Tensor part_of(const at::Tensor& t, int64_t first, at::IntArrayRef sizes)
+{
+    at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+    part.unsafeGetTensorImpl()->set_storage_offset(t.storage_offset() + first);
+    part.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return part;
+}
+
 // New tables of the same shapes, or the given ones.
 Tables outputs(PyObject* given, const Tables& in, int64_t pages, int64_t device)
 {
     if (given == Py_None) {
-        Tables t{at::empty_like(in.table), at::empty_like(in.lens), at::empty_like(in.refs), in.c};
+        // In one piece of memory, each from a whole 256 bytes on: an allocation takes the host 1.0 us.
+        const auto end = [](int64_t ints) { return (ints + 63) / 64 * 64; };
+        const int64_t lens = end(in.table.numel()), refs = lens + end(in.lens.numel());
+        const at::Tensor all = at::empty({refs + end(in.refs.numel())}, in.table.options());
+        Tables t{part_of(all, 0, in.table.sizes()), part_of(all, lens, in.lens.sizes()), part_of(all, refs, in.refs.sizes()), in.c};
         t.c.block_table = static_cast<int32_t*>(t.table.data_ptr());
         t.c.lens = static_cast<int32_t*>(t.lens.data_ptr());
         t.c.refs = static_cast<int32_t*>(t.refs.data_ptr());
