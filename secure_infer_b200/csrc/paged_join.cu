@@ -13,15 +13,18 @@ namespace {
 //
 // A block per group.  A page is common when every sequence of the group that has
 // new tokens names it in the same place, and all of its tokens lie before the
-// first new one of each: every new token sees all of them.  A warp compares a
-// sequence's row with the first one's, 32 pages at a time, to the first that
-// differs.  Once a step for all its layers: bound by the latency of its reads.
-constexpr int kPrefixThreads = 256;
+// first new one of each: every new token sees all of them.  A thread compares a
+// column of the sequences' rows with the first one's, 64 columns at a time until
+// one differs, eight rows on their way at once.  Once a step for all its layers:
+// bound by the latency of its reads.  Measured: 48 sequences with 64 pages in common
+// 3.4 us, four groups of six with up to 234 4.5, 1024 with 64 17 (78 by a warp a row).
+constexpr int kPrefixThreads = 1024;
+constexpr int kPrefixColumns = 64;
 
 __global__ void __launch_bounds__(kPrefixThreads) shared_prefix_kernel(const __grid_constant__ PrefixParams p)
 {
     __shared__ int first, end, lead, members, common;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x;
+    const int tid = threadIdx.x, g = blockIdx.x;
     wait_for_earlier_kernels();
     dependents_may_launch();
     if (tid == 0) {
@@ -55,18 +58,19 @@ __global__ void __launch_bounds__(kPrefixThreads) shared_prefix_kernel(const __g
     }
     __syncthreads();
     if (members > 1) {
-        const int32_t* row = p.table + lead * p.table_stride;
-        for (int s = first + warp; s < end; s += kPrefixThreads / 32) {
-            if (s == lead || new_tokens(s) == 0) continue;
-            const int32_t* other = p.table + s * p.table_stride;
-            const int pages = *static_cast<volatile int*>(&common);   // others may find fewer meanwhile
-            for (int c0 = 0; c0 < pages; c0 += 32) {
-                const int c = c0 + lane;
-                const uint32_t differ = __ballot_sync(0xffffffffu, c < pages && row[c] != other[c]);
-                if (differ == 0) continue;
-                if (lane == 0) atomicMin(&common, c0 + __ffs(differ) - 1);
-                break;
+        constexpr int kRowsAtOnce = kPrefixThreads / kPrefixColumns;
+        for (int c0 = 0; c0 < common; c0 += kPrefixColumns) {
+            const int c = c0 + tid % kPrefixColumns;
+            bool differs = false;
+            if (c < common) {
+                const int32_t page = p.table[lead * p.table_stride + c];
+#pragma unroll 8
+                for (int s = first + tid / kPrefixColumns; s < end; s += kRowsAtOnce)
+                    differs |= p.table[s * p.table_stride + c] != page && new_tokens(s) != 0;
             }
+            __syncthreads();   // all have read how many there are
+            if (differs) atomicMin(&common, c);
+            __syncthreads();
         }
     }
     __syncthreads();

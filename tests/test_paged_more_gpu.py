@@ -188,6 +188,22 @@ def test_long_contexts_with_sinks_repeat(paged, lens, window, sinks):
         assert torch.equal(out, again) and torch.equal(lse, again_lse)
 
 
+def test_many_sequences_of_both_kinds_with_sinks(paged):
+    """More sequences than a block has threads, chunks among single tokens and drafts; the same bits again."""
+    c = Seen(paged, [(40 if i % 7 == 0 else 1 + i % 4, 40 + (i * 37) % 500) for i in range(1400)], 8, 2)
+    out, lse = c.attend(paged, 60, 5)
+    c.check(out, lse, window=60, sinks=5)
+    again, again_lse = c.attend(paged, 60, 5)
+    assert torch.equal(out, again) and torch.equal(lse, again_lse)
+
+
+@pytest.mark.parametrize("lens", [[(1, 20000)] * 30 + [(30, 50)], [(2000, 2100)] + [(1, 40)] * 3, [(24, 300), (25, 300), (3, 9000)]])
+def test_one_kind_has_most_of_the_work(paged, lens):
+    c = Seen(paged, lens, 4, 4)
+    out, lse = c.attend(paged, 9000, 8)
+    c.check(out, lse, window=9000, sinks=8)
+
+
 @pytest.mark.parametrize("layout", ["heads", "joint"])
 def test_layouts_with_sinks(paged, layout):
     c = Seen(paged, [(1, 700), (3, 300), (150, 800)], 12, 2, layout=layout)
