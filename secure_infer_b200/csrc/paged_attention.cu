@@ -88,8 +88,8 @@ constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + 2 * kRows * 
 // Units up to which a tile is not cut where there is little work, with a cost of 1.
 // One sequence of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
 constexpr int kRowsWhole = 4;
-// Pages that a tile's beginning and end are worth.  Measured: its queries 0.7 us, its end 1.1, where a page takes 1.1 to
-// 1.4; the usual call keeps the 1 that its results' order of sums goes by.
+// Pages that a tile's beginning and end are worth: with sinks and shared prefixes 2, where 48 answers to 8192 take 45.2 us
+// (1: 50.5, 3: 47.6); the usual call keeps the 1 that its results' order of sums goes by.
 template <int M>
 constexpr int kRowsCost = M == kPlain ? 1 : 2;
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
@@ -1442,7 +1442,10 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 //
 // Sequences of few rows beside chunks, or beside the prefixes that they share: one
 // launch, in which a CTA does the one or the other.  As two launches the second's
-// CTAs started 3.6 us later, where the first's had counted the work and left.
+// CTAs started 3.6 us later, where the first's had counted the work and left: 777
+// tokens and 3 single ones with sinks 45.5 us for 43.5 (floor 8.6), drawn calls up
+// to 16 % more, 48 answers to a prompt of 8192 45.5 for 47.8 (floor 18.3, reading
+// their pages).  Bound by its start, 5 us to the first scores, and by tiles' ends.
 template <typename T, int M>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_attend_both_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
