@@ -62,6 +62,7 @@ struct AttendParams {
     Cut* cuts;                      // [grid]
     float* slots;                   // [2 * grid] partial results of tiles
     float* row_slots;               // and of the kernel for few rows
+    int32_t few_cuts;               // little work for tiles: few of them are cut
     int32_t both;                   // the call has a launch for few rows, and then one for the others, on the same SMs
     int32_t sinks;                  // kSinks: the first tokens that stay visible
     const int32_t* prefix;          // kShared: [seqs] keys in common with the sequence's group

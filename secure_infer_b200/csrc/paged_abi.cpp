@@ -346,6 +346,13 @@ SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_
     // Hidden scores are -inf before they are scaled, so the scale is never zero; at 1e-30 all weights are 1.
     if (p.scale_log2 > -1e-30f && p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
     attend_workspace(workspace, &p);
+    // At most eight units of work for each of 148 SMs, by the pages that a tile may see.
+    const uint64_t rows = static_cast<uint64_t>(chunk->tokens) * group;
+    const uint64_t seen = (static_cast<uint64_t>(p.window) + 256 / group) / kPage + 2 + sinks / kPage + 1;
+    const uint64_t span = p.window != 0 && seen < chunk->table_width ? seen : chunk->table_width;
+    const uint64_t several = rows / (kFewRows + 1) < chunk->seqs ? rows / (kFewRows + 1) : chunk->seqs;
+    const uint64_t tiles_most = (groups > 0 ? 2 : 1) * rows / 256 + several + groups + 1;
+    p.few_cuts = work.tiles && tiles_most * pages->heads * (span + 2) <= 8 * 148;
     const auto st = static_cast<cudaStream_t>(stream);
     // One call's launches follow one another on the stream: they hand the workspace on.
     static std::mutex launches;

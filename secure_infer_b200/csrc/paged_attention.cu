@@ -1499,9 +1499,12 @@ static_assert(kControlBytes + kRowsSmem <= kTilesSmem, "either kind's memory");
 // in many pieces has more warps.  Bound by reading the pieces from L2 and by
 // latency, so all blocks are there at once: two warps each (eight, with four of
 // them on a value's pieces, had to take turns: 10 us more where every CTA ends a
-// tile).
-constexpr int kJoinThreads = 64;
-constexpr int kJoinBlocks = kTileRows / 32 * (kDim / 16) / (kJoinThreads / 32);
+// tile).  Most blocks find no cut, and take a while to come and go all the same:
+// where the work is little, and few tiles are cut, blocks of eight warps (a call
+// with little for tiles 14.4 us for 18.0; 777 tokens with sinks 44.3 for 43.4), and
+// with sinks or shared prefixes never less than four (48 answers 46.0 for 47.9).
+constexpr int kJoinThreads = 256;   // at most
+constexpr int kJoinWarps = kTileRows / 32 * (kDim / 16);
 template <typename T, int M, int kFours>
 __device__ __forceinline__ void join_values(const AttendParams& p, const Cut& cut, int r, int tile_row, int d4)
 {
@@ -1601,7 +1604,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attend_join_kernel(const _
     if (cut.cta1 == 0) return;
     const int sharers = cut.cta1 - cut.cta0, k = blockIdx.y - cut.cta0 - 1;
     const int fours = sharers >= 4 ? 1 : sharers >= 2 ? 2 : 4;
-    const int part = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), d4 = part % 8 * 4 + k * fours;
+    const int part = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5), d4 = part % 8 * 4 + k * fours;
     const int rows_per_tile = 128 / p.group * p.group, r = part / 8 * 32 + (threadIdx.x & 31);
     const int tile_row = r < 128 ? (r < rows_per_tile ? r : cut.rows) : (r - 128 < rows_per_tile ? rows_per_tile + r - 128 : cut.rows);
     if (k * fours >= 4 || tile_row >= cut.rows) return;
@@ -1677,6 +1680,14 @@ int launch_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Attend
 }
 
 template <typename T, int M>
+cudaError_t launch_tiles_join(const AttendParams& p, cudaStream_t stream)
+{
+    const int threads = p.few_cuts ? kJoinThreads : M == kPlain ? 64 : 128;
+    return launch(paged_attend_join_kernel<T, M>, dim3(kJoinWarps / (threads / 32), attend_grid()), threads, 0, kKernAttendJoin,
+                  stream, p);
+}
+
+template <typename T, int M>
 int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p,
                  cudaStream_t stream)
 {
@@ -1687,7 +1698,7 @@ int launch_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUten
     e = launch(paged_attend_tiles_kernel<T, M>, dim3(grid), kTileThreads, kTilesSmem, kKernAttendTiles, stream, q_map, k_map,
                v_map, p);
     if (e != cudaSuccess) return e;
-    return launch(paged_attend_join_kernel<T, M>, dim3(kJoinBlocks, grid), kJoinThreads, 0, kKernAttendJoin, stream, p);
+    return launch_tiles_join<T, M>(p, stream);
 }
 
 template <typename T, int M>
@@ -1701,7 +1712,7 @@ int launch_both(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtens
     e = launch(paged_attend_both_kernel<T, M>, dim3(grid), kTileThreads, kTilesSmem, kKernAttendBoth, stream, q_map, k_map, v_map,
                k_quarters, v_quarters, few, many);
     if (e != cudaSuccess) return e;
-    return launch(paged_attend_join_kernel<T, M>, dim3(kJoinBlocks, grid), kJoinThreads, 0, kKernAttendJoin, stream, many);
+    return launch_tiles_join<T, M>(many, stream);
 }
 
 // f(type, mode) for the call's type and mode.
