@@ -76,7 +76,7 @@ struct AttendParams {
 // Launchers (cudaError_t values).
 int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, Mode mode,
                        uint32_t dtype, cudaStream_t stream);
-// q_map: boxes of [128 / group tokens][group heads][64 values].
+// q_map: boxes of [128 / group tokens][group heads][64 values].  Not for kShared, which has several sequences.
 int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
                         const AttendParams& p, Mode mode, uint32_t dtype, cudaStream_t stream);
 // Both kinds of sequences in one launch, not for kPlain.  quarters: the maps of the rows' kernel; few and many: the

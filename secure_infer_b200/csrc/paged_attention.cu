@@ -1715,18 +1715,11 @@ int launch_both(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtens
     return launch_tiles_join<T, M>(many, stream);
 }
 
-// f(type, mode) for the call's type and mode.
+// f(type) for the call's type.
 template <class F>
-int by_type_and_mode(uint32_t dtype, Mode mode, F f)
+int by_type(uint32_t dtype, F f)
 {
-    const auto by_mode = [&](auto type) {
-        switch (mode) {
-            case kSinks: return f(type, std::integral_constant<int, kSinks>{});
-            case kShared: return f(type, std::integral_constant<int, kShared>{});
-            default: return f(type, std::integral_constant<int, kPlain>{});
-        }
-    };
-    return dtype == SECURE_INFER_FP16 ? by_mode(__half{}) : by_mode(__nv_bfloat16{});
+    return dtype == SECURE_INFER_FP16 ? f(__half{}) : f(__nv_bfloat16{});
 }
 
 }  // namespace
@@ -1734,16 +1727,21 @@ int by_type_and_mode(uint32_t dtype, Mode mode, F f)
 int launch_attend_tiles(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map,
                         const AttendParams& p, Mode mode, uint32_t dtype, cudaStream_t stream)
 {
-    return by_type_and_mode(dtype, mode, [&](auto type, auto m) {
-        return launch_tiles<decltype(type), decltype(m)::value>(q_map, k_map, v_map, p, stream);
+    return by_type(dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        return mode == kSinks ? launch_tiles<T, kSinks>(q_map, k_map, v_map, p, stream)
+                              : launch_tiles<T, kPlain>(q_map, k_map, v_map, p, stream);
     });
 }
 
 int launch_attend_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const AttendParams& p, Mode mode,
                        uint32_t dtype, cudaStream_t stream)
 {
-    return by_type_and_mode(dtype, mode, [&](auto type, auto m) {
-        return launch_rows<decltype(type), decltype(m)::value>(k_map, v_map, p, stream);
+    return by_type(dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        return mode == kSinks    ? launch_rows<T, kSinks>(k_map, v_map, p, stream)
+               : mode == kShared ? launch_rows<T, kShared>(k_map, v_map, p, stream)
+                                 : launch_rows<T, kPlain>(k_map, v_map, p, stream);
     });
 }
 
@@ -1751,11 +1749,11 @@ int launch_attend_both(const CUtensorMap& q_map, const CUtensorMap& k_map, const
                        const CUtensorMap& k_quarters, const CUtensorMap& v_quarters, const AttendParams& few,
                        const AttendParams& many, Mode mode, uint32_t dtype, cudaStream_t stream)
 {
-    const auto with = [&](auto type) -> int {
-        return mode == kSinks ? launch_both<decltype(type), kSinks>(q_map, k_map, v_map, k_quarters, v_quarters, few, many, stream)
-                              : launch_both<decltype(type), kShared>(q_map, k_map, v_map, k_quarters, v_quarters, few, many, stream);
-    };
-    return dtype == SECURE_INFER_FP16 ? with(__half{}) : with(__nv_bfloat16{});
+    return by_type(dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        return mode == kSinks ? launch_both<T, kSinks>(q_map, k_map, v_map, k_quarters, v_quarters, few, many, stream)
+                              : launch_both<T, kShared>(q_map, k_map, v_map, k_quarters, v_quarters, few, many, stream);
+    });
 }
 
 uint64_t attend_workspace_bytes()
