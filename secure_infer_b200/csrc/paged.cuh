@@ -553,14 +553,6 @@ struct Kind {
     int later;    // in one launch: how much later than the other kind's its first scores are there, in the measure of time
 };
 
-// All threads of the block take part; `warp_sums` holds three values per warp.
-// Where no tile has more than `whole` units a CTA gets the largest one's:
-// cutting it would cost more than the few pages that it would save.  Where the
-// call has work of both kinds each gets SMs by the time that its units take:
-// the first CTAs of a launch work and the others leave theirs to the other
-// launch, so reading pages for few rows goes on beside the products of many: 333
-// tokens after 2167 and 15 single tokens of up to 4000 take 53 us, 62 one kind
-// after the other.
 // SMs for `units` of a kind beside `others` of the other, in launches of their own.
 __device__ __forceinline__ int sms_of(const Kind& kind, int units, const Kind& other, int others)
 {
@@ -587,6 +579,14 @@ __device__ __forceinline__ int sms_for_few(const Kind& few, int units, const Kin
     return end(high) < end(low) ? high : low;
 }
 
+// All threads of the block take part; `warp_sums` holds three values per warp.
+// Where no tile has more than `whole` units a CTA gets the largest one's:
+// cutting it would cost more than the few pages that it would save.  Where the
+// call has work of both kinds each gets SMs by the time that its units take:
+// the first CTAs of a launch work and the others leave theirs to the other
+// launch, so reading pages for few rows goes on beside the products of many: 333
+// tokens after 2167 and 15 single tokens of up to 4000 take 53 us, 62 one kind
+// after the other.
 template <int kThreads, int M>
 __device__ __forceinline__ void find_share(const AttendParams& p, const Kind& kind, const Kind& other, Share* share,
                                            int32_t* warp_sums)
