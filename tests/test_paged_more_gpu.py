@@ -631,6 +631,32 @@ def test_trim(paged, seqs, width, pages, window, sinks):
     assert all(torch.equal(a, b) for a, b in zip(cache.trim(t, [], window), t))
 
 
+def test_new_tables_are_tensors_like_others(paged):
+    """Whatever memory they share: written in place, saved, moved, made in inference mode and in a graph."""
+    import io
+
+    t, data, cache = model_of(paged, 8, 20, 200, 9)
+    want = trimmed(t, [0, 2, 4, 6], 100, 3)
+    for mode in (torch.inference_mode, torch.no_grad, torch.enable_grad):
+        with mode():
+            new = cache.trim(t, [0, 2, 4, 6], 100, 3)
+            assert all(torch.equal(a.cpu(), b) and a.is_contiguous() for a, b in zip(new, want))
+            new.lens.add_(1)
+            new.refs.zero_()
+            assert torch.equal(new.block_table.cpu(), want[0]) and torch.equal(new.lens.cpu(), want[1] + 1)
+    file = io.BytesIO()
+    torch.save(tuple(new), file)
+    file.seek(0)
+    assert all(torch.equal(a, b) for a, b in zip(torch.load(file), new))
+    named, graph = ints([0, 2, 4, 6]), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        made = cache.trim(cache.trim(t, named, 100, 3), named, 100, 3)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(made, want))
+
+
 def test_tables_after_a_trim(paged):
     """Trimmed sequences grow, fork, move and end like others."""
     t, data, cache = model_of(paged, 12, 40, 400, 3, share=False)
