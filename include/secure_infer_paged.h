@@ -137,7 +137,8 @@ int secure_infer_shared_prefix(const secure_infer_chunk* chunk, const int32_t* c
 /* Attention over all keys from attention over n sets of them that have none in
  * common, 1 <= n <= SECURE_INFER_JOIN_PARTS: lse = log sum e^lse_i and out = sum
  * e^(lse_i - lse) out_i.  A part with lse_i = -inf counts for nothing, whatever
- * its out_i holds; where all are, out is 0 and lse -inf.  A part's out:
+ * its out_i holds; where all are, out is 0 and lse -inf.  One of NaN, as attention
+ * that failed gives it, makes out and lse NaN beside any others.  A part's out:
  * [tokens][heads][128] of `dtype` with its strides (token, head) in elements,
  * multiples of 16 bytes; its lse: [tokens][heads] with strides.  out, lse: dense;
  * out may be one part's own where that is dense. */

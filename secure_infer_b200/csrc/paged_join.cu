@@ -147,9 +147,9 @@ __global__ void __launch_bounds__(kJoinPartsThreads) join_parts_kernel(const __g
         x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(part.out) + token * part.out_stride[0] +
                                                head * part.out_stride[1] + sub * 8);
     }
-    float top = lse[0];
+    float top = lse[0];   // NaN where one of them is, which fmaxf would pass over: the row failed then
 #pragma unroll
-    for (int i = 1; i < kParts; ++i) top = fmaxf(top, lse[i]);
+    for (int i = 1; i < kParts; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(lse[i]));
     const float base = top == -INFINITY ? 0.0f : top;
     float total = 0.0f, y[8] = {};
 #pragma unroll

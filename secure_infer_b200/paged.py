@@ -294,7 +294,8 @@ def join(outs, lses, *, out: torch.Tensor | None = None):
     ``lses`` float32 ``[tokens, heads]``, as ``attend`` returns them with
     ``return_lse``.  Returns ``out`` (given: it may be one of ``outs``) and the
     logarithms of all sums.  A part whose logarithm is -inf counts for nothing,
-    whatever it holds; a row that sees no key of any gives 0 and -inf."""
+    whatever it holds; a row that sees no key of any gives 0 and -inf, and one with
+    a logarithm of NaN, as ``attend`` leaves it where it failed, gives NaN."""
     outs, lses = tuple(outs), tuple(lses)
     if not outs or not isinstance(outs[0], torch.Tensor) or not outs[0].is_cuda:
         raise ValueError("outs must be tensors on a CUDA device")

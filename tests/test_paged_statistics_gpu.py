@@ -1,0 +1,77 @@
+"""Statistics that are not numbers on their way through joins: a row that failed
+stays one that failed, however many parts it is joined from and in whatever order."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_paged_gpu import Case  # noqa: E402
+from test_paged_more_gpu import joined  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def paged():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from secure_infer_b200 import paged
+    return paged
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", range(1, 9))
+def test_a_logarithm_of_nan_is_kept_beside_any_others(paged, n, dtype):
+    """One part's is NaN, at every place, the others' all -inf, all finite, all +inf, or some of each."""
+    others = [[-math.inf], [0.5], [math.inf], [-math.inf, 0.5], [-math.inf, math.inf], [-3e38, -math.inf]]
+    rows = [(at, other) for at in range(n) for other in others]
+    lse = torch.tensor([[math.nan if i == at else other[i % len(other)] for i in range(n)] for at, other in rows], device="cuda")
+    outs = [torch.full((len(rows), 1, 128), float(i + 1), dtype=dtype, device="cuda") for i in range(n)]
+    out, got = paged.join(outs, [lse[:, i:i + 1] for i in range(n)])
+    assert torch.isnan(out).all() and torch.isnan(got).all()
+
+
+@pytest.mark.parametrize("n", range(1, 9))
+def test_rows_that_see_nothing_and_rows_beside_failed_ones(paged, n):
+    """What is -inf in every part stays so, and a NaN stays in its own row and head."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    outs = [torch.randn((60, 3, 128), generator=g, device="cuda").bfloat16() for _ in range(n)]
+    lses = [3 * torch.randn((60, 3), generator=g, device="cuda") for _ in range(n)]
+    for i, x in enumerate(lses):
+        x[:20] = -math.inf
+        x[20:30] = -math.inf if i else 1.0
+    lses[-1][5, 1] = lses[0][40, 2] = math.nan
+    failed = torch.zeros((60, 3), dtype=torch.bool, device="cuda")
+    failed[5, 1] = failed[40, 2] = True
+    none = torch.zeros_like(failed)
+    none[:20] = True
+    none &= ~failed
+    out, lse = paged.join(outs, lses)
+    assert torch.equal(torch.isnan(lse), failed) and torch.equal(torch.isnan(out).any(2), failed)
+    assert torch.equal(lse == -math.inf, none) and (out[none] == 0).all()
+    clean = [torch.where(torch.isnan(x), 0.0, x) for x in lses]
+    want, want_lse, bound = joined(outs, clean)
+    rest = ~failed & ~none
+    assert ((out.double() - want).abs() <= bound)[rest].all()
+    assert ((lse.double() - want_lse).abs() <= 2e-7 * want_lse.abs() + 1e-6)[rest].all()
+
+
+def test_a_failed_call_is_seen_through_joins_in_stages(paged):
+    """attend with a workspace that is down gives NaN; joined with parts that see nothing, and then with one that does,
+    its rows are NaN still."""
+    for lens in ([(1, 300), (3, 700)], [(200, 900), (1, 256)]):
+        c = Case(paged, lens, 8, 2)
+        workspace = paged.attend_workspace("cuda:0")
+        workspace.view(torch.int32)[0] = 1
+        failed = paged.attend(c.pages, c.chunk, c.q, return_lse=True, workspace=workspace)
+        nothing = (torch.zeros_like(c.q), torch.full(c.q.shape[:2], -math.inf, device="cuda"))
+        sound = paged.attend(c.pages, c.chunk, c.q, return_lse=True)
+        c.check(*sound)
+        for first in ([failed, nothing], [nothing, failed], [nothing, failed, nothing]):
+            stage = paged.join(*zip(*first))
+            out, lse = paged.join(*zip(stage, sound))
+            assert torch.isnan(out).all() and torch.isnan(lse).all()
+        out, lse = paged.join(*zip(paged.join(*zip(nothing, nothing)), sound))
+        assert torch.equal(out, sound[0]) and (lse - sound[1]).abs().max() <= 2e-6
