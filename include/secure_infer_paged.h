@@ -87,6 +87,11 @@ uint64_t secure_infer_capture_id(void* stream);
  * units of work (a page for a tile of rows and a KV head), by the longest context
  * that the table's width can hold. */
 int secure_infer_attend_fits(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads);
+/* The same for a call with a window and sinks, whose tiles count a page more.
+ * (A shared prefix refuses nothing: where its work would pass that the call goes
+ * without it.) */
+int secure_infer_attend_fits_window(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads,
+                                    uint32_t window, uint32_t sinks);
 /* Waits for the stream, which is the one exception here.  *status: 0, or 1 if a
  * wait ran out in a call with this workspace; then its state is zero again and
  * the next call computes.  -1 while the stream is captured. */

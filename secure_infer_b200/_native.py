@@ -151,6 +151,7 @@ PAGED_SIGNATURES = {
 HOST_SIGNATURES.update(PAGED_SIGNATURES)
 HOST_SIGNATURES["secure_infer_capture_id"] = ([P], U64)
 HOST_SIGNATURES["secure_infer_attend_fits"] = ([P, P, U32], I32)
+HOST_SIGNATURES["secure_infer_attend_fits_window"] = ([P, P, U32, U32, U32], I32)
 HOST_SIGNATURES["secure_infer_attend_status"] = ([P, P, P], I32)
 HOST_SIGNATURES["secure_infer_attend"] = ([P, P, P, I64, I64, U32, P, P, ct.c_float, U32, U32, P, P, P], I32)
 HOST_SIGNATURES["secure_infer_attend_parts"] = ([P, P, U32, P], U64)

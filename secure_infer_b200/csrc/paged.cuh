@@ -32,6 +32,16 @@ enum Mode : int {
     kShared    // groups of sequences whose first pages are the same: these are attended once for all of a group's rows
 };
 
+// Pages that the beginning and the end of a tile are worth, which the kernels count with its pages and the host when it
+// bounds what they count.  Of few rows: with sinks and shared prefixes 2, where 48 answers to 8192 take 45.2 us (1: 50.5,
+// 3: 47.6); the usual call keeps the 1 that its results' order of sums goes by.
+constexpr int rows_cost(Mode mode) { return mode == kPlain ? 1 : 2; }
+// Of a pair of tiles.  With shared prefixes partial results are twice as long, and 4.5 us go besides the pages where
+// sequences fill both tiles (`full`).  Eight chunks of up to 40 tokens of 7 rows on 30000: 194 us with 2, 131 with 4; four
+// times six drafts of 5 of 8 rows on up to 30000, one tile each: 35.2 and 37.1.
+constexpr int kTilesCost = 2, kFullTilesCost = 4;
+inline int tiles_cost(Mode mode, bool full) { return mode == kShared && full ? kFullTilesCost : kTilesCost; }
+
 // A group of sequences with a common prefix, as secure_infer_shared_prefix
 // leaves it behind the sequences' own prefixes.
 struct Group {
@@ -68,7 +78,7 @@ struct AttendParams {
     const int32_t* prefix;          // kShared: [seqs] keys in common with the sequence's group
     const Group* shared;            // [groups]
     int32_t groups;
-    int32_t tiles_cost;             // pages that the beginning and the end of a pair of tiles are worth
+    int32_t tiles_cost;             // tiles_cost() of the call
     float* parts;                   // [2][rows of the output][128] sums over the group's and over a sequence's own keys, then
                                     // [2][rows] maxima and sums of weights
 };

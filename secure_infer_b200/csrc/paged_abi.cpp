@@ -105,10 +105,30 @@ struct Work {
     bool fits() const { return rows_units <= INT_MAX && tiles_units <= INT_MAX; }
 };
 
-// `groups` of sequences share a prefix: all their rows make tiles of it.
-Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, uint32_t q_heads, uint32_t groups = 0)
+// What rows see behind a window (0: none) with sinks.
+struct Sight {
+    int32_t window, sinks;
+    Mode mode;
+};
+Sight sight_of(const secure_infer_chunk& chunk, uint32_t window, uint32_t sinks)
+{
+    // As many tokens as a table can hold hide nothing, and positions less such a window might pass 32 bits.
+    const uint64_t most = static_cast<uint64_t>(chunk.table_width) * kPage;
+    if (window == 0 || window >= most || sinks >= most) return {0, 0, kPlain};
+    return {static_cast<int32_t>(window), static_cast<int32_t>(sinks), sinks > 0 ? kSinks : kPlain};
+}
+
+// Whether sequences that share prefixes fill pairs of tiles.
+bool tiles_full(const secure_infer_chunk& chunk, uint64_t group)
+{
+    return chunk.tokens * group > uint64_t(128) * (chunk.seqs < chunk.tokens ? chunk.seqs : chunk.tokens);
+}
+
+// `groups` of sequences share a prefix (kShared): all their rows make tiles of it.
+Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, uint32_t q_heads, Mode mode, uint32_t groups = 0)
 {
     Work w{q_heads / pages.heads, false, 0, 0};
+    const uint64_t a_tile = rows_cost(mode), a_pair = tiles_cost(mode, tiles_full(chunk, w.group));
     const uint32_t max_q = chunk.max_q == 0 || chunk.max_q > chunk.tokens ? chunk.tokens : chunk.max_q;
     const uint64_t max_rows = static_cast<uint64_t>(max_q) * w.group, rows = static_cast<uint64_t>(chunk.tokens) * w.group;
     // Up to kFewRows rows per KV head a sequence is bound by reading K and V once, which the kernel for few rows does
@@ -119,10 +139,10 @@ Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, u
     };
     const uint64_t seqs = uint64_t(chunk.seqs) + groups, all = groups > 0 ? 2 * rows : rows;
     if (max_rows > INT_MAX || (groups > 0 && rows > INT_MAX)) w.rows_units = UINT64_MAX;
-    else if (!w.tiles) w.rows_units = units(all / 8 + seqs, 1);
+    else if (!w.tiles) w.rows_units = units(all / 8 + seqs, a_tile);
     else {
-        w.rows_units = seqs > 1 ? units(seqs * (kFewRows / 8), 1) : 0;
-        w.tiles_units = units(all / (2 * (128 / w.group * w.group)) + seqs, 2);
+        w.rows_units = seqs > 1 ? units(seqs * (kFewRows / 8), a_tile) : 0;
+        w.tiles_units = units(all / (2 * (128 / w.group * w.group)) + seqs, a_pair);
     }
     return w;
 }
@@ -156,7 +176,7 @@ uint32_t shared_groups(const secure_infer_pages& pages, const secure_infer_chunk
     const int64_t cost = largest > kFewRows || group > 128 || tokens * group <= kFewRows ? kShareCost : kShareTilesCost;
     const double saved = static_cast<double>(apart - together) * common * pages.heads;
     const bool worth = saved > static_cast<double>(cost) + static_cast<double>(tokens * q_heads) / 6;
-    return worth && work_of(pages, chunk, q_heads, groups).fits() ? groups : 0;
+    return worth && work_of(pages, chunk, q_heads, kShared, groups).fits() ? groups : 0;
 }
 
 bool tables_ok(const secure_infer_tables* in, const secure_infer_tables* out)
@@ -215,7 +235,13 @@ static bool call_ok(const secure_infer_pages* pages, const secure_infer_chunk* c
 
 SI_EXPORT int secure_infer_attend_fits(const secure_infer_pages* pages, const secure_infer_chunk* chunk, uint32_t q_heads)
 {
-    return call_ok(pages, chunk, q_heads) && work_of(*pages, *chunk, q_heads).fits();
+    return call_ok(pages, chunk, q_heads) && work_of(*pages, *chunk, q_heads, kPlain).fits();
+}
+
+SI_EXPORT int secure_infer_attend_fits_window(const secure_infer_pages* pages, const secure_infer_chunk* chunk,
+                                              uint32_t q_heads, uint32_t window, uint32_t sinks)
+{
+    return call_ok(pages, chunk, q_heads) && work_of(*pages, *chunk, q_heads, sight_of(*chunk, window, sinks).mode).fits();
 }
 
 SI_EXPORT uint64_t secure_infer_attend_parts(const secure_infer_pages* pages, const secure_infer_chunk* chunk,
@@ -295,7 +321,9 @@ SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_
     if (!aligned16(q) || !aligned16(out) || !stride_ok(q_token_stride) || !stride_ok(q_head_stride) ||
         (groups > 0 && !aligned16(options->parts)))
         return -1;
-    const Work work = work_of(*pages, *chunk, q_heads, groups);
+    const Sight sight = sight_of(*chunk, window, sinks);
+    const Mode mode = groups > 0 ? kShared : sight.mode;
+    const Work work = work_of(*pages, *chunk, q_heads, mode, groups);
     if (!work.fits()) return -1;
     const uint32_t group = work.group;
 
@@ -325,22 +353,14 @@ SI_EXPORT int secure_infer_attend(const secure_infer_pages* pages, const secure_
     p.rows_min = 1;
     p.rows_max = INT_MAX;
     p.causal = causal != 0;
-    // As many tokens as a table can hold hide nothing, and positions less such a window might pass 32 bits.
-    const uint64_t most = static_cast<uint64_t>(chunk->table_width) * kPage;
-    p.window = window >= most || sinks >= most ? 0 : static_cast<int32_t>(window);
-    p.sinks = p.window != 0 ? static_cast<int32_t>(sinks) : 0;
-    Mode mode = p.sinks > 0 ? kSinks : kPlain;
+    p.window = sight.window;
+    p.sinks = sight.sinks;
     if (groups > 0) {
-        mode = kShared;
         p.prefix = options->plan;
         p.shared = reinterpret_cast<const Group*>(options->plan + group_offset(chunk->seqs));
         p.groups = static_cast<int32_t>(groups);
         p.parts = options->parts;
-        // Partial results are twice as long: a pair of tiles takes 4.5 us besides its pages, where sequences fill both. Eight
-        // chunks of up to 40 tokens of 7 rows on 30000: 194 us with 2, 131 with 4; four times six drafts of 5 of 8 rows on
-        // up to 30000, one tile each: 35.2 and 37.1.
-        const uint64_t seqs = chunk->seqs < chunk->tokens ? chunk->seqs : chunk->tokens;
-        p.tiles_cost = uint64_t(chunk->tokens) * group > 128 * seqs ? 4 : 2;
+        p.tiles_cost = tiles_cost(kShared, tiles_full(*chunk, group));
     }
     p.scale_log2 = scale * 1.4426950408889634f;
     // Hidden scores are -inf before they are scaled, so the scale is never zero; at 1e-30 all weights are 1.

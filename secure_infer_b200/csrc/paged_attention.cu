@@ -88,21 +88,18 @@ constexpr uint32_t kRowsSmem = 1024 + kRowsStages * 2 * kPageTile + 2 * kRows * 
 // Units up to which a tile is not cut where there is little work, with a cost of 1.
 // One sequence of 200 tokens: 6.7 us in whole tiles, 7.9 cut; of 512: 8.4 and 8.1.
 constexpr int kRowsWhole = 4;
-// Pages that a tile's beginning and end are worth: with sinks and shared prefixes 2, where 48 answers to 8192 take 45.2 us
-// (1: 50.5, 3: 47.6); the usual call keeps the 1 that its results' order of sums goes by.
 template <int M>
-constexpr int kRowsCost = M == kPlain ? 1 : 2;
+constexpr int kRowsCost = rows_cost(static_cast<Mode>(M));
 // Rows of partial results (512 bytes each) that one CTA joins: reading 80 KiB takes it about as long as counting once
 // more in a second step.
 constexpr int kJoinRows = 160;
 // Partial result of a CTA: [rows][128] sums, [rows] maxima, [rows] sums.
 constexpr int kRowSlot = kRows * (kDim + 2);
 
-// Pages that a pair of tiles' beginning and end are worth.
 template <int M>
 __device__ __forceinline__ int tiles_cost(const AttendParams& p)
 {
-    return M == kShared ? p.tiles_cost : 2;
+    return M == kShared ? p.tiles_cost : kTilesCost;
 }
 
 // An SM takes 1.1 us of a page for few rows where fewer than 120 of 148 SMs read (58 GB/s each; 120 to 130 get nearly

@@ -174,7 +174,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
                                     want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, static_cast<float>(scale),
                                     causal, static_cast<uint32_t>(window), &options, workspace.data_ptr(),
                                     address<void>(a[10])) != 0) {
-                need(secure_infer_attend_fits(pages, &chunk, static_cast<uint32_t>(r.heads)),
+                need(secure_infer_attend_fits_window(pages, &chunk, static_cast<uint32_t>(r.heads), static_cast<uint32_t>(window),
+                                                     options.sinks),
                      "more work than one call takes: fewer tokens, or a narrower block table");
                 return failed("secure_infer_attend");
             }
