@@ -311,14 +311,14 @@ __device__ __forceinline__ bool zero_sum_odd(uint32_t sum)
 }
 
 // The sequence of a token, by a warp: the last s with cu[s] <= token, 32 probes at
-// a time.
+// a time.  From L2, since some kernels read them before they have waited.
 __device__ __forceinline__ int find_seq(const int32_t* cu, int seqs, int token)
 {
     const int lane = threadIdx.x & 31;
     int lo = 0, hi = seqs;   // cu[lo] <= token, and the answer lies in [lo, hi)
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const uint32_t below = __ballot_sync(0xffffffffu, at < hi && cu[at] <= token);
+        const uint32_t below = __ballot_sync(0xffffffffu, at < hi && __ldcg(cu + at) <= token);
         const int k = below == 0 ? 0 : 31 - __clz(below);
         lo += k * step;
         hi = min(hi, lo + step);

@@ -3,6 +3,8 @@ where there is no GPU."""
 from __future__ import annotations
 
 import ctypes as ct
+import re
+from pathlib import Path
 
 import pytest
 
@@ -68,3 +70,17 @@ def test_work_with_a_shared_prefix_is_bounded_by_what_its_kernels_count(lib, seq
     assert units(width, 1, 2) < 2 ** 31 <= units(width, 2, 4)
     assert not together(width) and not together(width + 1)
     assert units(width - 3, 2, 4) < 2 ** 31 and together(width - 3)
+
+
+CSRC = Path(__file__).resolve().parents[1] / "secure_infer_b200" / "csrc"
+
+
+@pytest.mark.parametrize("function,arrays", [("find_seq", "cu"), ("load_any", "p.cu|p.kv|p.prefix|p.shared")])
+def test_what_is_read_before_a_kernel_has_waited_comes_from_l2(function, arrays):
+    """Lines that an earlier kernel on the SM left in L1 may be older than what the call was given."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / "paged.cuh").read_text())
+    at = re.search(r"%s\([^;]*?\)\n\{" % function, text).end()
+    body = text[at:text.index("\n}\n", at)]
+    names = "|".join(re.escape(n) for n in arrays.split("|"))
+    reads = re.findall(r"(?:__ldcg\((?:reinterpret_cast<const int4\*>\()?)?(?<![\w.])(?:%s)(?![\w.])" % names, body)
+    assert reads and all(r.startswith("__ldcg(") for r in reads), reads

@@ -1,5 +1,6 @@
 """Statistics that are not numbers on their way through joins: a row that failed
-stays one that failed, however many parts it is joined from and in whatever order."""
+stays one that failed, however many parts it is joined from and in whatever order.
+And sequences whose tokens move from call to call under one plan's groups."""
 from __future__ import annotations
 
 import math
@@ -10,7 +11,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_paged_gpu import Case  # noqa: E402
-from test_paged_more_gpu import joined  # noqa: E402
+from test_paged_more_gpu import Family, joined, together  # noqa: E402
 
 
 @pytest.fixture(scope="module")
@@ -75,3 +76,40 @@ def test_a_failed_call_is_seen_through_joins_in_stages(paged):
             assert torch.isnan(out).all() and torch.isnan(lse).all()
         out, lse = paged.join(*zip(paged.join(*zip(nothing, nothing)), sound))
         assert torch.equal(out, sound[0]) and (lse - sound[1]).abs().max() <= 2e-6
+
+
+@pytest.mark.parametrize("lens,groups", [([(1, 700 + 9 * i) for i in range(12)], [(12, 5)]), ([(3, 500), (1, 520), (30, 600), (1, 700)], [(4, 3)])])
+def test_offsets_that_change_before_every_call(paged, lens, groups):
+    """New tokens change hands between calls that follow one another without a pause, in eager mode and in a graph: every
+    call's rows are those of the offsets that it was given."""
+    c = Family(paged, lens, groups, 8, 2, seed=11)
+    assert together(c.pages, c.chunk, c.q, c.shared)
+    tokens = c.cu[-1]
+    # Sequence s has a token or none, by turns; the others' tokens stay where the offsets say.
+    offsets = []
+    for turn in range(4):
+        n = [(k if (s + turn) % 3 else 0) for s, (k, _) in enumerate(lens)]
+        offsets.append([sum(n[:s]) for s in range(len(lens) + 1)])
+    offsets = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+
+    def steps(outs):
+        for cu, out in zip(offsets, outs):
+            c.chunk.cu_q.copy_(cu)
+            c.shared.update()
+            paged.attend(c.pages, c.chunk, c.q, shared=c.shared, out=out)
+
+    outs = [torch.full_like(c.q, 7.0) for _ in offsets]
+    steps(outs)
+    graph, again = torch.cuda.CUDAGraph(), [torch.full_like(c.q, 7.0) for _ in offsets]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        steps(again)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    all_lens, all_cu, q = c.lens, c.cu, c.q
+    for cu, out, other in zip(offsets.tolist(), outs, again):
+        assert (out[cu[-1]:] == 7.0).all() and torch.equal(out, other)
+        c.lens, c.cu, c.q = [(b - a, kv) for a, b, (_, kv) in zip(cu, cu[1:], all_lens)], cu, q[:cu[-1]]
+        c.check(out[:cu[-1]])
+    assert tokens == all_cu[-1]
