@@ -225,7 +225,7 @@ int secure_infer_paged_free(const secure_infer_tables* in, const secure_infer_ta
 /* trim: the sequences give up the pages that no later token sees when it is
  * attended with this window and these sinks: those behind the first `sinks`
  * tokens that lie wholly before the window of the token at position lens.
- * window >= 1.  Their entries become -1, lengths stay. */
+ * 1 <= window < 2^31, sinks < 2^31 - 128.  Their entries become -1, lengths stay. */
 int secure_infer_trim(const secure_infer_tables* in, const secure_infer_tables* out, const int32_t* seqs, uint32_t n,
                       uint32_t window, uint32_t sinks, void* scratch, void* stream);
 

@@ -456,14 +456,16 @@ PyObject* trim(PyObject*, PyObject* const* a, Py_ssize_t n)
         const int64_t window = PyLong_AsLongLong(a[6]), sinks = PyLong_AsLongLong(a[7]);
         if (PyErr_Occurred()) return nullptr;
         need(window > 0 && window < int64_t(1) << 31, "window must be positive");
-        need(sinks >= 0 && sinks < (int64_t(1) << 31) - 256, "sinks must be zero or positive");
+        need(sinks >= 0 && sinks < int64_t(1) << 31, "sinks must be zero or positive, and below 2^31");
+        // As many as a table can hold keep every page.
+        constexpr int64_t most = int64_t(1) << 30;
         const Tables in = tables(a, pages, device), out = outputs(a[9], in, pages, device);
         const at::Tensor& seqs = tensor(a[5], "seqs");
         const int32_t* named = ints(seqs, 1, device, kRequests);
         const uint32_t asked = requests(seqs, seqs);
         at::Tensor scratch = scratch_of(in, asked);
-        if (secure_infer_trim(&in.c, &out.c, named, asked, static_cast<uint32_t>(window), static_cast<uint32_t>(sinks),
-                              scratch.data_ptr(), address<void>(a[8])) != 0)
+        if (secure_infer_trim(&in.c, &out.c, named, asked, static_cast<uint32_t>(window),
+                              static_cast<uint32_t>(std::min(sinks, most)), scratch.data_ptr(), address<void>(a[8])) != 0)
             return failed("secure_infer_trim");
         return results({out.table, out.lens, out.refs});
     });

@@ -113,3 +113,21 @@ def test_offsets_that_change_before_every_call(paged, lens, groups):
         c.lens, c.cu, c.q = [(b - a, kv) for a, b, (_, kv) in zip(cu, cu[1:], all_lens)], cu, q[:cu[-1]]
         c.check(out[:cu[-1]])
     assert tokens == all_cu[-1]
+
+
+@pytest.mark.parametrize("sinks", [2 ** 31 - 1, 2 ** 31 - 256, 2 ** 31 - 257, 2 ** 30, 1 << 23])
+def test_trim_takes_the_sinks_that_attend_takes(paged, sinks):
+    """As many sinks as a context has tokens keep all of its pages."""
+    c = Family(paged, [(1, 700), (1, 650)], [(2, 4)], 8, 2)
+    cache = paged.CachePages([[c.k, c.v]])
+    out = paged.attend(c.pages, c.chunk, c.q, window=8, sinks=sinks)
+    c.check(out)
+    refs = torch.zeros(cache.pages, dtype=torch.int32, device="cuda")
+    held = c.chunk.block_table[c.chunk.block_table >= 0].long()
+    refs.index_add_(0, held, torch.ones_like(held, dtype=torch.int32))
+    t = paged.PageTables(c.chunk.block_table, c.chunk.kv_lens, refs)
+    new = cache.trim(t, [0, 1], 8, sinks)
+    assert all(torch.equal(a, b) for a, b in zip(new, t))
+    for bad in (2 ** 31, -1):
+        with pytest.raises(ValueError):
+            cache.trim(t, [0, 1], 8, bad)
