@@ -133,8 +133,9 @@ uint64_t secure_infer_attend_parts(const secure_infer_pages* pages, const secure
  * group with new tokens names in the same places, as far as all their tokens lie
  * before the new ones of each.  plan: secure_infer_shared_prefix_ints() int32,
  * 16-byte aligned: the common tokens of each sequence [seqs], then the kernels'
- * own.  It goes with the chunk's contents when this runs: lengths and tables that
- * change (other than by more tokens behind the common ones) need another. */
+ * own.  It goes with the chunk's contents when this runs: offsets, lengths and
+ * tables that change need another.  Only kv_lens may grow meanwhile, under the same
+ * cu_q: rows that the plan does not know would read what nobody has written. */
 uint64_t secure_infer_shared_prefix_ints(uint32_t seqs, uint32_t groups);
 int secure_infer_shared_prefix(const secure_infer_chunk* chunk, const int32_t* cu_seqs, uint32_t groups, int32_t* plan,
                                void* stream);

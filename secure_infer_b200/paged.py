@@ -138,7 +138,8 @@ class SharedPrefix:
 
     Found on the device, on the current stream, from what the chunk's tensors
     hold at that time.  ``update`` finds it again where they have changed, as a
-    captured graph does that holds this call.
+    captured graph does that holds this call.  Only ``kv_lens`` may grow without it:
+    with other offsets or tables than it was found for ``attend`` gives wrong rows.
 
     Whether ``attend`` goes by it is a matter of time, and judged on the host by
     the numbers of sequences, groups, tokens and heads, and by ``max_common``: no

@@ -131,3 +131,28 @@ def test_trim_takes_the_sinks_that_attend_takes(paged, sinks):
     for bad in (2 ** 31, -1):
         with pytest.raises(ValueError):
             cache.trim(t, [0, 1], 8, bad)
+
+
+@pytest.mark.parametrize("lens,groups", [([(1, 700), (1, 650), (1, 643)], [(3, 4)]), ([(5, 900), (40, 1000), (1, 790)], [(3, 5)])])
+def test_a_plan_outlives_lengths_that_grow(paged, lens, groups):
+    """Under the same offsets a plan holds for longer sequences, eagerly and in a graph that has no update."""
+    c = Family(paged, lens, groups, 8, 2, seed=12)
+    whole, rows = c.lens, c.rows
+    at = lambda back: ([(n, kv - back) for n, kv in whole], [[x[:kv - back] for x in r] for r, (_, kv) in zip(rows, whole)])  # noqa: E731
+    c.chunk.kv_lens.sub_(3)
+    c.lens, c.rows = at(3)
+    c.shared.update()
+    out, lse = c.run(paged)
+    c.check(out, lse)
+    captured, graph = torch.empty_like(c.q), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        paged.attend(c.pages, c.chunk, c.q, shared=c.shared, out=captured)
+    for back in (2, 1, 0):
+        c.chunk.kv_lens.add_(1)
+        c.lens, c.rows = at(back)
+        out, lse = paged.attend(c.pages, c.chunk, c.q, shared=c.shared, return_lse=True)
+        c.check(out, lse)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, out)
