@@ -99,7 +99,7 @@ def run(layers=4, prefix_blocks=6, chunk_tokens=75, answers=4, steps=6, check=Fa
             tables, granted = cache.reserve(tables, ints(alive), tables.lens[rows] + 1)
             assert granted.all()
             chunk = paged.Chunk(tables.block_table[rows], ints(list(range(len(alive) + 1))), tables.lens[rows], max_q=1)
-            shared = paged.SharedPrefix(chunk)
+            shared = paged.SharedPrefix(chunk, max_common=length)   # no answer shares more than the prompt
             for i, layer in enumerate(stack):
                 x = layer(x, cache.layers[i], chunk, rotary, shared=shared)
         say(f"{steps} tokens for each answer; lengths {tables.lens.tolist()}")

@@ -152,11 +152,14 @@ Work work_of(const secure_infer_pages& pages, const secure_infer_chunk& chunk, u
 // the caller says they may be.  A page takes an SM 4 units of time (1.1 us) for
 // eight rows in the kernel for few rows, as long for 128 rows in tiles and 7 for
 // 256.  It costs the joining of the parts (0.17 units a row) and, in a call that has
-// no tiles otherwise, the tiles' kernel and its own join.  Together and apart, us:
-// single tokens of 8 KV heads of 4 rows, 2 sequences with 512, 2048 and 8192 tokens in
-// common 10.2 and 8.4, 11.9 and 9.8, 14.4 and 16.5; 8 sequences with 2048, 8192 and
-// 30000 (tiles) 22.0 and 16.4, 25.7 and 32.4, 50.7 and 87; 8 chunks of up to 40
-// tokens of 4 rows with 2048, 8192, 30000 41 and 37, 65 and 71, 146 and 202.
+// no tiles otherwise, the tiles' kernel and its own join.  Together and apart, us, in
+// a graph: single tokens of 8 KV heads of 4 rows, 2 sequences with 512, 2048 and 8192
+// tokens in common 9.7 and 8.3, 12.3 and 9.7, 14.5 and 16.0; 8 sequences with 2048,
+// 8192 and 30000 (tiles) 18.3 and 16.1, 23.1 and 31.7, 44.1 and 86.5; 8 chunks of up to
+// 40 tokens of 4 rows with 2048, 8192, 30000 33 and 34, 56 and 74, 132 and 249; 5
+// chunks of up to 300 tokens of 7 rows with 6144 127 and 108.  Where nothing is said
+// of how much is common this stands for the table's width, and is wrong in wide ones:
+// 48 single tokens that share nothing 166 and 145.
 constexpr int64_t kShareCost = 1000, kShareTilesCost = 12000;
 int64_t page_time(uint64_t rows)
 {

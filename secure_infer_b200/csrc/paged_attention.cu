@@ -103,7 +103,7 @@ __device__ __forceinline__ int tiles_cost(const AttendParams& p)
 }
 
 // An SM takes 1.1 us of a page for few rows where fewer than 120 of 148 SMs read (58 GB/s each; 120 to 130 get nearly
-// all that memory gives), and 1.95 us of a page for a pair of tiles, whose kernel begins 5.5 us later.
+// all that memory gives), and 1.95 us of a page for a pair of tiles, whose first scores in one launch are there 2 us later.
 template <int M>
 __device__ __forceinline__ Kind rows_kind()
 {
@@ -1440,9 +1440,11 @@ paged_attend_tiles_kernel(const __grid_constant__ CUtensorMap q_map, const __gri
 // Sequences of few rows beside chunks, or beside the prefixes that they share: one
 // launch, in which a CTA does the one or the other.  As two launches the second's
 // CTAs started 3.6 us later, where the first's had counted the work and left: 777
-// tokens and 3 single ones with sinks 45.5 us for 43.5 (floor 8.6), drawn calls up
-// to 16 % more, 48 answers to a prompt of 8192 45.5 for 47.8 (floor 18.3, reading
-// their pages).  Bound by its start, 5 us to the first scores, and by tiles' ends.
+// tokens and 3 single ones with sinks 45.5 us for 43.5 (floor 8.6), 48 answers to a
+// prompt of 8192 45.5 for 47.8 (floor 18.3, reading their pages).  Bound by its start,
+// 5 us to the first scores, and by tiles' ends.  In the 96 registers that it starts
+// with it spills 156 bytes a thread with shared prefixes and 188 with sinks, where
+// either kind's own kernel spills nothing.
 template <typename T, int M>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_attend_both_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,

@@ -123,8 +123,9 @@ __global__ void __launch_bounds__(32 * kPartsWarps) attend_parts_kernel(const __
 //
 // Bound by reading every part's rows and writing one's.  Sixteen lanes a row,
 // 16-byte accesses, every part on its way at once.  Measured: three parts of 8000
-// tokens of 28 heads 37.5 us, 6.2 TB/s, where the copy rate would take 35.7; two of
-// 16 tokens 1.9.
+// tokens of 28 heads 37.7 us in a graph, where a part of the inputs is in L2, and 41.4
+// by calls with cold ones, 5.6 TB/s, where the copy rate would take 35.7; two of 16
+// tokens 1.6 and 6.0, which is the host's time.
 constexpr int kJoinPartsThreads = 256;
 constexpr int kJoinPartsRows = kJoinPartsThreads / 16;
 

@@ -143,9 +143,11 @@ class SharedPrefix:
 
     Whether ``attend`` goes by it is a matter of time, and judged on the host by
     the numbers of sequences, groups, tokens and heads, and by ``max_common``: no
-    group has more tokens in common (by default as many as the block table is wide
-    for; given, it keeps short prefixes in wide tables from costing more than they
-    save)."""
+    group has more tokens in common.  Give it wherever the host knows it, as one
+    that forked the sequences does.  By default it is as many as the block table is
+    wide for, and a table for long contexts then makes ``attend`` go by prefixes that
+    are short, or not there at all, which takes it up to a fifth longer than without
+    ``shared``."""
 
     def __init__(self, chunk: Chunk, cu_seqs: torch.Tensor | None = None, max_common: int | None = None):
         _need(isinstance(chunk, Chunk), "chunk must be a Chunk")
@@ -268,8 +270,8 @@ def attend(pages: LayerPages, chunk: Chunk, q: torch.Tensor, *, scale: float | N
     ``window`` of them and, behind these, the sequence's first ``sinks``;
     otherwise all of its sequence.  ``shared``, of this chunk and without a
     window: what its groups have in common is attended once for all of a group's
-    rows, which gives the same up to the order of sums.  Returns ``[tokens,
-    q heads, 128]``, and with ``return_lse`` the natural logarithms of the
+    rows, which gives the same up to the order of sums and the rounding of weights
+    to the cache's type.  Returns ``[tokens, q heads, 128]``, and with ``return_lse`` the natural logarithms of the
     softmax sums, float32 ``[tokens, q heads]``, to join it with attention over
     other keys.  A row that sees no key gives 0 and -inf; rows of tokens past
     the chunk's last are left as they were.  ``workspace``:
