@@ -115,7 +115,8 @@ int secure_infer_paged_attend(const secure_infer_pages* pages, const secure_infe
  * alone: max_common says that no group has more tokens in common (0: as many as the
  * table holds, which in tables much wider than the prefixes may take the slower
  * way).  parts: secure_infer_attend_parts() bytes, 16-byte aligned, for
- * this call alone; null where that is 0.  options may be null. */
+ * this call alone; null where that is 0, else 1040 bytes for every token of the call
+ * and query head.  options may be null. */
 typedef struct {
     const int32_t* plan;
     float* parts;

@@ -156,3 +156,23 @@ def test_a_plan_outlives_lengths_that_grow(paged, lens, groups):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(captured, out)
+
+
+def test_work_beyond_32_bits_with_sinks_is_refused(paged):
+    """1024 sequences of one token on 8 KV heads in a table of 87380 pages: three tiles of few rows each make
+    24576 * 87381 units by the usual count, which fits, and 24576 * 87382 with sinks, which does not."""
+    width = 87380
+    assert 24576 * (width + 1) < 2 ** 31 <= 24576 * (width + 2)
+    k, v = (torch.zeros((2, 128, 8, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cu = torch.arange(1025, dtype=torch.int32, device="cuda")
+    table, none = torch.zeros((1024, width), dtype=torch.int32, device="cuda"), torch.zeros(1024, dtype=torch.int32, device="cuda")
+    pages, chunk, q = paged.LayerPages(k, v), paged.Chunk(table, cu, none), torch.ones((1024, 8, 128), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="more work than one call takes"):
+        paged.attend(pages, chunk, q, window=5000, sinks=4)
+    for kw in (dict(window=5000), dict(), dict(shared=paged.SharedPrefix(chunk))):
+        out, lse = paged.attend(pages, chunk, q, return_lse=True, **kw)
+        assert not out.any() and (lse == -math.inf).all()
+    # A column less, and it fits.
+    narrow = paged.Chunk(table[:, :width - 1], cu, none)
+    out, lse = paged.attend(pages, narrow, q, window=5000, sinks=4, return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
